@@ -47,7 +47,7 @@ typedef enum rkv_dtype {
     RKV_F32 = 0,
     RKV_BF16 = 1,
     RKV_Q8_0 = 2,
-    RKV_F16 = 3   /* source type of rkv_capture_rows only */
+    RKV_F16 = 3   /* sources of rkv_capture_rows, paged caches, rkv_sink_attention */
 } rkv_dtype;
 
 /* Stage-1 scoring engine. */
@@ -318,6 +318,121 @@ int rkv_evict_compact(const void* Q, const void* K, const void* V, int dtype, in
                       int* kept, int kept_stride, int* n_kept, void* K_out, void* V_out, int out_len,
                       long long out_item_stride, void* workspace, size_t workspace_bytes, int engine,
                       void* stream);
+
+/* ---- paged KV cache ---------------------------------------------------------
+ * The dense counterpart of stage 2, and the eviction that watches it: a cache
+ * whose rows live in pages of `page_size` tokens, one token attended over all
+ * of it (or over a window and a few first tokens), rows appended, and the
+ * least attended tokens evicted.  No counterpart in the reference, which
+ * keeps one contiguous cache per sequence in llama.cpp.
+ *
+ * Token t of sequence b and KV head h is row t % page_size of page
+ * block_table[b * table_stride + t / page_size]: bytes
+ *   page * page_stride + h * head_stride + (t % page_size) * token_stride
+ * from K and from V alike (strides in bytes, so [page][head][token][dim] and
+ * [page][token][head][dim] pools are both served), dim_head values of dtype
+ * RKV_F32, RKV_BF16 or RKV_F16.  dim_head: a multiple of 8, at most 256.
+ * K, V and every stride are multiples of 16 bytes.  lens[b] counts the tokens
+ * of sequence b; it is read on the device and clamped to
+ * [0, min(max_len, table_stride * page_size)].  Pages may be shared between
+ * sequences that only read them.  A page index outside [0, num_pages) is
+ * never followed: its tokens are left out (not read, not written). */
+typedef struct rkv_paged_cache {
+    void* K;
+    void* V;
+    int dtype;
+    int num_heads_kv;
+    int dim_head;
+    int page_size;             /* tokens per page, >= 1                        */
+    int num_pages;             /* pages in the pool                            */
+    int table_stride;          /* table entries per sequence                   */
+    long long page_stride, head_stride, token_stride;
+    const int* block_table;    /* device [batch][table_stride]                 */
+    const int* lens;           /* device [batch]                               */
+} rkv_paged_cache;
+
+/* Writes the newest rows of every sequence into its pages: lens already
+ * counts them, so row i of the n = n_new[b] (all n_rows where n_new is NULL)
+ * goes to token lens[b] - n + i; rows whose token lies outside
+ * [0, table_stride * page_size) are skipped.  n_new is clamped to
+ * [0, n_rows].  k, v: device, element (b, i, h, d) at b * src_item_stride +
+ * i * src_token_stride + h * src_head_stride + d * element size, the cache's
+ * dtype, strides in bytes and multiples of the element size (rows of a fused
+ * projection are read in place).  The source must not overlap the pages, and
+ * no two written tokens may share a row.  Asynchronous on `stream`. */
+int rkv_paged_append(const rkv_paged_cache* cache, const void* k, const void* v, int n_rows, int batch,
+                     long long src_item_stride, long long src_token_stride, long long src_head_stride,
+                     const int* n_new, void* stream);
+
+/* Attention of one new token per sequence over its paged cache.
+ * Q: [batch] items of [num_heads][dim_head] in the cache's dtype,
+ * q_item_stride bytes apart (16-byte aligned); num_heads a multiple of
+ * num_heads_kv.  Token t of n = lens[b] is visible when window == 0, or
+ * t < sinks, or t >= n - window.  Scores are q.k / sqrt(dim_head).
+ * O: [batch][num_heads][dim_head] fp32; lse (nullable): [batch][num_heads]
+ * natural log of the sum of exponentials.  A sequence with no visible token
+ * gets O = 0 and lse = -inf.  weights (nullable): fp32
+ * [batch][num_heads_kv][weight_stride], weight_stride >= max_len; every
+ * visible token's attention weight, summed over the query heads of its KV
+ * head, is added to its entry (other entries keep their values), which is
+ * what rkv_weight_evict ranks by.  max_len: host bound on lens (it fixes the
+ * launch, so a captured call serves every length up to it).  The cache's
+ * length is split over CTAs by (batch, heads, max_len) alone and the parts are
+ * joined in a fixed order: results repeat bit for bit.
+ * Workspace: device, 16-byte aligned, not shared with a call that may run at
+ * the same time; with_weights: whether weights will be passed.  Asynchronous
+ * on `stream`; allocates nothing. */
+int rkv_paged_decode_workspace_size(int num_heads, int num_heads_kv, int dim_head, int max_len, int batch,
+                                    int with_weights, size_t* bytes);
+int rkv_paged_decode(const void* Q, long long q_item_stride, int num_heads, const rkv_paged_cache* cache,
+                     int max_len, int batch, int sinks, int window, float* O, float* lse, float* weights,
+                     int weight_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated attention weight: every (sequence, KV head) with
+ * more than `budget` tokens keeps its first `sinks`, its last `recent` and,
+ * of the tokens between, the budget - sinks - recent with the largest weights
+ * (ties to the lower index; a NaN weight ranks below every number); sinks +
+ * recent <= budget.  Sequences of at most `budget` tokens keep all.
+ * kept: [batch][num_heads_kv][kept_stride] ascending token indices, -1 behind
+ * them up to min(budget, max_len) <= kept_stride; new_lens: [batch], receives
+ * min(lens[b], budget) and must not be cache->lens.  Then the kept rows of K
+ * and V become rows 0, 1, ... of the sequence in `out` and the kept weights
+ * entries 0, 1, ... of weights_out (strides as the inputs'), entries behind
+ * them up to max_len set to zero.  out NULL (or the same pools and table):
+ * in place; rows from new_lens[b] on keep what they held.  Otherwise `out` is
+ * a cache of the same dtype, heads and dim_head whose pages the input's
+ * sequences do not use (the same pools may hold them); only its first
+ * min(budget, max_len) tokens per sequence are written and its lens is not
+ * read.  weights_out NULL or weights: in place.  In place, no page may belong
+ * to two sequences.  Asynchronous on `stream`; allocates nothing. */
+int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, int weight_stride, int max_len, int batch,
+                     int budget, int sinks, int recent, const rkv_paged_cache* out, float* weights_out,
+                     int* kept, int kept_stride, int* new_lens, void* stream);
+
+/* ---- prefill attention with a sliding window and sinks ------------------------
+ * The causal attention that produces a prompt's cache: query i is at position
+ * p = i + len_k - len_q (len_q <= len_k; the first len_k - len_q keys are a
+ * cached prefix) and sees key j <= p when window == 0, or j < sinks, or
+ * j > p - window.  lens (nullable): device [batch], the valid keys of each
+ * item of a padded batch; keys from lens[b] on are never read and query rows
+ * at positions from lens[b] on are left as they were.
+ * Q: [batch][num_heads][len_q][dim_head], K, V: [batch][num_heads_kv][len_k]
+ * [dim_head], O as Q, all of dtype (RKV_F32, RKV_BF16, RKV_F16; sums and
+ * softmax in fp32), at the given strides (bytes, multiples of 16; NULL: rows,
+ * heads and items back to back).  dim_head: a multiple of 8, at most 256;
+ * num_heads a multiple of num_heads_kv.  lse (nullable):
+ * [batch][num_heads][len_q] fp32.  O must not overlap the inputs.
+ * Workspace: device, 16-byte aligned; holds the error word that
+ * rkv_workspace_status reads.  Asynchronous on `stream`; allocates nothing. */
+typedef struct rkv_row_strides {
+    long long item, head, token;
+} rkv_row_strides;
+int rkv_sink_attention_workspace_size(size_t* bytes);
+int rkv_sink_attention(const void* Q, const void* K, const void* V, int dtype, int len_q, int len_k, int batch,
+                       int num_heads, int num_heads_kv, int dim_head, const rkv_row_strides* q_strides,
+                       const rkv_row_strides* kv_strides, const int* lens, int sinks, int window, void* O,
+                       const rkv_row_strides* o_strides, float* lse, void* workspace, size_t workspace_bytes,
+                       void* stream);
 
 /* ---- errors raised inside kernels ----------------------------------------
  * Kernels record a failed bounded wait in the workspace.  This synchronises

@@ -1,0 +1,583 @@
+// paged.cu -- a paged KV cache on the device: rows appended to its pages, and
+// the attention of one new token over it.
+//
+// The attention.  For query head h of KV head hk the scores of the visible
+// tokens are x_t = (q . k_t) log2(e) / sqrt(D); with m the largest score seen
+// and the running pair (l, o) = (sum 2^(x_t - m), sum 2^(x_t - m) v_t), a new
+// token with a larger score rescales the pair by 2^(m_old - m_new), so K and V
+// are read once.  Pairs of disjoint token sets join the same way, which is
+// what splits the cache's length over CTAs: each CTA leaves (m, l, o) of its
+// part and a second kernel joins the parts in order.  O = o / l,
+// lse = (m + log2 l) ln 2.
+#include <float.h>
+
+#include "paged.cuh"
+
+namespace rkv {
+namespace {
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+struct AppendArgs {
+    PagedView c;
+    const uint8_t* k;
+    const uint8_t* v;
+    const int* n_new;
+    long long item_stride, src_token, src_head;  // bytes
+    int n_rows, HK, vpr;                         // vpr: vectors per row
+};
+
+// Consecutive threads take consecutive vectors of (row, head), so source rows
+// that lie back to back are read in whole lines.
+template <typename VT>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
+    const int b = blockIdx.y;
+    const int n = a.n_new ? min(max(a.n_new[b], 0), a.n_rows) : a.n_rows;
+    const int first = a.c.lens[b] - n;
+    const long long cap = (long long)a.c.table_stride * a.c.page_size;
+    const int per = a.HK * a.vpr;
+    const long long total = (long long)n * per;
+    for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (long long)gridDim.x * blockDim.x) {
+        const int i = (int)(e / per), r = (int)(e - (long long)i * per);
+        const int h = r / a.vpr, vec = r - h * a.vpr;
+        const long long t = (long long)first + i;
+        if (t < 0 || t >= cap) continue;
+        const long long off = paged_offset(a.c, b, h, (int)t);
+        if (off < 0) continue;
+        const size_t s = (size_t)b * a.item_stride + (size_t)i * a.src_token + (size_t)h * a.src_head;
+        reinterpret_cast<VT*>(a.c.K + off)[vec] = reinterpret_cast<const VT*>(a.k + s)[vec];
+        reinterpret_cast<VT*>(a.c.V + off)[vec] = reinterpret_cast<const VT*>(a.v + s)[vec];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// decode
+// ---------------------------------------------------------------------------
+constexpr int kWarps = 4;
+constexpr int kTile = 32;       // tokens a warp takes at a time
+constexpr int kMinChunk = 128;  // visible tokens per CTA at least
+constexpr int kMaxSplits = 1024;
+
+struct DecodeArgs {
+    PagedView c;
+    const uint8_t* Q;
+    long long q_stride;
+    int H, HK, G, D, max_len, sinks, window;
+    int ngroups;         // groups of query heads per KV head
+    int splits, chunk;   // parts of the visible tokens, tokens per part
+    int vmax;            // row stride of the scores
+    float scale2;        // log2(e) / sqrt(D)
+    float* O;
+    float* lse;
+    float* weights;
+    int weight_stride;
+    float* part_o;       // [batch][H][splits][D]
+    float2* part_ml;     // [batch][H][splits]
+    float* scores;       // [batch][H][vmax], base-2 scores (with weights)
+    long long o_blocks;  // join: CTAs that join O; the others add weights
+    int w_blocks;        // join: CTAs per (item, KV head) that add weights
+};
+
+// The visible tokens are numbered 0 .. nvis - 1: the sinks, then the window.
+struct Visible {
+    int n, sinks, gap, nvis;
+    __device__ int token(int v) const { return v < sinks ? v : v + gap; }
+};
+__device__ __forceinline__ Visible visible(const DecodeArgs& a, int b) {
+    Visible s;
+    s.n = paged_len(a.c, b, a.max_len);
+    const int w = a.window > 0 ? min(a.window, s.n) : s.n;
+    const int start = s.n - w;
+    s.sinks = min(a.sinks, start);
+    s.gap = start - s.sinks;
+    s.nvis = s.sinks + w;
+    return s;
+}
+
+template <typename T>
+struct Vec;  // 16 bytes of T as floats
+template <>
+struct Vec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void get(const uint4& u, float* f) {
+        f[0] = __uint_as_float(u.x);
+        f[1] = __uint_as_float(u.y);
+        f[2] = __uint_as_float(u.z);
+        f[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ float one(const void* p, int i) { return static_cast<const float*>(p)[i]; }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(const uint4& u, float* f) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ float one(const void* p, int i) {
+        return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+    }
+};
+template <>
+struct Vec<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(const uint4& u, float* f) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = v.x;
+            f[2 * i + 1] = v.y;
+        }
+    }
+    static __device__ __forceinline__ float one(const void* p, int i) {
+        return __half2float(static_cast<const __half*>(p)[i]);
+    }
+};
+
+__device__ __forceinline__ uint4 load16(const uint8_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+// 0 in place of -inf, so that a set with nothing in it subtracts no infinities.
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
+
+size_t simt_smem(int GT, int D) { return sizeof(float) * ((size_t)GT * D + kWarps * GT * kTile + 2 * kWarps * GT + (size_t)kWarps * GT * D); }
+
+// Fused multiply-adds on the CUDA cores, any type: one CTA per (item, KV
+// head, group of up to GT query heads, part).  Every warp takes 32 tokens at a
+// time on its own: 8 lanes form the scores of a token (four tokens per lane
+// and pass), a lane per token forms the weights, and LR lanes of 16 bytes add
+// up a V row.  VL: 16-byte vectors of a V row per lane.
+template <typename T, int GT, int VL>
+__global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const DecodeArgs a) {
+    constexpr int N = Vec<T>::N;
+    extern __shared__ __align__(16) float sm[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int D = a.D, VPR = D / N;
+    float* qs = sm;                                         // [GT][D]
+    float* pw = qs + GT * D + warp * GT * kTile;            // [GT][32] of this warp
+    float* ms = qs + GT * D + kWarps * GT * kTile;          // [warps][GT]
+    float* ls = ms + kWarps * GT;                           // [warps][GT]
+    float* os = ls + kWarps * GT;                           // [warps][GT][D]
+
+    long long id = blockIdx.x;
+    const int split = (int)(id % a.splits);
+    id /= a.splits;
+    const int grp = (int)(id % a.ngroups);
+    id /= a.ngroups;
+    const int hk = (int)(id % a.HK), b = (int)(id / a.HK);
+    const Visible vis = visible(a, b);
+    const long long v_lo = (long long)split * a.chunk;
+    if (split > 0 && v_lo >= vis.nvis) return;  // the join takes the parts that hold tokens
+    const int v0 = (int)v_lo, v1 = (int)min((long long)vis.nvis, v_lo + a.chunk);
+    const int h0 = hk * a.G + grp * GT, ng = min(GT, a.G - grp * GT);
+
+    const uint8_t* q = a.Q + (size_t)b * a.q_stride;
+    for (int i = tid; i < GT * D; i += kWarps * 32) {
+        const int g = i / D;
+        qs[i] = g < ng ? Vec<T>::one(q, (h0 + g) * D + (i - g * D)) * a.scale2 : 0.0f;
+    }
+    __syncthreads();
+
+    int LR = 1;
+    while (LR < VPR && LR < 32) LR <<= 1;
+    const int TPS = 32 / LR, vl0 = lane & (LR - 1), tsub = lane / LR;
+    float m[GT], l[GT], acc[VL][N][GT];
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+        m[g] = -INFINITY;
+        l[g] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+#pragma unroll
+            for (int g = 0; g < GT; ++g) acc[i][e][g] = 0.0f;
+
+    for (int t0 = v0 + warp * kTile; t0 < v1; t0 += kWarps * kTile) {
+        const int v = t0 + lane;
+        const long long off = v < v1 ? paged_offset(a.c, b, hk, vis.token(v)) : -1;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            long long o[4];
+            float s[4][GT];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] = __shfl_sync(0xffffffffu, off, half * 16 + j * 4 + (lane >> 3));
+#pragma unroll
+                for (int g = 0; g < GT; ++g) s[j][g] = 0.0f;
+            }
+            for (int vec = lane & 7; vec < VPR; vec += 8) {
+                uint4 x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    x[j] = o[j] >= 0 ? load16(a.c.K + o[j] + vec * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float f[N];
+                    Vec<T>::get(x[j], f);
+#pragma unroll
+                    for (int g = 0; g < GT; ++g)
+#pragma unroll
+                        for (int e = 0; e < N; ++e) s[j][g] = fmaf(f[e], qs[g * D + vec * N + e], s[j][g]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int g = 0; g < GT; ++g) {
+                    float x = s[j][g];
+                    x += __shfl_xor_sync(0xffffffffu, x, 1);
+                    x += __shfl_xor_sync(0xffffffffu, x, 2);
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    if ((lane & 7) == g) pw[g * kTile + half * 16 + j * 4 + (lane >> 3)] = x;
+                }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+            const float x = off >= 0 ? pw[g * kTile + lane] : -INFINITY;
+            if (a.scores && v < v1 && g < ng) a.scores[((size_t)b * a.H + h0 + g) * a.vmax + v] = x;
+            const float mn = fmaxf(m[g], warp_max(x)), mf = finite_max(mn);
+            const float corr = exp2f(m[g] - mf), p = exp2f(x - mf);
+            m[g] = mn;
+            l[g] = l[g] * corr + p;
+            pw[g * kTile + lane] = p;
+#pragma unroll
+            for (int i = 0; i < VL; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[i][e][g] *= corr;
+        }
+        __syncwarp();
+#pragma unroll 4
+        for (int s0 = 0; s0 < kTile; s0 += TPS) {
+            const int t = s0 + tsub;
+            const long long o = __shfl_sync(0xffffffffu, off, t);
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+                const int vec = vl0 + i * 32;
+                const uint4 x = o >= 0 && vec < VPR ? load16(a.c.V + o + vec * 16) : make_uint4(0, 0, 0, 0);
+                float f[N];
+                Vec<T>::get(x, f);
+#pragma unroll
+                for (int g = 0; g < GT; ++g) {
+                    const float p = pw[g * kTile + t];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) acc[i][e][g] = fmaf(p, f[e], acc[i][e][g]);
+                }
+            }
+        }
+        __syncwarp();
+    }
+    // the token groups of a warp, then the warps
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+        l[g] = warp_sum(l[g]);
+        if (lane == 0) {
+            ms[warp * GT + g] = m[g];
+            ls[warp * GT + g] = l[g];
+        }
+#pragma unroll
+        for (int i = 0; i < VL; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                float x = acc[i][e][g];
+                for (int o = LR; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                const int vec = vl0 + i * 32;
+                if (tsub == 0 && vec < VPR) os[(warp * GT + g) * D + vec * N + e] = x;
+            }
+    }
+    __syncthreads();
+    for (int i = tid; i < ng * D; i += kWarps * 32) {
+        const int g = i / D, d = i - g * D;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ms[w * GT + g]);
+        const float mf = finite_max(mm);
+        float ll = 0.0f, oo = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float c = exp2f(ms[w * GT + g] - mf);
+            ll = fmaf(ls[w * GT + g], c, ll);
+            oo = fmaf(os[(w * GT + g) * D + d], c, oo);
+        }
+        const size_t head = (size_t)b * a.H + h0 + g;
+        if (a.splits == 1) {
+            a.O[head * D + d] = ll == 0.0f ? 0.0f : oo / ll;
+            if (d == 0 && a.lse) a.lse[head] = ll == 0.0f ? -INFINITY : (mf + log2f(ll)) * 0.693147180559945f;
+        }
+        if (a.part_o) {
+            if (a.splits > 1) a.part_o[(head * a.splits + split) * D + d] = oo;
+            if (d == 0) a.part_ml[head * a.splits + split] = make_float2(mm, ll);
+        }
+    }
+}
+
+// m and l of all parts of a head (one warp): the same order whatever the grid.
+__device__ __forceinline__ float2 join_ml(const float2* ml, int parts, int lane) {
+    float m = -INFINITY;
+    for (int s = lane; s < parts; s += 32) m = fmaxf(m, ml[s].x);
+    m = finite_max(warp_max(m));
+    float l = 0.0f;
+    for (int s = lane; s < parts; s += 32) {
+        const float2 x = ml[s];
+        l = fmaf(x.y, exp2f(x.x - m), l);
+    }
+    return make_float2(m, warp_sum(l));
+}
+
+// Joins the parts.  The first o_blocks CTAs take one query head each; the
+// others add the weights of a stretch of tokens of one KV head.
+__global__ void __launch_bounds__(128) paged_join_kernel(const DecodeArgs a) {
+    extern __shared__ __align__(16) float sm[];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    long long id = blockIdx.x;
+    if (id < a.o_blocks) {
+        const int b = (int)(id / a.H);
+        const int nvis = visible(a, b).nvis;
+        const int parts = max(1, (nvis + a.chunk - 1) / a.chunk);
+        const float2* ml = a.part_ml + id * a.splits;
+        if (warp == 0) {
+            const float2 j = join_ml(ml, parts, lane);
+            const float inv = j.y == 0.0f ? 0.0f : 1.0f / j.y;
+            for (int s = lane; s < parts; s += 32) sm[s] = exp2f(ml[s].x - j.x) * inv;
+            if (lane == 0 && a.lse) a.lse[id] = j.y == 0.0f ? -INFINITY : (j.x + log2f(j.y)) * 0.693147180559945f;
+        }
+        __syncthreads();
+        for (int d = tid; d < a.D; d += 128) {
+            const float* po = a.part_o + (size_t)id * a.splits * a.D + d;
+            float o = 0.0f;
+#pragma unroll 8
+            for (int s = 0; s < parts; ++s) o = fmaf(po[(size_t)s * a.D], sm[s], o);
+            a.O[id * a.D + d] = o;
+        }
+        return;
+    }
+    id -= a.o_blocks;
+    const int blk = (int)(id % a.w_blocks);
+    id /= a.w_blocks;
+    const int hk = (int)(id % a.HK), b = (int)(id / a.HK);
+    const Visible vis = visible(a, b);
+    const int parts = max(1, (vis.nvis + a.chunk - 1) / a.chunk);
+    if ((long long)blk * 1024 >= vis.nvis) return;
+    float2* st = reinterpret_cast<float2*>(sm);  // [G] (m, 1 / l)
+    for (int g = warp; g < a.G; g += 4) {
+        const float2 j = join_ml(a.part_ml + ((size_t)b * a.H + hk * a.G + g) * a.splits, parts, lane);
+        if (lane == 0) st[g] = make_float2(j.x, j.y == 0.0f ? 0.0f : 1.0f / j.y);
+    }
+    __syncthreads();
+    const float* x = a.scores + ((size_t)b * a.H + hk * a.G) * a.vmax;
+    float* w = a.weights + ((size_t)b * a.HK + hk) * a.weight_stride;
+    const int v_end = min(vis.nvis, blk * 1024 + 1024);
+    for (int v = blk * 1024 + tid; v < v_end; v += 128) {
+        float s = 0.0f;
+        for (int g = 0; g < a.G; ++g) s = fmaf(exp2f(x[(size_t)g * a.vmax + v] - st[g].x), st[g].y, s);
+        const int t = vis.token(v);
+        w[t] += s;
+    }
+}
+
+struct DecodePlan {
+    int gt, ngroups, splits, chunk, vmax;
+    size_t off_ml, off_o, off_scores, bytes;
+};
+
+// The parts of the visible tokens: enough CTAs for a few waves over the GPU,
+// at least kMinChunk tokens each.
+DecodePlan decode_plan(int H, int HK, int D, long long visible_max, int max_len, int batch, bool weights) {
+    DecodePlan p{};
+    const int G = H / HK;
+    p.gt = G >= 5 ? 8 : G >= 3 ? 4 : G;
+    p.ngroups = (G + p.gt - 1) / p.gt;
+    const long long units = (long long)batch * HK * p.ngroups;
+    const long long target = 148 * 16;
+    long long splits = units > 0 ? (target + units - 1) / units : 1;
+    const long long most = (visible_max + kMinChunk - 1) / kMinChunk;
+    if (splits > most) splits = most;
+    if (splits > kMaxSplits) splits = kMaxSplits;
+    if (splits < 1) splits = 1;
+    const size_t most_parts = (size_t)splits;
+    long long chunk = (visible_max + splits - 1) / splits;
+    chunk = (chunk + kTile - 1) / kTile * kTile;
+    if (chunk < kTile) chunk = kTile;
+    p.chunk = (int)chunk;
+    splits = (visible_max + p.chunk - 1) / p.chunk;
+    p.splits = splits < 1 ? 1 : (int)splits;
+    p.vmax = (max_len + 3) / 4 * 4;
+    // the parts before rounding bound the layout: they grow with visible_max, so the workspace of max_len
+    // serves every window
+    const size_t heads = (size_t)batch * H;
+    size_t off = kWorkspaceHeader;
+    p.off_ml = off;
+    off = align_up(off + heads * most_parts * sizeof(float2), kWorkspaceAlign);
+    p.off_o = off;
+    if (most_parts > 1) off = align_up(off + heads * most_parts * D * sizeof(float), kWorkspaceAlign);
+    p.off_scores = off;
+    if (weights) off = align_up(off + heads * (size_t)p.vmax * sizeof(float), kWorkspaceAlign);
+    p.bytes = off;
+    return p;
+}
+
+template <typename T, int GT>
+int launch_simt(const DecodeArgs& a, long long blocks, cudaStream_t st) {
+    const int vpr = a.D / Vec<T>::N;
+    const size_t smem = simt_smem(GT, a.D);
+    if (vpr > 32)
+        paged_decode_simt_kernel<T, GT, 2><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
+    else
+        paged_decode_simt_kernel<T, GT, 1><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
+    return launched();
+}
+
+template <typename T>
+int launch_decode(const DecodeArgs& a, int gt, long long blocks, cudaStream_t st) {
+    switch (gt) {
+        case 1: return launch_simt<T, 1>(a, blocks, st);
+        case 2: return launch_simt<T, 2>(a, blocks, st);
+        case 4: return launch_simt<T, 4>(a, blocks, st);
+        default: return launch_simt<T, 8>(a, blocks, st);
+    }
+}
+
+}  // namespace
+}  // namespace rkv
+
+using namespace rkv;
+
+extern "C" int rkv_paged_append(const rkv_paged_cache* cache, const void* k, const void* v, int n_rows, int batch,
+                                long long src_item_stride, long long src_token_stride, long long src_head_stride,
+                                const int* n_new, void* stream) {
+    const int rc = paged_check(cache, true);
+    if (rc) return rc;
+    if (n_rows < 0 || batch < 0) return RKV_ERR_INVALID_ARG;
+    if (n_rows == 0 || batch == 0 || cache->num_pages == 0 || cache->table_stride == 0) return RKV_OK;
+    if (batch > 65535) return RKV_ERR_UNSUPPORTED;
+    const int es = elem_size(cache->dtype);
+    const long long rowb = (long long)cache->dim_head * es;
+    if (!k || !v || src_item_stride < 0 || src_token_stride < 0 || src_head_stride < 0) return RKV_ERR_INVALID_ARG;
+    uintptr_t al = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | (uintptr_t)rowb;
+    if (batch > 1) al |= (uintptr_t)src_item_stride;
+    if (n_rows > 1) al |= (uintptr_t)src_token_stride;
+    if (cache->num_heads_kv > 1) al |= (uintptr_t)src_head_stride;
+    if (al & (es - 1)) return RKV_ERR_INVALID_ARG;
+    const int vb = (al & 15) == 0 ? 16 : (al & 7) == 0 ? 8 : (al & 3) == 0 ? 4 : 2;
+    AppendArgs a{};
+    a.c = paged_view(*cache);
+    a.k = static_cast<const uint8_t*>(k);
+    a.v = static_cast<const uint8_t*>(v);
+    a.n_new = n_new;
+    a.item_stride = src_item_stride;
+    a.src_token = src_token_stride;
+    a.src_head = src_head_stride;
+    a.n_rows = n_rows;
+    a.HK = cache->num_heads_kv;
+    a.vpr = (int)(rowb / vb);
+    if ((long long)a.HK * a.vpr > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
+    const long long total = (long long)n_rows * a.HK * a.vpr;
+    long long gx = (total + 255) / 256;
+    const long long most = 148 * 16 / batch + 1;
+    if (gx > most) gx = most;
+    const dim3 grid((unsigned)gx, batch);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (vb) {
+        case 16: paged_append_kernel<uint4><<<grid, 256, 0, st>>>(a); break;
+        case 8: paged_append_kernel<uint2><<<grid, 256, 0, st>>>(a); break;
+        case 4: paged_append_kernel<uint32_t><<<grid, 256, 0, st>>>(a); break;
+        default: paged_append_kernel<uint16_t><<<grid, 256, 0, st>>>(a); break;
+    }
+    return launched();
+}
+
+static int decode_shape_check(int H, int HK, int D, int max_len, int batch) {
+    if (H <= 0 || HK <= 0 || H % HK != 0 || D <= 0 || max_len < 0 || batch < 0) return RKV_ERR_INVALID_ARG;
+    if (D % 8 != 0 || D > 256) return RKV_ERR_UNSUPPORTED;
+    if (H / HK > 1024 || max_len > kMaxLen) return RKV_ERR_UNSUPPORTED;
+    return RKV_OK;
+}
+
+extern "C" int rkv_paged_decode_workspace_size(int num_heads, int num_heads_kv, int dim_head, int max_len, int batch,
+                                               int with_weights, size_t* bytes) {
+    const int rc = decode_shape_check(num_heads, num_heads_kv, dim_head, max_len, batch);
+    if (rc || !bytes) return rc ? rc : (int)RKV_ERR_INVALID_ARG;
+    *bytes = decode_plan(num_heads, num_heads_kv, dim_head, max_len, max_len, batch, with_weights != 0).bytes;
+    return RKV_OK;
+}
+
+extern "C" int rkv_paged_decode(const void* Q, long long q_item_stride, int num_heads, const rkv_paged_cache* cache,
+                                int max_len, int batch, int sinks, int window, float* O, float* lse, float* weights,
+                                int weight_stride, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = paged_check(cache, true);
+    if (!rc) rc = decode_shape_check(num_heads, cache->num_heads_kv, cache->dim_head, max_len, batch);
+    if (rc) return rc;
+    if (sinks < 0 || window < 0) return RKV_ERR_INVALID_ARG;
+    if (batch == 0) return RKV_OK;
+    const int D = cache->dim_head;
+    const long long q_bytes = (long long)num_heads * D * elem_size(cache->dtype);
+    if (!Q || !O || (reinterpret_cast<uintptr_t>(Q) & 15)) return RKV_ERR_INVALID_ARG;
+    if (batch > 1 && (q_item_stride < q_bytes || (q_item_stride & 15))) return RKV_ERR_INVALID_ARG;
+    if (weights && weight_stride < max_len) return RKV_ERR_INVALID_ARG;
+    long long vis = max_len;
+    if (window > 0 && (long long)sinks + window < vis) vis = (long long)sinks + window;
+    const DecodePlan p = decode_plan(num_heads, cache->num_heads_kv, D, vis, max_len, batch, weights != nullptr);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < p.bytes) return RKV_ERR_WORKSPACE;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    DecodeArgs a{};
+    a.c = paged_view(*cache);
+    a.Q = static_cast<const uint8_t*>(Q);
+    a.q_stride = q_item_stride;
+    a.H = num_heads;
+    a.HK = cache->num_heads_kv;
+    a.G = num_heads / cache->num_heads_kv;
+    a.D = D;
+    a.max_len = max_len;
+    a.sinks = sinks;
+    a.window = window;
+    a.ngroups = p.ngroups;
+    a.splits = p.splits;
+    a.chunk = p.chunk;
+    a.vmax = p.vmax;
+    a.scale2 = 1.4426950408889634f / sqrtf((float)D);
+    a.O = O;
+    a.lse = lse;
+    a.weights = weights;
+    a.weight_stride = weight_stride;
+    const bool join = p.splits > 1 || weights;
+    if (join) {
+        a.part_ml = reinterpret_cast<float2*>(ws + p.off_ml);
+        a.part_o = reinterpret_cast<float*>(ws + p.off_o);
+    }
+    if (weights) a.scores = reinterpret_cast<float*>(ws + p.off_scores);
+    const long long blocks = (long long)batch * a.HK * p.ngroups * p.splits;
+    a.o_blocks = p.splits > 1 ? (long long)batch * a.H : 0;
+    a.w_blocks = weights ? (int)((vis + 1023) / 1024) : 0;
+    const long long jblocks = a.o_blocks + (long long)batch * a.HK * a.w_blocks;
+    if (blocks > 0x7FFFFFFFLL || jblocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
+    switch (cache->dtype) {
+        case RKV_F32: rc = launch_decode<float>(a, p.gt, blocks, st); break;
+        case RKV_BF16: rc = launch_decode<__nv_bfloat16>(a, p.gt, blocks, st); break;
+        default: rc = launch_decode<__half>(a, p.gt, blocks, st); break;
+    }
+    if (rc || !join || jblocks == 0) return rc;
+    size_t smem = (size_t)p.splits * sizeof(float);
+    if (weights && smem < (size_t)a.G * sizeof(float2)) smem = (size_t)a.G * sizeof(float2);
+    const cudaError_t e = launch_pdl(paged_join_kernel, dim3((unsigned)jblocks), dim3(128), smem, st, a);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
+}

@@ -37,7 +37,9 @@ EXPORTS = [
     "rkv_hsa_workspace_size", "rkv_hsa_decode", "rkv_hybrid_sparse_decode_host",
     "rkv_hsa_decode_host_ex", "rkv_workspace_status", "rkv_hsa_decode_noalloc", "rkv_hsa_decode_noalloc_status",
     "rkv_selftest_wait_timeout", "rkv_compact_kv", "rkv_hsa_summary_size", "rkv_hsa_build_summary",
-    "rkv_hsa_decode_summary", "rkv_capture_rows", "rkv_evict_compact",
+    "rkv_hsa_decode_summary", "rkv_capture_rows", "rkv_evict_compact", "rkv_paged_append",
+    "rkv_paged_decode_workspace_size", "rkv_paged_decode", "rkv_weight_evict",
+    "rkv_sink_attention_workspace_size", "rkv_sink_attention",
 ]
 
 
@@ -57,6 +59,18 @@ class _Budget(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in (
         "token_budget", "sequence_length", "max_new_tokens", "capacity_budget",
         "prompt_budget", "chunk_size", "r", "k")] + [("compression_ratio", ctypes.c_float)]
+
+
+class _PagedCache(ctypes.Structure):
+    _fields_ = ([("K", ctypes.c_void_p), ("V", ctypes.c_void_p)]
+                + [(n, ctypes.c_int) for n in ("dtype", "num_heads_kv", "dim_head", "page_size", "num_pages",
+                                               "table_stride")]
+                + [(n, ctypes.c_longlong) for n in ("page_stride", "head_stride", "token_stride")]
+                + [("block_table", ctypes.c_void_p), ("lens", ctypes.c_void_p)])
+
+
+class _RowStrides(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_longlong) for n in ("item", "head", "token")]
 
 
 @dataclass
@@ -99,6 +113,8 @@ _I = ctypes.c_int
 _LL = ctypes.c_longlong
 _SZ = ctypes.c_size_t
 _CFGP = ctypes.POINTER(_Config)
+_PCP = ctypes.POINTER(_PagedCache)
+_RSP = ctypes.POINTER(_RowStrides)
 
 
 def lib() -> ctypes.CDLL:
@@ -141,6 +157,13 @@ def lib() -> ctypes.CDLL:
         "rkv_hsa_build_summary": ([_VP, _I, _I, _I, _I, _LL, _CFGP, _VP, _VP], _I),
         "rkv_hsa_decode_summary": ([_VP, _VP, _VP, _VP, _I, _I, _I, _I, _LL, _LL, _CFGP, _I, _I, _VP, _VP, _I,
                                     _VP, _VP, _SZ, _VP], _I),
+        "rkv_paged_append": ([_PCP, _VP, _VP, _I, _I, _LL, _LL, _LL, _VP, _VP], _I),
+        "rkv_paged_decode_workspace_size": ([_I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)], _I),
+        "rkv_paged_decode": ([_VP, _LL, _I, _PCP, _I, _I, _I, _I, _VP, _VP, _VP, _I, _VP, _SZ, _VP], _I),
+        "rkv_weight_evict": ([_PCP, _VP, _I, _I, _I, _I, _I, _I, _PCP, _VP, _VP, _I, _VP, _VP], _I),
+        "rkv_sink_attention_workspace_size": ([ctypes.POINTER(_SZ)], _I),
+        "rkv_sink_attention": ([_VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _RSP, _RSP, _VP, _I, _I, _VP, _RSP, _VP,
+                                _VP, _SZ, _VP], _I),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -429,3 +452,230 @@ class HsaDecoder:
 
     def status(self, stream=None) -> int:
         return lib().rkv_workspace_status(_ptr(self.ws), _stream(stream))
+
+
+# ---------------------------------------------------------------------------
+# Paged KV cache: append, dense decode, eviction by accumulated weight
+# ---------------------------------------------------------------------------
+def _on(tensor, stream, call):
+    """Runs call(stream) with the tensor's device current (a stream belongs to one)."""
+    import torch
+    if tensor.device.index == torch.cuda.current_device():
+        return call(_stream(stream))
+    with torch.cuda.device(tensor.device):
+        return call(_stream(stream))
+
+
+def _int32(t, device, what):
+    import torch
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        raise TypeError(f"{what}: a contiguous int32 tensor on {device} is needed")
+
+
+class PagedCache:
+    """K and V pages [num_pages, HK, page_size, D] (float32, bfloat16 or
+    float16; unit stride along D, any 16-byte multiple along the others, so a
+    [num_pages, page_size, HK, D] pool is passed as pool.transpose(1, 2)),
+    block_table [B, table_stride] int32 and lens [B] int32, all on one device.
+    Holds the tensors; lens may be replaced or updated in place between calls."""
+
+    def __init__(self, K, V, block_table, lens):
+        if K.shape != V.shape or K.stride() != V.stride() or K.dtype != V.dtype or K.dim() != 4:
+            raise ValueError("K and V: [num_pages, HK, page_size, D], of one layout and type")
+        if not K.is_cuda or V.device != K.device:
+            raise TypeError("K and V: CUDA tensors on one device")
+        pages, hk, page, d = K.shape
+        if d > 1 and K.stride(3) != 1:
+            raise ValueError("unit stride along the last dimension is needed")
+        dt = _dtype_of(K)
+        if dt == Q8_0:
+            raise TypeError("a paged cache holds float32, bfloat16 or float16")
+        _int32(block_table, K.device, "block_table")
+        if block_table.dim() != 2:
+            raise ValueError("block_table: [batch, pages per sequence]")
+        self.K, self.V, self.block_table = K, V, block_table
+        es = K.element_size()
+        # the stride of a dimension of one entry is never used: any value passes
+        st = [K.stride(i) * es if K.shape[i] > 1 else 16 * ((d * es + 15) // 16) for i in range(3)]
+        self.c = _PagedCache(_ptr(K), _ptr(V), dt, hk, d, page, pages, block_table.shape[1], st[0], st[1], st[2],
+                             _ptr(block_table), None)
+        self.ref = ctypes.byref(self.c)
+        self.batch = block_table.shape[0]
+        self.lens = lens
+
+    @property
+    def lens(self):
+        return self._lens
+
+    @lens.setter
+    def lens(self, t):
+        if t is not None:
+            _int32(t, self.K.device, "lens")
+            if t.numel() != self.batch:
+                raise ValueError("lens: one entry per row of block_table")
+        self._lens = t
+        self.c.lens = _ptr(t)
+
+
+def paged_append(cache: PagedCache, k, v, n_new=None, stream=None):
+    """Newest rows into the pages (rkv_paged_append).  k, v: [B, n_rows, HK, D]
+    (or [B, HK, D] for one row) of the cache's type, unit stride along D, equal
+    strides; cache.lens already counts them, and n_new [B] int32 (nullable)
+    says how many of the n_rows each sequence has."""
+    if k.dim() == 3:
+        k, v = k[:, None], v[:, None]
+    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != cache.K.dtype or v.dtype != k.dtype:
+        raise ValueError("k and v: one shape, layout and the cache's type")
+    B, n, hk, d = k.shape
+    if B != cache.batch or hk != cache.K.shape[1] or d != cache.K.shape[3] or (d > 1 and k.stride(3) != 1):
+        raise ValueError("k, v: [B, n_rows, HK, D] of the cache's geometry, unit stride along D")
+    if k.device != cache.K.device or v.device != k.device:
+        raise TypeError("k and v: on the cache's device")
+    if n_new is not None:
+        _int32(n_new, k.device, "n_new")
+        if n_new.numel() != B:
+            raise ValueError("n_new: one entry per sequence")
+    es = k.element_size()
+    _on(k, stream, lambda st: _check(lib().rkv_paged_append(
+        cache.ref, _ptr(k), _ptr(v), n, B, k.stride(0) * es, k.stride(1) * es, k.stride(2) * es, _ptr(n_new), st),
+        "rkv_paged_append"))
+
+
+class PagedDecoder:
+    """One new token per sequence attended over a paged cache
+    (rkv_paged_decode), with its outputs O [B, H, D] and lse [B, H] float32 and
+    its workspace.  window > 0: only the first `sinks` and the last `window`
+    tokens are seen.  weights=True reserves what a call that accumulates
+    attention weights needs."""
+
+    def __init__(self, num_heads: int, num_heads_kv: int, dim_head: int, max_len: int, batch: int, device, sinks: int = 0,
+                 window: int = 0, weights: bool = False):
+        import torch
+        b = _SZ(0)
+        _check(lib().rkv_paged_decode_workspace_size(num_heads, num_heads_kv, dim_head, max_len, batch, int(weights),
+                                                     ctypes.byref(b)), "rkv_paged_decode_workspace_size")
+        self.num_heads, self.num_heads_kv, self.dim_head = num_heads, num_heads_kv, dim_head
+        self.max_len, self.batch, self.sinks, self.window = max_len, batch, sinks, window
+        self.ws_bytes = b.value
+        self.ws = _workspace(b.value, device)
+        self.O = torch.zeros((batch, num_heads, dim_head), dtype=torch.float32, device=device)
+        self.lse = torch.zeros((batch, num_heads), dtype=torch.float32, device=device)
+
+    def __call__(self, Q, cache: PagedCache, weights=None, stream=None):
+        """Q [B, H, D] of the cache's type.  weights (nullable): float32
+        [B, HK, >= max_len]; every visible token's attention weight, summed over
+        its KV head's query heads, is added.  Returns O."""
+        if tuple(Q.shape) != (self.batch, self.num_heads, self.dim_head) or not Q.is_contiguous():
+            raise ValueError("Q: contiguous [B, H, D] of the decoder's sizes")
+        if (Q.dtype != cache.K.dtype or Q.device != cache.K.device or Q.device != self.ws.device
+                or cache.batch != self.batch or cache._lens is None):
+            raise ValueError("Q, the cache and the decoder: one type, device and batch, and the cache's lens set")
+        if (cache.c.num_heads_kv, cache.c.dim_head) != (self.num_heads_kv, self.dim_head):
+            raise ValueError("the cache's heads are not the decoder's")
+        wstride = _check_weights(weights, self.batch, self.num_heads_kv, self.max_len, Q.device)
+        _on(Q, stream, lambda st: _check(lib().rkv_paged_decode(
+            _ptr(Q), self.num_heads * self.dim_head * Q.element_size(), self.num_heads, cache.ref, self.max_len,
+            self.batch, self.sinks, self.window, _ptr(self.O), _ptr(self.lse), _ptr(weights), wstride, _ptr(self.ws),
+            self.ws_bytes, st), "rkv_paged_decode"))
+        return self.O
+
+
+def _check_weights(w, batch, heads, max_len, device) -> int:
+    """Row stride of accumulated weights [B, HK, >= max_len] (0 for None)."""
+    import torch
+    if w is None:
+        return 0
+    if (w.dtype != torch.float32 or w.device != device or not w.is_contiguous() or w.dim() != 3
+            or w.shape[0] != batch or w.shape[1] != heads or w.shape[2] < max_len):
+        raise ValueError("weights: contiguous float32 [B, HK, >= max_len] on the cache's device")
+    return w.shape[2]
+
+
+class WeightEvictor:
+    """Eviction by accumulated attention weight (rkv_weight_evict): every
+    (sequence, KV head) keeps its first `sinks`, its last `recent` and the
+    heaviest of its other tokens, `budget` in all."""
+
+    def __init__(self, num_heads_kv: int, max_len: int, batch: int, budget: int, device, sinks: int = 0, recent: int = 0):
+        import torch
+        self.num_heads_kv, self.max_len, self.batch = num_heads_kv, max_len, batch
+        self.budget, self.sinks, self.recent = budget, sinks, recent
+        self.kept = torch.full((batch, num_heads_kv, max(0, min(budget, max_len))), -1, dtype=torch.int32, device=device)
+        self.new_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+
+    def __call__(self, cache: PagedCache, weights, out: PagedCache | None = None, weights_out=None, stream=None):
+        """In place without out / weights_out.  Returns (kept [B, HK, min(budget,
+        max_len)] int32 ascending with -1 behind, new_lens [B] int32): the
+        caller's next calls take new_lens (copied, or as the cache's lens)."""
+        if cache.batch != self.batch or cache.c.num_heads_kv != self.num_heads_kv or cache._lens is None or weights is None:
+            raise ValueError("the evictor's batch and KV heads, lens and weights are needed")
+        if out is not None and (out.batch != self.batch or out.K.device != cache.K.device):
+            raise ValueError("out: the same batch, on the cache's device")
+        if self.kept.device != cache.K.device:
+            raise ValueError("the cache is not on the evictor's device")
+        ws = _check_weights(weights, self.batch, self.num_heads_kv, self.max_len, cache.K.device)
+        if weights_out is not None and _check_weights(weights_out, self.batch, self.num_heads_kv, self.max_len,
+                                                      cache.K.device) != ws:
+            raise ValueError("weights_out: the layout of weights")
+        _on(cache.K, stream, lambda st: _check(lib().rkv_weight_evict(
+            cache.ref, _ptr(weights), ws, self.max_len, self.batch, self.budget, self.sinks, self.recent,
+            out.ref if out is not None else None, _ptr(weights_out), _ptr(self.kept), self.kept.shape[2],
+            _ptr(self.new_lens), st), "rkv_weight_evict"))
+        return self.kept, self.new_lens
+
+
+def _row_strides(t, what):
+    """(item, head, token) byte strides of [B, H, len, D] with unit stride along D."""
+    if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
+        raise ValueError(f"{what}: [B, heads, len, D] with unit stride along D")
+    es = t.element_size()
+    row = 16 * ((t.shape[3] * es + 15) // 16)  # the stride of a dimension of one entry is never used
+    return _RowStrides(*[t.stride(i) * es if t.shape[i] > 1 else row for i in range(3)])
+
+
+class SinkAttention:
+    """Causal prefill attention over a sliding window and a few first tokens
+    that stay visible (rkv_sink_attention); window 0: every key up to the
+    query.  Holds the workspace."""
+
+    def __init__(self, sinks: int = 0, window: int = 0, device="cuda"):
+        b = _SZ(0)
+        _check(lib().rkv_sink_attention_workspace_size(ctypes.byref(b)), "rkv_sink_attention_workspace_size")
+        self.sinks, self.window, self.ws_bytes = sinks, window, b.value
+        self.ws = _workspace(b.value, device)
+
+    def __call__(self, Q, K, V, lens=None, out=None, lse=None, stream=None):
+        """Q [B, H, len_q, D], K, V [B, HK, len_k, D] (float32, bfloat16 or
+        float16; unit stride along D, K and V strided alike); lens (nullable) [B]
+        int32: valid keys of each item, query rows at positions from lens[b] on
+        are left as they were.  out: as Q (allocated without); lse: float32
+        [B, H, len_q].  Returns out."""
+        import torch
+        if K.shape != V.shape or K.stride() != V.stride() or not (Q.dtype == K.dtype == V.dtype):
+            raise ValueError("K and V: one shape and layout; Q, K, V: one type")
+        if not (Q.device == K.device == V.device == self.ws.device):
+            raise ValueError("Q, K, V and the workspace: one device")
+        if out is None:
+            out = torch.zeros(Q.shape, dtype=Q.dtype, device=Q.device)
+        if out.shape != Q.shape or out.dtype != Q.dtype or out.device != Q.device:
+            raise ValueError("out: Q's shape, type and device")
+        B, H, Lq, D = Q.shape
+        if K.shape[0] != B or K.shape[3] != D:
+            raise ValueError("K, V: [B, HK, len_k, D] of Q's batch and D")
+        dt = _dtype_of(Q)
+        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, Lq) or not lse.is_contiguous()
+                                or lse.device != Q.device):
+            raise ValueError("lse: contiguous float32 [B, H, len_q] on Q's device")
+        if lens is not None:
+            _int32(lens, Q.device, "lens")
+            if lens.numel() != B:
+                raise ValueError("lens: one entry per item")
+        qs, ks, os_ = _row_strides(Q, "Q"), _row_strides(K, "K, V"), _row_strides(out, "out")
+        _on(Q, stream, lambda st: _check(lib().rkv_sink_attention(
+            _ptr(Q), _ptr(K), _ptr(V), dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(qs), ctypes.byref(ks),
+            _ptr(lens), self.sinks, self.window, _ptr(out), ctypes.byref(os_), _ptr(lse), _ptr(self.ws), self.ws_bytes,
+            st), "rkv_sink_attention"))
+        return out
+
+    def status(self, stream=None) -> int:
+        return _on(self.ws, stream, lambda st: lib().rkv_workspace_status(_ptr(self.ws), st))
