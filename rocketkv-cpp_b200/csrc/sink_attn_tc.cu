@@ -1,0 +1,396 @@
+// sink_attn_tc.cu -- the sink-window prefill attention of 16-bit inputs on the
+// tcgen05 tensor cores (dim_head <= 128).
+//
+// A CTA takes two units -- a unit is 128 queries of one query head -- of one
+// KV head, so that both use every K and V tile that is loaded: 128 keys at a
+// time, S = Q K^T into tensor memory, P = 2^(S - m) rounded to the inputs'
+// type back into tensor memory in S's place, O += P V.  While one unit's
+// softmax runs on its four warps (a thread per query row), the tensor cores
+// work on the other unit.
+//
+//   warp 0       copies Q and the K, V tiles (one TMA box per 64 columns) into
+//                shared memory; K and V share a ring of stages
+//   warp 1       issues the products: per tile and unit P V, then the next S
+//   warps 4-7, 8-11   softmax of unit 0, 1, and their output rows
+//
+// Two roundings to 16 bits: P (relative half a step of the type, as the
+// products take both operands in one type) and the output.  Scores, m, l and
+// the accumulator are fp32.  The accumulator is rescaled only when a row's
+// largest score has grown by more than 2^8 since its last rescale: P stays
+// below 2^8 then, which both types hold, and O and l carry the same factor.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "sink_attn.cuh"
+#include "tc_common.cuh"
+
+namespace rkv {
+namespace {
+
+constexpr int kTile = 128;            // queries of a unit, keys of a tile
+constexpr int kThreads = 384;
+constexpr int kBlk = kTile * 128;     // bytes of a 128-row block of 64 columns
+constexpr float kGrow = 8.0f;         // log2 growth of a row's maximum that is carried without a rescale
+
+__host__ __device__ constexpr int stages(int kb) { return kb == 1 ? 8 : 4; }
+
+struct TcBars {
+    uint64_t q_full, o_full;
+    uint64_t s_full[2], p_ready[2];
+    uint64_t full[8], empty[8];
+    uint32_t tmem;
+    int abort;
+};
+
+// S or O += A B with A in shared memory / A (16-bit pairs) in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    mma_issue_w<false>(d, a, b, idesc, acc);
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// Shared-memory descriptor of a V tile as the N x K operand, N (columns of V)
+// contiguous, 128-byte swizzle: 64 columns x 8 keys per 1024-byte group, the
+// groups of further keys 1024 bytes apart, further 64 columns kBlk apart.
+__device__ __forceinline__ uint64_t v_desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kBlk >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+
+// 32 columns of this thread's lane, not waited for.
+__device__ __forceinline__ void ld32_async(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+          "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+// Values that a wait has made valid: keeps their uses behind it.
+__device__ __forceinline__ void pin32(uint32_t* r) {
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if (BF) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort) {
+    return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, err, abort));
+}
+
+// KB: blocks of 64 columns (dim_head <= 64 KB; columns behind dim_head are
+// filled with zeros by the copies).
+template <int KB, bool BF>
+__global__ void __launch_bounds__(kThreads, 1)
+    sink_tc_kernel(const SinkArgs a, const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                   const __grid_constant__ CUtensorMap tv) {
+    constexpr int NS = stages(KB);
+    constexpr uint32_t kStage = KB * kBlk;
+    constexpr uint32_t kColO = 256;  // tensor memory: S0, S1 (128 columns each), O0, O1 (64 KB each)
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    TcBars& B = *reinterpret_cast<TcBars*>(sm);
+    volatile int* abort_flag = &B.abort;
+    uint8_t* sq = sm + 1024;
+    uint8_t* ring = sq + 2 * kStage;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // the units: (query tile, head of the group), the latest queries (the longest rows) first
+    const int units = a.G * a.qtiles, pairs = (units + 1) / 2;
+    const int heads = a.HK;
+    const int per = (int)(gridDim.x / pairs);  // batch * KV heads
+    const int u0 = 2 * (pairs - 1 - (int)(blockIdx.x / per));
+    const int bh = (int)(blockIdx.x % per), b = bh / heads, hk = bh % heads;
+    const int nu = min(2, units - u0);
+    const int qt0 = u0 / a.G, qt1 = (u0 + nu - 1) / a.G;
+    const SinkRange rg = sink_range(a, b, qt0 * kTile, (qt1 - qt0 + 1) * kTile, kTile);
+    const int tiles = rg.count();
+    if (tiles == 0) return;
+
+    if (tid == 0) {
+        mbar_init(&B.q_full, 1);
+        mbar_init(&B.o_full, 1);
+        for (int u = 0; u < 2; ++u) {
+            mbar_init(&B.s_full[u], 1);
+            mbar_init(&B.p_ready[u], 4);
+        }
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&B.full[i], 1);
+            mbar_init(&B.empty[i], 1);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc(&B.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = B.tmem;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            mbar_arrive_expect_tx_w(&B.q_full, nu * kStage);
+            for (int u = 0; u < nu; ++u)
+                for (int kb = 0; kb < KB; ++kb)
+                    tma_load_4d_w(sq + u * kStage + kb * kBlk, &tq, kb * 64, (u0 + u) / a.G * kTile, hk * a.G + (u0 + u) % a.G, b,
+                                  &B.q_full);
+            int q = 0;
+            for (; q < 2 * tiles; ++q) {
+                const int s = q % NS;
+                if (q >= NS && !warp_wait(&B.empty[s], (uint32_t)((q / NS - 1) & 1), a.err, abort_flag)) break;
+                mbar_arrive_expect_tx_w(&B.full[s], kStage);
+                for (int kb = 0; kb < KB; ++kb)
+                    tma_load_4d_w(ring + s * kStage + kb * kBlk, (q & 1) ? &tv : &tk, kb * 64, rg.tile(q >> 1) * kTile, hk, b,
+                                  &B.full[s]);
+            }
+            // every copy has landed before the CTA may end
+            mbar_wait_bounded(&B.q_full, 0, a.err);
+            for (int s = 0; s < min(q, NS); ++s) mbar_wait_bounded(&B.full[s], (uint32_t)(((q - 1 - s) / NS) & 1), a.err);
+        } else if (warp == 1) {
+            const uint32_t ids = mma_idesc(BF ? 1u : 0u, kTile);
+            const uint32_t idv = mma_idesc(BF ? 1u : 0u, KB * 64) | (1u << 16);  // B with N contiguous
+            auto scores = [&](int u, uint32_t kaddr) {
+                const uint32_t qaddr = smem_u32(sq + u * kStage);
+#pragma unroll
+                for (int ks = 0; ks < KB * 4; ++ks) {
+                    const uint32_t o = (ks >> 2) * kBlk + (ks & 3) * 32;
+                    mma_ss(tbase + u * 128, mma_desc_sw128(qaddr + o), mma_desc_sw128(kaddr + o), ids, ks > 0);
+                }
+                mma_commit_w(&B.s_full[u]);
+            };
+            bool ok = warp_wait(&B.q_full, 0, a.err, abort_flag) && warp_wait(&B.full[0], 0, a.err, abort_flag);
+            if (ok) {
+                tc_fence_after();
+                for (int u = 0; u < nu; ++u) scores(u, smem_u32(ring));
+                mma_commit_w(&B.empty[0]);
+            }
+            for (int j = 0; j < tiles && ok; ++j) {
+                const int qv = 2 * j + 1, sv = qv % NS, qk = qv + 1, sk = qk % NS;
+                uint8_t* vt = ring + sv * kStage;
+                if (!(ok = warp_wait(&B.full[sv], (uint32_t)((qv / NS) & 1), a.err, abort_flag))) break;
+                const int behind = rg.n - rg.tile(j) * kTile;  // keys of the tile that exist
+                if (behind < kTile && rg.n < a.len_k) {
+                    // the padding behind a sequence's end may hold anything, and 0 * NaN is NaN
+                    for (int e = lane; e < (kTile - behind) * 8; e += 32)
+#pragma unroll
+                        for (int kb = 0; kb < KB; ++kb)
+                            *reinterpret_cast<uint4*>(vt + kb * kBlk + behind * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                for (int u = 0; u < nu; ++u) {
+                    if (!(ok = warp_wait(&B.p_ready[u], (uint32_t)(j & 1), a.err, abort_flag))) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)
+                        mma_ts(tbase + kColO + u * (KB * 64), tbase + u * 128 + ks * 8, v_desc(smem_u32(vt) + ks * 2048), idv,
+                               (j | ks) > 0);
+                    if (u == nu - 1) mma_commit_w(&B.empty[sv]);
+                    if (j + 1 < tiles) {
+                        if (u == 0) {
+                            if (!(ok = warp_wait(&B.full[sk], (uint32_t)((qk / NS) & 1), a.err, abort_flag))) break;
+                            tc_fence_after();
+                        }
+                        scores(u, smem_u32(ring + sk * kStage));
+                        if (u == nu - 1) mma_commit_w(&B.empty[sk]);
+                    }
+                }
+            }
+            if (ok) mma_commit_w(&B.o_full);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int u = (warp >> 2) - 1, q4 = warp & 3, row = q4 * 32 + lane;
+        const int qt = (u0 + u) / a.G, h = hk * a.G + (u0 + u) % a.G;
+        const int p0 = qt * kTile + a.len_k - a.len_q, p = p0 + row;
+        const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+        const uint32_t ts = tbase + u * 128 + lane_off, to = tbase + kColO + u * (KB * 64) + lane_off;
+        float m = -INFINITY, l = 0.0f;
+        bool ok = u < nu;
+        for (int j = 0; j < tiles && ok; ++j) {
+            if (!(ok = warp_wait(&B.s_full[u], (uint32_t)(j & 1), a.err, abort_flag))) break;
+            tc_fence_after();
+            uint32_t r[128];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) ld32_async(ts + c * 32, r + c * 32);
+            wait_ld();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) pin32(r + c * 32);
+            const int j0 = rg.tile(j) * kTile;
+            const bool whole = j0 + kTile - 1 <= p0 && j0 + kTile <= rg.n &&
+                               (a.window <= 0 || j0 > p0 + kTile - 1 - a.window || j0 + kTile <= a.sinks);
+            if (!whole) {
+                const int hi = min(p, rg.n - 1) - j0, lo = a.window > 0 ? p - a.window + 1 - j0 : 0, sk = a.sinks - j0;
+#pragma unroll
+                for (int c = 0; c < 128; ++c)
+                    if (!(c <= hi && (c >= lo || c < sk))) r[c] = 0xFF800000u;  // -inf
+            }
+            float mt = -INFINITY;
+            {
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(r[c]));
+                mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            }
+            const bool need = (mt - m) * a.scale2 > kGrow;  // true for a row's first key, false while it has none
+            if (__any_sync(0xffffffffu, need)) {
+                const float corr = need ? ex2_approx((m - mt) * a.scale2) : 1.0f;
+                l *= corr;
+                if (need) m = mt;
+                if (j > 0) {  // the products up to here are complete: this tile's scores were issued behind them
+#pragma unroll 1
+                    for (int c = 0; c < KB * 2; ++c) {
+                        uint32_t o[32];
+                        ld32_async(to + c * 32, o);
+                        wait_ld();
+                        pin32(o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                        st32(to + c * 32, o);
+                    }
+                }
+            }
+            const float ms = (m == -INFINITY ? 0.0f : m) * a.scale2;
+            const float2 sc = make_float2(a.scale2, a.scale2), nm = make_float2(-ms, -ms);
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+            for (int c = 0; c < 64; ++c) {
+                float2 x = __ffma2_rn(make_float2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), sc, nm);
+                x.x = ex2_approx(x.x);
+                x.y = ex2_approx(x.y);
+                sum[c & 1] = __fadd2_rn(sum[c & 1], x);
+                r[c] = pack2<BF>(x.x, x.y);
+                if (c == 31) st32(ts, r);
+            }
+            st32(ts + 32, r + 32);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(&B.p_ready[u]);
+        }
+        if (ok && (ok = warp_wait(&B.o_full, 0, a.err, abort_flag))) {
+            tc_fence_after();
+            const int i = qt * kTile + row;
+            const bool real = i < a.len_q && p < rg.n;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            uint8_t* po = a.O + (size_t)b * a.os.item + (size_t)h * a.os.head + (size_t)i * a.os.token;
+#pragma unroll 1
+            for (int c = 0; c < KB * 2; ++c) {
+                uint32_t o[32];
+                ld32_async(to + c * 32, o);
+                wait_ld();
+                pin32(o);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i2 = 0; i2 < 4; ++i2)
+                        w[i2] = pack2<BF>(__uint_as_float(o[v * 8 + 2 * i2]) * inv, __uint_as_float(o[v * 8 + 2 * i2 + 1]) * inv);
+                    if (real && c * 32 + v * 8 < a.D)
+                        *reinterpret_cast<uint4*>(po + (c * 32 + v * 8) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            if (real && a.lse)
+                a.lse[((size_t)b * a.H + h) * a.len_q + i] =
+                    l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) * a.scale2 + log2f(l)) * 0.693147180559945f;
+            tc_fence_before();
+        }
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tbase, 512);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
+// [batch][heads][rows][D] with byte strides; boxes of 64 columns x 128 rows, 128-byte swizzle, zeros
+// outside.  A stride of a dimension of one entry is not used and set to a valid value.
+bool encode(CUtensorMap* m, const void* base, bool bf, int D, int rows, int heads, int batch, const rkv_row_strides& s) {
+    auto enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t rowb = (cuuint64_t)D * 2;
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
+    const cuuint64_t st[3] = {rows > 1 ? (cuuint64_t)s.token : rowb, heads > 1 ? (cuuint64_t)s.head : rowb,
+                              batch > 1 ? (cuuint64_t)s.item : rowb};
+    const cuuint32_t box[4] = {64u, (cuuint32_t)kTile, 1u, 1u}, one[4] = {1u, 1u, 1u, 1u};
+    return enc(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, st,
+               box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int KB, bool BF>
+int launch_kb(const SinkArgs& a, long long blocks, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+              cudaStream_t st) {
+    const int smem = 2048 + (2 + stages(KB)) * KB * kBlk;  // the barriers, and up to 1023 bytes of alignment
+    if (cudaFuncSetAttribute(sink_tc_kernel<KB, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return RKV_ERR_CUDA;
+    }
+    sink_tc_kernel<KB, BF><<<(unsigned)blocks, kThreads, smem, st>>>(a, tq, tk, tv);
+    return cudaGetLastError() == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
+}
+
+}  // namespace
+
+bool sink_tc_supported(const SinkArgs& a, int dtype) { return dtype != RKV_F32 && a.D <= 128; }
+
+int launch_sink_tc(SinkArgs a, int dtype, int batch, cudaStream_t st) {
+    const bool bf = dtype == RKV_BF16;
+    CUtensorMap tq, tk, tv;
+    if (!encode(&tq, a.Q, bf, a.D, a.len_q, a.H, batch, a.qs) || !encode(&tk, a.K, bf, a.D, a.len_k, a.HK, batch, a.ks) ||
+        !encode(&tv, a.V, bf, a.D, a.len_k, a.HK, batch, a.ks))
+        return RKV_ERR_CUDA;
+    a.qtiles = (a.len_q + kTile - 1) / kTile;
+    const long long units = (long long)a.G * a.qtiles, blocks = (units + 1) / 2 * batch * a.HK;
+    if (units > 0x7FFFFFFELL || blocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
+    if (a.D <= 64) return bf ? launch_kb<1, true>(a, blocks, tq, tk, tv, st) : launch_kb<1, false>(a, blocks, tq, tk, tv, st);
+    return bf ? launch_kb<2, true>(a, blocks, tq, tk, tv, st) : launch_kb<2, false>(a, blocks, tq, tk, tv, st);
+}
+
+}  // namespace rkv
