@@ -58,6 +58,7 @@ constexpr int kWarps = 4;
 constexpr int kTile = 32;       // tokens a warp takes at a time
 constexpr int kMinChunk = 128;  // visible tokens per CTA at least
 constexpr int kMaxSplits = 1024;
+constexpr long long kTargetCtas = 148 * 8;
 
 struct DecodeArgs {
     PagedView c;
@@ -95,52 +96,7 @@ __device__ __forceinline__ Visible visible(const DecodeArgs& a, int b) {
     return s;
 }
 
-template <typename T>
-struct Vec;  // 16 bytes of T as floats
-template <>
-struct Vec<float> {
-    static constexpr int N = 4;
-    static __device__ __forceinline__ void get(const uint4& u, float* f) {
-        f[0] = __uint_as_float(u.x);
-        f[1] = __uint_as_float(u.y);
-        f[2] = __uint_as_float(u.z);
-        f[3] = __uint_as_float(u.w);
-    }
-    static __device__ __forceinline__ float one(const void* p, int i) { return static_cast<const float*>(p)[i]; }
-};
-template <>
-struct Vec<__nv_bfloat16> {
-    static constexpr int N = 8;
-    static __device__ __forceinline__ void get(const uint4& u, float* f) {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-    static __device__ __forceinline__ float one(const void* p, int i) {
-        return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
-    }
-};
-template <>
-struct Vec<__half> {
-    static constexpr int N = 8;
-    static __device__ __forceinline__ void get(const uint4& u, float* f) {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            f[2 * i] = v.x;
-            f[2 * i + 1] = v.y;
-        }
-    }
-    static __device__ __forceinline__ float one(const void* p, int i) {
-        return __half2float(static_cast<const __half*>(p)[i]);
-    }
-};
-
-__device__ __forceinline__ uint4 load16(const uint8_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ float4 load16(const uint8_t* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
 
 __device__ __forceinline__ float warp_max(float x) {
 #pragma unroll
@@ -155,16 +111,46 @@ __device__ __forceinline__ float warp_sum(float x) {
 // 0 in place of -inf, so that a set with nothing in it subtracts no infinities.
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// Joins the warps' (m, l, o) of ng heads from shared memory (ms, ls [warps][rows], os [warps][rows][pitch])
+// and writes the part, or the output where there is one part.
+__device__ __forceinline__ void merge_warps(const DecodeArgs& a, size_t head0, int ng, int split, const float* ms,
+                                            const float* ls, const float* os, int rows, int pitch) {
+    const int D = a.D;
+    for (int i = threadIdx.x; i < ng * D; i += kWarps * 32) {
+        const int g = i / D, d = i - g * D;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ms[w * rows + g]);
+        const float mf = finite_max(mm);
+        float ll = 0.0f, oo = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float c = exp2f(ms[w * rows + g] - mf);
+            ll = fmaf(ls[w * rows + g], c, ll);
+            oo = fmaf(os[(w * rows + g) * pitch + d], c, oo);
+        }
+        const size_t head = head0 + g;
+        if (a.splits == 1) {
+            a.O[head * D + d] = ll == 0.0f ? 0.0f : oo / ll;
+            if (d == 0 && a.lse) a.lse[head] = ll == 0.0f ? -INFINITY : (mf + log2f(ll)) * 0.693147180559945f;
+        }
+        if (a.part_o) {
+            if (a.splits > 1) a.part_o[(head * a.splits + split) * D + d] = oo;
+            if (d == 0) a.part_ml[head * a.splits + split] = make_float2(mm, ll);
+        }
+    }
+}
+
 size_t simt_smem(int GT, int D) { return sizeof(float) * ((size_t)GT * D + kWarps * GT * kTile + 2 * kWarps * GT + (size_t)kWarps * GT * D); }
 
-// Fused multiply-adds on the CUDA cores, any type: one CTA per (item, KV
+// fp32 caches, fused multiply-adds on the CUDA cores: one CTA per (item, KV
 // head, group of up to GT query heads, part).  Every warp takes 32 tokens at a
 // time on its own: 8 lanes form the scores of a token (four tokens per lane
 // and pass), a lane per token forms the weights, and LR lanes of 16 bytes add
 // up a V row.  VL: 16-byte vectors of a V row per lane.
-template <typename T, int GT, int VL>
+template <int GT, int VL>
 __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const DecodeArgs a) {
-    constexpr int N = Vec<T>::N;
+    constexpr int N = 4;  // floats of a 16-byte vector
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int D = a.D, VPR = D / N;
@@ -186,10 +172,10 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const De
     const int v0 = (int)v_lo, v1 = (int)min((long long)vis.nvis, v_lo + a.chunk);
     const int h0 = hk * a.G + grp * GT, ng = min(GT, a.G - grp * GT);
 
-    const uint8_t* q = a.Q + (size_t)b * a.q_stride;
+    const float* q = reinterpret_cast<const float*>(a.Q + (size_t)b * a.q_stride);
     for (int i = tid; i < GT * D; i += kWarps * 32) {
         const int g = i / D;
-        qs[i] = g < ng ? Vec<T>::one(q, (h0 + g) * D + (i - g * D)) * a.scale2 : 0.0f;
+        qs[i] = g < ng ? q[(h0 + g) * D + (i - g * D)] * a.scale2 : 0.0f;
     }
     __syncthreads();
 
@@ -223,14 +209,13 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const De
                 for (int g = 0; g < GT; ++g) s[j][g] = 0.0f;
             }
             for (int vec = lane & 7; vec < VPR; vec += 8) {
-                uint4 x[4];
+                float4 x[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    x[j] = o[j] >= 0 ? load16(a.c.K + o[j] + vec * 16) : make_uint4(0, 0, 0, 0);
+                    x[j] = o[j] >= 0 ? load16(a.c.K + o[j] + vec * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float f[N];
-                    Vec<T>::get(x[j], f);
+                    const float f[N] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
                     for (int g = 0; g < GT; ++g)
 #pragma unroll
@@ -271,9 +256,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const De
 #pragma unroll
             for (int i = 0; i < VL; ++i) {
                 const int vec = vl0 + i * 32;
-                const uint4 x = o >= 0 && vec < VPR ? load16(a.c.V + o + vec * 16) : make_uint4(0, 0, 0, 0);
-                float f[N];
-                Vec<T>::get(x, f);
+                const float4 x = o >= 0 && vec < VPR ? load16(a.c.V + o + vec * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float f[N] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int g = 0; g < GT; ++g) {
                     const float p = pw[g * kTile + t];
@@ -303,29 +287,297 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const De
             }
     }
     __syncthreads();
-    for (int i = tid; i < ng * D; i += kWarps * 32) {
-        const int g = i / D, d = i - g * D;
-        float mm = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ms[w * GT + g]);
-        const float mf = finite_max(mm);
-        float ll = 0.0f, oo = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float c = exp2f(ms[w * GT + g] - mf);
-            ll = fmaf(ls[w * GT + g], c, ll);
-            oo = fmaf(os[(w * GT + g) * D + d], c, oo);
-        }
-        const size_t head = (size_t)b * a.H + h0 + g;
-        if (a.splits == 1) {
-            a.O[head * D + d] = ll == 0.0f ? 0.0f : oo / ll;
-            if (d == 0 && a.lse) a.lse[head] = ll == 0.0f ? -INFINITY : (mf + log2f(ll)) * 0.693147180559945f;
-        }
-        if (a.part_o) {
-            if (a.splits > 1) a.part_o[(head * a.splits + split) * D + d] = oo;
-            if (d == 0) a.part_ml[head * a.splits + split] = make_float2(mm, ll);
-        }
+    merge_warps(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, GT, D);
+}
+
+// ---------------------------------------------------------------------------
+// 16-bit caches: matrix instructions on tiles of 16 tokens
+// ---------------------------------------------------------------------------
+constexpr int kKeys = 16;     // tokens of a tile
+constexpr int kMmaStages = 3; // tiles of a warp in shared memory, one in use and the others on their way
+
+template <bool BF>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    if (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// 16 bytes global -> shared, or zeros (nothing is read) where !real.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float ex2(float t) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+    return y;
+}
+// The two values as 16-bit pair, and what the rounding left of them.
+template <bool BF>
+__device__ __forceinline__ uint32_t split2(float& x, float& y) {
+    if (BF) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(&v);
+        x -= __uint_as_float(u << 16);
+        y -= __uint_as_float(u & 0xFFFF0000u);
+        return u;
     }
+    const __half2 v = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(v);
+    x -= f.x;
+    y -= f.y;
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__host__ __device__ constexpr int mma_stage_bytes(int DP) { return kKeys * DP * 2 * 2; }  // K rows, V rows
+constexpr size_t mma_smem(int DP, int NT) {
+    const size_t ring = (size_t)kWarps * kMmaStages * mma_stage_bytes(DP);
+    const size_t merge = sizeof(float) * kWarps * 8 * NT * (2 + DP + 4);
+    return ring > merge ? ring : merge;
+}
+
+// One CTA per (item, KV head, group of up to 8 NT query heads, part); every
+// warp takes tiles of 16 tokens on its own.  The tile's K and V rows arrive in
+// the warp's ring by 16-byte asynchronous copies, rows of DP columns with the
+// 16-byte chunk c of row r at c ^ (r % 8), so that the eight rows of a matrix
+// load lie in different banks.  Scores: K (16 tokens x 16 columns per step) by
+// q^T (8 heads); output: V^T (16 columns x 16 tokens) by P (8 heads), whose
+// fragment is the transpose of the scores'.  P keeps fp32's precision: it
+// enters as a sum of 16-bit parts (three for bf16, two for fp16), one product
+// each, which costs nothing here, since the kernel is bound by its reads.
+// A row's maximum is raised only when a score exceeds it by more than 2^8
+// (both types hold P then); fp16's P is kept 2^7 larger, away from the type's
+// smallest numbers.
+template <bool BF, int DP, int NT>
+__global__ void __launch_bounds__(kWarps * 32) paged_decode_mma_kernel(const DecodeArgs a) {
+    constexpr int kStage = mma_stage_bytes(DP), CH = DP / 8;  // 16-byte chunks of a row
+    constexpr int PARTS = BF ? 3 : 2;
+    constexpr float kLift = BF ? 0.0f : 7.0f, kGrow = 8.0f;
+    constexpr int RPI = 32 / CH;                              // rows a warp copies per instruction
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int D = a.D;
+
+    long long id = blockIdx.x;
+    const int split = (int)(id % a.splits);
+    id /= a.splits;
+    const int grp = (int)(id % a.ngroups);
+    id /= a.ngroups;
+    const int hk = (int)(id % a.HK), b = (int)(id / a.HK);
+    const Visible vis = visible(a, b);
+    const long long v_lo = (long long)split * a.chunk;
+    if (split > 0 && v_lo >= vis.nvis) return;  // the join takes the parts that hold tokens
+    const int v0 = (int)v_lo, v1 = (int)min((long long)vis.nvis, v_lo + a.chunk);
+    const int h0 = hk * a.G + grp * 8 * NT, ng = min(8 * NT, a.G - grp * 8 * NT);
+
+    uint8_t* ring = smem + warp * kMmaStages * kStage;
+    const uint32_t ring_u = smem_u32(ring);
+    if (D < DP)  // the columns behind D count as zeros and are never copied
+        for (int e = lane; e < kMmaStages * 2 * kKeys * CH; e += 32) {
+            const int row = e / CH, c = e % CH;
+            if ((c ^ (row & 7)) >= D / 8) *reinterpret_cast<uint4*>(ring + row * DP * 2 + c * 16) = make_uint4(0, 0, 0, 0);
+        }
+
+    // the tile's tokens: lane i (and i + 16) has the row of token i
+    const int ntiles = v1 > v0 ? (v1 - v0 + kKeys - 1) / kKeys : 0;
+    auto row_of = [&](int tile) -> long long {
+        const int v = v0 + tile * kKeys + (lane & 15);
+        return tile < ntiles && v < v1 ? paged_offset(a.c, b, hk, vis.token(v)) : -1;
+    };
+    const int cchunk = lane % CH, crow = lane / CH;
+    auto fetch = [&](int slot, long long off) {
+#pragma unroll
+        for (int i = 0; i < kKeys / RPI; ++i) {
+            const int r = i * RPI + crow;
+            const long long o = __shfl_sync(0xffffffffu, off, r);
+            if (cchunk < D / 8) {
+                const uint32_t dst = ring_u + slot * kStage + r * DP * 2 + ((cchunk ^ (r & 7)) << 4);
+                copy16(dst, o >= 0 ? a.c.K + o + cchunk * 16 : a.Q, o >= 0);
+                copy16(dst + kKeys * DP * 2, o >= 0 ? a.c.V + o + cchunk * 16 : a.Q, o >= 0);
+            }
+        }
+    };
+    long long off_next = row_of(warp);
+    uint32_t real[kMmaStages];  // which of the tile's tokens there are
+#pragma unroll
+    for (int s = 0; s < kMmaStages - 1; ++s) {
+        const long long off = off_next;
+        off_next = row_of(warp + (s + 1) * kWarps);
+        real[s] = __ballot_sync(0xffffffffu, off >= 0);
+        if (warp + s * kWarps < ntiles) fetch(s, off);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    // q^T fragments: columns 2 t, 2 t + 1 (and + 8) of head g
+    uint32_t q[NT][DP / 16][2];
+    const uint8_t* qb = a.Q + (size_t)b * a.q_stride;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int d = k * 16 + e * 8 + 2 * t;
+                q[n][k][e] = n * 8 + g < ng && d < D
+                                 ? __ldg(reinterpret_cast<const uint32_t*>(qb + ((size_t)(h0 + n * 8 + g) * D + d) * 2))
+                                 : 0u;
+            }
+    float m[NT][2], l[NT][2], o[NT][DP / 16][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][k][e] = 0.0f;
+    }
+    // matrix loads: lane i gives the address of row i % 8 of block i / 8
+    const int kr = lane & 15, kc = lane >> 4;                       // K: rows 0-15, column halves
+    const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;  // V^T: column halves first, then rows
+
+    int slot = 0;
+    for (int tile = warp; tile < ntiles; tile += kWarps) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kMmaStages - 2) : "memory");
+        __syncwarp();
+        const uint32_t here = real[0];
+#pragma unroll
+        for (int s = 0; s + 1 < kMmaStages - 1; ++s) real[s] = real[s + 1];
+        {
+            const int ahead = tile + (kMmaStages - 1) * kWarps;
+            const long long off = off_next;
+            off_next = row_of(ahead + kWarps);
+            real[kMmaStages - 2] = __ballot_sync(0xffffffffu, off >= 0);
+            int fs = slot + kMmaStages - 1;
+            if (fs >= kMmaStages) fs -= kMmaStages;
+            if (ahead < ntiles) fetch(fs, off);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        const uint32_t kb = ring_u + slot * kStage, vb = kb + kKeys * DP * 2;
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            uint32_t f[4];
+            ldmatrix4<false>(f, kb + kr * DP * 2 + (((2 * k + kc) ^ (kr & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<BF>(s[n], f, q[n][k][0], q[n][k][1]);
+        }
+        // scores of tokens g and g + 8, heads 2 t and 2 t + 1
+        const bool r0 = (here >> g) & 1, r1 = (here >> (g + 8)) & 1;
+        bool need = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            s[n][0] = r0 ? s[n][0] * a.scale2 : -INFINITY;
+            s[n][1] = r0 ? s[n][1] * a.scale2 : -INFINITY;
+            s[n][2] = r1 ? s[n][2] * a.scale2 : -INFINITY;
+            s[n][3] = r1 ? s[n][3] * a.scale2 : -INFINITY;
+            need |= fmaxf(s[n][0], s[n][2]) > m[n][0] + kGrow || fmaxf(s[n][1], s[n][3]) > m[n][1] + kGrow;
+            if (a.scores) {
+                const int v = v0 + tile * kKeys + g;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int h = n * 8 + 2 * t + (e & 1), ve = v + (e >> 1) * 8;
+                    if (h < ng && ve < v1) a.scores[((size_t)b * a.H + h0 + h) * a.vmax + ve] = s[n][e];
+                }
+            }
+        }
+        if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = fmaxf(s[n][e], s[n][e + 2]);
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+                    x = fmaxf(m[n][e], x);
+                    const float corr = ex2(m[n][e] - finite_max(x));
+                    m[n][e] = x;
+                    l[n][e] *= corr;
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        o[n][k][e] *= corr;
+                        o[n][k][e + 2] *= corr;
+                    }
+                }
+        }
+        uint32_t p[NT][PARTS][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float m0 = finite_max(m[n][0]) - kLift, m1 = finite_max(m[n][1]) - kLift;
+            float x[4] = {ex2(s[n][0] - m0), ex2(s[n][1] - m1), ex2(s[n][2] - m0), ex2(s[n][3] - m1)};
+            l[n][0] += x[0] + x[2];
+            l[n][1] += x[1] + x[3];
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+                p[n][i][0] = transpose8x8(split2<BF>(x[0], x[1]));
+                p[n][i][1] = transpose8x8(split2<BF>(x[2], x[3]));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            uint32_t f[4];
+            ldmatrix4<true>(f, vb + vr * DP * 2 + (((2 * k + vc) ^ (vr & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < PARTS; ++i) mma16816<BF>(o[n][k], f, p[n][i][0], p[n][i][1]);
+        }
+        if (++slot == kMmaStages) slot = 0;
+    }
+    // the warps' (m, l, o) meet in shared memory, over the ring
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    float* ms = reinterpret_cast<float*>(smem);  // [warps][8 NT]
+    float* ls = ms + kWarps * 8 * NT;
+    float* os = ls + kWarps * 8 * NT;            // [warps][8 NT][DP + 4]
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float x = l[n][e];
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+            const int h = warp * 8 * NT + n * 8 + 2 * t + e;
+            if (g == 0) {
+                ms[h] = m[n][e] - kLift;
+                ls[h] = x;
+            }
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                os[h * (DP + 4) + k * 16 + g] = o[n][k][e];
+                os[h * (DP + 4) + k * 16 + g + 8] = o[n][k][e + 2];
+            }
+        }
+    __syncthreads();
+    merge_warps(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, 8 * NT, DP + 4);
 }
 
 // m and l of all parts of a head (one warp): the same order whatever the grid.
@@ -398,26 +650,36 @@ struct DecodePlan {
     size_t off_ml, off_o, off_scores, bytes;
 };
 
-// The parts of the visible tokens: enough CTAs for a few waves over the GPU,
-// at least kMinChunk tokens each.
-DecodePlan decode_plan(int H, int HK, int D, long long visible_max, int max_len, int batch, bool weights) {
+// Query heads of a KV head that one CTA takes: up to 8 by fused multiply-adds (fp32); 8 or 16 by matrix
+// instructions, 8 where 16 heads of 256 columns would not fit in registers.
+int head_group(int dtype, int G, int D) {
+    if (dtype == RKV_F32) return G >= 5 ? 8 : G >= 3 ? 4 : G;
+    return G > 8 && D <= 128 ? 16 : 8;
+}
+
+// Parts of the visible tokens: enough CTAs for a few waves over the GPU, at
+// least kMinChunk tokens each.  Grows with `visible_max`.
+long long decode_parts(int dtype, int H, int HK, int D, long long visible_max, int batch) {
+    const int G = H / HK, gt = head_group(dtype, G, D);
+    const long long units = (long long)batch * HK * ((G + gt - 1) / gt);
+    long long parts = units > 0 ? (kTargetCtas + units - 1) / units : 1;
+    const long long most = (visible_max + kMinChunk - 1) / kMinChunk;
+    if (parts > most) parts = most;
+    if (parts > kMaxSplits) parts = kMaxSplits;
+    return parts < 1 ? 1 : parts;
+}
+
+DecodePlan decode_plan(int dtype, int H, int HK, int D, long long visible_max, int max_len, int batch, bool weights) {
     DecodePlan p{};
     const int G = H / HK;
-    p.gt = G >= 5 ? 8 : G >= 3 ? 4 : G;
+    p.gt = head_group(dtype, G, D);
     p.ngroups = (G + p.gt - 1) / p.gt;
-    const long long units = (long long)batch * HK * p.ngroups;
-    const long long target = 148 * 16;
-    long long splits = units > 0 ? (target + units - 1) / units : 1;
-    const long long most = (visible_max + kMinChunk - 1) / kMinChunk;
-    if (splits > most) splits = most;
-    if (splits > kMaxSplits) splits = kMaxSplits;
-    if (splits < 1) splits = 1;
-    const size_t most_parts = (size_t)splits;
-    long long chunk = (visible_max + splits - 1) / splits;
+    const long long parts = decode_parts(dtype, H, HK, D, visible_max, batch);
+    long long chunk = (visible_max + parts - 1) / parts;
     chunk = (chunk + kTile - 1) / kTile * kTile;
     if (chunk < kTile) chunk = kTile;
     p.chunk = (int)chunk;
-    splits = (visible_max + p.chunk - 1) / p.chunk;
+    const long long splits = (visible_max + chunk - 1) / chunk;
     p.splits = splits < 1 ? 1 : (int)splits;
     p.vmax = (max_len + 3) / 4 * 4;
     // the parts before rounding bound the layout: they grow with visible_max, so the workspace of max_len
@@ -425,34 +687,51 @@ DecodePlan decode_plan(int H, int HK, int D, long long visible_max, int max_len,
     const size_t heads = (size_t)batch * H;
     size_t off = kWorkspaceHeader;
     p.off_ml = off;
-    off = align_up(off + heads * most_parts * sizeof(float2), kWorkspaceAlign);
+    off = align_up(off + heads * parts * sizeof(float2), kWorkspaceAlign);
     p.off_o = off;
-    if (most_parts > 1) off = align_up(off + heads * most_parts * D * sizeof(float), kWorkspaceAlign);
+    if (parts > 1) off = align_up(off + heads * parts * D * sizeof(float), kWorkspaceAlign);
     p.off_scores = off;
     if (weights) off = align_up(off + heads * (size_t)p.vmax * sizeof(float), kWorkspaceAlign);
     p.bytes = off;
     return p;
 }
 
-template <typename T, int GT>
+template <int GT>
 int launch_simt(const DecodeArgs& a, long long blocks, cudaStream_t st) {
-    const int vpr = a.D / Vec<T>::N;
+    const int vpr = a.D / 4;
     const size_t smem = simt_smem(GT, a.D);
     if (vpr > 32)
-        paged_decode_simt_kernel<T, GT, 2><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
+        paged_decode_simt_kernel<GT, 2><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
     else
-        paged_decode_simt_kernel<T, GT, 1><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
+        paged_decode_simt_kernel<GT, 1><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
     return launched();
 }
 
-template <typename T>
-int launch_decode(const DecodeArgs& a, int gt, long long blocks, cudaStream_t st) {
+int launch_f32(const DecodeArgs& a, int gt, long long blocks, cudaStream_t st) {
     switch (gt) {
-        case 1: return launch_simt<T, 1>(a, blocks, st);
-        case 2: return launch_simt<T, 2>(a, blocks, st);
-        case 4: return launch_simt<T, 4>(a, blocks, st);
-        default: return launch_simt<T, 8>(a, blocks, st);
+        case 1: return launch_simt<1>(a, blocks, st);
+        case 2: return launch_simt<2>(a, blocks, st);
+        case 4: return launch_simt<4>(a, blocks, st);
+        default: return launch_simt<8>(a, blocks, st);
     }
+}
+
+template <bool BF, int DP, int NT>
+int launch_mma(const DecodeArgs& a, long long blocks, cudaStream_t st) {
+    constexpr size_t smem = mma_smem(DP, NT);
+    if (cudaFuncSetAttribute(paged_decode_mma_kernel<BF, DP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+        cudaSuccess) {
+        (void)cudaGetLastError();
+        return RKV_ERR_CUDA;
+    }
+    paged_decode_mma_kernel<BF, DP, NT><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
+    return launched();
+}
+template <bool BF>
+int launch_16(const DecodeArgs& a, int gt, long long blocks, cudaStream_t st) {
+    if (a.D <= 64) return gt == 16 ? launch_mma<BF, 64, 2>(a, blocks, st) : launch_mma<BF, 64, 1>(a, blocks, st);
+    if (a.D <= 128) return gt == 16 ? launch_mma<BF, 128, 2>(a, blocks, st) : launch_mma<BF, 128, 1>(a, blocks, st);
+    return launch_mma<BF, 256, 1>(a, blocks, st);
 }
 
 }  // namespace
@@ -515,7 +794,11 @@ extern "C" int rkv_paged_decode_workspace_size(int num_heads, int num_heads_kv, 
                                                int with_weights, size_t* bytes) {
     const int rc = decode_shape_check(num_heads, num_heads_kv, dim_head, max_len, batch);
     if (rc || !bytes) return rc ? rc : (int)RKV_ERR_INVALID_ARG;
-    *bytes = decode_plan(num_heads, num_heads_kv, dim_head, max_len, max_len, batch, with_weights != 0).bytes;
+    *bytes = 0;  // the largest over the types
+    for (int dtype : {RKV_F32, RKV_BF16}) {
+        const size_t n = decode_plan(dtype, num_heads, num_heads_kv, dim_head, max_len, max_len, batch, with_weights != 0).bytes;
+        if (n > *bytes) *bytes = n;
+    }
     return RKV_OK;
 }
 
@@ -534,7 +817,7 @@ extern "C" int rkv_paged_decode(const void* Q, long long q_item_stride, int num_
     if (weights && weight_stride < max_len) return RKV_ERR_INVALID_ARG;
     long long vis = max_len;
     if (window > 0 && (long long)sinks + window < vis) vis = (long long)sinks + window;
-    const DecodePlan p = decode_plan(num_heads, cache->num_heads_kv, D, vis, max_len, batch, weights != nullptr);
+    const DecodePlan p = decode_plan(cache->dtype, num_heads, cache->num_heads_kv, D, vis, max_len, batch, weights != nullptr);
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < p.bytes) return RKV_ERR_WORKSPACE;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -570,9 +853,9 @@ extern "C" int rkv_paged_decode(const void* Q, long long q_item_stride, int num_
     const long long jblocks = a.o_blocks + (long long)batch * a.HK * a.w_blocks;
     if (blocks > 0x7FFFFFFFLL || jblocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
     switch (cache->dtype) {
-        case RKV_F32: rc = launch_decode<float>(a, p.gt, blocks, st); break;
-        case RKV_BF16: rc = launch_decode<__nv_bfloat16>(a, p.gt, blocks, st); break;
-        default: rc = launch_decode<__half>(a, p.gt, blocks, st); break;
+        case RKV_F32: rc = launch_f32(a, p.gt, blocks, st); break;
+        case RKV_BF16: rc = launch_16<true>(a, p.gt, blocks, st); break;
+        default: rc = launch_16<false>(a, p.gt, blocks, st); break;
     }
     if (rc || !join || jblocks == 0) return rc;
     size_t smem = (size_t)p.splits * sizeof(float);
