@@ -198,6 +198,20 @@ def _stream(stream) -> int:
     return int(stream)
 
 
+_raw_stream = None
+
+
+def _current_stream(index: int) -> int:
+    """The device's current stream as a number; torch's Stream object, which
+    costs microseconds to make, only where torch lacks the direct query."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)
+
+
 # ---------------------------------------------------------------------------
 # rocket.h mirror (host buffers, synchronous)
 # ---------------------------------------------------------------------------
@@ -457,13 +471,17 @@ class HsaDecoder:
 # ---------------------------------------------------------------------------
 # Paged KV cache: append, dense decode, eviction by accumulated weight
 # ---------------------------------------------------------------------------
-def _on(tensor, stream, call):
-    """Runs call(stream) with the tensor's device current (a stream belongs to one)."""
+def _launch(device, stream, what, fn, *args) -> None:
+    """fn(*args, stream) with the tensors' device current (a stream belongs to one)."""
     import torch
-    if tensor.device.index == torch.cuda.current_device():
-        return call(_stream(stream))
-    with torch.cuda.device(tensor.device):
-        return call(_stream(stream))
+    i = device.index
+    if i == torch.cuda.current_device():
+        st = fn(*args, _current_stream(i) if stream is None else int(stream))
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, _current_stream(i) if stream is None else int(stream))
+    if st != RKV_OK:
+        raise RkvError(st, what)
 
 
 def _int32(t, device, what):
@@ -536,9 +554,9 @@ def paged_append(cache: PagedCache, k, v, n_new=None, stream=None):
         if n_new.numel() != B:
             raise ValueError("n_new: one entry per sequence")
     es = k.element_size()
-    _on(k, stream, lambda st: _check(lib().rkv_paged_append(
-        cache.ref, _ptr(k), _ptr(v), n, B, k.stride(0) * es, k.stride(1) * es, k.stride(2) * es, _ptr(n_new), st),
-        "rkv_paged_append"))
+    si, st, sh, _ = k.stride()
+    _launch(k.device, stream, "rkv_paged_append", lib().rkv_paged_append, cache.ref, k.data_ptr(), v.data_ptr(), n, B,
+            si * es, st * es, sh * es, _ptr(n_new))
 
 
 class PagedDecoder:
@@ -565,18 +583,19 @@ class PagedDecoder:
         """Q [B, H, D] of the cache's type.  weights (nullable): float32
         [B, HK, >= max_len]; every visible token's attention weight, summed over
         its KV head's query heads, is added.  Returns O."""
-        if tuple(Q.shape) != (self.batch, self.num_heads, self.dim_head) or not Q.is_contiguous():
+        if Q.shape != self.O.shape or not Q.is_contiguous():
             raise ValueError("Q: contiguous [B, H, D] of the decoder's sizes")
-        if (Q.dtype != cache.K.dtype or Q.device != cache.K.device or Q.device != self.ws.device
+        dev = Q.device
+        if (Q.dtype != cache.K.dtype or dev != cache.K.device or dev != self.ws.device
                 or cache.batch != self.batch or cache._lens is None):
             raise ValueError("Q, the cache and the decoder: one type, device and batch, and the cache's lens set")
         if (cache.c.num_heads_kv, cache.c.dim_head) != (self.num_heads_kv, self.dim_head):
             raise ValueError("the cache's heads are not the decoder's")
-        wstride = _check_weights(weights, self.batch, self.num_heads_kv, self.max_len, Q.device)
-        _on(Q, stream, lambda st: _check(lib().rkv_paged_decode(
-            _ptr(Q), self.num_heads * self.dim_head * Q.element_size(), self.num_heads, cache.ref, self.max_len,
-            self.batch, self.sinks, self.window, _ptr(self.O), _ptr(self.lse), _ptr(weights), wstride, _ptr(self.ws),
-            self.ws_bytes, st), "rkv_paged_decode"))
+        wstride = _check_weights(weights, self.batch, self.num_heads_kv, self.max_len, dev)
+        _launch(dev, stream, "rkv_paged_decode", lib().rkv_paged_decode, Q.data_ptr(),
+                self.num_heads * self.dim_head * Q.element_size(), self.num_heads, cache.ref, self.max_len, self.batch,
+                self.sinks, self.window, self.O.data_ptr(), self.lse.data_ptr(), _ptr(weights), wstride,
+                self.ws.data_ptr(), self.ws_bytes)
         return self.O
 
 
@@ -607,20 +626,19 @@ class WeightEvictor:
         """In place without out / weights_out.  Returns (kept [B, HK, min(budget,
         max_len)] int32 ascending with -1 behind, new_lens [B] int32): the
         caller's next calls take new_lens (copied, or as the cache's lens)."""
+        dev = cache.K.device
         if cache.batch != self.batch or cache.c.num_heads_kv != self.num_heads_kv or cache._lens is None or weights is None:
             raise ValueError("the evictor's batch and KV heads, lens and weights are needed")
-        if out is not None and (out.batch != self.batch or out.K.device != cache.K.device):
+        if out is not None and (out.batch != self.batch or out.K.device != dev):
             raise ValueError("out: the same batch, on the cache's device")
-        if self.kept.device != cache.K.device:
+        if self.kept.device != dev:
             raise ValueError("the cache is not on the evictor's device")
-        ws = _check_weights(weights, self.batch, self.num_heads_kv, self.max_len, cache.K.device)
-        if weights_out is not None and _check_weights(weights_out, self.batch, self.num_heads_kv, self.max_len,
-                                                      cache.K.device) != ws:
+        ws = _check_weights(weights, self.batch, self.num_heads_kv, self.max_len, dev)
+        if weights_out is not None and _check_weights(weights_out, self.batch, self.num_heads_kv, self.max_len, dev) != ws:
             raise ValueError("weights_out: the layout of weights")
-        _on(cache.K, stream, lambda st: _check(lib().rkv_weight_evict(
-            cache.ref, _ptr(weights), ws, self.max_len, self.batch, self.budget, self.sinks, self.recent,
-            out.ref if out is not None else None, _ptr(weights_out), _ptr(self.kept), self.kept.shape[2],
-            _ptr(self.new_lens), st), "rkv_weight_evict"))
+        _launch(dev, stream, "rkv_weight_evict", lib().rkv_weight_evict, cache.ref, weights.data_ptr(), ws, self.max_len,
+                self.batch, self.budget, self.sinks, self.recent, out.ref if out is not None else None, _ptr(weights_out),
+                self.kept.data_ptr(), self.kept.shape[2], self.new_lens.data_ptr())
         return self.kept, self.new_lens
 
 
@@ -629,8 +647,9 @@ def _row_strides(t, what):
     if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
         raise ValueError(f"{what}: [B, heads, len, D] with unit stride along D")
     es = t.element_size()
-    row = 16 * ((t.shape[3] * es + 15) // 16)  # the stride of a dimension of one entry is never used
-    return _RowStrides(*[t.stride(i) * es if t.shape[i] > 1 else row for i in range(3)])
+    (i, h, n, d), (si, sh, sn, _) = t.shape, t.stride()
+    row = 16 * ((d * es + 15) // 16)  # the stride of a dimension of one entry is never used
+    return _RowStrides(si * es if i > 1 else row, sh * es if h > 1 else row, sn * es if n > 1 else row)
 
 
 class SinkAttention:
@@ -671,11 +690,12 @@ class SinkAttention:
             if lens.numel() != B:
                 raise ValueError("lens: one entry per item")
         qs, ks, os_ = _row_strides(Q, "Q"), _row_strides(K, "K, V"), _row_strides(out, "out")
-        _on(Q, stream, lambda st: _check(lib().rkv_sink_attention(
-            _ptr(Q), _ptr(K), _ptr(V), dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(qs), ctypes.byref(ks),
-            _ptr(lens), self.sinks, self.window, _ptr(out), ctypes.byref(os_), _ptr(lse), _ptr(self.ws), self.ws_bytes,
-            st), "rkv_sink_attention"))
+        _launch(Q.device, stream, "rkv_sink_attention", lib().rkv_sink_attention, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
+                dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(qs), ctypes.byref(ks), _ptr(lens), self.sinks,
+                self.window, out.data_ptr(), ctypes.byref(os_), _ptr(lse), self.ws.data_ptr(), self.ws_bytes)
         return out
 
     def status(self, stream=None) -> int:
-        return _on(self.ws, stream, lambda st: lib().rkv_workspace_status(_ptr(self.ws), st))
+        import torch
+        with torch.cuda.device(self.ws.device):
+            return lib().rkv_workspace_status(_ptr(self.ws), _stream(stream))
