@@ -306,6 +306,8 @@ EVICT = [
     ("f16", 72, 5, 32, [9000, 4097], 4096, 0, 0, "hnd", 32),
     ("bf16", 64, 2, 64, [70001, 20000], 5001, 4, 100, "hnd", 64),
     ("f32", 8, 1, 16, [300000], 100000, 4, 100, "hnd", 128),
+    ("f32", 8, 1, 16, [500000, 90000], 100000, 4, 100, "nhd", 128),  # more weights than a cluster's shared memory holds
+    ("bf16", 8, 1, 64, [420000], 0, 0, 0, "hnd", 16),
 ]
 
 
