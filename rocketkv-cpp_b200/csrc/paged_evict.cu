@@ -18,9 +18,8 @@ namespace cg = cooperative_groups;
 namespace rkv {
 namespace {
 
-constexpr int kSelNT = 512, kSelWarps = kSelNT / 32;
 constexpr int kBins = 2048, kPasses = 3;
-constexpr int kSliceMax = 49152;  // weights of a slice in shared memory (192 KB beside the counts)
+constexpr int kSliceMax = 32768;  // tokens of a slice whose keys and lists are in shared memory (192 KB beside the counts)
 
 struct WEvictArgs {
     PagedView c, o;  // source and destination
@@ -32,80 +31,125 @@ struct WEvictArgs {
     int* new_lens;
     int vpr;      // 16-byte vectors of a row
     int slice;    // tokens of a CTA's slice
+    int list_cap; // entries of a warp's list where the slice is not in shared memory
     int inplace;  // rows move within their own pages
 };
 
 // Larger weight, larger key; -0 ranks as 0, NaN below every number.
-__device__ __forceinline__ uint32_t weight_key(float w) { return w != w ? 0u : float_key(w + 0.0f); }
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    const int b = __float_as_int(w + 0.0f);
+    return w != w ? 0u : (uint32_t)(b ^ ((b >> 31) | (int)0x80000000));
+}
+// The weight of a key (-0 has become 0, a NaN is the canonical one).
+__device__ __forceinline__ float key_weight(uint32_t k) {
+    return k == 0u ? __int_as_float(0x7FC00000) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+
+constexpr int kMaxCluster = 8;
 
 struct SelShared {
     unsigned hist[kPasses][kBins];
-    unsigned warp_sum[kSelWarps];
+    unsigned warp_sum[32];
     unsigned digit, above;
     int count[2];               // tokens of the slice that stay outright, ties
-    int wcount[2][kSelWarps];
+    int wcount[2][32];
 };
 
-// One cluster per (item, KV head).  RESIDENT: the slice stays in shared
-// memory and the kept weights are written from there (so in place is safe:
-// every slice has been read before the first cluster barrier); otherwise the
-// weights are read again from global memory and moved by weight_shift_kernel.
-template <bool RESIDENT>
-__global__ void __launch_bounds__(kSelNT) weight_select_kernel(const WEvictArgs a) {
+static_assert(sizeof(SelShared) % 16 == 0, "keys behind it are 16-byte aligned");
+
+// dst[i] = 0 for lo <= i < hi, the cluster's threads in turn.
+__device__ __forceinline__ void zero_tail(float* dst, int lo, int hi, int thread, int threads) {
+    const int mis = (int)((reinterpret_cast<uintptr_t>(dst + lo) >> 2) & 3);
+    const int body = min(hi, lo + (mis ? 4 - mis : 0)), quads = (hi - body) / 4;
+    if (thread < body - lo) dst[lo + thread] = 0.0f;
+    for (int i = thread; i < quads; i += threads)
+        *reinterpret_cast<float4*>(dst + body + 4 * i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (thread < hi - body - 4 * quads) dst[body + 4 * quads + thread] = 0.0f;
+}
+
+// One cluster per (item, KV head); every CTA has a slice of the tokens, every
+// warp a stretch of the slice.  All weights are looked at twice, for the first
+// and the second digit; in the second look each warp lists, in order, the
+// tokens whose first digit is at or above the threshold's (a few per cent of a
+// long cache), and the third digit, the counts and the output work on those
+// lists.  RESIDENT: the slice's keys stay in shared memory, lists always fit,
+// and the kept weights are written from there (in place is safe: every slice
+// has been read before the first cluster barrier).  Otherwise the second look
+// reads L2, a list holds keys too, a warp whose list is full looks at its
+// whole stretch again instead, and in place weight_shift_kernel moves the
+// weights afterwards.
+template <int NT, bool RESIDENT, bool CLUSTER>
+__global__ void __launch_bounds__(NT) weight_select_kernel(const WEvictArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");
+    constexpr int W = NT / 32;
+    constexpr int EB = 8;  // words of 32 tokens whose loads are on their way together
     extern __shared__ __align__(16) uint8_t smem[];
     SelShared& S = *reinterpret_cast<SelShared*>(smem);
-    float* sw = reinterpret_cast<float*>(smem + sizeof(SelShared));
+    uint32_t* skey = reinterpret_cast<uint32_t*>(smem + sizeof(SelShared));  // [slice] keys, or [W][list_cap] of the lists
+    uint16_t* sidx = reinterpret_cast<uint16_t*>(skey + (RESIDENT ? a.slice : W * a.list_cap));
     cg::cluster_group cl = cg::this_cluster();
-    const int CS = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    const int CS = CLUSTER ? (int)cl.num_blocks() : 1, rank = CLUSTER ? (int)cl.block_rank() : 0;
+    auto sync_all = [&] {
+        if (CLUSTER)
+            cl.sync();
+        else
+            __syncthreads();
+    };
     const int unit = blockIdx.x / CS, hk = unit % a.HK, b = unit / a.HK;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ct = rank * NT + tid, cthreads = CS * NT;  // thread of the cluster
     const int n = paged_len(a.c, b, a.max_len), keep = min(n, a.budget);
     int* kept = a.kept + (size_t)unit * a.kept_stride;
     const float* w = a.w + (size_t)unit * a.w_stride;
     float* wo = a.wo + (size_t)unit * a.w_stride;
-    const int lo_t = min(n, rank * a.slice), hi_t = min(n, lo_t + a.slice), ns = hi_t - lo_t;  // this slice
+    const bool write_w = RESIDENT || wo != w;
 
     if (rank == 0 && hk == 0 && tid == 0) a.new_lens[b] = keep;
-    for (int i = keep + rank * kSelNT + tid; i < a.list; i += CS * kSelNT) kept[i] = -1;
+    for (int i = keep + ct; i < a.list; i += cthreads) kept[i] = -1;
     if (n <= a.budget) {
-        for (int i = rank * kSelNT + tid; i < n; i += CS * kSelNT) {
+        for (int i = ct; i < n; i += cthreads) {
             kept[i] = i;
-            if (RESIDENT && wo != w) wo[i] = w[i];
+            if (wo != w) wo[i] = w[i];
         }
-        if (RESIDENT)
-            for (int i = keep + rank * kSelNT + tid; i < a.max_len; i += CS * kSelNT) wo[i] = 0.0f;
+        if (write_w) zero_tail(wo, keep, a.max_len, ct, cthreads);
         return;  // the same for every CTA of the cluster
     }
-    const int first = a.sinks, last = n - a.recent;  // the tokens that compete: first .. last - 1, more than m
-    const int m = a.budget - a.sinks - a.recent;
-    for (int i = tid; i < kPasses * kBins; i += kSelNT) (&S.hist[0][0])[i] = 0;
-    if (RESIDENT)
-        for (int i = tid; i < ns; i += kSelNT) sw[i] = w[lo_t + i];
+    for (int i = tid; i < kPasses * kBins / 4; i += NT) reinterpret_cast<uint4*>(S.hist)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    auto weight = [&](int i) { return RESIDENT ? sw[i] : w[lo_t + i]; };
-    const int c0 = max(0, first - lo_t), c1 = min(ns, last - lo_t);  // competing part of the slice
+    const int lo_t = (int)min((long long)n, (long long)rank * a.slice);
+    const int ns = min(n - lo_t, a.slice);  // this slice
+    const float* ws = w + lo_t;
+    // the part of the slice that competes: more than m tokens over all slices
+    const int c0 = max(0, a.sinks - lo_t), c1 = min(ns, n - a.recent - lo_t);
+    const int m = a.budget - a.sinks - a.recent;
+    const int per = ((ns + W - 1) / W + 31) / 32 * 32;
+    const int t0 = min(ns, warp * per), t1 = min(ns, t0 + per);  // this warp's stretch
+    const int cap = RESIDENT ? per : a.list_cap;
+    uint16_t* li = sidx + (RESIDENT ? t0 : warp * a.list_cap);
+    uint32_t* lk = skey + warp * a.list_cap;  // keys of the list (not RESIDENT)
+    int nlist = 0;
+    bool dense = !RESIDENT && per > 65536;  // indices of a stretch have 16 bits
+
     uint32_t prefix = 0;
     unsigned need = m;  // still to be taken among the keys that share the prefix
-#pragma unroll
-    for (int pass = 0; pass < kPasses; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-        const uint32_t mask = pass == 0 ? 0u : 0xFFFFFFFFu << (shift + bits);
-        for (int i = c0 + tid; i < c1; i += kSelNT) {
-            const uint32_t k = weight_key(weight(i));
-            if ((k & mask) == prefix) atomicAdd(&S.hist[pass][(k >> shift) & ((1 << bits) - 1)], 1u);
-        }
-        cl.sync();
-        // thread i sums bins 4 i .. 4 i + 3 from the top over the cluster; a scan finds where `need` falls
-        constexpr int BPT = kBins / kSelNT;
+    // the digit at which `need` falls, over the cluster's counts: thread i sums BPT bins from the top
+    auto find_digit = [&](int pass, int shift) {
+        sync_all();
+        constexpr int BPT = kBins / NT;  // 2 or 4
         unsigned v[BPT], sum = 0;
 #pragma unroll
         for (int e = 0; e < BPT; ++e) v[e] = 0;
-        for (int r = 0; r < CS; ++r) {
-            const unsigned* h = cl.map_shared_rank(&S.hist[pass][0], r);
-            const uint4 x = *reinterpret_cast<const uint4*>(h + kBins - BPT * (tid + 1));
-            v[0] += x.w, v[1] += x.z, v[2] += x.y, v[3] += x.x;
-        }
+#pragma unroll
+        for (int r = 0; r < (CLUSTER ? kMaxCluster : 1); ++r)
+            if (r < CS) {
+                const unsigned* h = CLUSTER ? cl.map_shared_rank(&S.hist[pass][0], r) : &S.hist[pass][0];
+                h += kBins - BPT * (tid + 1);
+#pragma unroll
+                for (int e = 0; e < BPT; e += 2) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(h + BPT - 2 - e);
+                    v[e] += x.y, v[e + 1] += x.x;
+                }
+            }
 #pragma unroll
         for (int e = 0; e < BPT; ++e) sum += v[e];
         unsigned inc = sum;
@@ -116,69 +160,129 @@ __global__ void __launch_bounds__(kSelNT) weight_select_kernel(const WEvictArgs 
         }
         if (lane == 31) S.warp_sum[warp] = inc;
         __syncthreads();
-        unsigned before = inc - sum;
-        for (int x = 0; x < warp; ++x) before += S.warp_sum[x];
+        unsigned before = __reduce_add_sync(0xffffffffu, lane < warp ? S.warp_sum[lane] : 0u) + inc - sum;
         if (before < need && before + sum >= need) {  // one thread, unless need is 0
             int e = 0;
             while (before + v[e] < need) before += v[e++];
             S.digit = kBins - 1 - (BPT * tid + e);
             S.above = before;
         }
-        if (need == 0 && tid == 0) S.digit = kBins - 1, S.above = 0;
+        if (need == 0 && tid == 0) S.digit = 0, S.above = 0;
         __syncthreads();
         prefix |= S.digit << shift;
         need -= S.above;
-    }
-    // what stays: sinks, recent, keys above prefix; of those equal to it the first `need`.  m == 0: nothing
-    // competes (prefix is then the largest key, which no weight but a NaN with that sign has, and need is 0)
-    auto flags = [&](int i, bool& stay, bool& tie) {
-        const int t = lo_t + i;
-        const bool forced = t < first || t >= last;
-        const uint32_t k = weight_key(weight(i));
-        stay = forced || (m > 0 && k > prefix);
-        tie = !forced && m > 0 && k == prefix;
     };
-    // every warp takes a stretch of the slice: counts, then the places
-    const int per = ((ns + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
-    const int w0 = min(ns, warp * per), w1 = min(ns, w0 + per);
-    int cs = 0, ct = 0;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        bool stay = false, tie = false;
-        if (i0 + lane < w1) flags(i0 + lane, stay, tie);
-        cs += __popc(__ballot_sync(0xffffffffu, stay));
-        ct += __popc(__ballot_sync(0xffffffffu, tie));
+
+    // first digit
+    for (int i0 = t0; i0 < t1; i0 += 32 * EB) {
+        float x[EB];
+#pragma unroll
+        for (int e = 0; e < EB; ++e) {
+            const int i = i0 + e * 32 + lane;
+            x[e] = i < t1 ? ws[i] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < EB; ++e) {
+            const int i = i0 + e * 32 + lane;
+            const uint32_t k = weight_key(x[e]);
+            if (RESIDENT && i < t1) skey[i] = k;
+            if (i < t1 && i >= c0 && i < c1) atomicAdd(&S.hist[0][k >> 21], 1u);
+        }
     }
-    if (lane == 0) S.wcount[0][warp] = cs, S.wcount[1][warp] = ct;
+    find_digit(0, 21);
+    if (write_w) zero_tail(wo, keep, a.max_len, ct, cthreads);
+    // second digit, and the lists
+    for (int i0 = t0; i0 < t1; i0 += 32 * EB) {
+        uint32_t k[EB];
+#pragma unroll
+        for (int e = 0; e < EB; ++e) {
+            const int i = i0 + e * 32 + lane;
+            k[e] = i < t1 ? (RESIDENT ? skey[i] : __float_as_uint(ws[i])) : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < EB; ++e) {
+            const int i = i0 + e * 32 + lane;
+            if (!RESIDENT) k[e] = weight_key(__uint_as_float(k[e]));
+            const bool in = i < t1, comp = in && i >= c0 && i < c1;
+            if (comp && (k[e] >> 21) == (prefix >> 21)) atomicAdd(&S.hist[1][(k[e] >> 10) & 2047], 1u);
+            const bool may = comp ? m > 0 && k[e] >= prefix : in;
+            const unsigned mm = __ballot_sync(0xffffffffu, may);
+            if (mm && !dense) {
+                const int c = __popc(mm);
+                if (nlist + c > cap) {
+                    dense = true;
+                } else {
+                    if (may) {
+                        const int at = nlist + __popc(mm & ((1u << lane) - 1));
+                        li[at] = (uint16_t)(i - t0);
+                        if (!RESIDENT) lk[at] = k[e];
+                    }
+                    nlist += c;
+                }
+            }
+        }
+    }
+    __syncwarp();
+    // entry j of the warp's list (of its stretch where that is dense): token and key
+    const int items = dense ? t1 - t0 : nlist;
+    auto entry = [&](int j, int& i, uint32_t& k) {
+        i = t0 + (dense ? j : (int)li[j]);
+        k = RESIDENT ? skey[i] : dense ? weight_key(ws[i]) : lk[j];
+        return i >= c0 && i < c1;  // competes
+    };
+    find_digit(1, 10);
+    for (int j = lane; j < items; j += 32) {
+        int i;
+        uint32_t k;
+        if (entry(j, i, k) && (k >> 10) == (prefix >> 10)) atomicAdd(&S.hist[2][k & 1023], 1u);
+    }
+    find_digit(2, 0);
+    // What stays: sinks, recent, keys above prefix; of those equal to it the first `need`.  Where nothing
+    // competes (m == 0) no key may count: cut is out of reach then.
+    const uint32_t cut = m > 0 ? prefix : 0xFFFFFFFFu;
+    int stays = 0, ties = 0;
+    for (int j = lane; j < items; j += 32) {
+        int i;
+        uint32_t k;
+        const bool comp = entry(j, i, k);
+        stays += !comp || k > cut;
+        ties += comp && k == cut;
+    }
+    stays = __reduce_add_sync(0xffffffffu, stays);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) S.wcount[0][warp] = stays, S.wcount[1][warp] = ties;
     __syncthreads();
-    if (tid < 2) {
-        int x = 0;
-        for (int i = 0; i < kSelWarps; ++i) x += S.wcount[tid][i];
-        S.count[tid] = x;
+    // stays and ties before this warp's stretch
+    int bs = __reduce_add_sync(0xffffffffu, lane < warp ? S.wcount[0][lane] : 0);
+    int bt = __reduce_add_sync(0xffffffffu, lane < warp ? S.wcount[1][lane] : 0);
+    if (CLUSTER) {
+        if (warp == W - 1 && lane == 0) S.count[0] = bs + stays, S.count[1] = bt + ties;
+        cl.sync();
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r)
+            if (r < rank) {
+                const int* c = cl.map_shared_rank(&S.count[0], r);
+                bs += c[0], bt += c[1];
+            }
     }
-    cl.sync();
-    int bs = 0, bt = 0;  // stays and ties before this warp's stretch
-    for (int r = 0; r < rank; ++r) {
-        const int* c = cl.map_shared_rank(&S.count[0], r);
-        bs += c[0], bt += c[1];
-    }
-    for (int i = 0; i < warp; ++i) bs += S.wcount[0][i], bt += S.wcount[1][i];
     const int nt = (int)need;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        bool stay = false, tie = false;
-        if (i0 + lane < w1) flags(i0 + lane, stay, tie);
-        const unsigned ms = __ballot_sync(0xffffffffu, stay), mt = __ballot_sync(0xffffffffu, tie), lt = (1u << lane) - 1;
+    const unsigned lt = (1u << lane) - 1;
+    for (int j0 = 0; j0 < items; j0 += 32) {
+        int i = 0;
+        uint32_t k = 0;
+        const bool in = j0 + lane < items, comp = in && entry(j0 + lane, i, k);
+        const bool stay = in && (!comp || k > cut), tie = comp && k == cut;
+        const unsigned ms = __ballot_sync(0xffffffffu, stay), mt = __ballot_sync(0xffffffffu, tie);
         const int tb = bt + __popc(mt & lt);
         if (stay || (tie && tb < nt)) {
             const int pos = bs + __popc(ms & lt) + min(tb, nt);
-            kept[pos] = lo_t + i0 + lane;
-            if (RESIDENT) wo[pos] = weight(i0 + lane);
+            kept[pos] = lo_t + i;
+            if (write_w) wo[pos] = key_weight(k);
         }
         bs += __popc(ms);
         bt += __popc(mt);
     }
-    if (RESIDENT)
-        for (int i = keep + rank * kSelNT + tid; i < a.max_len; i += CS * kSelNT) wo[i] = 0.0f;
-    cl.sync();  // no CTA leaves while its counts are being read
+    if (CLUSTER) cl.sync();  // no CTA leaves while its counts are being read
 }
 
 // The kept weights to the front where the selection did not hold them (chunk
@@ -196,7 +300,7 @@ __global__ void __launch_bounds__(1024) weight_shift_kernel(const WEvictArgs a) 
         if (i < keep) wo[i] = x;
         __syncthreads();
     }
-    for (int i = keep + threadIdx.x; i < a.max_len; i += 1024) wo[i] = 0.0f;
+    zero_tail(wo, keep, a.max_len, threadIdx.x, 1024);
 }
 
 constexpr int kMoveNT = 256;
@@ -282,10 +386,10 @@ __global__ void __launch_bounds__(kMoveNT) weight_move_kernel(const WEvictArgs a
     }
 }
 
-template <bool RESIDENT>
+template <int NT, bool RESIDENT, bool CLUSTER>
 int launch_select(const WEvictArgs& a, long long units, int CS, cudaStream_t st) {
-    const size_t smem = sizeof(SelShared) + (RESIDENT ? (size_t)a.slice * sizeof(float) : 0);
-    if (cudaFuncSetAttribute(weight_select_kernel<RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+    const size_t smem = sizeof(SelShared) + (RESIDENT ? (size_t)a.slice : (size_t)(NT / 32) * a.list_cap) * 6;  // keys, indices
+    if (cudaFuncSetAttribute(weight_select_kernel<NT, RESIDENT, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
         cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
@@ -296,12 +400,12 @@ int launch_select(const WEvictArgs& a, long long units, int CS, cudaStream_t st)
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t lc{};
     lc.gridDim = dim3((unsigned)(units * CS));
-    lc.blockDim = dim3(kSelNT);
+    lc.blockDim = dim3(NT);
     lc.dynamicSmemBytes = smem;
     lc.stream = st;
     lc.attrs = at;
-    lc.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&lc, weight_select_kernel<RESIDENT>, a);
+    lc.numAttrs = CLUSTER ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&lc, weight_select_kernel<NT, RESIDENT, CLUSTER>, a);
     if (e != cudaSuccess) (void)cudaGetLastError();
     return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }
@@ -355,12 +459,21 @@ extern "C" int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, in
          out->table_stride != cache->table_stride || out->num_pages != cache->num_pages))
         return RKV_ERR_INVALID_ARG;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // CTAs of a cluster: slices of about 4096 tokens (8 weights a thread), at most eight
+    // Short lists: a CTA of 512 threads each, four to an SM.  Longer ones: CTAs of 1024 threads, one to an SM,
+    // as many to a list as give every SM one (a second wave costs more than a longer slice).
     int CS = 1;
-    while (CS < 8 && max_len > CS * 4096) CS *= 2;
-    a.slice = (max_len + CS - 1) / CS;
+    const bool small = max_len <= 8192;
+    if (!small)
+        while (CS < kMaxCluster && units * CS * 2 <= 148 && max_len > CS * 4096) CS *= 2;
+    a.slice = ((max_len + CS - 1) / CS + 3) / 4 * 4;
     const bool resident = a.slice <= kSliceMax;
-    rc = resident ? launch_select<true>(a, units, CS, st) : launch_select<false>(a, units, CS, st);
+    a.list_cap = kSliceMax / 32;
+    if (small)
+        rc = launch_select<512, true, false>(a, units, 1, st);
+    else if (resident)
+        rc = CS > 1 ? launch_select<1024, true, true>(a, units, CS, st) : launch_select<1024, true, false>(a, units, 1, st);
+    else
+        rc = CS > 1 ? launch_select<1024, false, true>(a, units, CS, st) : launch_select<1024, false, false>(a, units, 1, st);
     if (rc) return rc;
     cudaError_t e = cudaSuccess;
     if (list == 0) {
@@ -382,7 +495,7 @@ extern "C" int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, in
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
-    if (resident) return RKV_OK;
+    if (resident || a.wo != a.w) return RKV_OK;
     weight_shift_kernel<<<(unsigned)units, 1024, 0, st>>>(a);
     return launched();
 }
