@@ -11,6 +11,8 @@
 // threads, or moved in place.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace cg = cooperative_groups;
@@ -69,10 +71,10 @@ __device__ __forceinline__ void zero_tail(float* dst, int lo, int hi, int thread
 
 // One cluster per (item, KV head); every CTA has a slice of the tokens, every
 // warp a stretch of the slice.  All weights are looked at twice, for the first
-// and the second digit; in the second look each warp lists, in order, the
-// tokens whose first digit is at or above the threshold's (a few per cent of a
-// long cache), and the third digit, the counts and the output work on those
-// lists.  RESIDENT: the slice's keys stay in shared memory, lists always fit,
+// and the second digit; in the second look each warp of a CTA of 1024 threads
+// lists, in order, the tokens whose first digit is at or above the threshold's
+// (a few per cent of a long cache), and the third digit, the counts and the
+// output work on those lists.  RESIDENT: the slice's keys stay in shared memory, lists always fit,
 // and the kept weights are written from there (in place is safe: every slice
 // has been read before the first cluster barrier).  Otherwise the second look
 // reads L2, a list holds keys too, a warp whose list is full looks at its
@@ -82,7 +84,9 @@ template <int NT, bool RESIDENT, bool CLUSTER>
 __global__ void __launch_bounds__(NT) weight_select_kernel(const WEvictArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");
     constexpr int W = NT / 32;
-    constexpr int EB = 8;  // words of 32 tokens whose loads are on their way together
+    constexpr bool LISTS = NT == 1024;  // short lists of tokens are looked at whole
+    static_assert(LISTS || RESIDENT, "without lists the keys are in shared memory");
+    constexpr int EB = 4;  // loads of four weights that a thread has on their way together
     extern __shared__ __align__(16) uint8_t smem[];
     SelShared& S = *reinterpret_cast<SelShared*>(smem);
     uint32_t* skey = reinterpret_cast<uint32_t*>(smem + sizeof(SelShared));  // [slice] keys, or [W][list_cap] of the lists
@@ -128,7 +132,7 @@ __global__ void __launch_bounds__(NT) weight_select_kernel(const WEvictArgs a) {
     uint16_t* li = sidx + (RESIDENT ? t0 : warp * a.list_cap);
     uint32_t* lk = skey + warp * a.list_cap;  // keys of the list (not RESIDENT)
     int nlist = 0;
-    bool dense = !RESIDENT && per > 65536;  // indices of a stretch have 16 bits
+    bool dense = !LISTS || per > 65536;  // indices of a stretch have 16 bits
 
     uint32_t prefix = 0;
     unsigned need = m;  // still to be taken among the keys that share the prefix
@@ -173,54 +177,119 @@ __global__ void __launch_bounds__(NT) weight_select_kernel(const WEvictArgs a) {
         need -= S.above;
     };
 
+    // four weights at a time where the rows are 16-byte aligned (a.slice is a multiple of four)
+    const bool vec4 = ((reinterpret_cast<uintptr_t>(ws)) & 15) == 0;
+    const int qlo = t0 / 4, qfull = t1 / 4, qend = t1 > t0 ? (t1 + 3) / 4 : qfull;
+    auto weights4 = [&](int q, auto vec, float (&x)[4]) {
+        if (decltype(vec)::value) {
+            const float4 y = q < qfull ? *reinterpret_cast<const float4*>(ws + 4 * q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = q < qfull ? ws[4 * q + e] : 0.0f;
+        }
+    };
+    auto tail4 = [&](float (&x)[4]) {  // the quad that the slice ends in
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = 4 * qfull + e < t1 ? ws[4 * qfull + e] : 0.0f;
+    };
     // first digit
-    for (int i0 = t0; i0 < t1; i0 += 32 * EB) {
-        float x[EB];
+    auto count4 = [&](int q, const float (&x)[4]) {
+        const int at = 4 * q;
+        uint32_t k[4];
 #pragma unroll
-        for (int e = 0; e < EB; ++e) {
-            const int i = i0 + e * 32 + lane;
-            x[e] = i < t1 ? ws[i] : 0.0f;
-        }
+        for (int e = 0; e < 4; ++e) k[e] = weight_key(x[e]);
+        if (RESIDENT) *reinterpret_cast<uint4*>(skey + at) = make_uint4(k[0], k[1], k[2], k[3]);
+        if (at >= c0 && at + 4 <= c1) {
 #pragma unroll
-        for (int e = 0; e < EB; ++e) {
-            const int i = i0 + e * 32 + lane;
-            const uint32_t k = weight_key(x[e]);
-            if (RESIDENT && i < t1) skey[i] = k;
-            if (i < t1 && i >= c0 && i < c1) atomicAdd(&S.hist[0][k >> 21], 1u);
+            for (int e = 0; e < 4; ++e) atomicAdd(&S.hist[0][k[e] >> 21], 1u);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (at + e >= c0 && at + e < c1) atomicAdd(&S.hist[0][k[e] >> 21], 1u);
         }
-    }
+    };
+    auto first_digit = [&](auto vec) {
+        for (int q0 = qlo + lane; q0 < qfull; q0 += 32 * EB) {
+            float x[EB][4];
+#pragma unroll
+            for (int u = 0; u < EB; ++u) weights4(q0 + 32 * u, vec, x[u]);
+#pragma unroll
+            for (int u = 0; u < EB; ++u)
+                if (q0 + 32 * u < qfull) count4(q0 + 32 * u, x[u]);
+        }
+        if (qfull < qend && lane == 0) {
+            float x[4];
+            tail4(x);
+            count4(qfull, x);
+        }
+    };
+    if (vec4)
+        first_digit(std::true_type{});
+    else
+        first_digit(std::false_type{});
     find_digit(0, 21);
     if (write_w) zero_tail(wo, keep, a.max_len, ct, cthreads);
-    // second digit, and the lists
-    for (int i0 = t0; i0 < t1; i0 += 32 * EB) {
-        uint32_t k[EB];
-#pragma unroll
-        for (int e = 0; e < EB; ++e) {
-            const int i = i0 + e * 32 + lane;
-            k[e] = i < t1 ? (RESIDENT ? skey[i] : __float_as_uint(ws[i])) : 0u;
+    // Second digit, and the lists: tokens whose key is at or above the prefix.  A lane looks at 16 tokens in a
+    // row, so one scan over the lanes places 512 tokens; what it marks is compared as floats where it comes
+    // from global memory, and a prefix of -infinity's digit or below (3: keys there are no numbers) marks all.
+    const bool all = (prefix >> 21) <= 3u;
+    const float bar = key_weight(prefix);
+    if (!LISTS)
+        for (int i = t0 + lane; i < t1; i += 32) {
+            const uint32_t k = skey[i];
+            if ((k >> 21) == (prefix >> 21) && i >= c0 && i < c1) atomicAdd(&S.hist[1][(k >> 10) & 2047], 1u);
         }
+    for (int g0 = t0; LISTS && g0 < t1; g0 += 512) {
+        const int i0 = g0 + lane * 16;
+        unsigned f = 0;
+        if (i0 + 16 <= t1 && (RESIDENT || vec4)) {
+            uint4 y[4];
 #pragma unroll
-        for (int e = 0; e < EB; ++e) {
-            const int i = i0 + e * 32 + lane;
-            if (!RESIDENT) k[e] = weight_key(__uint_as_float(k[e]));
-            const bool in = i < t1, comp = in && i >= c0 && i < c1;
-            if (comp && (k[e] >> 21) == (prefix >> 21)) atomicAdd(&S.hist[1][(k[e] >> 10) & 2047], 1u);
-            const bool may = comp ? m > 0 && k[e] >= prefix : in;
-            const unsigned mm = __ballot_sync(0xffffffffu, may);
-            if (mm && !dense) {
-                const int c = __popc(mm);
-                if (nlist + c > cap) {
-                    dense = true;
-                } else {
-                    if (may) {
-                        const int at = nlist + __popc(mm & ((1u << lane) - 1));
-                        li[at] = (uint16_t)(i - t0);
-                        if (!RESIDENT) lk[at] = k[e];
-                    }
-                    nlist += c;
-                }
+            for (int u = 0; u < 4; ++u)
+                y[u] = RESIDENT ? *reinterpret_cast<const uint4*>(skey + i0 + 4 * u)
+                                : *reinterpret_cast<const uint4*>(ws + i0 + 4 * u);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint32_t k[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    f |= (RESIDENT ? k[e] >= prefix : __uint_as_float(k[e]) >= bar) ? 1u << (4 * u + e) : 0u;
             }
+        } else {
+            for (int e = 0; e < 16; ++e)
+                if (i0 + e < t1) f |= (RESIDENT ? skey[i0 + e] >= prefix : ws[i0 + e] >= bar) ? 1u << e : 0u;
         }
+        if (all) f = 0xFFFFu;
+        if (m == 0) f = 0;
+        if (i0 < c0 || i0 + 16 > c1)  // sinks and recent tokens are listed, nothing behind the stretch
+            for (int e = 0; e < 16; ++e) {
+                const int i = i0 + e;
+                if (i < c0 || i >= c1 || i >= t1) f = i < t1 ? f | 1u << e : f & ~(1u << e);
+            }
+        const int c = __popc(f);
+        int inc = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        const int total = __shfl_sync(0xffffffffu, inc, 31);
+        if (nlist + total > cap) dense = true;
+        int to = nlist + inc - c;
+        while (f) {
+            const int i = i0 + __ffs(f) - 1;
+            f &= f - 1;
+            const uint32_t k = RESIDENT ? skey[i] : weight_key(ws[i]);
+            if (!dense) {
+                li[to] = (uint16_t)(i - t0);
+                if (!RESIDENT) lk[to] = k;
+                ++to;
+            }
+            if ((k >> 21) == (prefix >> 21) && i >= c0 && i < c1) atomicAdd(&S.hist[1][(k >> 10) & 2047], 1u);
+        }
+        __syncwarp();
+        if (!dense) nlist += total;
     }
     __syncwarp();
     // entry j of the warp's list (of its stretch where that is dense): token and key
@@ -388,7 +457,8 @@ __global__ void __launch_bounds__(kMoveNT) weight_move_kernel(const WEvictArgs a
 
 template <int NT, bool RESIDENT, bool CLUSTER>
 int launch_select(const WEvictArgs& a, long long units, int CS, cudaStream_t st) {
-    const size_t smem = sizeof(SelShared) + (RESIDENT ? (size_t)a.slice : (size_t)(NT / 32) * a.list_cap) * 6;  // keys, indices
+    // keys, and 16-bit indices where there are lists
+    const size_t smem = sizeof(SelShared) + (RESIDENT ? (size_t)a.slice : (size_t)(NT / 32) * a.list_cap) * (NT == 1024 ? 6 : 4);
     if (cudaFuncSetAttribute(weight_select_kernel<NT, RESIDENT, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
         cudaSuccess) {
         (void)cudaGetLastError();
