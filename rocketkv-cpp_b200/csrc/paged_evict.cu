@@ -376,7 +376,7 @@ constexpr int kMoveNT = 256;
 
 // Rows to other pages: 2^lg lanes per row (the row's vectors, rounded up),
 // K and V by the same thread, kCopyRows rows in flight per thread.
-constexpr int kCopyRows = 4;
+constexpr int kCopyRows = 2;
 __global__ void __launch_bounds__(kMoveNT) weight_copy_kernel(const WEvictArgs a, int lg) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int unit = blockIdx.y, hk = unit % a.HK, b = unit / a.HK;
