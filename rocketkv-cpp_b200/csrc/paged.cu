@@ -9,8 +9,6 @@
 // what splits the cache's length over CTAs: each CTA leaves (m, l, o) of its
 // part and a second kernel joins the parts in order.  O = o / l,
 // lse = (m + log2 l) ln 2.
-#include <float.h>
-
 #include "paged.cuh"
 
 namespace rkv {
@@ -152,6 +150,7 @@ template <int GT, int VL>
 __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const DecodeArgs a) {
     constexpr int N = 4;  // floats of a 16-byte vector
     extern __shared__ __align__(16) float sm[];
+    asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled (it waits for this grid)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int D = a.D, VPR = D / N;
     float* qs = sm;                                         // [GT][D]
@@ -379,6 +378,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma_kernel(const Dec
     constexpr float kLift = BF ? 0.0f : 7.0f, kGrow = 8.0f;
     constexpr int RPI = 32 / CH;                              // rows a warp copies per instruction
     extern __shared__ __align__(128) uint8_t smem[];
+    asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled (it waits for this grid)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int D = a.D;
 
@@ -593,11 +593,15 @@ __device__ __forceinline__ float2 join_ml(const float2* ml, int parts, int lane)
     return make_float2(m, warp_sum(l));
 }
 
+constexpr int kJoinTokens = 512;  // tokens whose weights one CTA of the join adds
+constexpr int kJoinAhead = 16;    // parts of a column read before the shares are known
+
 // Joins the parts.  The first o_blocks CTAs take one query head each; the
-// others add the weights of a stretch of tokens of one KV head.
+// others add the weights of a stretch of tokens of one KV head.  Launched
+// while the parts are still being made: what they do not write is read before
+// the wait.
 __global__ void __launch_bounds__(128) paged_join_kernel(const DecodeArgs a) {
     extern __shared__ __align__(16) float sm[];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     long long id = blockIdx.x;
     if (id < a.o_blocks) {
@@ -605,6 +609,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const DecodeArgs a) {
         const int nvis = visible(a, b).nvis;
         const int parts = max(1, (nvis + a.chunk - 1) / a.chunk);
         const float2* ml = a.part_ml + id * a.splits;
+        const float* po = a.part_o + (size_t)id * a.splits * a.D;
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        float x[kJoinAhead];
+#pragma unroll
+        for (int s = 0; s < kJoinAhead; ++s) x[s] = s < parts && tid < a.D ? po[(size_t)s * a.D + tid] : 0.0f;
         if (warp == 0) {
             const float2 j = join_ml(ml, parts, lane);
             const float inv = j.y == 0.0f ? 0.0f : 1.0f / j.y;
@@ -613,10 +622,12 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const DecodeArgs a) {
         }
         __syncthreads();
         for (int d = tid; d < a.D; d += 128) {
-            const float* po = a.part_o + (size_t)id * a.splits * a.D + d;
             float o = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kJoinAhead; ++s)
+                if (s < parts) o = fmaf(d == tid ? x[s] : po[(size_t)s * a.D + d], sm[s], o);
 #pragma unroll 8
-            for (int s = 0; s < parts; ++s) o = fmaf(po[(size_t)s * a.D], sm[s], o);
+            for (int s = kJoinAhead; s < parts; ++s) o = fmaf(po[(size_t)s * a.D + d], sm[s], o);
             a.O[id * a.D + d] = o;
         }
         return;
@@ -627,22 +638,36 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const DecodeArgs a) {
     const int hk = (int)(id % a.HK), b = (int)(id / a.HK);
     const Visible vis = visible(a, b);
     const int parts = max(1, (vis.nvis + a.chunk - 1) / a.chunk);
-    if ((long long)blk * 1024 >= vis.nvis) return;
+    const int v0 = blk * kJoinTokens, v1 = min(vis.nvis, v0 + kJoinTokens);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (v0 >= vis.nvis) return;
     float2* st = reinterpret_cast<float2*>(sm);  // [G] (m, 1 / l)
     for (int g = warp; g < a.G; g += 4) {
         const float2 j = join_ml(a.part_ml + ((size_t)b * a.H + hk * a.G + g) * a.splits, parts, lane);
         if (lane == 0) st[g] = make_float2(j.x, j.y == 0.0f ? 0.0f : 1.0f / j.y);
     }
     __syncthreads();
-    const float* x = a.scores + ((size_t)b * a.H + hk * a.G) * a.vmax;
+    const float* x = a.scores + ((size_t)b * a.H + hk * a.G) * a.vmax + v0;
     float* w = a.weights + ((size_t)b * a.HK + hk) * a.weight_stride;
-    const int v_end = min(vis.nvis, blk * 1024 + 1024);
-    for (int v = blk * 1024 + tid; v < v_end; v += 128) {
-        float s = 0.0f;
-        for (int g = 0; g < a.G; ++g) s = fmaf(exp2f(x[(size_t)g * a.vmax + v] - st[g].x), st[g].y, s);
-        const int t = vis.token(v);
-        w[t] += s;
+    constexpr int U = kJoinTokens / 128;  // tokens of a thread, all on their way together
+    float old[U], sum[U];
+    int t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int v = v0 + tid + u * 128;
+        t[u] = v < v1 ? vis.token(v) : -1;
+        old[u] = t[u] >= 0 ? w[t[u]] : 0.0f;
+        sum[u] = 0.0f;
     }
+    for (int g = 0; g < a.G; ++g) {
+        const float2 j = st[g];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (t[u] >= 0) sum[u] = fmaf(exp2f(x[(size_t)g * a.vmax + tid + u * 128] - j.x), j.y, sum[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (t[u] >= 0) w[t[u]] = old[u] + sum[u];
 }
 
 struct DecodePlan {
@@ -849,7 +874,7 @@ extern "C" int rkv_paged_decode(const void* Q, long long q_item_stride, int num_
     if (weights) a.scores = reinterpret_cast<float*>(ws + p.off_scores);
     const long long blocks = (long long)batch * a.HK * p.ngroups * p.splits;
     a.o_blocks = p.splits > 1 ? (long long)batch * a.H : 0;
-    a.w_blocks = weights ? (int)((vis + 1023) / 1024) : 0;
+    a.w_blocks = weights ? (int)((vis + kJoinTokens - 1) / kJoinTokens) : 0;
     const long long jblocks = a.o_blocks + (long long)batch * a.HK * a.w_blocks;
     if (blocks > 0x7FFFFFFFLL || jblocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
     switch (cache->dtype) {
