@@ -56,7 +56,9 @@ constexpr int kWarps = 4;
 constexpr int kTile = 32;       // tokens a warp takes at a time
 constexpr int kMinChunk = 128;  // visible tokens per CTA at least
 constexpr int kMaxSplits = 1024;
-constexpr long long kTargetCtas = 148 * 8;
+constexpr int kSms = 148;
+constexpr int kMaxWaves = 8;       // of CTAs that a cache is split into at most
+constexpr int kStartTokens = 128;  // what a CTA costs before and behind its tokens, in tokens
 
 struct DecodeArgs {
     PagedView c;
@@ -682,16 +684,45 @@ int head_group(int dtype, int G, int D) {
     return G > 8 && D <= 128 ? 16 : 8;
 }
 
-// Parts of the visible tokens: enough CTAs for a few waves over the GPU, at
-// least kMinChunk tokens each.  Grows with `visible_max`.
-long long decode_parts(int dtype, int H, int HK, int D, long long visible_max, int batch) {
+// CTAs that run at a time: what shared memory (16-bit) or registers (fp32) let the SMs hold.
+int decode_slots(int dtype, int gt, int D) {
+    if (dtype == RKV_F32) return kSms * (gt <= 2 ? 6 : gt == 4 ? 4 : 3);
+    return kSms * (D <= 64 ? 4 : D <= 128 ? 2 : 1);
+}
+long long decode_units(int dtype, int H, int HK, int D, int batch) {
     const int G = H / HK, gt = head_group(dtype, G, D);
-    const long long units = (long long)batch * HK * ((G + gt - 1) / gt);
-    long long parts = units > 0 ? (kTargetCtas + units - 1) / units : 1;
+    return (long long)batch * HK * ((G + gt - 1) / gt);
+}
+// The most parts that decode_parts gives up to visible_max, which it grows with.
+long long decode_parts_bound(int dtype, int H, int HK, int D, long long visible_max, int batch) {
+    const long long units = decode_units(dtype, H, HK, D, batch);
+    const long long slots = decode_slots(dtype, head_group(dtype, H / HK, D), D);
+    long long p = units > 0 ? kMaxWaves * slots / units : 1;
     const long long most = (visible_max + kMinChunk - 1) / kMinChunk;
-    if (parts > most) parts = most;
-    if (parts > kMaxSplits) parts = kMaxSplits;
-    return parts < 1 ? 1 : parts;
+    if (p > most) p = most;
+    if (p > kMaxSplits) p = kMaxSplits;
+    return p < 1 ? 1 : p;
+}
+// Parts of the visible tokens.  With w waves of CTAs as full as they get, a
+// wave takes the time of a part and of about kStartTokens tokens more (start,
+// first reads, join); the w with the least time in all.  Measured: 16 x 3717
+// tokens with weights in 2 / 4 / 6 / 9 / 10 parts (0.9 / 1.7 / 2.6 / 3.9 / 4.3
+// waves) 50 / 54 / 56 / 59 / 62 us; 8 x 131072 in 4 / 9 / 19 / 23 parts (0.9 /
+// 1.9 / 4.1 / 5.0 waves) 686 / 650 / 705 / 654 us.  (One wave with equal
+// stretches of all sequences' tokens, balanced on the device, was slower: 64
+// ragged sequences 247 us against 198; the SMs do not stream at one rate.)
+long long decode_parts(int dtype, int H, int HK, int D, long long visible_max, int batch) {
+    const long long units = decode_units(dtype, H, HK, D, batch), bound = decode_parts_bound(dtype, H, HK, D, visible_max, batch);
+    const long long slots = decode_slots(dtype, head_group(dtype, H / HK, D), D);
+    long long best = 1, best_cost = -1;
+    for (int w = 0; w <= kMaxWaves; ++w) {
+        long long p = w == 0 || units == 0 ? 1 : w * slots / units;
+        if (p < 1) p = 1;
+        if (p > bound) p = bound;
+        const long long cost = ((units * p + slots - 1) / slots) * (kStartTokens + (visible_max + p - 1) / p);
+        if (best_cost < 0 || cost < best_cost) best = p, best_cost = cost;
+    }
+    return best;
 }
 
 DecodePlan decode_plan(int dtype, int H, int HK, int D, long long visible_max, int max_len, int batch, bool weights) {
@@ -707,14 +738,14 @@ DecodePlan decode_plan(int dtype, int H, int HK, int D, long long visible_max, i
     const long long splits = (visible_max + chunk - 1) / chunk;
     p.splits = splits < 1 ? 1 : (int)splits;
     p.vmax = (max_len + 3) / 4 * 4;
-    // the parts before rounding bound the layout: they grow with visible_max, so the workspace of max_len
+    // the bound, not the parts, gives the layout: it grows with visible_max, so the workspace of max_len
     // serves every window
-    const size_t heads = (size_t)batch * H;
+    const size_t heads = (size_t)batch * H, bound = (size_t)decode_parts_bound(dtype, H, HK, D, visible_max, batch);
     size_t off = kWorkspaceHeader;
     p.off_ml = off;
-    off = align_up(off + heads * parts * sizeof(float2), kWorkspaceAlign);
+    off = align_up(off + heads * bound * sizeof(float2), kWorkspaceAlign);
     p.off_o = off;
-    if (parts > 1) off = align_up(off + heads * parts * D * sizeof(float), kWorkspaceAlign);
+    if (bound > 1) off = align_up(off + heads * bound * D * sizeof(float), kWorkspaceAlign);
     p.off_scores = off;
     if (weights) off = align_up(off + heads * (size_t)p.vmax * sizeof(float), kWorkspaceAlign);
     p.bytes = off;
