@@ -145,12 +145,13 @@ size_t simt_smem(int GT, int D) { return sizeof(float) * ((size_t)GT * D + kWarp
 
 // fp32 caches, fused multiply-adds on the CUDA cores: one CTA per (item, KV
 // head, group of up to GT query heads, part).  Every warp takes 32 tokens at a
-// time on its own: 8 lanes form the scores of a token (four tokens per lane
-// and pass), a lane per token forms the weights, and LR lanes of 16 bytes add
+// time on its own: 8 lanes form the scores of a token, a lane per token forms the weights, and LR lanes of 16 bytes add
 // up a V row.  VL: 16-byte vectors of a V row per lane.
 template <int GT, int VL>
 __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const DecodeArgs a) {
-    constexpr int N = 4;  // floats of a 16-byte vector
+    constexpr int N = 4;                // floats of a 16-byte vector
+    constexpr int J = GT <= 2 ? 8 : 4;  // tokens whose scores a lane forms together
+    constexpr int UV = GT <= 2 ? 16 : 4;  // V rows a lane has on their way together
     extern __shared__ __align__(16) float sm[];
     asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled (it waits for this grid)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -200,22 +201,23 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const De
         const int v = t0 + lane;
         const long long off = v < v1 ? paged_offset(a.c, b, hk, vis.token(v)) : -1;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            long long o[4];
-            float s[4][GT];
+        for (int pass = 0; pass < 8 / J; ++pass) {
+            long long o[J];
+            float s[J][GT];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                o[j] = __shfl_sync(0xffffffffu, off, half * 16 + j * 4 + (lane >> 3));
+            for (int j = 0; j < J; ++j) {
+                o[j] = __shfl_sync(0xffffffffu, off, (pass * J + j) * 4 + (lane >> 3));
 #pragma unroll
                 for (int g = 0; g < GT; ++g) s[j][g] = 0.0f;
             }
+#pragma unroll 2
             for (int vec = lane & 7; vec < VPR; vec += 8) {
-                float4 x[4];
+                float4 x[J];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < J; ++j)
                     x[j] = o[j] >= 0 ? load16(a.c.K + o[j] + vec * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < J; ++j) {
                     const float f[N] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
                     for (int g = 0; g < GT; ++g)
@@ -224,14 +226,14 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const De
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < J; ++j)
 #pragma unroll
                 for (int g = 0; g < GT; ++g) {
                     float x = s[j][g];
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
                     x += __shfl_xor_sync(0xffffffffu, x, 2);
                     x += __shfl_xor_sync(0xffffffffu, x, 4);
-                    if ((lane & 7) == g) pw[g * kTile + half * 16 + j * 4 + (lane >> 3)] = x;
+                    if ((lane & 7) == g) pw[g * kTile + (pass * J + j) * 4 + (lane >> 3)] = x;
                 }
         }
         __syncwarp();
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const De
                 for (int e = 0; e < N; ++e) acc[i][e][g] *= corr;
         }
         __syncwarp();
-#pragma unroll 4
+#pragma unroll UV
         for (int s0 = 0; s0 < kTile; s0 += TPS) {
             const int t = s0 + tsub;
             const long long o = __shfl_sync(0xffffffffu, off, t);
@@ -686,7 +688,7 @@ int head_group(int dtype, int G, int D) {
 
 // CTAs that run at a time: what shared memory (16-bit) or registers (fp32) let the SMs hold.
 int decode_slots(int dtype, int gt, int D) {
-    if (dtype == RKV_F32) return kSms * (gt <= 2 ? 6 : gt == 4 ? 4 : 3);
+    if (dtype == RKV_F32) return kSms * (gt <= 4 ? 4 : 3);
     return kSms * (D <= 64 ? 4 : D <= 128 ? 2 : 1);
 }
 long long decode_units(int dtype, int H, int HK, int D, int batch) {
