@@ -52,8 +52,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
 // ---------------------------------------------------------------------------
 // decode
 // ---------------------------------------------------------------------------
-constexpr int kWarps = 4;
-constexpr int kTile = 32;       // tokens a warp takes at a time
+constexpr int kTile = 32;       // parts are multiples of this many tokens
 constexpr int kMinChunk = 128;  // visible tokens per CTA at least
 constexpr int kMaxSplits = 1024;
 constexpr int kSms = 148;
@@ -96,8 +95,6 @@ __device__ __forceinline__ Visible visible(const DecodeArgs& a, int b) {
     return s;
 }
 
-__device__ __forceinline__ float4 load16(const uint8_t* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
-
 __device__ __forceinline__ float warp_max(float x) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -113,18 +110,19 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 
 // Joins the warps' (m, l, o) of ng heads from shared memory (ms, ls [warps][rows], os [warps][rows][pitch])
 // and writes the part, or the output where there is one part.
+template <int W>
 __device__ __forceinline__ void merge_warps(const DecodeArgs& a, size_t head0, int ng, int split, const float* ms,
                                             const float* ls, const float* os, int rows, int pitch) {
     const int D = a.D;
-    for (int i = threadIdx.x; i < ng * D; i += kWarps * 32) {
+    for (int i = threadIdx.x; i < ng * D; i += W * 32) {
         const int g = i / D, d = i - g * D;
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ms[w * rows + g]);
+        for (int w = 0; w < W; ++w) mm = fmaxf(mm, ms[w * rows + g]);
         const float mf = finite_max(mm);
         float ll = 0.0f, oo = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float c = exp2f(ms[w * rows + g] - mf);
             ll = fmaf(ls[w * rows + g], c, ll);
             oo = fmaf(os[(w * rows + g) * pitch + d], c, oo);
@@ -141,173 +139,27 @@ __device__ __forceinline__ void merge_warps(const DecodeArgs& a, size_t head0, i
     }
 }
 
-size_t simt_smem(int GT, int D) { return sizeof(float) * ((size_t)GT * D + kWarps * GT * kTile + 2 * kWarps * GT + (size_t)kWarps * GT * D); }
-
-// fp32 caches, fused multiply-adds on the CUDA cores: one CTA per (item, KV
-// head, group of up to GT query heads, part).  Every warp takes 32 tokens at a
-// time on its own: 8 lanes form the scores of a token, a lane per token forms the weights, and LR lanes of 16 bytes add
-// up a V row.  VL: 16-byte vectors of a V row per lane.
-template <int GT, int VL>
-__global__ void __launch_bounds__(kWarps * 32) paged_decode_simt_kernel(const DecodeArgs a) {
-    constexpr int N = 4;                // floats of a 16-byte vector
-    constexpr int J = GT <= 2 ? 8 : 4;  // tokens whose scores a lane forms together
-    constexpr int UV = GT <= 2 ? 16 : 4;  // V rows a lane has on their way together
-    extern __shared__ __align__(16) float sm[];
-    asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled (it waits for this grid)
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int D = a.D, VPR = D / N;
-    float* qs = sm;                                         // [GT][D]
-    float* pw = qs + GT * D + warp * GT * kTile;            // [GT][32] of this warp
-    float* ms = qs + GT * D + kWarps * GT * kTile;          // [warps][GT]
-    float* ls = ms + kWarps * GT;                           // [warps][GT]
-    float* os = ls + kWarps * GT;                           // [warps][GT][D]
-
-    long long id = blockIdx.x;
-    const int split = (int)(id % a.splits);
-    id /= a.splits;
-    const int grp = (int)(id % a.ngroups);
-    id /= a.ngroups;
-    const int hk = (int)(id % a.HK), b = (int)(id / a.HK);
-    const Visible vis = visible(a, b);
-    const long long v_lo = (long long)split * a.chunk;
-    if (split > 0 && v_lo >= vis.nvis) return;  // the join takes the parts that hold tokens
-    const int v0 = (int)v_lo, v1 = (int)min((long long)vis.nvis, v_lo + a.chunk);
-    const int h0 = hk * a.G + grp * GT, ng = min(GT, a.G - grp * GT);
-
-    const float* q = reinterpret_cast<const float*>(a.Q + (size_t)b * a.q_stride);
-    for (int i = tid; i < GT * D; i += kWarps * 32) {
-        const int g = i / D;
-        qs[i] = g < ng ? q[(h0 + g) * D + (i - g * D)] * a.scale2 : 0.0f;
-    }
-    __syncthreads();
-
-    int LR = 1;
-    while (LR < VPR && LR < 32) LR <<= 1;
-    const int TPS = 32 / LR, vl0 = lane & (LR - 1), tsub = lane / LR;
-    float m[GT], l[GT], acc[VL][N][GT];
-#pragma unroll
-    for (int g = 0; g < GT; ++g) {
-        m[g] = -INFINITY;
-        l[g] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < VL; ++i)
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-#pragma unroll
-            for (int g = 0; g < GT; ++g) acc[i][e][g] = 0.0f;
-
-    for (int t0 = v0 + warp * kTile; t0 < v1; t0 += kWarps * kTile) {
-        const int v = t0 + lane;
-        const long long off = v < v1 ? paged_offset(a.c, b, hk, vis.token(v)) : -1;
-#pragma unroll
-        for (int pass = 0; pass < 8 / J; ++pass) {
-            long long o[J];
-            float s[J][GT];
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                o[j] = __shfl_sync(0xffffffffu, off, (pass * J + j) * 4 + (lane >> 3));
-#pragma unroll
-                for (int g = 0; g < GT; ++g) s[j][g] = 0.0f;
-            }
-#pragma unroll 2
-            for (int vec = lane & 7; vec < VPR; vec += 8) {
-                float4 x[J];
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-                    x[j] = o[j] >= 0 ? load16(a.c.K + o[j] + vec * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    const float f[N] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-                    for (int g = 0; g < GT; ++g)
-#pragma unroll
-                        for (int e = 0; e < N; ++e) s[j][g] = fmaf(f[e], qs[g * D + vec * N + e], s[j][g]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-#pragma unroll
-                for (int g = 0; g < GT; ++g) {
-                    float x = s[j][g];
-                    x += __shfl_xor_sync(0xffffffffu, x, 1);
-                    x += __shfl_xor_sync(0xffffffffu, x, 2);
-                    x += __shfl_xor_sync(0xffffffffu, x, 4);
-                    if ((lane & 7) == g) pw[g * kTile + (pass * J + j) * 4 + (lane >> 3)] = x;
-                }
-        }
-        __syncwarp();
-#pragma unroll
-        for (int g = 0; g < GT; ++g) {
-            const float x = off >= 0 ? pw[g * kTile + lane] : -INFINITY;
-            if (a.scores && v < v1 && g < ng) a.scores[((size_t)b * a.H + h0 + g) * a.vmax + v] = x;
-            const float mn = fmaxf(m[g], warp_max(x)), mf = finite_max(mn);
-            const float corr = exp2f(m[g] - mf), p = exp2f(x - mf);
-            m[g] = mn;
-            l[g] = l[g] * corr + p;
-            pw[g * kTile + lane] = p;
-#pragma unroll
-            for (int i = 0; i < VL; ++i)
-#pragma unroll
-                for (int e = 0; e < N; ++e) acc[i][e][g] *= corr;
-        }
-        __syncwarp();
-#pragma unroll UV
-        for (int s0 = 0; s0 < kTile; s0 += TPS) {
-            const int t = s0 + tsub;
-            const long long o = __shfl_sync(0xffffffffu, off, t);
-#pragma unroll
-            for (int i = 0; i < VL; ++i) {
-                const int vec = vl0 + i * 32;
-                const float4 x = o >= 0 && vec < VPR ? load16(a.c.V + o + vec * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const float f[N] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int g = 0; g < GT; ++g) {
-                    const float p = pw[g * kTile + t];
-#pragma unroll
-                    for (int e = 0; e < N; ++e) acc[i][e][g] = fmaf(p, f[e], acc[i][e][g]);
-                }
-            }
-        }
-        __syncwarp();
-    }
-    // the token groups of a warp, then the warps
-#pragma unroll
-    for (int g = 0; g < GT; ++g) {
-        l[g] = warp_sum(l[g]);
-        if (lane == 0) {
-            ms[warp * GT + g] = m[g];
-            ls[warp * GT + g] = l[g];
-        }
-#pragma unroll
-        for (int i = 0; i < VL; ++i)
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                float x = acc[i][e][g];
-                for (int o = LR; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                const int vec = vl0 + i * 32;
-                if (tsub == 0 && vec < VPR) os[(warp * GT + g) * D + vec * N + e] = x;
-            }
-    }
-    __syncthreads();
-    merge_warps(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, GT, D);
-}
-
 // ---------------------------------------------------------------------------
-// 16-bit caches: matrix instructions on tiles of 16 tokens
+// The decode kernel: matrix instructions on tiles of 16 tokens
 // ---------------------------------------------------------------------------
-constexpr int kKeys = 16;     // tokens of a tile
-constexpr int kMmaStages = 3; // tiles of a warp in shared memory, one in use and the others on their way
+constexpr int kKeys = 16;  // tokens of a tile
 
-template <bool BF>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if (BF)
+enum { KIND_F16 = 0, KIND_BF16 = 1, KIND_F32 = 2 };
+
+template <int KIND>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (KIND == KIND_BF16)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                      "{%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
+    else if (KIND == KIND_F16)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                      "{%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -324,6 +176,11 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                      : "r"(addr)
                      : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -355,36 +212,67 @@ __device__ __forceinline__ uint32_t split2(float& x, float& y) {
     y -= f.y;
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-
-__host__ __device__ constexpr int mma_stage_bytes(int DP) { return kKeys * DP * 2 * 2; }  // K rows, V rows
-constexpr size_t mma_smem(int DP, int NT) {
-    const size_t ring = (size_t)kWarps * kMmaStages * mma_stage_bytes(DP);
-    const size_t merge = sizeof(float) * kWarps * 8 * NT * (2 + DP + 4);
-    return ring > merge ? ring : merge;
+// What a tf32 operand (the top 19 bits) leaves of a value.
+__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) {
+    return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u));
 }
 
+// Shapes of the kernel: DP columns (dim_head rounded up), 8 NT query heads, W warps, ring slots of a warp,
+// CTAs of an SM.
+template <int KIND_, int DP_, int NT_>
+struct Shape {
+    static constexpr int KIND = KIND_, DP = DP_, NT = NT_;
+    static constexpr int SIZE = KIND == KIND_F32 ? 4 : 2;
+    static constexpr int ROW = DP * SIZE;             // bytes of a row in shared memory
+    static constexpr int SLOT = kKeys * ROW;          // 16 rows of K or of V
+    static constexpr int W = ROW > 512 ? 4 : 8;
+    static constexpr int SLOTS = ROW > 128 ? 3 : 5;   // odd: K and V take the slots in turn
+    static constexpr int CTAS = ROW > 256 ? 1 : 2;
+    static constexpr bool QS = KIND == KIND_F32 || NT > 1;  // q in shared memory, else in registers
+    static constexpr int QBYTES = !QS ? 0 : KIND == KIND_F32 ? DP / 8 * NT * 512 : DP / 16 * NT * 256;
+    static constexpr int RING = W * SLOTS * SLOT;
+    static constexpr int PITCH = DP + 4;
+    static constexpr int MERGE = (int)sizeof(float) * W * 8 * NT * (2 + PITCH);
+    static constexpr int SMEM = QBYTES + (RING > MERGE ? RING : MERGE);
+};
+
 // One CTA per (item, KV head, group of up to 8 NT query heads, part); every
-// warp takes tiles of 16 tokens on its own.  The tile's K and V rows arrive in
-// the warp's ring by 16-byte asynchronous copies, rows of DP columns with the
-// 16-byte chunk c of row r at c ^ (r % 8), so that the eight rows of a matrix
-// load lie in different banks.  Scores: K (16 tokens x 16 columns per step) by
-// q^T (8 heads); output: V^T (16 columns x 16 tokens) by P (8 heads), whose
-// fragment is the transpose of the scores'.  P keeps fp32's precision: it
-// enters as a sum of 16-bit parts (three for bf16, two for fp16), one product
-// each, which costs nothing here, since the kernel is bound by its reads.
+// warp takes tiles of 16 tokens on its own.  K rows and V rows arrive in turn
+// in the warp's ring by 16-byte asynchronous copies, SLOTS - 1 of them ahead;
+// masked rows and the columns behind dim_head arrive as zeros.
+//
+// Scores: K (16 tokens x 16 or 8 columns per step) by q^T (8 heads); output:
+// V^T (16 columns x 16 or 8 tokens) by P (8 heads).  The 16-byte chunks of a
+// row are stored at other places of the row (swizzled by the row's number), so
+// that what one matrix load or one 128-bit load of eight lanes touches lies in
+// different banks.
+//
+// 16 bit: fragments by ldmatrix; P's fragment is the transpose of the scores'.
+// P keeps fp32's precision: it enters as a sum of 16-bit parts (three for
+// bf16, two for fp16), one product each, which costs little here, since the
+// kernel is bound by its reads.  fp32: tf32 products, each operand as its top
+// 19 bits and the rest, three products (hi hi + lo hi + hi lo); the columns a
+// lane needs for four steps are one 16-byte chunk, since the order in which a
+// product sums its columns (or tokens) is free.
+//
 // A row's maximum is raised only when a score exceeds it by more than 2^8
-// (both types hold P then); fp16's P is kept 2^7 larger, away from the type's
+// (all types hold P then); fp16's P is kept 2^7 larger, away from the type's
 // smallest numbers.
-template <bool BF, int DP, int NT>
-__global__ void __launch_bounds__(kWarps * 32) paged_decode_mma_kernel(const DecodeArgs a) {
-    constexpr int kStage = mma_stage_bytes(DP), CH = DP / 8;  // 16-byte chunks of a row
+template <typename S>
+__global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const DecodeArgs a) {
+    constexpr int KIND = S::KIND, DP = S::DP, NT = S::NT, W = S::W, SLOTS = S::SLOTS;
+    constexpr bool F32 = KIND == KIND_F32, BF = KIND == KIND_BF16;
+    constexpr int CH = S::ROW / 16;                       // 16-byte chunks of a row
+    constexpr int LPR = CH < 32 ? CH : 32;                // lanes that copy a row
+    constexpr int RPI = 32 / LPR, CPL = CH / LPR;         // rows per copy instruction, chunks of a lane
+    constexpr int LEAD = (SLOTS - 1) / 2;                 // tiles that the copies are ahead
+    constexpr int MT = DP / 16;                           // output tiles of 16 columns
     constexpr int PARTS = BF ? 3 : 2;
-    constexpr float kLift = BF ? 0.0f : 7.0f, kGrow = 8.0f;
-    constexpr int RPI = 32 / CH;                              // rows a warp copies per instruction
+    constexpr float kLift = KIND == KIND_F16 ? 7.0f : 0.0f, kGrow = 8.0f;
     extern __shared__ __align__(128) uint8_t smem[];
     asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled (it waits for this grid)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int D = a.D;
+    const int D = a.D, chunks = D * S::SIZE / 16;
 
     long long id = blockIdx.x;
     const int split = (int)(id % a.splits);
@@ -398,13 +286,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma_kernel(const Dec
     const int v0 = (int)v_lo, v1 = (int)min((long long)vis.nvis, v_lo + a.chunk);
     const int h0 = hk * a.G + grp * 8 * NT, ng = min(8 * NT, a.G - grp * 8 * NT);
 
-    uint8_t* ring = smem + warp * kMmaStages * kStage;
-    const uint32_t ring_u = smem_u32(ring);
-    if (D < DP)  // the columns behind D count as zeros and are never copied
-        for (int e = lane; e < kMmaStages * 2 * kKeys * CH; e += 32) {
-            const int row = e / CH, c = e % CH;
-            if ((c ^ (row & 7)) >= D / 8) *reinterpret_cast<uint4*>(ring + row * DP * 2 + c * 16) = make_uint4(0, 0, 0, 0);
-        }
+    uint8_t* qsm = smem;
+    const uint32_t ring = smem_u32(smem + S::QBYTES) + warp * SLOTS * S::SLOT;
 
     // the tile's tokens: lane i (and i + 16) has the row of token i
     const int ntiles = v1 > v0 ? (v1 - v0 + kKeys - 1) / kKeys : 0;
@@ -412,87 +295,143 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma_kernel(const Dec
         const int v = v0 + tile * kKeys + (lane & 15);
         return tile < ntiles && v < v1 ? paged_offset(a.c, b, hk, vis.token(v)) : -1;
     };
-    const int cchunk = lane % CH, crow = lane / CH;
-    auto fetch = [&](int slot, long long off) {
+    const int clane = lane % LPR, crow = lane / LPR;
+    auto fetch = [&](const uint8_t* base, bool isv, int slot, long long off) {
 #pragma unroll
         for (int i = 0; i < kKeys / RPI; ++i) {
             const int r = i * RPI + crow;
             const long long o = __shfl_sync(0xffffffffu, off, r);
-            if (cchunk < D / 8) {
-                const uint32_t dst = ring_u + slot * kStage + r * DP * 2 + ((cchunk ^ (r & 7)) << 4);
-                copy16(dst, o >= 0 ? a.c.K + o + cchunk * 16 : a.Q, o >= 0);
-                copy16(dst + kKeys * DP * 2, o >= 0 ? a.c.V + o + cchunk * 16 : a.Q, o >= 0);
+            const int swz = !F32 || isv ? r & 7 : (r & 1) << 2;
+#pragma unroll
+            for (int c0 = 0; c0 < CPL; ++c0) {
+                const int c = c0 * LPR + clane;
+                const bool real = o >= 0 && c < chunks;
+                copy16(ring + slot * S::SLOT + r * S::ROW + ((c ^ swz) << 4), real ? base + o + c * 16 : a.Q, real);
             }
         }
     };
-    long long off_next = row_of(warp);
-    uint32_t real[kMmaStages];  // which of the tile's tokens there are
+    // copies are numbered K0 V0 K1 V1 ...: number f is in slot f % SLOTS
+    long long off_next = row_of(warp), off = -1;
+    uint32_t real[LEAD];  // which tokens there are, of this tile and the next
 #pragma unroll
-    for (int s = 0; s < kMmaStages - 1; ++s) {
-        const long long off = off_next;
-        off_next = row_of(warp + (s + 1) * kWarps);
-        real[s] = __ballot_sync(0xffffffffu, off >= 0);
-        if (warp + s * kWarps < ntiles) fetch(s, off);
+    for (int i = 0; i < LEAD; ++i) {
+        const int tile = warp + i * W;
+        off = off_next;
+        off_next = row_of(tile + W);
+        real[i] = __ballot_sync(0xffffffffu, off >= 0);
+        if (tile < ntiles) fetch(a.c.K, false, 2 * i, off);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (tile < ntiles) fetch(a.c.V, true, 2 * i + 1, off);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
-    // q^T fragments: columns 2 t, 2 t + 1 (and + 8) of head g
-    uint32_t q[NT][DP / 16][2];
+    // q^T fragments
     const uint8_t* qb = a.Q + (size_t)b * a.q_stride;
+    uint32_t q[S::QS ? 1 : NT][S::QS ? 1 : DP / 16][2];
+    if (F32) {
+        // step (blk, e): columns 32 blk + 4 t + e and 16 further of head g, and their rests
+        for (int i = warp; i < DP / 8 * NT; i += W) {
+            const int n = i / (DP / 8), st = i % (DP / 8), d = (st >> 2) * 32 + 4 * t + (st & 3);
+            const bool have = n * 8 + g < ng;
+            const float* row = reinterpret_cast<const float*>(qb) + (size_t)(h0 + n * 8 + g) * D;
+            const uint32_t b0 = have && d < D ? __float_as_uint(__ldg(row + d)) : 0u;
+            const uint32_t b1 = have && d + 16 < D ? __float_as_uint(__ldg(row + d + 16)) : 0u;
+            reinterpret_cast<uint4*>(qsm)[i * 32 + lane] = make_uint4(b0, b1, tf32_rest(b0), tf32_rest(b1));
+        }
+        __syncthreads();
+    } else {
+        // step k: columns 16 k + 2 t, 2 t + 1 (and + 8) of head g
+        auto frag = [&](int n, int k, int e) {
+            const int d = k * 16 + e * 8 + 2 * t;
+            return n * 8 + g < ng && d < D
+                       ? __ldg(reinterpret_cast<const uint32_t*>(qb + ((size_t)(h0 + n * 8 + g) * D + d) * 2))
+                       : 0u;
+        };
+        if (S::QS) {
+            for (int i = warp; i < DP / 16 * NT; i += W)
+                reinterpret_cast<uint2*>(qsm)[i * 32 + lane] = make_uint2(frag(i % NT, i / NT, 0), frag(i % NT, i / NT, 1));
+            __syncthreads();
+        } else {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int d = k * 16 + e * 8 + 2 * t;
-                q[n][k][e] = n * 8 + g < ng && d < D
-                                 ? __ldg(reinterpret_cast<const uint32_t*>(qb + ((size_t)(h0 + n * 8 + g) * D + d) * 2))
-                                 : 0u;
-            }
-    float m[NT][2], l[NT][2], o[NT][DP / 16][4];
+                for (int k = 0; k < DP / 16; ++k) {
+                    q[S::QS ? 0 : n][S::QS ? 0 : k][0] = frag(n, k, 0);
+                    q[S::QS ? 0 : n][S::QS ? 0 : k][1] = frag(n, k, 1);
+                }
+        }
+    }
+    float m[NT][2], l[NT][2], o[NT][MT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         m[n][0] = m[n][1] = -INFINITY;
         l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
+        for (int k = 0; k < MT; ++k)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][k][e] = 0.0f;
     }
-    // matrix loads: lane i gives the address of row i % 8 of block i / 8
-    const int kr = lane & 15, kc = lane >> 4;                       // K: rows 0-15, column halves
-    const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;  // V^T: column halves first, then rows
 
-    int slot = 0;
-    for (int tile = warp; tile < ntiles; tile += kWarps) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kMmaStages - 2) : "memory");
+    int slot = 0;  // of this tile's K; its V is in the next
+    auto after = [&](int s, int k) { return s + k >= SLOTS ? s + k - SLOTS : s + k; };
+    for (int tile = warp; tile < ntiles; tile += W) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 2) : "memory");
         __syncwarp();
         const uint32_t here = real[0];
 #pragma unroll
-        for (int s = 0; s + 1 < kMmaStages - 1; ++s) real[s] = real[s + 1];
-        {
-            const int ahead = tile + (kMmaStages - 1) * kWarps;
-            const long long off = off_next;
-            off_next = row_of(ahead + kWarps);
-            real[kMmaStages - 2] = __ballot_sync(0xffffffffu, off >= 0);
-            int fs = slot + kMmaStages - 1;
-            if (fs >= kMmaStages) fs -= kMmaStages;
-            if (ahead < ntiles) fetch(fs, off);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-        const uint32_t kb = ring_u + slot * kStage, vb = kb + kKeys * DP * 2;
+        for (int i = 0; i + 1 < LEAD; ++i) real[i] = real[i + 1];
+        const bool more = tile + LEAD * W < ntiles;
+        off = off_next;
+        off_next = row_of(tile + (LEAD + 1) * W);
+        real[LEAD - 1] = __ballot_sync(0xffffffffu, off >= 0);
+        if (more) fetch(a.c.K, false, after(slot, SLOTS - 1), off);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+
+        const uint32_t kb = ring + slot * S::SLOT;
         float s[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+        if (F32) {
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            uint32_t f[4];
-            ldmatrix4<false>(f, kb + kr * DP * 2 + (((2 * k + kc) ^ (kr & 7)) << 4));
+            for (int blk = 0; blk < DP / 32; ++blk) {
+                // rows g and g + 8 (one parity), chunks t and t + 4 of the 32 columns
+                const int c = blk * 8 + t, swz = (g & 1) << 2;
+                const uint4 x0 = lds16(kb + g * S::ROW + ((c ^ swz) << 4)), x1 = lds16(kb + (g + 8) * S::ROW + ((c ^ swz) << 4));
+                const uint4 x2 = lds16(kb + g * S::ROW + (((c + 4) ^ swz) << 4)),
+                            x3 = lds16(kb + (g + 8) * S::ROW + (((c + 4) ^ swz) << 4));
+                const uint32_t k0[4] = {x0.x, x0.y, x0.z, x0.w}, k1[4] = {x1.x, x1.y, x1.z, x1.w};
+                const uint32_t k2[4] = {x2.x, x2.y, x2.z, x2.w}, k3[4] = {x3.x, x3.y, x3.z, x3.w};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<BF>(s[n], f, q[n][k][0], q[n][k][1]);
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t hi[4] = {k0[e], k1[e], k2[e], k3[e]};
+                    const uint32_t lo[4] = {tf32_rest(k0[e]), tf32_rest(k1[e]), tf32_rest(k2[e]), tf32_rest(k3[e])};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint4 qq = reinterpret_cast<const uint4*>(qsm)[(n * (DP / 8) + blk * 4 + e) * 32 + lane];
+                        mma16<KIND>(s[n], hi, qq.z, qq.w);
+                        mma16<KIND>(s[n], lo, qq.x, qq.y);
+                        mma16<KIND>(s[n], hi, qq.x, qq.y);
+                    }
+                }
+            }
+        } else {
+            const int kr = lane & 15, kc = lane >> 4;  // lane i addresses row i % 8 of block i / 8: rows, then column halves
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                uint32_t f[4];
+                ldmatrix4<false>(f, kb + kr * S::ROW + (((2 * k + kc) ^ (kr & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if (S::QS) {
+                        const uint2 qq = reinterpret_cast<const uint2*>(qsm)[(k * NT + n) * 32 + lane];
+                        mma16<KIND>(s[n], f, qq.x, qq.y);
+                    } else {
+                        mma16<KIND>(s[n], f, q[S::QS ? 0 : n][S::QS ? 0 : k][0], q[S::QS ? 0 : n][S::QS ? 0 : k][1]);
+                    }
+                }
+            }
         }
         // scores of tokens g and g + 8, heads 2 t and 2 t + 1
         const bool r0 = (here >> g) & 1, r1 = (here >> (g + 8)) & 1;
@@ -526,42 +465,86 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma_kernel(const Dec
                     m[n][e] = x;
                     l[n][e] *= corr;
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
+                    for (int k = 0; k < MT; ++k) {
                         o[n][k][e] *= corr;
                         o[n][k][e + 2] *= corr;
                     }
                 }
         }
-        uint32_t p[NT][PARTS][2];
+        // P's fragments: 16 bit [part][tokens 0-7, 8-15], fp32 [tokens 0-7, 8-15][token 2 t, 2 t + 1]
+        uint32_t p[NT][F32 ? 2 : PARTS][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const float m0 = finite_max(m[n][0]) - kLift, m1 = finite_max(m[n][1]) - kLift;
             float x[4] = {ex2(s[n][0] - m0), ex2(s[n][1] - m1), ex2(s[n][2] - m0), ex2(s[n][3] - m1)};
             l[n][0] += x[0] + x[2];
             l[n][1] += x[1] + x[3];
+            if (F32) {
 #pragma unroll
-            for (int i = 0; i < PARTS; ++i) {
-                p[n][i][0] = transpose8x8(split2<BF>(x[0], x[1]));
-                p[n][i][1] = transpose8x8(split2<BF>(x[2], x[3]));
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int from = (2 * t + e) * 4 + (g >> 1);  // the lane with token 2 t + e, head g
+                        const float y0 = __shfl_sync(0xffffffffu, x[2 * h], from), y1 = __shfl_sync(0xffffffffu, x[2 * h + 1], from);
+                        p[n][h][e] = __float_as_uint((g & 1) ? y1 : y0);
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PARTS; ++i) {
+                    p[n][i][0] = transpose8x8(split2<BF>(x[0], x[1]));
+                    p[n][i][1] = transpose8x8(split2<BF>(x[2], x[3]));
+                }
             }
         }
+        asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 2) : "memory");
+        __syncwarp();
+        if (more) fetch(a.c.V, true, slot, off);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+
+        const uint32_t vb = ring + after(slot, 1) * S::SLOT;
+        if (F32) {
+            // output tile 2 j + h: rows g and g + 8 are columns 4 (g + 8 j) + 2 h and + 1
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            uint32_t f[4];
-            ldmatrix4<true>(f, vb + vr * DP * 2 + (((2 * k + vc) ^ (vr & 7)) << 4));
+            for (int h8 = 0; h8 < 2; ++h8) {
+                const int row0 = h8 * 8 + 2 * t;  // this lane's tokens: row0, row0 + 1
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                for (int j = 0; j < DP / 32; ++j) {
+                    const int c = g + 8 * j;
+                    const uint4 u = lds16(vb + row0 * S::ROW + ((c ^ (row0 & 7)) << 4));
+                    const uint4 w = lds16(vb + (row0 + 1) * S::ROW + ((c ^ ((row0 + 1) & 7)) << 4));
 #pragma unroll
-                for (int i = 0; i < PARTS; ++i) mma16816<BF>(o[n][k], f, p[n][i][0], p[n][i][1]);
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t hi[4] = {h ? u.z : u.x, h ? u.w : u.y, h ? w.z : w.x, h ? w.w : w.y};
+                        const uint32_t lo[4] = {tf32_rest(hi[0]), tf32_rest(hi[1]), tf32_rest(hi[2]), tf32_rest(hi[3])};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma16<KIND>(o[n][2 * j + h], hi, tf32_rest(p[n][h8][0]), tf32_rest(p[n][h8][1]));
+                            mma16<KIND>(o[n][2 * j + h], lo, p[n][h8][0], p[n][h8][1]);
+                            mma16<KIND>(o[n][2 * j + h], hi, p[n][h8][0], p[n][h8][1]);
+                        }
+                    }
+                }
+            }
+        } else {
+            const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;  // blocks: column halves first, then rows
+#pragma unroll
+            for (int k = 0; k < MT; ++k) {
+                uint32_t f[4];
+                ldmatrix4<true>(f, vb + vr * S::ROW + (((2 * k + vc) ^ (vr & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < PARTS; ++i) mma16<KIND>(o[n][k], f, p[n][F32 ? 0 : i][0], p[n][F32 ? 0 : i][1]);
+            }
         }
-        if (++slot == kMmaStages) slot = 0;
+        slot = after(slot, 2);
     }
     // the warps' (m, l, o) meet in shared memory, over the ring
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    float* ms = reinterpret_cast<float*>(smem);  // [warps][8 NT]
-    float* ls = ms + kWarps * 8 * NT;
-    float* os = ls + kWarps * 8 * NT;            // [warps][8 NT][DP + 4]
+    float* ms = reinterpret_cast<float*>(smem + S::QBYTES);  // [warps][8 NT]
+    float* ls = ms + W * 8 * NT;
+    float* os = ls + W * 8 * NT;                             // [warps][8 NT][PITCH]
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -575,13 +558,14 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma_kernel(const Dec
                 ls[h] = x;
             }
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                os[h * (DP + 4) + k * 16 + g] = o[n][k][e];
-                os[h * (DP + 4) + k * 16 + g + 8] = o[n][k][e + 2];
+            for (int k = 0; k < MT; ++k) {
+                const int d0 = F32 ? 4 * (g + 8 * (k >> 1)) + 2 * (k & 1) : k * 16 + g, d1 = F32 ? d0 + 1 : d0 + 8;
+                os[h * S::PITCH + d0] = o[n][k][e];
+                os[h * S::PITCH + d1] = o[n][k][e + 2];
             }
         }
     __syncthreads();
-    merge_warps(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, 8 * NT, DP + 4);
+    merge_warps<W>(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, 8 * NT, S::PITCH);
 }
 
 // m and l of all parts of a head (one warp): the same order whatever the grid.
@@ -679,17 +663,13 @@ struct DecodePlan {
     size_t off_ml, off_o, off_scores, bytes;
 };
 
-// Query heads of a KV head that one CTA takes: up to 8 by fused multiply-adds (fp32); 8 or 16 by matrix
-// instructions, 8 where 16 heads of 256 columns would not fit in registers.
-int head_group(int dtype, int G, int D) {
-    if (dtype == RKV_F32) return G >= 5 ? 8 : G >= 3 ? 4 : G;
-    return G > 8 && D <= 128 ? 16 : 8;
-}
-
-// CTAs that run at a time: what shared memory (16-bit) or registers (fp32) let the SMs hold.
-int decode_slots(int dtype, int gt, int D) {
-    if (dtype == RKV_F32) return kSms * (gt <= 4 ? 4 : 3);
-    return kSms * (D <= 64 ? 4 : D <= 128 ? 2 : 1);
+// Query heads of a KV head that one CTA takes: 16 where more than 8 share a KV head of 16-bit rows of at
+// most 128 columns, else 8 (more would not fit in registers).
+int head_group(int dtype, int G, int D) { return dtype != RKV_F32 && G > 8 && D <= 128 ? 16 : 8; }
+// CTAs that run at a time (Shape::CTAS of an SM).
+int decode_slots(int dtype, int D) {
+    const int row = (D <= 64 ? 64 : D <= 128 ? 128 : 256) * (dtype == RKV_F32 ? 4 : 2);
+    return kSms * (row > 256 ? 1 : 2);
 }
 long long decode_units(int dtype, int H, int HK, int D, int batch) {
     const int G = H / HK, gt = head_group(dtype, G, D);
@@ -698,7 +678,7 @@ long long decode_units(int dtype, int H, int HK, int D, int batch) {
 // The most parts that decode_parts gives up to visible_max, which it grows with.
 long long decode_parts_bound(int dtype, int H, int HK, int D, long long visible_max, int batch) {
     const long long units = decode_units(dtype, H, HK, D, batch);
-    const long long slots = decode_slots(dtype, head_group(dtype, H / HK, D), D);
+    const long long slots = decode_slots(dtype, D);
     long long p = units > 0 ? kMaxWaves * slots / units : 1;
     const long long most = (visible_max + kMinChunk - 1) / kMinChunk;
     if (p > most) p = most;
@@ -715,7 +695,7 @@ long long decode_parts_bound(int dtype, int H, int HK, int D, long long visible_
 // ragged sequences 247 us against 198; the SMs do not stream at one rate.)
 long long decode_parts(int dtype, int H, int HK, int D, long long visible_max, int batch) {
     const long long units = decode_units(dtype, H, HK, D, batch), bound = decode_parts_bound(dtype, H, HK, D, visible_max, batch);
-    const long long slots = decode_slots(dtype, head_group(dtype, H / HK, D), D);
+    const long long slots = decode_slots(dtype, D);
     long long best = 1, best_cost = -1;
     for (int w = 0; w <= kMaxWaves; ++w) {
         long long p = w == 0 || units == 0 ? 1 : w * slots / units;
@@ -754,42 +734,25 @@ DecodePlan decode_plan(int dtype, int H, int HK, int D, long long visible_max, i
     return p;
 }
 
-template <int GT>
-int launch_simt(const DecodeArgs& a, long long blocks, cudaStream_t st) {
-    const int vpr = a.D / 4;
-    const size_t smem = simt_smem(GT, a.D);
-    if (vpr > 32)
-        paged_decode_simt_kernel<GT, 2><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
-    else
-        paged_decode_simt_kernel<GT, 1><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
-    return launched();
-}
-
-int launch_f32(const DecodeArgs& a, int gt, long long blocks, cudaStream_t st) {
-    switch (gt) {
-        case 1: return launch_simt<1>(a, blocks, st);
-        case 2: return launch_simt<2>(a, blocks, st);
-        case 4: return launch_simt<4>(a, blocks, st);
-        default: return launch_simt<8>(a, blocks, st);
-    }
-}
-
-template <bool BF, int DP, int NT>
-int launch_mma(const DecodeArgs& a, long long blocks, cudaStream_t st) {
-    constexpr size_t smem = mma_smem(DP, NT);
-    if (cudaFuncSetAttribute(paged_decode_mma_kernel<BF, DP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-        cudaSuccess) {
+template <int KIND, int DP, int NT>
+int launch_shape(const DecodeArgs& a, long long blocks, cudaStream_t st) {
+    using S = Shape<KIND, DP, NT>;
+    static_assert(S::SMEM * S::CTAS + 1024 * S::CTAS <= 228 * 1024, "the CTAs of an SM fit in its shared memory");
+    if (cudaFuncSetAttribute(paged_decode_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
-    paged_decode_mma_kernel<BF, DP, NT><<<(unsigned)blocks, kWarps * 32, smem, st>>>(a);
+    paged_decode_kernel<S><<<(unsigned)blocks, S::W * 32, S::SMEM, st>>>(a);
     return launched();
 }
-template <bool BF>
-int launch_16(const DecodeArgs& a, int gt, long long blocks, cudaStream_t st) {
-    if (a.D <= 64) return gt == 16 ? launch_mma<BF, 64, 2>(a, blocks, st) : launch_mma<BF, 64, 1>(a, blocks, st);
-    if (a.D <= 128) return gt == 16 ? launch_mma<BF, 128, 2>(a, blocks, st) : launch_mma<BF, 128, 1>(a, blocks, st);
-    return launch_mma<BF, 256, 1>(a, blocks, st);
+template <int KIND>
+int launch_kind(const DecodeArgs& a, int gt, long long blocks, cudaStream_t st) {
+    if constexpr (KIND != KIND_F32) {
+        if (gt == 16) return a.D <= 64 ? launch_shape<KIND, 64, 2>(a, blocks, st) : launch_shape<KIND, 128, 2>(a, blocks, st);
+    }
+    if (a.D <= 64) return launch_shape<KIND, 64, 1>(a, blocks, st);
+    if (a.D <= 128) return launch_shape<KIND, 128, 1>(a, blocks, st);
+    return launch_shape<KIND, 256, 1>(a, blocks, st);
 }
 
 }  // namespace
@@ -911,9 +874,9 @@ extern "C" int rkv_paged_decode(const void* Q, long long q_item_stride, int num_
     const long long jblocks = a.o_blocks + (long long)batch * a.HK * a.w_blocks;
     if (blocks > 0x7FFFFFFFLL || jblocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
     switch (cache->dtype) {
-        case RKV_F32: rc = launch_f32(a, p.gt, blocks, st); break;
-        case RKV_BF16: rc = launch_16<true>(a, p.gt, blocks, st); break;
-        default: rc = launch_16<false>(a, p.gt, blocks, st); break;
+        case RKV_F32: rc = launch_kind<KIND_F32>(a, p.gt, blocks, st); break;
+        case RKV_BF16: rc = launch_kind<KIND_BF16>(a, p.gt, blocks, st); break;
+        default: rc = launch_kind<KIND_F16>(a, p.gt, blocks, st); break;
     }
     if (rc || !join || jblocks == 0) return rc;
     size_t smem = (size_t)p.splits * sizeof(float);
