@@ -107,6 +107,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Bits 0 .. n - 1 (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort) {
     return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, err, abort));
 }
@@ -254,16 +261,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool whole = j0 + kTile - 1 <= p0 && j0 + kTile <= rg.n &&
                                (a.window <= 0 || j0 > p0 + kTile - 1 - a.window || j0 + kTile <= a.sinks);
             if (!whole) {
-                const int hi = min(p, rg.n - 1) - j0, lo = a.window > 0 ? p - a.window + 1 - j0 : 0, sk = a.sinks - j0;
+                const int hi = min(p, rg.n - 1) - j0 + 1, lo = a.window > 0 ? p - a.window + 1 - j0 : 0, sk = a.sinks - j0;
 #pragma unroll
-                for (int c = 0; c < 128; ++c)
-                    if (!(c <= hi && (c >= lo || c < sk))) r[c] = 0xFF800000u;  // -inf
+                for (int w = 0; w < 4; ++w) {  // a bit per column
+                    const uint32_t see = below(hi - 32 * w) & (~below(lo - 32 * w) | below(sk - 32 * w));
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (!(see & (1u << c))) r[32 * w + c] = 0xFF800000u;  // -inf
+                }
             }
             float mt = -INFINITY;
             {
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(r[c]));
+                for (int c = 0; c < 128; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(r[c]), __uint_as_float(r[c + 1]));
                 mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             }
             const bool need = (mt - m) * a.scale2 > kGrow;  // true for a row's first key, false while it has none
