@@ -31,14 +31,15 @@ namespace {
 
 constexpr int kTile = 128;            // queries of a unit, keys of a tile
 constexpr int kThreads = 384;
+constexpr int kSms = 148;
 constexpr int kBlk = kTile * 128;     // bytes of a 128-row block of 64 columns
 constexpr float kGrow = 8.0f;         // log2 growth of a row's maximum that is carried without a rescale
 
 __host__ __device__ constexpr int stages(int kb) { return kb == 1 ? 8 : 4; }
 
 struct TcBars {
-    uint64_t q_full, o_full;
-    uint64_t s_full[2], p_ready[2];
+    uint64_t q_full, q_empty, o_full, drained;
+    uint64_t s_full[2], p_half[2], p_ready[2], o_empty[2];  // of a unit
     uint64_t full[8], empty[8];
     uint32_t tmem;
     int abort;
@@ -118,12 +119,40 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
     return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, err, abort));
 }
 
+// A pair of units: (query tile, head of the group) numbers u0 and u0 + 1 of one KV head.
+struct Pair {
+    int b, hk, u0, nu;
+    SinkRange rg;
+    int tiles;
+};
+// Item i of the list, the latest queries (the longest rows) first.
+__device__ __forceinline__ Pair pair_of(const SinkArgs& a, int i, int per) {
+    const int units = a.G * a.qtiles, pairs = (units + 1) / 2;
+    Pair p;
+    p.u0 = 2 * (pairs - 1 - i / per);
+    const int bh = i % per;
+    p.b = bh / a.HK;
+    p.hk = bh - p.b * a.HK;
+    p.nu = min(2, units - p.u0);
+    const int qt0 = p.u0 / a.G, qt1 = (p.u0 + p.nu - 1) / a.G;
+    p.rg = sink_range(a, p.b, qt0 * kTile, (qt1 - qt0 + 1) * kTile, kTile);
+    p.tiles = p.rg.count();
+    return p;
+}
+// The k-th item of a CTA: the list goes round the CTAs to and fro, so that each gets long and short ones.
+__device__ __forceinline__ int item_of(int k) {
+    return k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
 // KB: blocks of 64 columns (dim_head <= 64 KB; columns behind dim_head are
-// filled with zeros by the copies).
+// filled with zeros by the copies).  One CTA per SM goes through its items
+// (pairs of units); every role keeps its own count of barrier phases over all
+// of them, so the copies, and the first scores, of an item run under the end
+// of the one before.
 template <int KB, bool BF>
 __global__ void __launch_bounds__(kThreads, 1)
-    sink_tc_kernel(const SinkArgs a, const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                   const __grid_constant__ CUtensorMap tv) {
+    sink_tc_kernel(const SinkArgs a, const int items, const int per, const __grid_constant__ CUtensorMap tq,
+                   const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
     constexpr int NS = stages(KB);
     constexpr uint32_t kStage = KB * kBlk;
     constexpr uint32_t kColO = 256;  // tensor memory: S0, S1 (128 columns each), O0, O1 (64 KB each)
@@ -135,24 +164,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* ring = sq + 2 * kStage;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    // the units: (query tile, head of the group), the latest queries (the longest rows) first
-    const int units = a.G * a.qtiles, pairs = (units + 1) / 2;
-    const int heads = a.HK;
-    const int per = (int)(gridDim.x / pairs);  // batch * KV heads
-    const int u0 = 2 * (pairs - 1 - (int)(blockIdx.x / per));
-    const int bh = (int)(blockIdx.x % per), b = bh / heads, hk = bh % heads;
-    const int nu = min(2, units - u0);
-    const int qt0 = u0 / a.G, qt1 = (u0 + nu - 1) / a.G;
-    const SinkRange rg = sink_range(a, b, qt0 * kTile, (qt1 - qt0 + 1) * kTile, kTile);
-    const int tiles = rg.count();
-    if (tiles == 0) return;
-
     if (tid == 0) {
         mbar_init(&B.q_full, 1);
+        mbar_init(&B.q_empty, 1);
         mbar_init(&B.o_full, 1);
+        mbar_init(&B.drained, 1);
         for (int u = 0; u < 2; ++u) {
             mbar_init(&B.s_full[u], 1);
+            mbar_init(&B.p_half[u], 4);
             mbar_init(&B.p_ready[u], 4);
+            mbar_init(&B.o_empty[u], 4);
         }
         for (int i = 0; i < NS; ++i) {
             mbar_init(&B.full[i], 1);
@@ -168,24 +189,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tbase = B.tmem;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        // 88 * 128 + 208 * 256 registers are the 168 * 384 of the launch
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 0) {
-            mbar_arrive_expect_tx_w(&B.q_full, nu * kStage);
-            for (int u = 0; u < nu; ++u)
-                for (int kb = 0; kb < KB; ++kb)
-                    tma_load_4d_w(sq + u * kStage + kb * kBlk, &tq, kb * 64, (u0 + u) / a.G * kTile, hk * a.G + (u0 + u) % a.G, b,
-                                  &B.q_full);
-            int q = 0;
-            for (; q < 2 * tiles; ++q) {
+            // copies number q of the ring: K and V of every tile in turn
+            int q = 0, nq = 0;
+            bool ok = true;
+            auto copy = [&](const Pair& P, int j, bool v) {
                 const int s = q % NS;
-                if (q >= NS && !warp_wait(&B.empty[s], (uint32_t)((q / NS - 1) & 1), a.err, abort_flag)) break;
+                if (q >= NS && !(ok = warp_wait(&B.empty[s], (uint32_t)((q / NS - 1) & 1), a.err, abort_flag))) return;
                 mbar_arrive_expect_tx_w(&B.full[s], kStage);
                 for (int kb = 0; kb < KB; ++kb)
-                    tma_load_4d_w(ring + s * kStage + kb * kBlk, (q & 1) ? &tv : &tk, kb * 64, rg.tile(q >> 1) * kTile, hk, b,
-                                  &B.full[s]);
+                    tma_load_4d_w(ring + s * kStage + kb * kBlk, v ? &tv : &tk, kb * 64, P.rg.tile(j) * kTile, P.hk, P.b, &B.full[s]);
+                ++q;
+            };
+            for (int k = 0; ok; ++k) {
+                const int it = item_of(k);
+                if (it >= items) break;
+                const Pair P = pair_of(a, it, per);
+                if (P.tiles == 0) continue;
+                copy(P, 0, false);
+                if (!ok || (nq > 0 && !(ok = warp_wait(&B.q_empty, (uint32_t)((nq - 1) & 1), a.err, abort_flag)))) break;
+                mbar_arrive_expect_tx_w(&B.q_full, P.nu * kStage);
+                for (int u = 0; u < P.nu; ++u)
+                    for (int kb = 0; kb < KB; ++kb)
+                        tma_load_4d_w(sq + u * kStage + kb * kBlk, &tq, kb * 64, (P.u0 + u) / a.G * kTile,
+                                      P.hk * a.G + (P.u0 + u) % a.G, P.b, &B.q_full);
+                ++nq;
+                for (int j = 0; j < P.tiles && ok; ++j) {
+                    copy(P, j, true);
+                    if (ok && j + 1 < P.tiles) copy(P, j + 1, false);
+                }
             }
             // every copy has landed before the CTA may end
-            mbar_wait_bounded(&B.q_full, 0, a.err);
+            if (nq > 0) mbar_wait_bounded(&B.q_full, (uint32_t)((nq - 1) & 1), a.err);
             for (int s = 0; s < min(q, NS); ++s) mbar_wait_bounded(&B.full[s], (uint32_t)(((q - 1 - s) / NS) & 1), a.err);
         } else if (warp == 1) {
             const uint32_t ids = mma_idesc(BF ? 1u : 0u, kTile);
@@ -199,148 +236,188 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 mma_commit_w(&B.s_full[u]);
             };
-            bool ok = warp_wait(&B.q_full, 0, a.err, abort_flag) && warp_wait(&B.full[0], 0, a.err, abort_flag);
-            if (ok) {
+            int q = 0, nq = 0;                  // ring copies, items
+            uint32_t tiles_ph = 0, out_ph = 0;  // a bit per unit: parity of its tiles and of its items
+            uint32_t used = 0;                  // the unit's output columns have been written before
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, int n) { return ok = warp_wait(bar, (uint32_t)(n & 1), a.err, abort_flag); };
+            for (int k = 0; ok; ++k) {
+                const int it = item_of(k);
+                if (it >= items) break;
+                const Pair P = pair_of(a, it, per);
+                if (P.tiles == 0) continue;
+                if (!wait(&B.q_full, nq) || !wait(&B.full[q % NS], q / NS)) break;
+                ++nq;
                 tc_fence_after();
-                for (int u = 0; u < nu; ++u) scores(u, smem_u32(ring));
-                mma_commit_w(&B.empty[0]);
-            }
-            for (int j = 0; j < tiles && ok; ++j) {
-                const int qv = 2 * j + 1, sv = qv % NS, qk = qv + 1, sk = qk % NS;
-                uint8_t* vt = ring + sv * kStage;
-                if (!(ok = warp_wait(&B.full[sv], (uint32_t)((qv / NS) & 1), a.err, abort_flag))) break;
-                const int behind = rg.n - rg.tile(j) * kTile;  // keys of the tile that exist
-                if (behind < kTile && rg.n < a.len_k) {
-                    // the padding behind a sequence's end may hold anything, and 0 * NaN is NaN
-                    for (int e = lane; e < (kTile - behind) * 8; e += 32)
+                for (int u = 0; u < P.nu; ++u) scores(u, smem_u32(ring + (q % NS) * kStage));
+                mma_commit_w(&B.empty[q % NS]);
+                if (P.tiles == 1) mma_commit_w(&B.q_empty);
+                ++q;
+                for (int j = 0; j < P.tiles && ok; ++j) {
+                    const int sv = q % NS, sk = (q + 1) % NS;
+                    uint8_t* vt = ring + sv * kStage;
+                    if (!wait(&B.full[sv], q / NS)) break;
+                    const int behind = P.rg.n - P.rg.tile(j) * kTile;  // keys of the tile that exist
+                    if (behind < kTile && P.rg.n < a.len_k) {
+                        // the padding behind a sequence's end may hold anything, and 0 * NaN is NaN
+                        for (int e = lane; e < (kTile - behind) * 8; e += 32)
 #pragma unroll
-                        for (int kb = 0; kb < KB; ++kb)
-                            *reinterpret_cast<uint4*>(vt + kb * kBlk + behind * 128 + e * 16) = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async();
-                    __syncwarp();
-                }
-                for (int u = 0; u < nu; ++u) {
-                    if (!(ok = warp_wait(&B.p_ready[u], (uint32_t)(j & 1), a.err, abort_flag))) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)
-                        mma_ts(tbase + kColO + u * (KB * 64), tbase + u * 128 + ks * 8, v_desc(smem_u32(vt) + ks * 2048), idv,
-                               (j | ks) > 0);
-                    if (u == nu - 1) mma_commit_w(&B.empty[sv]);
-                    if (j + 1 < tiles) {
-                        if (u == 0) {
-                            if (!(ok = warp_wait(&B.full[sk], (uint32_t)((qk / NS) & 1), a.err, abort_flag))) break;
-                            tc_fence_after();
-                        }
-                        scores(u, smem_u32(ring + sk * kStage));
-                        if (u == nu - 1) mma_commit_w(&B.empty[sk]);
+                            for (int kb = 0; kb < KB; ++kb)
+                                *reinterpret_cast<uint4*>(vt + kb * kBlk + behind * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async();
+                        __syncwarp();
                     }
+                    for (int u = 0; u < P.nu; ++u) {
+                        if (j == 0) {  // the output rows of the unit before have been read
+                            if ((used >> u) & 1u) {
+                                if (!wait(&B.o_empty[u], out_ph >> u)) break;
+                                out_ph ^= 1u << u;
+                            }
+                            used |= 1u << u;
+                        }
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            if (!wait(half ? &B.p_ready[u] : &B.p_half[u], tiles_ph >> u)) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int ks = half * 4; ks < half * 4 + 4; ++ks)
+                                mma_ts(tbase + kColO + u * (KB * 64), tbase + u * 128 + ks * 8, v_desc(smem_u32(vt) + ks * 2048), idv,
+                                       (j | ks) > 0);
+                        }
+                        if (!ok) break;
+                        tiles_ph ^= 1u << u;
+                        if (u == P.nu - 1) mma_commit_w(&B.empty[sv]);
+                        if (j + 1 < P.tiles) {
+                            if (u == 0) {
+                                if (!wait(&B.full[sk], (q + 1) / NS)) break;
+                                tc_fence_after();
+                            }
+                            scores(u, smem_u32(ring + sk * kStage));
+                            if (u == P.nu - 1) {
+                                mma_commit_w(&B.empty[sk]);
+                                if (j + 2 == P.tiles) mma_commit_w(&B.q_empty);
+                            }
+                        }
+                    }
+                    q += j + 1 < P.tiles ? 2 : 1;
                 }
+                if (ok) mma_commit_w(&B.o_full);
             }
-            if (ok) mma_commit_w(&B.o_full);
+            // the products have ended before the tensor memory is freed
+            mma_commit_w(&B.drained);
+            mbar_wait_bounded(&B.drained, 0, a.err);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int u = (warp >> 2) - 1, q4 = warp & 3, row = q4 * 32 + lane;
-        const int qt = (u0 + u) / a.G, h = hk * a.G + (u0 + u) % a.G;
-        const int p0 = qt * kTile + a.len_k - a.len_q, p = p0 + row;
         const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
         const uint32_t ts = tbase + u * 128 + lane_off, to = tbase + kColO + u * (KB * 64) + lane_off;
-        float m = -INFINITY, l = 0.0f;
-        bool ok = u < nu;
-        for (int j = 0; j < tiles && ok; ++j) {
-            if (!(ok = warp_wait(&B.s_full[u], (uint32_t)(j & 1), a.err, abort_flag))) break;
-            tc_fence_after();
-            uint32_t r[128];
+        const float2 sc = make_float2(a.scale2, a.scale2);
+        int nt = 0, ni = 0;  // tiles of this unit, items
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+            const int it = item_of(k);
+            if (it >= items) break;
+            const Pair P = pair_of(a, it, per);
+            if (P.tiles == 0) continue;
+            ++ni;
+            if (u >= P.nu) continue;
+            const int qt = (P.u0 + u) / a.G, h = P.hk * a.G + (P.u0 + u) % a.G;
+            const int p0 = qt * kTile + a.len_k - a.len_q, p = p0 + row, n = P.rg.n;
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < P.tiles; ++j, ++nt) {
+                if (!(ok = warp_wait(&B.s_full[u], (uint32_t)(nt & 1), a.err, abort_flag))) break;
+                tc_fence_after();
+                uint32_t r[128];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) ld32_async(ts + c * 32, r + c * 32);
-            wait_ld();
+                for (int c = 0; c < 4; ++c) ld32_async(ts + c * 32, r + c * 32);
+                wait_ld();
 #pragma unroll
-            for (int c = 0; c < 4; ++c) pin32(r + c * 32);
-            const int j0 = rg.tile(j) * kTile;
-            const bool whole = j0 + kTile - 1 <= p0 && j0 + kTile <= rg.n &&
-                               (a.window <= 0 || j0 > p0 + kTile - 1 - a.window || j0 + kTile <= a.sinks);
-            if (!whole) {
-                const int hi = min(p, rg.n - 1) - j0 + 1, lo = a.window > 0 ? p - a.window + 1 - j0 : 0, sk = a.sinks - j0;
+                for (int c = 0; c < 4; ++c) pin32(r + c * 32);
+                const int j0 = P.rg.tile(j) * kTile;
+                const bool whole = j0 + kTile - 1 <= p0 && j0 + kTile <= n &&
+                                   (a.window <= 0 || j0 > p0 + kTile - 1 - a.window || j0 + kTile <= a.sinks);
+                if (!whole) {
+                    const int hi = min(p, n - 1) - j0 + 1, lo = a.window > 0 ? p - a.window + 1 - j0 : 0, sk = a.sinks - j0;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {  // a bit per column
-                    const uint32_t see = below(hi - 32 * w) & (~below(lo - 32 * w) | below(sk - 32 * w));
+                    for (int w = 0; w < 4; ++w) {  // a bit per column
+                        const uint32_t see = below(hi - 32 * w) & (~below(lo - 32 * w) | below(sk - 32 * w));
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (!(see & (1u << c))) r[32 * w + c] = 0xFF800000u;  // -inf
+                        for (int c = 0; c < 32; ++c)
+                            if (!(see & (1u << c))) r[32 * w + c] = 0xFF800000u;  // -inf
+                    }
                 }
-            }
-            float mt = -INFINITY;
-            {
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < 128; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(r[c]), __uint_as_float(r[c + 1]));
-                mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            }
-            const bool need = (mt - m) * a.scale2 > kGrow;  // true for a row's first key, false while it has none
-            if (__any_sync(0xffffffffu, need)) {
-                const float corr = need ? ex2_approx((m - mt) * a.scale2) : 1.0f;
-                l *= corr;
-                if (need) m = mt;
-                if (j > 0) {  // the products up to here are complete: this tile's scores were issued behind them
+                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool need = (mt - m) * a.scale2 > kGrow;  // true for a row's first key, false while it has none
+                if (__any_sync(0xffffffffu, need)) {
+                    const float corr = need ? ex2_approx((m - mt) * a.scale2) : 1.0f;
+                    l *= corr;
+                    if (need) m = mt;
+                    if (j > 0) {  // the products up to here are complete: this tile's scores were issued behind them
 #pragma unroll 1
-                    for (int c = 0; c < KB * 2; ++c) {
-                        uint32_t o[32];
-                        ld32_async(to + c * 32, o);
-                        wait_ld();
-                        pin32(o);
+                        for (int c = 0; c < KB * 2; ++c) {
+                            uint32_t o[32];
+                            ld32_async(to + c * 32, o);
+                            wait_ld();
+                            pin32(o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                        st32(to + c * 32, o);
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                            st32(to + c * 32, o);
+                        }
                     }
                 }
-            }
-            const float ms = (m == -INFINITY ? 0.0f : m) * a.scale2;
-            const float2 sc = make_float2(a.scale2, a.scale2), nm = make_float2(-ms, -ms);
-            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                const float ms = (m == -INFINITY ? 0.0f : m) * a.scale2;
+                const float2 nm = make_float2(-ms, -ms);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-            for (int c = 0; c < 64; ++c) {
-                float2 x = __ffma2_rn(make_float2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), sc, nm);
-                x.x = ex2_approx(x.x);
-                x.y = ex2_approx(x.y);
-                sum[c & 1] = __fadd2_rn(sum[c & 1], x);
-                r[c] = pack2<BF>(x.x, x.y);
-                if (c == 31) st32(ts, r);
+                for (int half = 0; half < 2; ++half) {  // the products of the first 64 keys start under the second's exponentials
+#pragma unroll
+                    for (int c = half * 32; c < half * 32 + 32; ++c) {
+                        float2 x = __ffma2_rn(make_float2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), sc, nm);
+                        x.x = ex2_approx(x.x);
+                        x.y = ex2_approx(x.y);
+                        sum[c & 1] = __fadd2_rn(sum[c & 1], x);
+                        r[c] = pack2<BF>(x.x, x.y);
+                    }
+                    st32(ts + half * 32, r + half * 32);
+                    wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive1(half ? &B.p_ready[u] : &B.p_half[u]);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
-            st32(ts + 32, r + 32);
-            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-            wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive1(&B.p_ready[u]);
-        }
-        if (ok && (ok = warp_wait(&B.o_full, 0, a.err, abort_flag))) {
+            if (!ok || !(ok = warp_wait(&B.o_full, (uint32_t)((ni - 1) & 1), a.err, abort_flag))) break;
             tc_fence_after();
             const int i = qt * kTile + row;
-            const bool real = i < a.len_q && p < rg.n;
+            const bool real = i < a.len_q && p < n;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            uint8_t* po = a.O + (size_t)b * a.os.item + (size_t)h * a.os.head + (size_t)i * a.os.token;
-#pragma unroll 1
-            for (int c = 0; c < KB * 2; ++c) {
-                uint32_t o[32];
-                ld32_async(to + c * 32, o);
-                wait_ld();
-                pin32(o);
+            uint8_t* po = a.O + (size_t)P.b * a.os.item + (size_t)h * a.os.head + (size_t)i * a.os.token;
+            uint32_t o[KB * 64];
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    uint32_t w[4];
+            for (int c = 0; c < KB * 2; ++c) ld32_async(to + c * 32, o + c * 32);
+            wait_ld();
 #pragma unroll
-                    for (int i2 = 0; i2 < 4; ++i2)
-                        w[i2] = pack2<BF>(__uint_as_float(o[v * 8 + 2 * i2]) * inv, __uint_as_float(o[v * 8 + 2 * i2 + 1]) * inv);
-                    if (real && c * 32 + v * 8 < a.D)
-                        *reinterpret_cast<uint4*>(po + (c * 32 + v * 8) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
+            for (int c = 0; c < KB * 2; ++c) pin32(o + c * 32);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(&B.o_empty[u]);
+#pragma unroll
+            for (int v = 0; v < KB * 8; ++v) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[e] = pack2<BF>(__uint_as_float(o[v * 8 + 2 * e]) * inv, __uint_as_float(o[v * 8 + 2 * e + 1]) * inv);
+                if (real && v * 8 < a.D) *reinterpret_cast<uint4*>(po + v * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             if (real && a.lse)
-                a.lse[((size_t)b * a.H + h) * a.len_q + i] =
+                a.lse[((size_t)P.b * a.H + h) * a.len_q + i] =
                     l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) * a.scale2 + log2f(l)) * 0.693147180559945f;
-            tc_fence_before();
         }
+        tc_fence_before();
     }
     __syncthreads();
     tc_fence_after();
@@ -376,14 +453,14 @@ bool encode(CUtensorMap* m, const void* base, bool bf, int D, int rows, int head
 }
 
 template <int KB, bool BF>
-int launch_kb(const SinkArgs& a, long long blocks, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+int launch_kb(const SinkArgs& a, int items, int per, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
               cudaStream_t st) {
     const int smem = 2048 + (2 + stages(KB)) * KB * kBlk;  // the barriers, and up to 1023 bytes of alignment
     if (cudaFuncSetAttribute(sink_tc_kernel<KB, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
-    sink_tc_kernel<KB, BF><<<(unsigned)blocks, kThreads, smem, st>>>(a, tq, tk, tv);
+    sink_tc_kernel<KB, BF><<<items < kSms ? items : kSms, kThreads, smem, st>>>(a, items, per, tq, tk, tv);
     return cudaGetLastError() == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }
 
@@ -398,10 +475,11 @@ int launch_sink_tc(SinkArgs a, int dtype, int batch, cudaStream_t st) {
         !encode(&tv, a.V, bf, a.D, a.len_k, a.HK, batch, a.ks))
         return RKV_ERR_CUDA;
     a.qtiles = (a.len_q + kTile - 1) / kTile;
-    const long long units = (long long)a.G * a.qtiles, blocks = (units + 1) / 2 * batch * a.HK;
-    if (units > 0x7FFFFFFELL || blocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
-    if (a.D <= 64) return bf ? launch_kb<1, true>(a, blocks, tq, tk, tv, st) : launch_kb<1, false>(a, blocks, tq, tk, tv, st);
-    return bf ? launch_kb<2, true>(a, blocks, tq, tk, tv, st) : launch_kb<2, false>(a, blocks, tq, tk, tv, st);
+    const long long units = (long long)a.G * a.qtiles, per = (long long)batch * a.HK, items = (units + 1) / 2 * per;
+    if (units > 0x7FFFFFFELL || items > (1 << 30)) return RKV_ERR_UNSUPPORTED;
+    const int n = (int)items, p = (int)per;
+    if (a.D <= 64) return bf ? launch_kb<1, true>(a, n, p, tq, tk, tv, st) : launch_kb<1, false>(a, n, p, tq, tk, tv, st);
+    return bf ? launch_kb<2, true>(a, n, p, tq, tk, tv, st) : launch_kb<2, false>(a, n, p, tq, tk, tv, st);
 }
 
 }  // namespace rkv
