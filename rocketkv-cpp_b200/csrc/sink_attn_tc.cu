@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int* abort_flag = &B.abort;
     uint8_t* sq = sm + 1024;
     uint8_t* ring = sq + 2 * kStage;
+    uint8_t* stage_o = ring + NS * kStage;  // 4 KB per softmax warp
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -227,12 +228,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (warp == 1) {
             const uint32_t ids = mma_idesc(BF ? 1u : 0u, kTile);
             const uint32_t idv = mma_idesc(BF ? 1u : 0u, KB * 64) | (1u << 16);  // B with N contiguous
-            auto scores = [&](int u, uint32_t kaddr) {
-                const uint32_t qaddr = smem_u32(sq + u * kStage);
+            const uint64_t qd = mma_desc_sw128(smem_u32(sq)), kd = mma_desc_sw128(smem_u32(ring)), vd = v_desc(smem_u32(ring));
+            auto scores = [&](int u, int slot) {
+                const uint64_t da = qd + (uint32_t)(u * (kStage >> 4)), db = kd + (uint32_t)(slot * (kStage >> 4));
 #pragma unroll
                 for (int ks = 0; ks < KB * 4; ++ks) {
-                    const uint32_t o = (ks >> 2) * kBlk + (ks & 3) * 32;
-                    mma_ss(tbase + u * 128, mma_desc_sw128(qaddr + o), mma_desc_sw128(kaddr + o), ids, ks > 0);
+                    const uint32_t o = ((ks >> 2) * kBlk + (ks & 3) * 32) >> 4;
+                    mma_ss(tbase + u * 128, da + o, db + o, ids, ks > 0);
                 }
                 mma_commit_w(&B.s_full[u]);
             };
@@ -249,13 +251,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!wait(&B.q_full, nq) || !wait(&B.full[q % NS], q / NS)) break;
                 ++nq;
                 tc_fence_after();
-                for (int u = 0; u < P.nu; ++u) scores(u, smem_u32(ring + (q % NS) * kStage));
+                for (int u = 0; u < P.nu; ++u) scores(u, q % NS);
                 mma_commit_w(&B.empty[q % NS]);
                 if (P.tiles == 1) mma_commit_w(&B.q_empty);
                 ++q;
                 for (int j = 0; j < P.tiles && ok; ++j) {
                     const int sv = q % NS, sk = (q + 1) % NS;
                     uint8_t* vt = ring + sv * kStage;
+                    const uint64_t vdj = vd + (uint32_t)(sv * (kStage >> 4));
                     if (!wait(&B.full[sv], q / NS)) break;
                     const int behind = P.rg.n - P.rg.tile(j) * kTile;  // keys of the tile that exist
                     if (behind < kTile && P.rg.n < a.len_k) {
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tc_fence_after();
 #pragma unroll
                             for (int ks = half * 4; ks < half * 4 + 4; ++ks)
-                                mma_ts(tbase + kColO + u * (KB * 64), tbase + u * 128 + ks * 8, v_desc(smem_u32(vt) + ks * 2048), idv,
+                                mma_ts(tbase + kColO + u * (KB * 64), tbase + u * 128 + ks * 8, vdj + ks * 128, idv,
                                        (j | ks) > 0);
                         }
                         if (!ok) break;
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 if (!wait(&B.full[sk], (q + 1) / NS)) break;
                                 tc_fence_after();
                             }
-                            scores(u, smem_u32(ring + sk * kStage));
+                            scores(u, sk);
                             if (u == P.nu - 1) {
                                 mma_commit_w(&B.empty[sk]);
                                 if (j + 2 == P.tiles) mma_commit_w(&B.q_empty);
@@ -395,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int i = qt * kTile + row;
             const bool real = i < a.len_q && p < n;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            uint8_t* po = a.O + (size_t)P.b * a.os.item + (size_t)h * a.os.head + (size_t)i * a.os.token;
+            uint8_t* po = a.O + (size_t)P.b * a.os.item + (size_t)h * a.os.head;
             uint32_t o[KB * 64];
 #pragma unroll
             for (int c = 0; c < KB * 2; ++c) ld32_async(to + c * 32, o + c * 32);
@@ -405,13 +408,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive1(&B.o_empty[u]);
+            // through shared memory, 64 columns at a time, so that eight lanes write 128 bytes of a row (a lane
+            // per row wrote half sectors: 4000 cycles a pair); chunk c of row r is kept at c ^ (r % 8)
+            uint8_t* so = stage_o + (warp - 4) * 4096;
+            const uint32_t rows_ok = __ballot_sync(0xffffffffu, real);
 #pragma unroll
-            for (int v = 0; v < KB * 8; ++v) {
-                uint32_t w[4];
+            for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    w[e] = pack2<BF>(__uint_as_float(o[v * 8 + 2 * e]) * inv, __uint_as_float(o[v * 8 + 2 * e + 1]) * inv);
-                if (real && v * 8 < a.D) *reinterpret_cast<uint4*>(po + v * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int v = 0; v < 8; ++v) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = pack2<BF>(__uint_as_float(o[kb * 64 + v * 8 + 2 * e]) * inv, __uint_as_float(o[kb * 64 + v * 8 + 2 * e + 1]) * inv);
+                    *reinterpret_cast<uint4*>(so + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const int rr = x * 4 + (lane >> 3), v = lane & 7;
+                    const uint4 y = *reinterpret_cast<const uint4*>(so + rr * 128 + ((v ^ (rr & 7)) << 4));
+                    if (((rows_ok >> rr) & 1u) && kb * 64 + v * 8 < a.D)
+                        *reinterpret_cast<uint4*>(po + (size_t)(qt * kTile + q4 * 32 + rr) * a.os.token + kb * 128 + v * 16) = y;
+                }
+                __syncwarp();
             }
             if (real && a.lse)
                 a.lse[((size_t)P.b * a.H + h) * a.len_q + i] =
@@ -455,7 +474,8 @@ bool encode(CUtensorMap* m, const void* base, bool bf, int D, int rows, int head
 template <int KB, bool BF>
 int launch_kb(const SinkArgs& a, int items, int per, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
               cudaStream_t st) {
-    const int smem = 2048 + (2 + stages(KB)) * KB * kBlk;  // the barriers, and up to 1023 bytes of alignment
+    // the barriers, and up to 1023 bytes of alignment; Q and the ring; the output rows' stage
+    const int smem = 2048 + (2 + stages(KB)) * KB * kBlk + 8 * 4096;
     if (cudaFuncSetAttribute(sink_tc_kernel<KB, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
