@@ -278,7 +278,7 @@ extern "C" int rkv_sink_attention(const void* Q, const void* K, const void* V, i
     a.scale2 = 1.4426950408889634f / sqrtf((float)dim_head);
     a.err = static_cast<int*>(workspace);
     if (cudaMemsetAsync(a.err, 0, sizeof(int), st) != cudaSuccess) return RKV_ERR_CUDA;
-    if (sink_tc_supported(a, dtype)) return launch_sink_tc(a, dtype, batch, st);
+    if (sink_tc_supported(dtype)) return launch_sink_tc(a, dtype, batch, st);
     a.qtiles = (len_q + kBM - 1) / kBM;
     const long long blocks = (long long)a.qtiles * num_heads * batch;
     if (blocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;

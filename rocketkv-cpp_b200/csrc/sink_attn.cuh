@@ -48,8 +48,8 @@ __device__ __forceinline__ bool sink_sees(const SinkArgs& a, int n, int p, int j
     return j <= p && j < n && (a.window <= 0 || j < a.sinks || j > p - a.window);
 }
 
-// 16-bit inputs of dim_head <= 128 on the tensor cores (sink_attn_tc.cu)
-bool sink_tc_supported(const SinkArgs& a, int dtype);
+// 16-bit inputs on the tcgen05 tensor cores (sink_attn_tc.cu)
+bool sink_tc_supported(int dtype);
 int launch_sink_tc(SinkArgs a, int dtype, int batch, cudaStream_t st);
 
 }  // namespace rkv

@@ -1,5 +1,6 @@
 // sink_attn_tc.cu -- the sink-window prefill attention of 16-bit inputs on the
-// tcgen05 tensor cores (dim_head <= 128).
+// tcgen05 tensor cores: sink_tc_kernel for dim_head <= 128, sink_wide_kernel
+// for up to 256.
 //
 // A CTA takes two units -- a unit is 128 queries of one query head -- of one
 // KV head, so that both use every K and V tile that is loaded: 128 keys at a
@@ -59,9 +60,9 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 
 // Shared-memory descriptor of a V tile as the N x K operand, N (columns of V)
 // contiguous, 128-byte swizzle: 64 columns x 8 keys per 1024-byte group, the
-// groups of further keys 1024 bytes apart, further 64 columns kBlk apart.
-__device__ __forceinline__ uint64_t v_desc(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kBlk >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+// groups of further keys 1024 bytes apart, further 64 columns blk bytes apart.
+__device__ __forceinline__ uint64_t v_desc(uint32_t addr, uint32_t blk) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(blk >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
 
@@ -117,6 +118,30 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort) {
     return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, err, abort));
+}
+
+// 64 columns of a warp's 32 output rows (a row per lane in o) times inv, through 4 KB of shared memory, so that
+// eight lanes write 128 bytes of a row (a lane per row wrote half sectors); chunk c of row r is kept at c ^ (r % 8).
+template <bool BF>
+__device__ __forceinline__ void write_rows(uint8_t* so, const uint32_t* o, float inv, uint32_t rows_ok, uint8_t* po, int row0,
+                                           long long stride, int col0, int D, int lane) {
+#pragma unroll
+    for (int v = 0; v < 8; ++v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = pack2<BF>(__uint_as_float(o[v * 8 + 2 * e]) * inv, __uint_as_float(o[v * 8 + 2 * e + 1]) * inv);
+        *reinterpret_cast<uint4*>(so + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        const int r = x * 4 + (lane >> 3), v = lane & 7;
+        const uint4 y = *reinterpret_cast<const uint4*>(so + r * 128 + ((v ^ (r & 7)) << 4));
+        if (((rows_ok >> r) & 1u) && col0 + v * 8 < D)
+            *reinterpret_cast<uint4*>(po + (size_t)(row0 + r) * stride + (col0 + v * 8) * 2) = y;
+    }
+    __syncwarp();
 }
 
 // A pair of units: (query tile, head of the group) numbers u0 and u0 + 1 of one KV head.
@@ -228,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (warp == 1) {
             const uint32_t ids = mma_idesc(BF ? 1u : 0u, kTile);
             const uint32_t idv = mma_idesc(BF ? 1u : 0u, KB * 64) | (1u << 16);  // B with N contiguous
-            const uint64_t qd = mma_desc_sw128(smem_u32(sq)), kd = mma_desc_sw128(smem_u32(ring)), vd = v_desc(smem_u32(ring));
+            const uint64_t qd = mma_desc_sw128(smem_u32(sq)), kd = mma_desc_sw128(smem_u32(ring)), vd = v_desc(smem_u32(ring), kBlk);
             auto scores = [&](int u, int slot) {
                 const uint64_t da = qd + (uint32_t)(u * (kStage >> 4)), db = kd + (uint32_t)(slot * (kStage >> 4));
 #pragma unroll
@@ -408,32 +433,289 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive1(&B.o_empty[u]);
-            // through shared memory, 64 columns at a time, so that eight lanes write 128 bytes of a row (a lane
-            // per row wrote half sectors: 4000 cycles a pair); chunk c of row r is kept at c ^ (r % 8)
             uint8_t* so = stage_o + (warp - 4) * 4096;
             const uint32_t rows_ok = __ballot_sync(0xffffffffu, real);
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-                for (int v = 0; v < 8; ++v) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e] = pack2<BF>(__uint_as_float(o[kb * 64 + v * 8 + 2 * e]) * inv, __uint_as_float(o[kb * 64 + v * 8 + 2 * e + 1]) * inv);
-                    *reinterpret_cast<uint4*>(so + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-                __syncwarp();
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const int rr = x * 4 + (lane >> 3), v = lane & 7;
-                    const uint4 y = *reinterpret_cast<const uint4*>(so + rr * 128 + ((v ^ (rr & 7)) << 4));
-                    if (((rows_ok >> rr) & 1u) && kb * 64 + v * 8 < a.D)
-                        *reinterpret_cast<uint4*>(po + (size_t)(qt * kTile + q4 * 32 + rr) * a.os.token + kb * 128 + v * 16) = y;
-                }
-                __syncwarp();
-            }
+            for (int kb = 0; kb < KB; ++kb)
+                write_rows<BF>(so, o + kb * 64, inv, rows_ok, po, qt * kTile + q4 * 32, a.os.token, kb * 64, a.D, lane);
             if (real && a.lse)
                 a.lse[((size_t)P.b * a.H + h) * a.len_q + i] =
+                    l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) * a.scale2 + log2f(l)) * 0.693147180559945f;
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tbase, 512);
+}
+
+// dim_head 129 .. 256: the output of one unit takes 256 columns of tensor
+// memory, so a CTA has one unit, tiles of 64 keys, and two score buffers that
+// the tiles take in turn: the scores of the next tile are formed under this
+// tile's softmax.  Warp 0 copies, warp 1 issues, warps 4-7 are the softmax.
+constexpr int kWideKB = 4, kWideKeys = 64, kWideSlots = 4;
+constexpr int kWideThreads = 256;
+constexpr int kWideBlk = kWideKeys * 128;        // bytes of 64 rows of 64 columns
+constexpr int kWideSlot = kWideKB * kWideBlk;
+constexpr int kWideSmem = 2048 + kWideKB * kBlk + kWideSlots * kWideSlot + 4 * 4096;
+struct WideBars {
+    uint64_t q_full, q_empty, o_full, o_empty, pv_done, drained;
+    uint64_t s_full[2], p_ready[2];
+    uint64_t full[kWideSlots], empty[kWideSlots];
+    uint32_t tmem;
+    int abort;
+};
+struct WideItem {
+    int b, h, qt;
+    SinkRange rg;
+    int tiles;
+};
+__device__ __forceinline__ WideItem wide_item(const SinkArgs& a, int i, int per) {
+    WideItem w;
+    w.qt = a.qtiles - 1 - i / per;  // the longest rows first
+    const int bh = i % per;
+    w.b = bh / a.H;
+    w.h = bh - w.b * a.H;
+    w.rg = sink_range(a, w.b, w.qt * kTile, kTile, kWideKeys);
+    w.tiles = w.rg.count();
+    return w;
+}
+
+template <bool BF>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    sink_wide_kernel(const SinkArgs a, const int items, const int per, const __grid_constant__ CUtensorMap tq,
+                     const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
+    constexpr int KB = kWideKB, NS = kWideSlots;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    WideBars& B = *reinterpret_cast<WideBars*>(sm);
+    volatile int* abort_flag = &B.abort;
+    uint8_t* sq = sm + 1024;
+    uint8_t* ring = sq + KB * kBlk;
+    uint8_t* stage_o = ring + NS * kWideSlot;  // 4 KB per softmax warp
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        mbar_init(&B.q_full, 1);
+        mbar_init(&B.q_empty, 1);
+        mbar_init(&B.o_full, 1);
+        mbar_init(&B.o_empty, 4);
+        mbar_init(&B.pv_done, 1);
+        mbar_init(&B.drained, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&B.s_full[i], 1);
+            mbar_init(&B.p_ready[i], 4);
+        }
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&B.full[i], 1);
+            mbar_init(&B.empty[i], 1);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc(&B.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = B.tmem;  // output: columns 0-255, scores: 64 columns from 256 and from 384
+
+    if (warp == 0) {
+        int q = 0, nq = 0;
+        bool ok = true;
+        auto copy = [&](const WideItem& P, int j, bool v) {
+            const int s = q % NS;
+            if (q >= NS && !(ok = warp_wait(&B.empty[s], (uint32_t)((q / NS - 1) & 1), a.err, abort_flag))) return;
+            mbar_arrive_expect_tx_w(&B.full[s], kWideSlot);
+            for (int kb = 0; kb < KB; ++kb)
+                tma_load_4d_w(ring + s * kWideSlot + kb * kWideBlk, v ? &tv : &tk, kb * 64, P.rg.tile(j) * kWideKeys, P.h / a.G, P.b,
+                              &B.full[s]);
+            ++q;
+        };
+        for (int k = 0; ok; ++k) {
+            const int it = item_of(k);
+            if (it >= items) break;
+            const WideItem P = wide_item(a, it, per);
+            if (P.tiles == 0) continue;
+            copy(P, 0, false);
+            if (!ok || (nq > 0 && !(ok = warp_wait(&B.q_empty, (uint32_t)((nq - 1) & 1), a.err, abort_flag)))) break;
+            mbar_arrive_expect_tx_w(&B.q_full, KB * kBlk);
+            for (int kb = 0; kb < KB; ++kb) tma_load_4d_w(sq + kb * kBlk, &tq, kb * 64, P.qt * kTile, P.h, P.b, &B.q_full);
+            ++nq;
+            for (int j = 0; j < P.tiles && ok; ++j) {  // the scores run a tile ahead: K1 before V0
+                if (j + 1 < P.tiles) copy(P, j + 1, false);
+                if (ok) copy(P, j, true);
+            }
+        }
+        // every copy has landed before the CTA may end
+        if (nq > 0) mbar_wait_bounded(&B.q_full, (uint32_t)((nq - 1) & 1), a.err);
+        for (int s = 0; s < min(q, NS); ++s) mbar_wait_bounded(&B.full[s], (uint32_t)(((q - 1 - s) / NS) & 1), a.err);
+    } else if (warp == 1) {
+        const uint32_t ids = mma_idesc(BF ? 1u : 0u, kWideKeys);
+        const uint32_t idv = mma_idesc(BF ? 1u : 0u, KB * 64) | (1u << 16);  // B with N contiguous
+        const uint64_t qd = mma_desc_sw128(smem_u32(sq)), kd = mma_desc_sw128(smem_u32(ring));
+        const uint64_t vd = v_desc(smem_u32(ring), kWideBlk);
+        int q = 0, nq = 0, nt = 0, no = 0;  // ring copies, items, tiles, items whose output was begun
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, int n) { return ok = warp_wait(bar, (uint32_t)(n & 1), a.err, abort_flag); };
+        auto scores = [&](int t, int slot) {  // of tile number t of all
+            const uint64_t d = kd + (uint32_t)(slot * (kWideSlot >> 4));
+#pragma unroll
+            for (int ks = 0; ks < KB * 4; ++ks)
+                mma_ss(tbase + 256 + (t & 1) * 128, qd + (((ks >> 2) * kBlk + (ks & 3) * 32) >> 4),
+                       d + (((ks >> 2) * kWideBlk + (ks & 3) * 32) >> 4), ids, ks > 0);
+            mma_commit_w(&B.s_full[t & 1]);
+            mma_commit_w(&B.empty[slot]);
+        };
+        for (int k = 0; ok; ++k) {
+            const int it = item_of(k);
+            if (it >= items) break;
+            const WideItem P = wide_item(a, it, per);
+            if (P.tiles == 0) continue;
+            if (!wait(&B.q_full, nq) || !wait(&B.full[q % NS], q / NS)) break;
+            ++nq;
+            tc_fence_after();
+            scores(nt, q % NS);
+            if (P.tiles == 1) mma_commit_w(&B.q_empty);
+            ++q;
+            for (int j = 0; j < P.tiles; ++j, ++nt) {
+                if (j + 1 < P.tiles) {
+                    // its buffer held the P of the tile before, whose products are issued already
+                    if (!wait(&B.full[q % NS], q / NS)) break;
+                    tc_fence_after();
+                    scores(nt + 1, q % NS);
+                    if (j + 2 == P.tiles) mma_commit_w(&B.q_empty);
+                    ++q;
+                }
+                const int sv = q % NS;
+                if (!wait(&B.full[sv], q / NS)) break;
+                ++q;
+                const int behind = P.rg.n - P.rg.tile(j) * kWideKeys;  // keys of the tile that exist
+                if (behind < kWideKeys && P.rg.n < a.len_k) {
+                    // the padding behind a sequence's end may hold anything, and 0 * NaN is NaN
+                    uint8_t* vt = ring + sv * kWideSlot;
+                    for (int e = lane; e < (kWideKeys - behind) * 8; e += 32)
+#pragma unroll
+                        for (int kb = 0; kb < KB; ++kb)
+                            *reinterpret_cast<uint4*>(vt + kb * kWideBlk + behind * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                if (j == 0 && no++ > 0 && !wait(&B.o_empty, no)) break;  // the output rows before have been read
+                if (!wait(&B.p_ready[nt & 1], nt >> 1)) break;
+                tc_fence_after();
+                const uint64_t d = vd + (uint32_t)(sv * (kWideSlot >> 4));
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) mma_ts(tbase, tbase + 256 + (nt & 1) * 128 + ks * 8, d + ks * 128, idv, (j | ks) > 0);
+                mma_commit_w(&B.empty[sv]);
+                mma_commit_w(&B.pv_done);
+            }
+            if (ok) mma_commit_w(&B.o_full);
+        }
+        // the products have ended before the tensor memory is freed
+        mma_commit_w(&B.drained);
+        mbar_wait_bounded(&B.drained, 0, a.err);
+    } else if (warp >= 4) {
+        const int q4 = warp & 3, row = q4 * 32 + lane;
+        const uint32_t to = tbase + ((uint32_t)(q4 * 32) << 16);
+        uint8_t* so = stage_o + q4 * 4096;
+        const float2 sc = make_float2(a.scale2, a.scale2);
+        int nt = 0, ni = 0;
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+            const int it = item_of(k);
+            if (it >= items) break;
+            const WideItem P = wide_item(a, it, per);
+            if (P.tiles == 0) continue;
+            const int p0 = P.qt * kTile + a.len_k - a.len_q, p = p0 + row, n = P.rg.n;
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < P.tiles; ++j, ++nt) {
+                const uint32_t ts = to + 256 + (nt & 1) * 128;
+                if (!(ok = warp_wait(&B.s_full[nt & 1], (uint32_t)((nt >> 1) & 1), a.err, abort_flag))) break;
+                tc_fence_after();
+                uint32_t r[64];
+                ld32_async(ts, r);
+                ld32_async(ts + 32, r + 32);
+                wait_ld();
+                pin32(r);
+                pin32(r + 32);
+                const int j0 = P.rg.tile(j) * kWideKeys;
+                const bool whole = j0 + kWideKeys - 1 <= p0 && j0 + kWideKeys <= n &&
+                                   (a.window <= 0 || j0 > p0 + kTile - 1 - a.window || j0 + kWideKeys <= a.sinks);
+                if (!whole) {
+                    const int hi = min(p, n - 1) - j0 + 1, lo = a.window > 0 ? p - a.window + 1 - j0 : 0, sk = a.sinks - j0;
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {  // a bit per column
+                        const uint32_t see = below(hi - 32 * w) & (~below(lo - 32 * w) | below(sk - 32 * w));
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (!(see & (1u << c))) r[32 * w + c] = 0xFF800000u;  // -inf
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool need = (mt - m) * a.scale2 > kGrow;  // true for a row's first key, false while it has none
+                if (__any_sync(0xffffffffu, need)) {
+                    const float corr = need ? ex2_approx((m - mt) * a.scale2) : 1.0f;
+                    l *= corr;
+                    if (need) m = mt;
+                    if (j > 0) {  // behind the products of the tile before
+                        if (!(ok = warp_wait(&B.pv_done, (uint32_t)((nt - 1) & 1), a.err, abort_flag))) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < KB * 2; ++c) {
+                            uint32_t o[32];
+                            ld32_async(to + c * 32, o);
+                            wait_ld();
+                            pin32(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                            st32(to + c * 32, o);
+                        }
+                    }
+                }
+                const float ms = (m == -INFINITY ? 0.0f : m) * a.scale2;
+                const float2 nm = make_float2(-ms, -ms);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    float2 x = __ffma2_rn(make_float2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), sc, nm);
+                    x.x = ex2_approx(x.x);
+                    x.y = ex2_approx(x.y);
+                    sum[c & 1] = __fadd2_rn(sum[c & 1], x);
+                    r[c] = pack2<BF>(x.x, x.y);
+                }
+                st32(ts, r);
+                wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive1(&B.p_ready[nt & 1]);
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            }
+            if (!ok || !(ok = warp_wait(&B.o_full, (uint32_t)(ni++ & 1), a.err, abort_flag))) break;
+            tc_fence_after();
+            const int i = P.qt * kTile + row;
+            const bool real = i < a.len_q && p < n;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            uint8_t* po = a.O + (size_t)P.b * a.os.item + (size_t)P.h * a.os.head;
+            const uint32_t rows_ok = __ballot_sync(0xffffffffu, real);
+#pragma unroll 1
+            for (int kb = 0; kb < KB; ++kb) {
+                uint32_t o[64];
+                ld32_async(to + kb * 64, o);
+                ld32_async(to + kb * 64 + 32, o + 32);
+                wait_ld();
+                pin32(o);
+                pin32(o + 32);
+                if (kb == KB - 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive1(&B.o_empty);
+                }
+                write_rows<BF>(so, o, inv, rows_ok, po, P.qt * kTile + q4 * 32, a.os.token, kb * 64, a.D, lane);
+            }
+            if (real && a.lse)
+                a.lse[((size_t)P.b * a.H + P.h) * a.len_q + i] =
                     l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) * a.scale2 + log2f(l)) * 0.693147180559945f;
         }
         tc_fence_before();
@@ -456,16 +738,17 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// [batch][heads][rows][D] with byte strides; boxes of 64 columns x 128 rows, 128-byte swizzle, zeros
+// [batch][heads][rows][D] with byte strides; boxes of 64 columns x box_rows rows, 128-byte swizzle, zeros
 // outside.  A stride of a dimension of one entry is not used and set to a valid value.
-bool encode(CUtensorMap* m, const void* base, bool bf, int D, int rows, int heads, int batch, const rkv_row_strides& s) {
+bool encode(CUtensorMap* m, const void* base, bool bf, int D, int rows, int heads, int batch, const rkv_row_strides& s,
+            int box_rows) {
     auto enc = encode_fn();
     if (!enc) return false;
     const cuuint64_t rowb = (cuuint64_t)D * 2;
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
     const cuuint64_t st[3] = {rows > 1 ? (cuuint64_t)s.token : rowb, heads > 1 ? (cuuint64_t)s.head : rowb,
                               batch > 1 ? (cuuint64_t)s.item : rowb};
-    const cuuint32_t box[4] = {64u, (cuuint32_t)kTile, 1u, 1u}, one[4] = {1u, 1u, 1u, 1u};
+    const cuuint32_t box[4] = {64u, (cuuint32_t)box_rows, 1u, 1u}, one[4] = {1u, 1u, 1u, 1u};
     return enc(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, st,
                box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -484,17 +767,35 @@ int launch_kb(const SinkArgs& a, int items, int per, const CUtensorMap& tq, cons
     return cudaGetLastError() == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }
 
+template <bool BF>
+int launch_wide(const SinkArgs& a, int items, int per, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                cudaStream_t st) {
+    if (cudaFuncSetAttribute(sink_wide_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return RKV_ERR_CUDA;
+    }
+    sink_wide_kernel<BF><<<items < kSms ? items : kSms, kWideThreads, kWideSmem, st>>>(a, items, per, tq, tk, tv);
+    return cudaGetLastError() == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
+}
+
 }  // namespace
 
-bool sink_tc_supported(const SinkArgs& a, int dtype) { return dtype != RKV_F32 && a.D <= 128; }
+bool sink_tc_supported(int dtype) { return dtype != RKV_F32; }
 
 int launch_sink_tc(SinkArgs a, int dtype, int batch, cudaStream_t st) {
     const bool bf = dtype == RKV_BF16;
     CUtensorMap tq, tk, tv;
-    if (!encode(&tq, a.Q, bf, a.D, a.len_q, a.H, batch, a.qs) || !encode(&tk, a.K, bf, a.D, a.len_k, a.HK, batch, a.ks) ||
-        !encode(&tv, a.V, bf, a.D, a.len_k, a.HK, batch, a.ks))
+    const int keys = a.D <= 128 ? kTile : kWideKeys;
+    if (!encode(&tq, a.Q, bf, a.D, a.len_q, a.H, batch, a.qs, kTile) || !encode(&tk, a.K, bf, a.D, a.len_k, a.HK, batch, a.ks, keys) ||
+        !encode(&tv, a.V, bf, a.D, a.len_k, a.HK, batch, a.ks, keys))
         return RKV_ERR_CUDA;
     a.qtiles = (a.len_q + kTile - 1) / kTile;
+    if (a.D > 128) {
+        const long long per = (long long)batch * a.H, items = (long long)a.qtiles * per;
+        if (items > (1 << 30)) return RKV_ERR_UNSUPPORTED;
+        return bf ? launch_wide<true>(a, (int)items, (int)per, tq, tk, tv, st)
+                  : launch_wide<false>(a, (int)items, (int)per, tq, tk, tv, st);
+    }
     const long long units = (long long)a.G * a.qtiles, per = (long long)batch * a.HK, items = (units + 1) / 2 * per;
     if (units > 0x7FFFFFFELL || items > (1 << 30)) return RKV_ERR_UNSUPPORTED;
     const int n = (int)items, p = (int)per;

@@ -53,6 +53,9 @@ CASES = [
     ("bf16", 200, 2, 1, 129, 129, 0, 0, None),
     ("bf16", 128, 2, 2, 2050, 2050, 64, 512, None),
     ("f16", 128, 1, 1, 128, 4097, 130, 1000, [4000]),
+    ("f16", 256, 3, 1, 1100, 1100, 4, 500, [1100, 700, 64, 63, 0]),
+    ("bf16", 136, 24, 8, 700, 900, 0, 0, None),            # more units than SMs
+    ("f16", 192, 2, 2, 65, 2000, 70, 333, [2000, 1999]),
 ]
 
 
