@@ -10,211 +10,230 @@
 namespace rkv {
 namespace {
 
-constexpr int kBM = 64, kBN = 64, kNT = 256;
-constexpr int kPad = 4;  // floats behind each row of a transposed tile
+constexpr int kBN = 64;  // keys of a tile
 
-template <typename T>
-__device__ __forceinline__ void load4(const uint8_t* p, float* f);
-template <>
-__device__ __forceinline__ void load4<float>(const uint8_t* p, float* f) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-}
-template <>
-__device__ __forceinline__ void load4<__nv_bfloat16>(const uint8_t* p, float* f) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
-    f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
-}
-template <>
-__device__ __forceinline__ void load4<__half>(const uint8_t* p, float* f) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
-    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
-}
-template <typename T>
-__device__ __forceinline__ void store4(uint8_t* p, const float* f);
-template <>
-__device__ __forceinline__ void store4<float>(uint8_t* p, const float* f) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-}
-template <>
-__device__ __forceinline__ void store4<__nv_bfloat16>(uint8_t* p, const float* f) {
-    __nv_bfloat162 v[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
-    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
-}
-template <>
-__device__ __forceinline__ void store4<__half>(uint8_t* p, const float* f) {
-    __half2 v[2] = {__floats2half2_rn(f[0], f[1]), __floats2half2_rn(f[2], f[3])};
-    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
-}
+// fp32 inputs: tf32 products of each operand's top 19 bits and of what they
+// leave, three per product (hi hi + lo hi + hi lo).  One CTA per BM queries of
+// a head, a warp per 16 of them, 64 keys at a time; V arrives under the scores
+// and the next K under the output's products.
+//
+// S = Q K^T has the queries on the rows; its fragment is P's fragment for
+// O += P V when the keys 2 t and 2 t + 1 of eight count as steps t and t + 4,
+// and the order of a product's steps is free.  Likewise a lane's 16-byte chunk
+// of a K row gives four steps of columns, and one of a V row four columns of
+// the output.  Chunks are stored at other places of their rows (c ^ 4 (r % 2)
+// for Q and K, c ^ (r % 8) for V), so that eight lanes' loads lie in different
+// banks.
+template <int DP>
+struct F32Shape {
+    static constexpr int BM = DP <= 128 ? 128 : 64;
+    static constexpr int NT = BM * 2;             // threads: a warp per 16 queries
+    static constexpr int ROW = DP * 4;            // bytes
+    static constexpr int SMEM = (BM + 2 * kBN) * ROW;
+};
 
-// rows x D values of a tile into dst[d][row] (transposed) or dst[row][d];
-// rows from `valid` on become zero and are not read.
-template <typename T, bool TR>
-__device__ __forceinline__ void stage(const uint8_t* src, long long stride, int valid, int D, float* dst, int pitch) {
-    const int q4 = D / 4;
-    for (int e = threadIdx.x; e < 64 * q4; e += kNT) {
-        const int r = TR ? (e & 63) : e / q4, d = 4 * (TR ? (e >> 6) : e - r * q4);
-        float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (r < valid) load4<T>(src + r * stride + d * (int)sizeof(T), f);
-        if (TR) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dst[(d + i) * pitch + r] = f[i];
-        } else {
-            *reinterpret_cast<float4*>(dst + r * pitch + d) = make_float4(f[0], f[1], f[2], f[3]);
-        }
-    }
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
 }
-
-__host__ __device__ constexpr size_t simt_floats(int D) {
-    return (size_t)D * (kBM + kPad) + (size_t)(D * (kBN + kPad) > kBN * (D + kPad) ? D * (kBN + kPad) : kBN * (D + kPad)) +
-           (size_t)kBN * (kBM + kPad);
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// What a tf32 operand (the top 19 bits) leaves of a value.
+__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) {
+    return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u));
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int e) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; }
 
-// fp32 multiply-adds on the CUDA cores, any type: one CTA of 16 x 16 threads
-// per 64 queries of a head, 64 keys at a time; a thread holds 4 x 4 scores and
-// 4 rows x 4 NC columns of the output.
-template <typename T, int NC>
-__global__ void __launch_bounds__(kNT) sink_simt_kernel(const SinkArgs a) {
-    extern __shared__ __align__(16) float sm[];
-    const int D = a.D, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    float* Qs = sm;                                  // [D][64 + pad]
-    float* KV = Qs + D * (kBM + kPad);               // K [D][64 + pad], then V [64][D + pad]
-    float* Ps = KV + (simt_floats(D) - (size_t)D * (kBM + kPad) - (size_t)kBN * (kBM + kPad));  // [64 keys][64 + pad]
+template <int DP>
+__global__ void __launch_bounds__(F32Shape<DP>::NT) sink_f32_kernel(const SinkArgs a) {
+    using S = F32Shape<DP>;
+    constexpr int CH = DP / 4;  // 16-byte chunks of a row
+    extern __shared__ __align__(128) uint8_t smem[];
+    const uint32_t qs = smem_u32(smem), ks = qs + S::BM * S::ROW, vs = ks + kBN * S::ROW;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     long long id = blockIdx.x;
-    const int qt = a.qtiles - 1 - (int)(id % a.qtiles);  // the longest rows first
-    id /= a.qtiles;
-    const int h = (int)(id % a.H), b = (int)(id / a.H), hk = h / a.G;
-    const int i0 = qt * kBM;
-    const SinkRange rg = sink_range(a, b, i0, kBM, kBN);
+    const int rest = (int)(id % ((long long)a.H * a.batch));
+    const int qt = a.qtiles - 1 - (int)(id / ((long long)a.H * a.batch));  // the longest rows first
+    const int h = rest % a.H, b = rest / a.H, hk = h / a.G, i0 = qt * S::BM;
+    const SinkRange rg = sink_range(a, b, i0, S::BM, kBN);
     const int tiles = rg.count();
     if (tiles == 0) return;
     const uint8_t* K = a.K + (size_t)b * a.ks.item + (size_t)hk * a.ks.head;
     const uint8_t* V = a.V + (size_t)b * a.ks.item + (size_t)hk * a.ks.head;
-    const int qrows = min(min(kBM, a.len_q - i0), rg.n - rg.p0);
-    stage<T, true>(a.Q + (size_t)b * a.qs.item + (size_t)h * a.qs.head + (size_t)i0 * a.qs.token, a.qs.token, qrows, D, Qs,
-                   kBM + kPad);
-    float m[4], l[4], o[4][NC][4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[r][c][e] = 0.0f;
-    }
-    for (int it = 0; it < tiles; ++it) {
-        const int j0 = rg.tile(it) * kBN, valid = min(kBN, rg.n - j0);
-        __syncthreads();
-        stage<T, true>(K + (size_t)j0 * a.ks.token, a.ks.token, valid, D, KV, kBN + kPad);
-        __syncthreads();
-        float s[4][4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) s[r][c] = 0.0f;
-#pragma unroll 4
-        for (int d = 0; d < D; ++d) {
-            const float4 q = *reinterpret_cast<const float4*>(Qs + d * (kBM + kPad) + ty * 4);
-            const float4 k = *reinterpret_cast<const float4*>(KV + d * (kBN + kPad) + tx * 4);
-            const float qv[4] = {q.x, q.y, q.z, q.w}, kv[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) s[r][c] = fmaf(qv[r], kv[c], s[r][c]);
+    const uint8_t* Q = a.Q + (size_t)b * a.qs.item + (size_t)h * a.qs.head + (size_t)i0 * a.qs.token;
+    const int qrows = min(min(S::BM, a.len_q - i0), rg.n - rg.p0);  // rows that are written
+    const int chunks = a.D / 4;
+    // rows of a tile, zeros (nothing is read) behind `valid` rows and behind dim_head
+    auto fetch = [&](uint32_t dst, const uint8_t* src, long long stride, int rows, int valid, bool isv) {
+        for (int e = tid; e < rows * CH; e += S::NT) {
+            const int r = e / CH, c = e % CH;
+            const bool real = r < valid && c < chunks;
+            copy16(dst + r * S::ROW + ((c ^ (isv ? r & 7 : (r & 1) << 2)) << 4), real ? src + r * stride + c * 16 : a.Q, real);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto key_tile = [&](int it, bool isv) {
+        const int j0 = rg.tile(it) * kBN;
+        fetch(isv ? vs : ks, (isv ? V : K) + (size_t)j0 * a.ks.token, a.ks.token, kBN, min(kBN, rg.n - j0), isv);
+    };
+    fetch(qs, Q, a.qs.token, S::BM, qrows, false);
+    key_tile(0, false);
+
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // rows g and g + 8 of the warp's 16
+    float o[DP / 8][4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int p = rg.p0 + ty * 4 + r;
-            float mt = -INFINITY;
+    for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                s[r][c] = sink_sees(a, rg.n, p, j0 + tx * 4 + c) ? s[r][c] * a.scale2 : -INFINITY;
-                mt = fmaxf(mt, s[r][c]);
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
+    const uint32_t qw = qs + warp * 16 * S::ROW;
+    const int pg = rg.p0 + warp * 16 + g;  // position of row g
+    for (int it = 0; it < tiles; ++it) {
+        key_tile(it, true);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // K (and Q) are here, V is on its way
+        __syncthreads();
+        float s[8][4];
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+        const int swz = (g & 1) << 2;
+#pragma unroll 1
+        for (int blk = 0; blk < DP / 32; ++blk) {
+            // rows g and g + 8, chunks t and t + 4 of 32 columns
+            const int c = blk * 8 + t;
+            const uint4 x0 = lds16(qw + g * S::ROW + ((c ^ swz) << 4)), x1 = lds16(qw + (g + 8) * S::ROW + ((c ^ swz) << 4));
+            const uint4 x2 = lds16(qw + g * S::ROW + (((c + 4) ^ swz) << 4)), x3 = lds16(qw + (g + 8) * S::ROW + (((c + 4) ^ swz) << 4));
+            uint32_t qh[4][4], ql[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                qh[e][0] = word(x0, e), qh[e][1] = word(x1, e), qh[e][2] = word(x2, e), qh[e][3] = word(x3, e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ql[e][i] = tf32_rest(qh[e][i]);
             }
 #pragma unroll
-            for (int x = 1; x < 16; x <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+            for (int n = 0; n < 8; ++n) {
+                const uint32_t kr = ks + (n * 8 + g) * S::ROW;
+                const uint4 y0 = lds16(kr + ((c ^ swz) << 4)), y1 = lds16(kr + (((c + 4) ^ swz) << 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t b0 = word(y0, e), b1 = word(y1, e);
+                    mma_tf32(s[n], qh[e], tf32_rest(b0), tf32_rest(b1));
+                    mma_tf32(s[n], ql[e], b0, b1);
+                    mma_tf32(s[n], qh[e], b0, b1);
+                }
+            }
+        }
+        // columns 8 n + 2 t and + 1 of rows g (s[n][0], s[n][1]) and g + 8
+        const int j0 = rg.tile(it) * kBN, pw = pg - g;  // the warp's rows are at positions pw .. pw + 15
+        const bool whole = j0 + kBN - 1 <= pw && j0 + kBN <= rg.n && (a.window <= 0 || j0 > pw + 15 - a.window || j0 + kBN <= a.sinks);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int p = pg + 8 * r;
+            float mt = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float& x = s[n][2 * r + e];
+                    x = whole || sink_sees(a, rg.n, p, j0 + n * 8 + 2 * t + e) ? x * a.scale2 : -INFINITY;
+                    mt = fmaxf(mt, x);
+                }
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
             const float mn = fmaxf(m[r], mt), mf = mn == -INFINITY ? 0.0f : mn;
             const float corr = exp2f(m[r] - mf);
             m[r] = mn;
             float sum = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                s[r][c] = exp2f(s[r][c] - mf);
-                sum += s[r][c];
-            }
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s[n][2 * r + e] = exp2f(s[n][2 * r + e] - mf);
+                    sum += s[n][2 * r + e];
+                }
             l[r] = l[r] * corr + sum;
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[r][c][e] *= corr;
+            for (int n = 0; n < DP / 8; ++n) {
+                o[n][2 * r] *= corr;
+                o[n][2 * r + 1] *= corr;
+            }
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // V is here, and every warp is done with K
+        if (it + 1 < tiles) key_tile(it + 1, false);
+#pragma unroll 1
+        for (int n8 = 0; n8 < 8; ++n8) {
+            // keys 8 n8 + 2 t and + 1 are steps t and t + 4
+            uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<float4*>(Ps + (tx * 4 + c) * (kBM + kPad) + ty * 4) =
-                make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
-        __syncthreads();  // the scores are done with K; P is written
-        stage<T, false>(V + (size_t)j0 * a.ks.token, a.ks.token, valid, D, KV, D + kPad);
-        __syncthreads();
-#pragma unroll 2
-        for (int k = 0; k < kBN; ++k) {
-            const float4 p4 = *reinterpret_cast<const float4*>(Ps + k * (kBM + kPad) + ty * 4);
-            const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+            for (int n = 0; n < 8; ++n)
+                if (n == n8) {
+                    ph[0] = __float_as_uint(s[n][0]), ph[1] = __float_as_uint(s[n][2]);
+                    ph[2] = __float_as_uint(s[n][1]), ph[3] = __float_as_uint(s[n][3]);
+                }
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                if (tx * 4 + c * 64 < D) {
-                    const float4 v = *reinterpret_cast<const float4*>(KV + k * (D + kPad) + tx * 4 + c * 64);
+            for (int i = 0; i < 4; ++i) pl[i] = tf32_rest(ph[i]);
+            const int r0 = n8 * 8 + 2 * t;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        o[r][c][0] = fmaf(p[r], v.x, o[r][c][0]);
-                        o[r][c][1] = fmaf(p[r], v.y, o[r][c][1]);
-                        o[r][c][2] = fmaf(p[r], v.z, o[r][c][2]);
-                        o[r][c][3] = fmaf(p[r], v.w, o[r][c][3]);
-                    }
+            for (int j = 0; j < DP / 32; ++j) {
+                const int c = g + 8 * j;
+                const uint4 u = lds16(vs + r0 * S::ROW + ((c ^ (r0 & 7)) << 4));
+                const uint4 w = lds16(vs + (r0 + 1) * S::ROW + ((c ^ ((r0 + 1) & 7)) << 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t b0 = word(u, e), b1 = word(w, e);
+                    mma_tf32(o[4 * j + e], ph, tf32_rest(b0), tf32_rest(b1));
+                    mma_tf32(o[4 * j + e], pl, b0, b1);
+                    mma_tf32(o[4 * j + e], ph, b0, b1);
                 }
             }
         }
+        __syncthreads();  // every warp is done with V
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
-        const int row = ty * 4 + r;
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        const int row = warp * 16 + g + 8 * r;
         if (row >= qrows) continue;
         const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
-        uint8_t* po = a.O + (size_t)b * a.os.item + (size_t)h * a.os.head + (size_t)(i0 + row) * a.os.token;
+        float* po = reinterpret_cast<float*>(a.O + (size_t)b * a.os.item + (size_t)h * a.os.head + (size_t)(i0 + row) * a.os.token);
+        // output column 4 (i + 8 j) + e is column i of tile 4 j + e; this lane has i = 2 t and 2 t + 1
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int d = tx * 4 + c * 64;
-            if (d < D) {
-                const float f[4] = {o[r][c][0] * inv, o[r][c][1] * inv, o[r][c][2] * inv, o[r][c][3] * inv};
-                store4<T>(po + d * (int)sizeof(T), f);
+        for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int d = 4 * (2 * t + x + 8 * j);
+                if (d < a.D)
+                    *reinterpret_cast<float4*>(po + d) = make_float4(o[4 * j][2 * r + x] * inv, o[4 * j + 1][2 * r + x] * inv,
+                                                                     o[4 * j + 2][2 * r + x] * inv, o[4 * j + 3][2 * r + x] * inv);
             }
-        }
-        if (a.lse && tx == 0)
+        if (a.lse && t == 0)
             a.lse[((size_t)b * a.H + h) * a.len_q + i0 + row] =
                 l[r] == 0.0f ? -INFINITY : ((m[r] == -INFINITY ? 0.0f : m[r]) + log2f(l[r])) * 0.693147180559945f;
     }
 }
 
-template <typename T, int NC>
-int launch_simt(const SinkArgs& a, long long blocks, cudaStream_t st) {
-    const size_t smem = simt_floats(a.D) * sizeof(float);
-    if (cudaFuncSetAttribute(sink_simt_kernel<T, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+template <int DP>
+int launch_f32(SinkArgs a, cudaStream_t st) {
+    using S = F32Shape<DP>;
+    a.qtiles = (a.len_q + S::BM - 1) / S::BM;
+    const long long blocks = (long long)a.qtiles * a.H * a.batch;
+    if (blocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
+    if (cudaFuncSetAttribute(sink_f32_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
-    sink_simt_kernel<T, NC><<<(unsigned)blocks, kNT, smem, st>>>(a);
+    sink_f32_kernel<DP><<<(unsigned)blocks, S::NT, S::SMEM, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
-}
-template <typename T>
-int launch_simt_d(const SinkArgs& a, long long blocks, cudaStream_t st) {
-    if (a.D <= 64) return launch_simt<T, 1>(a, blocks, st);
-    if (a.D <= 128) return launch_simt<T, 2>(a, blocks, st);
-    return launch_simt<T, 4>(a, blocks, st);
 }
 
 }  // namespace
@@ -269,6 +288,7 @@ extern "C" int rkv_sink_attention(const void* Q, const void* K, const void* V, i
     a.lens = lens;
     a.len_q = len_q;
     a.len_k = len_k;
+    a.batch = batch;
     a.H = num_heads;
     a.HK = num_heads_kv;
     a.G = num_heads / num_heads_kv;
@@ -278,13 +298,8 @@ extern "C" int rkv_sink_attention(const void* Q, const void* K, const void* V, i
     a.scale2 = 1.4426950408889634f / sqrtf((float)dim_head);
     a.err = static_cast<int*>(workspace);
     if (cudaMemsetAsync(a.err, 0, sizeof(int), st) != cudaSuccess) return RKV_ERR_CUDA;
-    if (sink_tc_supported(dtype)) return launch_sink_tc(a, dtype, batch, st);
-    a.qtiles = (len_q + kBM - 1) / kBM;
-    const long long blocks = (long long)a.qtiles * num_heads * batch;
-    if (blocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
-    switch (dtype) {
-        case RKV_F32: return launch_simt_d<float>(a, blocks, st);
-        case RKV_BF16: return launch_simt_d<__nv_bfloat16>(a, blocks, st);
-        default: return launch_simt_d<__half>(a, blocks, st);
-    }
+    if (dtype != RKV_F32) return launch_sink_tc(a, dtype, batch, st);
+    if (dim_head <= 64) return launch_f32<64>(a, st);
+    if (dim_head <= 128) return launch_f32<128>(a, st);
+    return launch_f32<256>(a, st);
 }

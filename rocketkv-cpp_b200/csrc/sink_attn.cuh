@@ -13,7 +13,7 @@ struct SinkArgs {
     float* lse;
     const int* lens;
     rkv_row_strides qs, ks, os;  // bytes
-    int len_q, len_k, H, HK, G, D, sinks, window;
+    int batch, len_q, len_k, H, HK, G, D, sinks, window;
     int qtiles;
     float scale2;  // log2(e) / sqrt(D)
     int* err;
@@ -49,7 +49,6 @@ __device__ __forceinline__ bool sink_sees(const SinkArgs& a, int n, int p, int j
 }
 
 // 16-bit inputs on the tcgen05 tensor cores (sink_attn_tc.cu)
-bool sink_tc_supported(int dtype);
 int launch_sink_tc(SinkArgs a, int dtype, int batch, cudaStream_t st);
 
 }  // namespace rkv

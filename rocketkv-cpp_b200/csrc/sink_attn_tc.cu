@@ -780,8 +780,6 @@ int launch_wide(const SinkArgs& a, int items, int per, const CUtensorMap& tq, co
 
 }  // namespace
 
-bool sink_tc_supported(int dtype) { return dtype != RKV_F32; }
-
 int launch_sink_tc(SinkArgs a, int dtype, int batch, cudaStream_t st) {
     const bool bf = dtype == RKV_BF16;
     CUtensorMap tq, tk, tv;
