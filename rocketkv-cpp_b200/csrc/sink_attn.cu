@@ -41,7 +41,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -119,15 +119,22 @@ __global__ void __launch_bounds__(F32Shape<DP>::NT) sink_f32_kernel(const SinkAr
                 for (int i = 0; i < 4; ++i) ql[e][i] = tf32_rest(qh[e][i]);
             }
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                const uint32_t kr = ks + (n * 8 + g) * S::ROW;
-                const uint4 y0 = lds16(kr + ((c ^ swz) << 4)), y1 = lds16(kr + (((c + 4) ^ swz) << 4));
+            for (int n0 = 0; n0 < 8; n0 += 4) {  // products into four accumulators in turn: one alone waits for itself
+                uint4 y0[4], y1[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t kr = ks + ((n0 + n) * 8 + g) * S::ROW;
+                    y0[n] = lds16(kr + ((c ^ swz) << 4));
+                    y1[n] = lds16(kr + (((c + 4) ^ swz) << 4));
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t b0 = word(y0, e), b1 = word(y1, e);
-                    mma_tf32(s[n], qh[e], tf32_rest(b0), tf32_rest(b1));
-                    mma_tf32(s[n], ql[e], b0, b1);
-                    mma_tf32(s[n], qh[e], b0, b1);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mma_tf32(s[n0 + n], qh[e], tf32_rest(word(y0[n], e)), tf32_rest(word(y1[n], e)));
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mma_tf32(s[n0 + n], ql[e], word(y0[n], e), word(y1[n], e));
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mma_tf32(s[n0 + n], qh[e], word(y0[n], e), word(y1[n], e));
                 }
             }
         }
@@ -188,12 +195,11 @@ __global__ void __launch_bounds__(F32Shape<DP>::NT) sink_f32_kernel(const SinkAr
                 const uint4 u = lds16(vs + r0 * S::ROW + ((c ^ (r0 & 7)) << 4));
                 const uint4 w = lds16(vs + (r0 + 1) * S::ROW + ((c ^ ((r0 + 1) & 7)) << 4));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t b0 = word(u, e), b1 = word(w, e);
-                    mma_tf32(o[4 * j + e], ph, tf32_rest(b0), tf32_rest(b1));
-                    mma_tf32(o[4 * j + e], pl, b0, b1);
-                    mma_tf32(o[4 * j + e], ph, b0, b1);
-                }
+                for (int e = 0; e < 4; ++e) mma_tf32(o[4 * j + e], ph, tf32_rest(word(u, e)), tf32_rest(word(w, e)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mma_tf32(o[4 * j + e], pl, word(u, e), word(w, e));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mma_tf32(o[4 * j + e], ph, word(u, e), word(w, e));
             }
         }
         __syncthreads();  // every warp is done with V
