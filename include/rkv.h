@@ -376,9 +376,9 @@ int rkv_paged_append(const rkv_paged_cache* cache, const void* k, const void* v,
  * visible token's attention weight, summed over the query heads of its KV
  * head, is added to its entry (other entries keep their values), which is
  * what rkv_weight_evict ranks by.  max_len: host bound on lens (it fixes the
- * launch, so a captured call serves every length up to it).  The cache's
- * length is split over CTAs by (batch, heads, max_len) alone and the parts are
- * joined in a fixed order: results repeat bit for bit.
+ * launch, so a captured call serves every length up to it).  The split of the
+ * cache over CTAs does not depend on what lens holds and the parts are joined
+ * in a fixed order: results repeat bit for bit.
  * Workspace: device, 16-byte aligned, not shared with a call that may run at
  * the same time; with_weights: whether weights will be passed.  Asynchronous
  * on `stream`; allocates nothing. */
@@ -422,12 +422,15 @@ int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, int weight_st
  * heads and items back to back).  dim_head: a multiple of 8, at most 256;
  * num_heads a multiple of num_heads_kv.  lse (nullable):
  * [batch][num_heads][len_q] fp32.  O must not overlap the inputs.
- * Workspace: device, 16-byte aligned; holds the error word that
- * rkv_workspace_status reads.  Asynchronous on `stream`; allocates nothing. */
+ * Workspace: device, 16-byte aligned, not shared with a call that may run at
+ * the same time; the size serves every sinks and window.  It begins with the
+ * error word that rkv_workspace_status reads, and holds the parts of the keys
+ * where few queries meet many.  Asynchronous on `stream`; allocates nothing. */
 typedef struct rkv_row_strides {
     long long item, head, token;
 } rkv_row_strides;
-int rkv_sink_attention_workspace_size(size_t* bytes);
+int rkv_sink_attention_workspace_size(int dtype, int len_q, int len_k, int batch, int num_heads, int num_heads_kv,
+                                      int dim_head, size_t* bytes);
 int rkv_sink_attention(const void* Q, const void* K, const void* V, int dtype, int len_q, int len_k, int batch,
                        int num_heads, int num_heads_kv, int dim_head, const rkv_row_strides* q_strides,
                        const rkv_row_strides* kv_strides, const int* lens, int sinks, int window, void* O,

@@ -60,12 +60,21 @@ __global__ void __launch_bounds__(F32Shape<DP>::NT) sink_f32_kernel(const SinkAr
     const uint32_t qs = smem_u32(smem), ks = qs + S::BM * S::ROW, vs = ks + kBN * S::ROW;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     long long id = blockIdx.x;
+    const int part = (int)(id % a.parts);
+    id /= a.parts;
     const int rest = (int)(id % ((long long)a.H * a.batch));
     const int qt = a.qtiles - 1 - (int)(id / ((long long)a.H * a.batch));  // the longest rows first
     const int h = rest % a.H, b = rest / a.H, hk = h / a.G, i0 = qt * S::BM;
-    const SinkRange rg = sink_range(a, b, i0, S::BM, kBN);
-    const int tiles = rg.count();
-    if (tiles == 0) return;
+    SinkRange rg = sink_range(a, b, i0, S::BM, kBN);
+    const int tiles = rg.part(part, a.parts);
+    const size_t prow0 = (((size_t)part * a.batch + b) * a.H + h) * a.len_q + i0;  // the first row of the part
+    asm volatile("griddepcontrol.launch_dependents;");  // a join may be scheduled (it waits for this grid)
+    if (tiles == 0) {
+        if (a.parts > 1)
+            for (int i = tid; i < min(min(S::BM, a.len_q - i0), rg.n - rg.p0); i += S::NT)
+                a.part_ml[prow0 + i] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
     const uint8_t* K = a.K + (size_t)b * a.ks.item + (size_t)hk * a.ks.head;
     const uint8_t* V = a.V + (size_t)b * a.ks.item + (size_t)hk * a.ks.head;
     const uint8_t* Q = a.Q + (size_t)b * a.qs.item + (size_t)h * a.qs.head + (size_t)i0 * a.qs.token;
@@ -210,8 +219,10 @@ __global__ void __launch_bounds__(F32Shape<DP>::NT) sink_f32_kernel(const SinkAr
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         const int row = warp * 16 + g + 8 * r;
         if (row >= qrows) continue;
-        const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
-        float* po = reinterpret_cast<float*>(a.O + (size_t)b * a.os.item + (size_t)h * a.os.head + (size_t)(i0 + row) * a.os.token);
+        const float inv = a.parts > 1 ? 1.0f : l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+        float* po = a.parts > 1 ? a.part_o + (prow0 + row) * a.D
+                                : reinterpret_cast<float*>(a.O + (size_t)b * a.os.item + (size_t)h * a.os.head +
+                                                           (size_t)(i0 + row) * a.os.token);
         // output column 4 (i + 8 j) + e is column i of tile 4 j + e; this lane has i = 2 t and 2 t + 1
 #pragma unroll
         for (int j = 0; j < DP / 32; ++j)
@@ -222,17 +233,104 @@ __global__ void __launch_bounds__(F32Shape<DP>::NT) sink_f32_kernel(const SinkAr
                     *reinterpret_cast<float4*>(po + d) = make_float4(o[4 * j][2 * r + x] * inv, o[4 * j + 1][2 * r + x] * inv,
                                                                      o[4 * j + 2][2 * r + x] * inv, o[4 * j + 3][2 * r + x] * inv);
             }
-        if (a.lse && t == 0)
+        if (a.parts > 1) {
+            if (t == 0) a.part_ml[prow0 + row] = make_float2(m[r] == -INFINITY ? 0.0f : m[r], l[r]);
+        } else if (a.lse && t == 0)
             a.lse[((size_t)b * a.H + h) * a.len_q + i0 + row] =
                 l[r] == 0.0f ? -INFINITY : ((m[r] == -INFINITY ? 0.0f : m[r]) + log2f(l[r])) * 0.693147180559945f;
     }
+}
+
+// Joins the parts of the keys: a warp per row.  m and l of a part that saw no key are -inf (or 0) and 0.
+template <typename T>
+__device__ __forceinline__ void store4(uint8_t* p, const float4& v);
+template <>
+__device__ __forceinline__ void store4<float>(uint8_t* p, const float4& v) { *reinterpret_cast<float4*>(p) = v; }
+template <>
+__device__ __forceinline__ void store4<__nv_bfloat16>(uint8_t* p, const float4& v) {
+    __nv_bfloat162 x[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(x);
+}
+template <>
+__device__ __forceinline__ void store4<__half>(uint8_t* p, const float4& v) {
+    __half2 x[2] = {__floats2half2_rn(v.x, v.y), __floats2half2_rn(v.z, v.w)};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(x);
+}
+template <typename T>
+__global__ void __launch_bounds__(256) sink_join_kernel(const SinkArgs a) {
+    const long long rows = (long long)a.batch * a.H * a.len_q;
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    const int i = (int)(row % a.len_q), h = (int)(row / a.len_q % a.H), b = (int)(row / a.len_q / a.H);
+    const int n = a.lens ? min(max(a.lens[b], 0), a.len_k) : a.len_k;
+    if (i + a.len_k - a.len_q >= n) return;  // behind the sequence's end
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const float2 ml = lane < a.parts ? a.part_ml[lane * rows + row] : make_float2(-INFINITY, 0.0f);
+    // a part without a visible key has l = 0, whatever its m
+    float m = ml.y == 0.0f ? -INFINITY : ml.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float mf = m == -INFINITY ? 0.0f : m;
+    const float w = ml.y == 0.0f ? 0.0f : exp2f(ml.x - mf);
+    float l = ml.y * w;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint8_t* po = a.O + (size_t)b * a.os.item + (size_t)h * a.os.head + (size_t)i * a.os.token;
+    for (int c0 = 0; c0 < a.D / 4; c0 += 32) {
+        const int c = c0 + lane;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p = 0; p < a.parts; ++p) {
+            const float wp = __shfl_sync(0xffffffffu, w, p);
+            if (wp != 0.0f && c < a.D / 4) {  // (a NaN weight counts)
+                const float4 x = *reinterpret_cast<const float4*>(a.part_o + (p * rows + row) * a.D + 4 * c);
+                o.x = fmaf(x.x, wp, o.x), o.y = fmaf(x.y, wp, o.y), o.z = fmaf(x.z, wp, o.z), o.w = fmaf(x.w, wp, o.w);
+            }
+        }
+        if (c < a.D / 4) store4<T>(po + c * 4 * sizeof(T), make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    }
+    if (lane == 0 && a.lse) a.lse[row] = l == 0.0f ? -INFINITY : (mf + log2f(l)) * 0.693147180559945f;
+}
+template <typename T>
+int launch_join(const SinkArgs& a, cudaStream_t st) {
+    const long long rows = (long long)a.batch * a.H * a.len_q;
+    const cudaError_t e = launch_pdl(sink_join_kernel<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
+}
+
+// CTAs' worth of queries, and the rows and keys of one's tiles.
+long long sink_items(const SinkArgs& a, int dtype, int* rows, int* keys) {
+    if (dtype != RKV_F32) return sink_tc_items(a, rows, keys);
+    *rows = a.D <= 128 ? F32Shape<128>::BM : F32Shape<256>::BM;
+    *keys = kBN;
+    return (long long)((a.len_q + *rows - 1) / *rows) * a.batch * a.H;
+}
+struct SinkPlan {
+    int parts;
+    size_t off_ml, off_o, bytes;
+};
+// window 0: the most parts of any window.
+SinkPlan sink_plan(const SinkArgs& a, int dtype, int sinks, int window) {
+    int rows, keys;
+    const long long items = sink_items(a, dtype, &rows, &keys);
+    SinkPlan p{};
+    p.parts = sink_parts(items, sink_tiles_max(a.len_k, sinks, window, rows, keys));
+    p.off_ml = p.off_o = p.bytes = kWorkspaceHeader;
+    if (p.parts > 1) {
+        const size_t n = (size_t)p.parts * a.batch * a.H * a.len_q;
+        p.off_o = align_up(p.off_ml + n * sizeof(float2), kWorkspaceAlign);
+        p.bytes = align_up(p.off_o + n * a.D * sizeof(float), kWorkspaceAlign);
+    }
+    return p;
 }
 
 template <int DP>
 int launch_f32(SinkArgs a, cudaStream_t st) {
     using S = F32Shape<DP>;
     a.qtiles = (a.len_q + S::BM - 1) / S::BM;
-    const long long blocks = (long long)a.qtiles * a.H * a.batch;
+    const long long blocks = (long long)a.qtiles * a.H * a.batch * a.parts;
     if (blocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
     if (cudaFuncSetAttribute(sink_f32_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
         (void)cudaGetLastError();
@@ -247,9 +345,28 @@ int launch_f32(SinkArgs a, cudaStream_t st) {
 
 using namespace rkv;
 
-extern "C" int rkv_sink_attention_workspace_size(size_t* bytes) {
-    if (!bytes) return RKV_ERR_INVALID_ARG;
-    *bytes = kWorkspaceHeader;
+static int sink_shape_check(int dtype, int len_q, int len_k, int batch, int num_heads, int num_heads_kv, int dim_head) {
+    if (dtype != RKV_F32 && dtype != RKV_BF16 && dtype != RKV_F16) return RKV_ERR_INVALID_ARG;
+    if (len_q < 0 || len_k < len_q || batch < 0 || num_heads <= 0 || num_heads_kv <= 0 || num_heads % num_heads_kv != 0 ||
+        dim_head <= 0)
+        return RKV_ERR_INVALID_ARG;
+    if (dim_head % 8 != 0 || dim_head > 256 || len_k > (1 << 30)) return RKV_ERR_UNSUPPORTED;
+    return RKV_OK;
+}
+
+extern "C" int rkv_sink_attention_workspace_size(int dtype, int len_q, int len_k, int batch, int num_heads, int num_heads_kv,
+                                                 int dim_head, size_t* bytes) {
+    const int rc = sink_shape_check(dtype, len_q, len_k, batch, num_heads, num_heads_kv, dim_head);
+    if (rc || !bytes) return rc ? rc : (int)RKV_ERR_INVALID_ARG;
+    SinkArgs a{};
+    a.batch = batch;
+    a.len_q = len_q;
+    a.len_k = len_k;
+    a.H = num_heads;
+    a.HK = num_heads_kv;
+    a.G = num_heads / num_heads_kv;
+    a.D = dim_head;
+    *bytes = sink_plan(a, dtype, 0, 0).bytes;
     return RKV_OK;
 }
 
@@ -258,11 +375,9 @@ extern "C" int rkv_sink_attention(const void* Q, const void* K, const void* V, i
                                   const rkv_row_strides* kv_strides, const int* lens, int sinks, int window, void* O,
                                   const rkv_row_strides* o_strides, float* lse, void* workspace, size_t workspace_bytes,
                                   void* stream) {
-    if (dtype != RKV_F32 && dtype != RKV_BF16 && dtype != RKV_F16) return RKV_ERR_INVALID_ARG;
-    if (len_q < 0 || len_k < len_q || batch < 0 || num_heads <= 0 || num_heads_kv <= 0 || num_heads % num_heads_kv != 0 ||
-        dim_head <= 0 || sinks < 0 || window < 0)
-        return RKV_ERR_INVALID_ARG;
-    if (dim_head % 8 != 0 || dim_head > 256 || len_k > (1 << 30)) return RKV_ERR_UNSUPPORTED;
+    const int rc = sink_shape_check(dtype, len_q, len_k, batch, num_heads, num_heads_kv, dim_head);
+    if (rc) return rc;
+    if (sinks < 0 || window < 0) return RKV_ERR_INVALID_ARG;
     if (batch == 0 || len_q == 0) return RKV_OK;
     const long long rowb = (long long)dim_head * (dtype == RKV_F32 ? 4 : 2);
     SinkArgs a{};
@@ -283,8 +398,6 @@ extern "C" int rkv_sink_attention(const void* Q, const void* K, const void* V, i
     if ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V) |
          reinterpret_cast<uintptr_t>(O)) & 15)
         return RKV_ERR_INVALID_ARG;
-    if (!workspace || workspace_bytes < kWorkspaceHeader || (reinterpret_cast<uintptr_t>(workspace) & 15))
-        return RKV_ERR_WORKSPACE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     a.Q = static_cast<const uint8_t*>(Q);
     a.K = static_cast<const uint8_t*>(K);
@@ -303,9 +416,18 @@ extern "C" int rkv_sink_attention(const void* Q, const void* K, const void* V, i
     a.window = window < len_k ? window : len_k;   // mean the same and could overflow below
     a.scale2 = 1.4426950408889634f / sqrtf((float)dim_head);
     a.err = static_cast<int*>(workspace);
+    const SinkPlan plan = sink_plan(a, dtype, a.sinks, a.window);
+    if (!workspace || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)) return RKV_ERR_WORKSPACE;
+    a.parts = plan.parts;
+    a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.off_ml);
+    a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.off_o);
     if (cudaMemsetAsync(a.err, 0, sizeof(int), st) != cudaSuccess) return RKV_ERR_CUDA;
-    if (dtype != RKV_F32) return launch_sink_tc(a, dtype, batch, st);
-    if (dim_head <= 64) return launch_f32<64>(a, st);
-    if (dim_head <= 128) return launch_f32<128>(a, st);
-    return launch_f32<256>(a, st);
+    int done;
+    if (dtype != RKV_F32)
+        done = launch_sink_tc(a, dtype, batch, st);
+    else
+        done = dim_head <= 64 ? launch_f32<64>(a, st) : dim_head <= 128 ? launch_f32<128>(a, st) : launch_f32<256>(a, st);
+    if (done || a.parts == 1) return done;
+    return dtype == RKV_F32 ? launch_join<float>(a, st)
+           : dtype == RKV_BF16 ? launch_join<__nv_bfloat16>(a, st) : launch_join<__half>(a, st);
 }

@@ -32,7 +32,6 @@ namespace {
 
 constexpr int kTile = 128;            // queries of a unit, keys of a tile
 constexpr int kThreads = 384;
-constexpr int kSms = 148;
 constexpr int kBlk = kTile * 128;     // bytes of a 128-row block of 64 columns
 constexpr float kGrow = 8.0f;         // log2 growth of a row's maximum that is carried without a rescale
 
@@ -144,16 +143,33 @@ __device__ __forceinline__ void write_rows(uint8_t* so, const uint32_t* o, float
     __syncwarp();
 }
 
+// The same for 32 columns in fp32, of a part's rows (back to back).
+__device__ __forceinline__ void write_part(uint8_t* so, const uint32_t* o, uint32_t rows_ok, float* po, int col0, int D, int lane) {
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+        *reinterpret_cast<uint4*>(so + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        const int r = x * 4 + (lane >> 3), v = lane & 7;
+        const uint4 y = *reinterpret_cast<const uint4*>(so + r * 128 + ((v ^ (r & 7)) << 4));
+        if (((rows_ok >> r) & 1u) && col0 + v * 4 < D) *reinterpret_cast<uint4*>(po + (size_t)r * D + col0 + v * 4) = y;
+    }
+    __syncwarp();
+}
+
 // A pair of units: (query tile, head of the group) numbers u0 and u0 + 1 of one KV head.
 struct Pair {
     int b, hk, u0, nu;
     SinkRange rg;
-    int tiles;
+    int tiles, part;
 };
-// Item i of the list, the latest queries (the longest rows) first.
+// Item i of the list, the latest queries (the longest rows) first, the parts of their keys side by side.
 __device__ __forceinline__ Pair pair_of(const SinkArgs& a, int i, int per) {
     const int units = a.G * a.qtiles, pairs = (units + 1) / 2;
     Pair p;
+    p.part = i % a.parts;
+    i /= a.parts;
     p.u0 = 2 * (pairs - 1 - i / per);
     const int bh = i % per;
     p.b = bh / a.HK;
@@ -161,7 +177,7 @@ __device__ __forceinline__ Pair pair_of(const SinkArgs& a, int i, int per) {
     p.nu = min(2, units - p.u0);
     const int qt0 = p.u0 / a.G, qt1 = (p.u0 + p.nu - 1) / a.G;
     p.rg = sink_range(a, p.b, qt0 * kTile, (qt1 - qt0 + 1) * kTile, kTile);
-    p.tiles = p.rg.count();
+    p.tiles = p.rg.part(p.part, a.parts);
     return p;
 }
 // The k-th item of a CTA: the list goes round the CTAs to and fro, so that each gets long and short ones.
@@ -182,6 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t kStage = KB * kBlk;
     constexpr uint32_t kColO = 256;  // tensor memory: S0, S1 (128 columns each), O0, O1 (64 KB each)
     extern __shared__ uint8_t smem_raw[];
+    asm volatile("griddepcontrol.launch_dependents;");  // a join may be scheduled (it waits for this grid)
     uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     TcBars& B = *reinterpret_cast<TcBars*>(sm);
     volatile int* abort_flag = &B.abort;
@@ -347,11 +364,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int it = item_of(k);
             if (it >= items) break;
             const Pair P = pair_of(a, it, per);
-            if (P.tiles == 0) continue;
-            ++ni;
+            if (P.tiles > 0) ++ni;
             if (u >= P.nu) continue;
             const int qt = (P.u0 + u) / a.G, h = P.hk * a.G + (P.u0 + u) % a.G;
             const int p0 = qt * kTile + a.len_k - a.len_q, p = p0 + row, n = P.rg.n;
+            const int i = qt * kTile + row;
+            const bool real = i < a.len_q && p < n;
+            const size_t prow = (((size_t)P.part * a.batch + P.b) * a.H + h) * a.len_q + i;  // this row of the part
+            if (P.tiles == 0) {
+                if (a.parts > 1 && real) a.part_ml[prow] = make_float2(-INFINITY, 0.0f);
+                continue;
+            }
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < P.tiles; ++j, ++nt) {
                 if (!(ok = warp_wait(&B.s_full[u], (uint32_t)(nt & 1), a.err, abort_flag))) break;
@@ -420,8 +443,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (!ok || !(ok = warp_wait(&B.o_full, (uint32_t)((ni - 1) & 1), a.err, abort_flag))) break;
             tc_fence_after();
-            const int i = qt * kTile + row;
-            const bool real = i < a.len_q && p < n;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             uint8_t* po = a.O + (size_t)P.b * a.os.item + (size_t)h * a.os.head;
             uint32_t o[KB * 64];
@@ -435,6 +456,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive1(&B.o_empty[u]);
             uint8_t* so = stage_o + (warp - 4) * 4096;
             const uint32_t rows_ok = __ballot_sync(0xffffffffu, real);
+            if (a.parts > 1) {
+                if (real) a.part_ml[prow] = make_float2((m == -INFINITY ? 0.0f : m) * a.scale2, l);
+#pragma unroll
+                for (int kb = 0; kb < KB * 2; ++kb)
+                    write_part(so, o + kb * 32, rows_ok, a.part_o + (prow - lane) * a.D, kb * 32, a.D, lane);
+                continue;
+            }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
                 write_rows<BF>(so, o + kb * 64, inv, rows_ok, po, qt * kTile + q4 * 32, a.os.token, kb * 64, a.D, lane);
@@ -468,16 +496,18 @@ struct WideBars {
 struct WideItem {
     int b, h, qt;
     SinkRange rg;
-    int tiles;
+    int tiles, part;
 };
 __device__ __forceinline__ WideItem wide_item(const SinkArgs& a, int i, int per) {
     WideItem w;
+    w.part = i % a.parts;
+    i /= a.parts;
     w.qt = a.qtiles - 1 - i / per;  // the longest rows first
     const int bh = i % per;
     w.b = bh / a.H;
     w.h = bh - w.b * a.H;
     w.rg = sink_range(a, w.b, w.qt * kTile, kTile, kWideKeys);
-    w.tiles = w.rg.count();
+    w.tiles = w.rg.part(w.part, a.parts);
     return w;
 }
 
@@ -487,6 +517,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                      const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
     constexpr int KB = kWideKB, NS = kWideSlots;
     extern __shared__ uint8_t smem_raw[];
+    asm volatile("griddepcontrol.launch_dependents;");  // a join may be scheduled (it waits for this grid)
     uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     WideBars& B = *reinterpret_cast<WideBars*>(sm);
     volatile int* abort_flag = &B.abort;
@@ -624,8 +655,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             const int it = item_of(k);
             if (it >= items) break;
             const WideItem P = wide_item(a, it, per);
-            if (P.tiles == 0) continue;
             const int p0 = P.qt * kTile + a.len_k - a.len_q, p = p0 + row, n = P.rg.n;
+            const int i = P.qt * kTile + row;
+            const bool real = i < a.len_q && p < n;
+            const size_t prow = (((size_t)P.part * a.batch + P.b) * a.H + P.h) * a.len_q + i;  // this row of the part
+            if (P.tiles == 0) {
+                if (a.parts > 1 && real) a.part_ml[prow] = make_float2(-INFINITY, 0.0f);
+                continue;
+            }
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < P.tiles; ++j, ++nt) {
                 const uint32_t ts = to + 256 + (nt & 1) * 128;
@@ -694,8 +731,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
             if (!ok || !(ok = warp_wait(&B.o_full, (uint32_t)(ni++ & 1), a.err, abort_flag))) break;
             tc_fence_after();
-            const int i = P.qt * kTile + row;
-            const bool real = i < a.len_q && p < n;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             uint8_t* po = a.O + (size_t)P.b * a.os.item + (size_t)P.h * a.os.head;
             const uint32_t rows_ok = __ballot_sync(0xffffffffu, real);
@@ -712,7 +747,16 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive1(&B.o_empty);
                 }
-                write_rows<BF>(so, o, inv, rows_ok, po, P.qt * kTile + q4 * 32, a.os.token, kb * 64, a.D, lane);
+                if (a.parts > 1) {
+                    write_part(so, o, rows_ok, a.part_o + (prow - lane) * a.D, kb * 64, a.D, lane);
+                    write_part(so, o + 32, rows_ok, a.part_o + (prow - lane) * a.D, kb * 64 + 32, a.D, lane);
+                } else {
+                    write_rows<BF>(so, o, inv, rows_ok, po, P.qt * kTile + q4 * 32, a.os.token, kb * 64, a.D, lane);
+                }
+            }
+            if (a.parts > 1) {
+                if (real) a.part_ml[prow] = make_float2((m == -INFINITY ? 0.0f : m) * a.scale2, l);
+                continue;
             }
             if (real && a.lse)
                 a.lse[((size_t)P.b * a.H + P.h) * a.len_q + i] =
@@ -763,7 +807,7 @@ int launch_kb(const SinkArgs& a, int items, int per, const CUtensorMap& tq, cons
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
-    sink_tc_kernel<KB, BF><<<items < kSms ? items : kSms, kThreads, smem, st>>>(a, items, per, tq, tk, tv);
+    sink_tc_kernel<KB, BF><<<items < kSinkSms ? items : kSinkSms, kThreads, smem, st>>>(a, items, per, tq, tk, tv);
     return cudaGetLastError() == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }
 
@@ -774,7 +818,7 @@ int launch_wide(const SinkArgs& a, int items, int per, const CUtensorMap& tq, co
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
-    sink_wide_kernel<BF><<<items < kSms ? items : kSms, kWideThreads, kWideSmem, st>>>(a, items, per, tq, tk, tv);
+    sink_wide_kernel<BF><<<items < kSinkSms ? items : kSinkSms, kWideThreads, kWideSmem, st>>>(a, items, per, tq, tk, tv);
     return cudaGetLastError() == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }
 
@@ -789,16 +833,27 @@ int launch_sink_tc(SinkArgs a, int dtype, int batch, cudaStream_t st) {
         return RKV_ERR_CUDA;
     a.qtiles = (a.len_q + kTile - 1) / kTile;
     if (a.D > 128) {
-        const long long per = (long long)batch * a.H, items = (long long)a.qtiles * per;
+        const long long per = (long long)batch * a.H, items = (long long)a.qtiles * per * a.parts;
         if (items > (1 << 30)) return RKV_ERR_UNSUPPORTED;
         return bf ? launch_wide<true>(a, (int)items, (int)per, tq, tk, tv, st)
                   : launch_wide<false>(a, (int)items, (int)per, tq, tk, tv, st);
     }
-    const long long units = (long long)a.G * a.qtiles, per = (long long)batch * a.HK, items = (units + 1) / 2 * per;
+    const long long units = (long long)a.G * a.qtiles, per = (long long)batch * a.HK, items = (units + 1) / 2 * per * a.parts;
     if (units > 0x7FFFFFFELL || items > (1 << 30)) return RKV_ERR_UNSUPPORTED;
     const int n = (int)items, p = (int)per;
     if (a.D <= 64) return bf ? launch_kb<1, true>(a, n, p, tq, tk, tv, st) : launch_kb<1, false>(a, n, p, tq, tk, tv, st);
     return bf ? launch_kb<2, true>(a, n, p, tq, tk, tv, st) : launch_kb<2, false>(a, n, p, tq, tk, tv, st);
+}
+
+long long sink_tc_items(const SinkArgs& a, int* rows, int* keys) {
+    const long long qtiles = (a.len_q + kTile - 1) / kTile;
+    *keys = a.D <= 128 ? kTile : kWideKeys;
+    if (a.D > 128) {
+        *rows = kTile;
+        return qtiles * a.batch * a.H;
+    }
+    *rows = 2 * kTile;  // two units of different query tiles at most
+    return (a.G * qtiles + 1) / 2 * a.batch * a.HK;
 }
 
 }  // namespace rkv

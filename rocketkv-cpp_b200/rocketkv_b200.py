@@ -161,7 +161,7 @@ def lib() -> ctypes.CDLL:
         "rkv_paged_decode_workspace_size": ([_I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)], _I),
         "rkv_paged_decode": ([_VP, _LL, _I, _PCP, _I, _I, _I, _I, _VP, _VP, _VP, _I, _VP, _SZ, _VP], _I),
         "rkv_weight_evict": ([_PCP, _VP, _I, _I, _I, _I, _I, _I, _PCP, _VP, _VP, _I, _VP, _VP], _I),
-        "rkv_sink_attention_workspace_size": ([ctypes.POINTER(_SZ)], _I),
+        "rkv_sink_attention_workspace_size": ([_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)], _I),
         "rkv_sink_attention": ([_VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _RSP, _RSP, _VP, _I, _I, _VP, _RSP, _VP,
                                 _VP, _SZ, _VP], _I),
     }
@@ -655,13 +655,12 @@ def _row_strides(t, what):
 class SinkAttention:
     """Causal prefill attention over a sliding window and a few first tokens
     that stay visible (rkv_sink_attention); window 0: every key up to the
-    query.  Holds the workspace."""
+    query.  Holds the workspace, which grows with the calls' sizes: calls that
+    may run at the same time need an object each."""
 
     def __init__(self, sinks: int = 0, window: int = 0, device="cuda"):
-        b = _SZ(0)
-        _check(lib().rkv_sink_attention_workspace_size(ctypes.byref(b)), "rkv_sink_attention_workspace_size")
-        self.sinks, self.window, self.ws_bytes = sinks, window, b.value
-        self.ws = _workspace(b.value, device)
+        self.sinks, self.window = sinks, window
+        self.ws, self._outgrown = _workspace(0, device), []
 
     def __call__(self, Q, K, V, lens=None, out=None, lse=None, stream=None):
         """Q [B, H, len_q, D], K, V [B, HK, len_k, D] (float32, bfloat16 or
@@ -689,10 +688,16 @@ class SinkAttention:
             _int32(lens, Q.device, "lens")
             if lens.numel() != B:
                 raise ValueError("lens: one entry per item")
+        need = _SZ(0)
+        _check(lib().rkv_sink_attention_workspace_size(dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(need)),
+               "rkv_sink_attention_workspace_size")
+        if self.ws.numel() < need.value:
+            self._outgrown.append(self.ws)  # calls in flight and captured graphs may still use it
+            self.ws = _workspace(need.value, Q.device)
         qs, ks, os_ = _row_strides(Q, "Q"), _row_strides(K, "K, V"), _row_strides(out, "out")
         _launch(Q.device, stream, "rkv_sink_attention", lib().rkv_sink_attention, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
                 dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(qs), ctypes.byref(ks), _ptr(lens), self.sinks,
-                self.window, out.data_ptr(), ctypes.byref(os_), _ptr(lse), self.ws.data_ptr(), self.ws_bytes)
+                self.window, out.data_ptr(), ctypes.byref(os_), _ptr(lse), self.ws.data_ptr(), self.ws.numel())
         return out
 
     def status(self, stream=None) -> int:

@@ -56,6 +56,13 @@ CASES = [
     ("f16", 256, 3, 1, 1100, 1100, 4, 500, [1100, 700, 64, 63, 0]),
     ("bf16", 136, 24, 8, 700, 900, 0, 0, None),            # more units than SMs
     ("f16", 192, 2, 2, 65, 2000, 70, 333, [2000, 1999]),
+    # few queries over many keys: the keys are taken in parts
+    ("bf16", 128, 8, 2, 64, 8000, 0, 0, None),
+    ("bf16", 128, 3, 1, 300, 9000, 4, 2500, [9000, 8701, 8700, 3]),
+    ("f16", 64, 4, 4, 5, 7001, 600, 40, [7001, 7000, 6997, 6996]),
+    ("f32", 128, 2, 1, 33, 6000, 0, 0, [6000, 5970]),
+    ("f32", 256, 2, 2, 10, 5000, 130, 1000, None),
+    ("bf16", 256, 4, 1, 20, 6100, 0, 0, [6100, 6085]),
 ]
 
 
@@ -122,6 +129,15 @@ def test_repeats_and_graph(cuda):
     assert att.status() == 0
     _check(Q, K, V, 4, 200, lens.tolist(), out, lse, torch.zeros_like(out), torch.zeros_like(lse))
     want = out.clone()
+    # a larger call makes the workspace grow; the captured one still has its own
+    Ql, Kl, Vl = _inputs(13, 1, 8, 2, 60, 9000, 128, torch.bfloat16, cuda)
+    att(Ql, Kl, Vl)
+    junk = torch.full((1 << 22,), math.nan, device=cuda)
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    del junk
     both = [(rkv.SinkAttention(sinks=4, window=200, device=cuda), torch.zeros_like(Q), torch.cuda.Stream()) for _ in range(2)]
     torch.cuda.synchronize()
     for _ in range(3):

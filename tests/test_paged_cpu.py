@@ -118,8 +118,15 @@ def test_sink_attention_arguments():
     assert sink(ws=None) == WS and sink(wb=8) == WS and sink(ws=P + 1) == WS
     assert sink(lq=0) == OK and sink(batch=0) == OK
     b = ctypes.c_size_t(0)
-    assert rkv.lib().rkv_sink_attention_workspace_size(None) == INV
-    assert rkv.lib().rkv_sink_attention_workspace_size(ctypes.byref(b)) == OK and b.value >= 4
+    size = rkv.lib().rkv_sink_attention_workspace_size
+    assert size(rkv.BF16, 8, 8, 1, 4, 2, 64, None) == INV and size(rkv.BF16, 9, 8, 1, 4, 2, 64, ctypes.byref(b)) == INV
+    assert size(rkv.BF16, 8, 8, 1, 4, 2, 60, ctypes.byref(b)) == UNS
+    for dt, D in ((rkv.BF16, 64), (rkv.F16, 128), (rkv.F32, 128), (rkv.BF16, 256), (rkv.F32, 256)):
+        assert size(dt, 4, 8, 1, 4, 2, D, ctypes.byref(b)) == OK and b.value >= 4
+        # few queries over many keys: parts of the keys, whatever the window
+        assert size(dt, 4, 100000, 1, 4, 2, D, ctypes.byref(b)) == OK and b.value > 4 * 4 * D * 4
+        assert sink(dt=dt, D=D, lk=100000, window=0, wb=b.value - 1) == WS
+        assert sink(dt=dt, D=D, lk=100000, window=99999, wb=256) == WS
 
 
 def test_python_front_end_refuses_cpu_tensors():
