@@ -10,6 +10,7 @@
 // part and a second kernel joins the parts in order.  O = o / l,
 // lse = (m + log2 l) ln 2.
 #include "paged.cuh"
+#include "tf32.cuh"
 
 namespace rkv {
 namespace {
@@ -149,17 +150,17 @@ enum { KIND_F16 = 0, KIND_BF16 = 1, KIND_F32 = 2 };
 template <int KIND>
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if (KIND == KIND_BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                      "{%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else if (KIND == KIND_F16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                      "{%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                      "{%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -212,11 +213,6 @@ __device__ __forceinline__ uint32_t split2(float& x, float& y) {
     y -= f.y;
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// What a tf32 operand (the top 19 bits) leaves of a value.
-__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) {
-    return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u));
-}
-
 // Shapes of the kernel: DP columns (dim_head rounded up), 8 NT query heads, W warps, ring slots of a warp,
 // CTAs of an SM.
 template <int KIND_, int DP_, int NT_>
@@ -254,6 +250,10 @@ struct Shape {
 // 19 bits and the rest, three products (hi hi + lo hi + hi lo); the columns a
 // lane needs for four steps are one 16-byte chunk, since the order in which a
 // product sums its columns (or tokens) is free.
+//
+// A tile's products are summed by the matrix units from zero and then added to
+// the running output: their sums cut instead of rounding, which over the
+// thousands of tokens of a part would show (1.3e-6 against 5e-7).
 //
 // A row's maximum is raised only when a score exceeds it by more than 2^8
 // (all types hold P then); fp16's P is kept 2^7 larger, away from the type's
@@ -329,14 +329,17 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
     const uint8_t* qb = a.Q + (size_t)b * a.q_stride;
     uint32_t q[S::QS ? 1 : NT][S::QS ? 1 : DP / 16][2];
     if (F32) {
-        // step (blk, e): columns 32 blk + 4 t + e and 16 further of head g, and their rests
+        // step (blk, e): columns 32 blk + 4 t + e and 16 further of head g, as hi, hi, lo, lo
         for (int i = warp; i < DP / 8 * NT; i += W) {
             const int n = i / (DP / 8), st = i % (DP / 8), d = (st >> 2) * 32 + 4 * t + (st & 3);
             const bool have = n * 8 + g < ng;
             const float* row = reinterpret_cast<const float*>(qb) + (size_t)(h0 + n * 8 + g) * D;
             const uint32_t b0 = have && d < D ? __float_as_uint(__ldg(row + d)) : 0u;
             const uint32_t b1 = have && d + 16 < D ? __float_as_uint(__ldg(row + d + 16)) : 0u;
-            reinterpret_cast<uint4*>(qsm)[i * 32 + lane] = make_uint4(b0, b1, tf32_rest(b0), tf32_rest(b1));
+            uint4 f;
+            tf32_split(b0, f.x, f.z);
+            tf32_split(b1, f.y, f.w);
+            reinterpret_cast<uint4*>(qsm)[i * 32 + lane] = f;
         }
         __syncthreads();
     } else {
@@ -403,18 +406,30 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
                             x3 = lds16(kb + (g + 8) * S::ROW + (((c + 4) ^ swz) << 4));
                 const uint32_t k0[4] = {x0.x, x0.y, x0.z, x0.w}, k1[4] = {x1.x, x1.y, x1.z, x1.w};
                 const uint32_t k2[4] = {x2.x, x2.y, x2.z, x2.w}, k3[4] = {x3.x, x3.y, x3.z, x3.w};
+                float part[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) part[n][e] = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t hi[4] = {k0[e], k1[e], k2[e], k3[e]};
-                    const uint32_t lo[4] = {tf32_rest(k0[e]), tf32_rest(k1[e]), tf32_rest(k2[e]), tf32_rest(k3[e])};
+                    uint32_t hi[4], lo[4];
+                    tf32_split(k0[e], hi[0], lo[0]);
+                    tf32_split(k1[e], hi[1], lo[1]);
+                    tf32_split(k2[e], hi[2], lo[2]);
+                    tf32_split(k3[e], hi[3], lo[3]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         const uint4 qq = reinterpret_cast<const uint4*>(qsm)[(n * (DP / 8) + blk * 4 + e) * 32 + lane];
-                        mma16<KIND>(s[n], hi, qq.z, qq.w);
-                        mma16<KIND>(s[n], lo, qq.x, qq.y);
-                        mma16<KIND>(s[n], hi, qq.x, qq.y);
+                        mma16<KIND>(part[n], hi, qq.z, qq.w);
+                        mma16<KIND>(part[n], lo, qq.x, qq.y);
+                        mma16<KIND>(part[n], hi, qq.x, qq.y);
                     }
                 }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][e] += part[n][e];
             }
         } else {
             const int kr = lane & 15, kc = lane >> 4;  // lane i addresses row i % 8 of block i / 8: rows, then column halves
@@ -504,26 +519,42 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
         const uint32_t vb = ring + after(slot, 1) * S::SLOT;
         if (F32) {
             // output tile 2 j + h: rows g and g + 8 are columns 4 (g + 8 j) + 2 h and + 1
+            uint32_t ph[NT][2][2], pl[NT][2][2];
 #pragma unroll
-            for (int h8 = 0; h8 < 2; ++h8) {
-                const int row0 = h8 * 8 + 2 * t;  // this lane's tokens: row0, row0 + 1
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < DP / 32; ++j) {
-                    const int c = g + 8 * j;
+                for (int i = 0; i < 4; ++i) tf32_split(p[n][i >> 1][i & 1], ph[n][i >> 1][i & 1], pl[n][i >> 1][i & 1]);
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j) {
+                float part[NT][2][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) part[n][e >> 2][e & 3] = 0.0f;
+#pragma unroll
+                for (int h8 = 0; h8 < 2; ++h8) {
+                    const int row0 = h8 * 8 + 2 * t, c = g + 8 * j;  // this lane's tokens: row0, row0 + 1
                     const uint4 u = lds16(vb + row0 * S::ROW + ((c ^ (row0 & 7)) << 4));
                     const uint4 w = lds16(vb + (row0 + 1) * S::ROW + ((c ^ ((row0 + 1) & 7)) << 4));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t hi[4] = {h ? u.z : u.x, h ? u.w : u.y, h ? w.z : w.x, h ? w.w : w.y};
-                        const uint32_t lo[4] = {tf32_rest(hi[0]), tf32_rest(hi[1]), tf32_rest(hi[2]), tf32_rest(hi[3])};
+                        uint32_t hi[4], lo[4];
+                        tf32_split(h ? u.z : u.x, hi[0], lo[0]);
+                        tf32_split(h ? u.w : u.y, hi[1], lo[1]);
+                        tf32_split(h ? w.z : w.x, hi[2], lo[2]);
+                        tf32_split(h ? w.w : w.y, hi[3], lo[3]);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma16<KIND>(o[n][2 * j + h], hi, tf32_rest(p[n][h8][0]), tf32_rest(p[n][h8][1]));
-                            mma16<KIND>(o[n][2 * j + h], lo, p[n][h8][0], p[n][h8][1]);
-                            mma16<KIND>(o[n][2 * j + h], hi, p[n][h8][0], p[n][h8][1]);
+                            mma16<KIND>(part[n][h], hi, pl[n][h8][0], pl[n][h8][1]);
+                            mma16<KIND>(part[n][h], lo, ph[n][h8][0], ph[n][h8][1]);
+                            mma16<KIND>(part[n][h], hi, ph[n][h8][0], ph[n][h8][1]);
                         }
                     }
                 }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[n][2 * j + (e >> 2)][e & 3] += part[n][e >> 2][e & 3];
             }
         } else {
             const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;  // blocks: column halves first, then rows
@@ -532,9 +563,13 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
                 uint32_t f[4];
                 ldmatrix4<true>(f, vb + vr * S::ROW + (((2 * k + vc) ^ (vr & 7)) << 4));
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
+                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int i = 0; i < PARTS; ++i) mma16<KIND>(o[n][k], f, p[n][F32 ? 0 : i][0], p[n][F32 ? 0 : i][1]);
+                    for (int i = PARTS - 1; i >= 0; --i) mma16<KIND>(part, f, p[n][F32 ? 0 : i][0], p[n][F32 ? 0 : i][1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][k][e] += part[e];
+                }
             }
         }
         slot = after(slot, 2);

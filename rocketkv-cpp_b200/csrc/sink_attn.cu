@@ -6,14 +6,18 @@
 // l = sum 2^(x - m), o = sum 2^(x - m) v; tiles that neither hold a sink nor
 // meet the window of any row are not visited.  O = o / l, lse = (m + log2 l) ln 2.
 #include "sink_attn.cuh"
+#include "tf32.cuh"
 
 namespace rkv {
 namespace {
 
 constexpr int kBN = 64;  // keys of a tile
 
-// fp32 inputs: tf32 products of each operand's top 19 bits and of what they
-// leave, three per product (hi hi + lo hi + hi lo).  One CTA per BM queries of
+// fp32 inputs: tf32 products of each operand as its top 19 bits and the rest,
+// three per product (hi hi + lo hi + hi lo), summed by the matrix units over a
+// tile or less and then added (their sums cut instead of rounding).  The rate
+// of these products bounds it: 24/8 heads of 128, 2048 tokens, causal, run at
+// 40 TFLOP/s, which is 120 of products.  One CTA per BM queries of
 // a head, a warp per 16 of them, 64 keys at a time; V arrives under the scores
 // and the next K under the output's products.
 //
@@ -45,10 +49,6 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
                  "{%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// What a tf32 operand (the top 19 bits) leaves of a value.
-__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) {
-    return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u));
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int e) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; }
 
@@ -123,28 +123,42 @@ __global__ void __launch_bounds__(F32Shape<DP>::NT) sink_f32_kernel(const SinkAr
             uint32_t qh[4][4], ql[4][4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                qh[e][0] = word(x0, e), qh[e][1] = word(x1, e), qh[e][2] = word(x2, e), qh[e][3] = word(x3, e);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ql[e][i] = tf32_rest(qh[e][i]);
+                tf32_split(word(x0, e), qh[e][0], ql[e][0]);
+                tf32_split(word(x1, e), qh[e][1], ql[e][1]);
+                tf32_split(word(x2, e), qh[e][2], ql[e][2]);
+                tf32_split(word(x3, e), qh[e][3], ql[e][3]);
             }
 #pragma unroll
             for (int n0 = 0; n0 < 8; n0 += 4) {  // products into four accumulators in turn: one alone waits for itself
                 uint4 y0[4], y1[4];
+                float part[4][4];
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     const uint32_t kr = ks + ((n0 + n) * 8 + g) * S::ROW;
                     y0[n] = lds16(kr + ((c ^ swz) << 4));
                     y1[n] = lds16(kr + (((c + 4) ^ swz) << 4));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) part[n][e] = 0.0f;
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
+                    uint32_t h0[4], h1[4], l0[4], l1[4];
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) mma_tf32(s[n0 + n], qh[e], tf32_rest(word(y0[n], e)), tf32_rest(word(y1[n], e)));
+                    for (int n = 0; n < 4; ++n) {
+                        tf32_split(word(y0[n], e), h0[n], l0[n]);
+                        tf32_split(word(y1[n], e), h1[n], l1[n]);
+                    }
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) mma_tf32(s[n0 + n], ql[e], word(y0[n], e), word(y1[n], e));
+                    for (int n = 0; n < 4; ++n) mma_tf32(part[n], qh[e], l0[n], l1[n]);
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) mma_tf32(s[n0 + n], qh[e], word(y0[n], e), word(y1[n], e));
+                    for (int n = 0; n < 4; ++n) mma_tf32(part[n], ql[e], h0[n], h1[n]);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mma_tf32(part[n], qh[e], h0[n], h1[n]);
                 }
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n0 + n][e] += part[n][e];
             }
         }
         // columns 8 n + 2 t and + 1 of rows g (s[n][0], s[n][1]) and g + 8
@@ -185,31 +199,36 @@ __global__ void __launch_bounds__(F32Shape<DP>::NT) sink_f32_kernel(const SinkAr
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();  // V is here, and every warp is done with K
         if (it + 1 < tiles) key_tile(it + 1, false);
-#pragma unroll 1
-        for (int n8 = 0; n8 < 8; ++n8) {
-            // keys 8 n8 + 2 t and + 1 are steps t and t + 4
-            uint32_t ph[4], pl[4];
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
-                if (n == n8) {
-                    ph[0] = __float_as_uint(s[n][0]), ph[1] = __float_as_uint(s[n][2]);
-                    ph[2] = __float_as_uint(s[n][1]), ph[3] = __float_as_uint(s[n][3]);
-                }
+        for (int j = 0; j < DP / 32; ++j) {
+            float part[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pl[i] = tf32_rest(ph[i]);
-            const int r0 = n8 * 8 + 2 * t;
+            for (int e = 0; e < 16; ++e) part[e >> 2][e & 3] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < DP / 32; ++j) {
-                const int c = g + 8 * j;
+            for (int n8 = 0; n8 < 8; ++n8) {
+                // keys 8 n8 + 2 t and + 1 are steps t and t + 4
+                uint32_t ph[4], pl[4], h0[4], h1[4], l0[4], l1[4];
+                tf32_split(__float_as_uint(s[n8][0]), ph[0], pl[0]);
+                tf32_split(__float_as_uint(s[n8][2]), ph[1], pl[1]);
+                tf32_split(__float_as_uint(s[n8][1]), ph[2], pl[2]);
+                tf32_split(__float_as_uint(s[n8][3]), ph[3], pl[3]);
+                const int r0 = n8 * 8 + 2 * t, c = g + 8 * j;
                 const uint4 u = lds16(vs + r0 * S::ROW + ((c ^ (r0 & 7)) << 4));
                 const uint4 w = lds16(vs + (r0 + 1) * S::ROW + ((c ^ ((r0 + 1) & 7)) << 4));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mma_tf32(o[4 * j + e], ph, tf32_rest(word(u, e)), tf32_rest(word(w, e)));
+                for (int e = 0; e < 4; ++e) {
+                    tf32_split(word(u, e), h0[e], l0[e]);
+                    tf32_split(word(w, e), h1[e], l1[e]);
+                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mma_tf32(o[4 * j + e], pl, word(u, e), word(w, e));
+                for (int e = 0; e < 4; ++e) mma_tf32(part[e], ph, l0[e], l1[e]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mma_tf32(o[4 * j + e], ph, word(u, e), word(w, e));
+                for (int e = 0; e < 4; ++e) mma_tf32(part[e], pl, h0[e], h1[e]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mma_tf32(part[e], ph, h0[e], h1[e]);
             }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[4 * j + (e >> 2)][e & 3] += part[e >> 2][e & 3];
         }
         __syncthreads();  // every warp is done with V
     }
