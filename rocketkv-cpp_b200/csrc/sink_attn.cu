@@ -440,7 +440,7 @@ extern "C" int rkv_sink_attention(const void* Q, const void* K, const void* V, i
     a.parts = plan.parts;
     a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.off_ml);
     a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.off_o);
-    if (cudaMemsetAsync(a.err, 0, sizeof(int), st) != cudaSuccess) return RKV_ERR_CUDA;
+    if (cudaMemsetAsync(a.err, 0, (kSinkTicket + 1) * sizeof(int), st) != cudaSuccess) return RKV_ERR_CUDA;  // error word, ticket
     int done;
     if (dtype != RKV_F32)
         done = launch_sink_tc(a, dtype, batch, st);

@@ -24,6 +24,7 @@ struct SinkArgs {
 };
 
 constexpr int kSinkSms = 148;
+constexpr int kSinkTicket = 1;  // word of the workspace header from which CTAs draw their further items
 constexpr int kSinkMaxParts = 16;
 constexpr int kSinkPartTiles = 4;  // key tiles of a part at least
 // Parts of the keys for `items` CTAs' worth of queries that visit at most `tiles` key tiles each.

@@ -10,7 +10,8 @@
 // work on the other unit.
 //
 //   warp 0       copies Q and the K, V tiles (one TMA box per 64 columns) into
-//                shared memory; K and V share a ring of stages
+//                shared memory; a stage of the ring holds the V of a tile and
+//                the K of the next, which the products take one after the other
 //   warp 1       issues the products: per tile and unit P V, then the next S
 //   warps 4-7, 8-11   softmax of unit 0, 1, and their output rows
 //
@@ -19,6 +20,20 @@
 // the accumulator are fp32.  The accumulator is rescaled only when a row's
 // largest score has grown by more than 2^8 since its last rescale: P stays
 // below 2^8 then, which both types hold, and O and l carry the same factor.
+//
+// What bounds it.  24/8 heads of 128, causal: 4096 tokens 104 us (994
+// TFLOP/s), 8192 tokens under a window of 2048 186 us (970).  A pair of tiles
+// takes 3300 cycles, 2048 of them products at their full rate: a unit's
+// chain is 2100 of softmax, then 1200 of its last products with P and its next
+// scores, and the two units fill each other's gaps only in part.  Power bounds
+// it too: some milliseconds of it bring the GPU to its 1000 W cap (1.74 GHz
+// sampled, of 1.97), where the 186 us become 210, and shortening one part of
+// the chain gives little: leaving out the maximum or the exponentials (wrong
+// results, to see) makes it 3 and 9 % faster.  Measured and not kept, on the
+// 186 us: 64 keys a tile with two score buffers 237 (200 with a second
+// issuing warp for P V); one thread that issues everything 224; two issuing
+// warps 213; 16 softmax warps 197; P handed over whole 197; the maximum taken
+// under the first half's exponentials 203.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -35,15 +50,8 @@ constexpr int kThreads = 384;
 constexpr int kBlk = kTile * 128;     // bytes of a 128-row block of 64 columns
 constexpr float kGrow = 8.0f;         // log2 growth of a row's maximum that is carried without a rescale
 
-__host__ __device__ constexpr int stages(int kb) { return kb == 1 ? 8 : 4; }
+__host__ __device__ constexpr int stages(int kb) { return kb == 1 ? 4 : 2; }  // of a V and a K tile
 
-struct TcBars {
-    uint64_t q_full, q_empty, o_full, drained;
-    uint64_t s_full[2], p_half[2], p_ready[2], o_empty[2];  // of a unit
-    uint64_t full[8], empty[8];
-    uint32_t tmem;
-    int abort;
-};
 
 // S or O += A B with A in shared memory / A (16-bit pairs) in tensor memory.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -180,10 +188,50 @@ __device__ __forceinline__ Pair pair_of(const SinkArgs& a, int i, int per) {
     p.tiles = p.rg.part(p.part, a.parts);
     return p;
 }
-// The k-th item of a CTA: the list goes round the CTAs to and fro, so that each gets long and short ones.
-__device__ __forceinline__ int item_of(int k) {
-    return k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-}
+// A CTA's items: the first by its number, then the next that no CTA has taken, so that CTAs with short ones take
+// more (causal, 4096 tokens: 104 us, 107 with a fixed order to and fro).  The copying warp draws them and hands them to the other roles through two places in shared memory.
+struct Items {
+    uint64_t full[2], empty[2];
+    volatile int at[2];
+    __device__ void init(int readers) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], readers);
+        }
+    }
+    // the copying warp's
+    __device__ int draw(int items, int* err, int lane) {
+        int n = 0;
+        if (items > (int)gridDim.x && lane == 0) n = (int)atomicAdd(reinterpret_cast<unsigned*>(err) + kSinkTicket, 1u);
+        return items > (int)gridDim.x ? (int)gridDim.x + __shfl_sync(0xffffffffu, n, 0) : items;
+    }
+    __device__ bool put(int k, int item, int* err, volatile int* abort, int lane) {
+        if (k >= 2 && !warp_wait(&empty[k & 1], (uint32_t)(((k >> 1) - 1) & 1), err, abort)) return false;
+        if (lane == 0) {
+            at[k & 1] = item;
+            mbar_arrive1(&full[k & 1]);
+        }
+        __syncwarp();
+        return true;
+    }
+    // a reading warp's k-th item; past every item where the wait gave up
+    __device__ int get(int k, int* err, volatile int* abort, int lane) {
+        if (!warp_wait(&full[k & 1], (uint32_t)((k >> 1) & 1), err, abort)) return 0x7FFFFFFF;
+        const int item = at[k & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(&empty[k & 1]);
+        return item;
+    }
+};
+
+struct TcBars {
+    uint64_t q_full, q_empty, o_full, drained;
+    uint64_t s_full[2], p_half[2], p_ready[2], o_empty[2];  // of a unit
+    uint64_t full[4], empty[4];
+    Items items;
+    uint32_t tmem;
+    int abort;
+};
 
 // KB: blocks of 64 columns (dim_head <= 64 KB; columns behind dim_head are
 // filled with zeros by the copies).  One CTA per SM goes through its items
@@ -195,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     sink_tc_kernel(const SinkArgs a, const int items, const int per, const __grid_constant__ CUtensorMap tq,
                    const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
     constexpr int NS = stages(KB);
-    constexpr uint32_t kStage = KB * kBlk;
+    constexpr uint32_t kOne = KB * kBlk, kStage = 2 * kOne;  // a tile of Q, V or K; the V of a tile, then the K of the next
     constexpr uint32_t kColO = 256;  // tensor memory: S0, S1 (128 columns each), O0, O1 (64 KB each)
     extern __shared__ uint8_t smem_raw[];
     asm volatile("griddepcontrol.launch_dependents;");  // a join may be scheduled (it waits for this grid)
@@ -203,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     TcBars& B = *reinterpret_cast<TcBars*>(sm);
     volatile int* abort_flag = &B.abort;
     uint8_t* sq = sm + 1024;
-    uint8_t* ring = sq + 2 * kStage;
+    uint8_t* ring = sq + 2 * kOne;
     uint8_t* stage_o = ring + NS * kStage;  // 4 KB per softmax warp
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -212,6 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&B.q_empty, 1);
         mbar_init(&B.o_full, 1);
         mbar_init(&B.drained, 1);
+        B.items.init(9);
         for (int u = 0; u < 2; ++u) {
             mbar_init(&B.s_full[u], 1);
             mbar_init(&B.p_half[u], 4);
@@ -235,34 +284,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         // 88 * 128 + 208 * 256 registers are the 168 * 384 of the launch
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 0) {
-            // copies number q of the ring: K and V of every tile in turn
+            // stage number q of the ring: an item of t tiles takes t + 1, V of tile j - 1 and K of tile j in stage j
             int q = 0, nq = 0;
             bool ok = true;
-            auto copy = [&](const Pair& P, int j, bool v) {
+            auto copy = [&](const Pair& P, int j) {
                 const int s = q % NS;
                 if (q >= NS && !(ok = warp_wait(&B.empty[s], (uint32_t)((q / NS - 1) & 1), a.err, abort_flag))) return;
-                mbar_arrive_expect_tx_w(&B.full[s], kStage);
-                for (int kb = 0; kb < KB; ++kb)
-                    tma_load_4d_w(ring + s * kStage + kb * kBlk, v ? &tv : &tk, kb * 64, P.rg.tile(j) * kTile, P.hk, P.b, &B.full[s]);
+                mbar_arrive_expect_tx_w(&B.full[s], j == 0 || j == P.tiles ? kOne : kStage);
+                for (int kb = 0; kb < KB && j < P.tiles; ++kb)
+                    tma_load_4d_w(ring + s * kStage + kOne + kb * kBlk, &tk, kb * 64, P.rg.tile(j) * kTile, P.hk, P.b, &B.full[s]);
+                for (int kb = 0; kb < KB && j > 0; ++kb)
+                    tma_load_4d_w(ring + s * kStage + kb * kBlk, &tv, kb * 64, P.rg.tile(j - 1) * kTile, P.hk, P.b, &B.full[s]);
                 ++q;
             };
-            for (int k = 0; ok; ++k) {
-                const int it = item_of(k);
+            int it = blockIdx.x;
+            for (int k = 0; ok; ++k, it = B.items.draw(items, a.err, lane)) {
+                if (!B.items.put(k, it, a.err, abort_flag, lane)) break;
                 if (it >= items) break;
                 const Pair P = pair_of(a, it, per);
                 if (P.tiles == 0) continue;
-                copy(P, 0, false);
+                copy(P, 0);
                 if (!ok || (nq > 0 && !(ok = warp_wait(&B.q_empty, (uint32_t)((nq - 1) & 1), a.err, abort_flag)))) break;
-                mbar_arrive_expect_tx_w(&B.q_full, P.nu * kStage);
+                mbar_arrive_expect_tx_w(&B.q_full, P.nu * kOne);
                 for (int u = 0; u < P.nu; ++u)
                     for (int kb = 0; kb < KB; ++kb)
-                        tma_load_4d_w(sq + u * kStage + kb * kBlk, &tq, kb * 64, (P.u0 + u) / a.G * kTile,
+                        tma_load_4d_w(sq + u * kOne + kb * kBlk, &tq, kb * 64, (P.u0 + u) / a.G * kTile,
                                       P.hk * a.G + (P.u0 + u) % a.G, P.b, &B.q_full);
                 ++nq;
-                for (int j = 0; j < P.tiles && ok; ++j) {
-                    copy(P, j, true);
-                    if (ok && j + 1 < P.tiles) copy(P, j + 1, false);
-                }
+                for (int j = 1; j <= P.tiles && ok; ++j) copy(P, j);
             }
             // every copy has landed before the CTA may end
             if (nq > 0) mbar_wait_bounded(&B.q_full, (uint32_t)((nq - 1) & 1), a.err);
@@ -270,9 +319,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (warp == 1) {
             const uint32_t ids = mma_idesc(BF ? 1u : 0u, kTile);
             const uint32_t idv = mma_idesc(BF ? 1u : 0u, KB * 64) | (1u << 16);  // B with N contiguous
-            const uint64_t qd = mma_desc_sw128(smem_u32(sq)), kd = mma_desc_sw128(smem_u32(ring)), vd = v_desc(smem_u32(ring), kBlk);
+            const uint64_t qd = mma_desc_sw128(smem_u32(sq)), kd = mma_desc_sw128(smem_u32(ring) + kOne);
+            const uint64_t vd = v_desc(smem_u32(ring), kBlk);
             auto scores = [&](int u, int slot) {
-                const uint64_t da = qd + (uint32_t)(u * (kStage >> 4)), db = kd + (uint32_t)(slot * (kStage >> 4));
+                const uint64_t da = qd + (uint32_t)(u * (kOne >> 4)), db = kd + (uint32_t)(slot * (kStage >> 4));
 #pragma unroll
                 for (int ks = 0; ks < KB * 4; ++ks) {
                     const uint32_t o = ((ks >> 2) * kBlk + (ks & 3) * 32) >> 4;
@@ -280,31 +330,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 mma_commit_w(&B.s_full[u]);
             };
-            int q = 0, nq = 0;                  // ring copies, items
+            int q = 0, nq = 0;                  // stages, items
             uint32_t tiles_ph = 0, out_ph = 0;  // a bit per unit: parity of its tiles and of its items
             uint32_t used = 0;                  // the unit's output columns have been written before
             bool ok = true;
             auto wait = [&](uint64_t* bar, int n) { return ok = warp_wait(bar, (uint32_t)(n & 1), a.err, abort_flag); };
             for (int k = 0; ok; ++k) {
-                const int it = item_of(k);
+                const int it = B.items.get(k, a.err, abort_flag, lane);
                 if (it >= items) break;
                 const Pair P = pair_of(a, it, per);
                 if (P.tiles == 0) continue;
                 if (!wait(&B.q_full, nq) || !wait(&B.full[q % NS], q / NS)) break;
                 ++nq;
                 tc_fence_after();
-                for (int u = 0; u < P.nu; ++u) scores(u, q % NS);
+                scores(0, q % NS);
+                if (P.nu > 1) scores(1, q % NS);
                 mma_commit_w(&B.empty[q % NS]);
                 if (P.tiles == 1) mma_commit_w(&B.q_empty);
                 ++q;
-                for (int j = 0; j < P.tiles && ok; ++j) {
-                    const int sv = q % NS, sk = (q + 1) % NS;
-                    uint8_t* vt = ring + sv * kStage;
-                    const uint64_t vdj = vd + (uint32_t)(sv * (kStage >> 4));
-                    if (!wait(&B.full[sv], q / NS)) break;
+                for (int j = 0; j < P.tiles && ok; ++j, ++q) {
+                    const int slot = q % NS;
+                    const uint64_t vdj = vd + (uint32_t)(slot * (kStage >> 4));
+                    if (!wait(&B.full[slot], q / NS)) break;
                     const int behind = P.rg.n - P.rg.tile(j) * kTile;  // keys of the tile that exist
                     if (behind < kTile && P.rg.n < a.len_k) {
                         // the padding behind a sequence's end may hold anything, and 0 * NaN is NaN
+                        uint8_t* vt = ring + slot * kStage;
                         for (int e = lane; e < (kTile - behind) * 8; e += 32)
 #pragma unroll
                             for (int kb = 0; kb < KB; ++kb)
@@ -312,7 +363,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         fence_proxy_async();
                         __syncwarp();
                     }
-                    for (int u = 0; u < P.nu; ++u) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        if (u >= P.nu) break;
                         if (j == 0) {  // the output rows of the unit before have been read
                             if ((used >> u) & 1u) {
                                 if (!wait(&B.o_empty[u], out_ph >> u)) break;
@@ -331,20 +384,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         if (!ok) break;
                         tiles_ph ^= 1u << u;
-                        if (u == P.nu - 1) mma_commit_w(&B.empty[sv]);
-                        if (j + 1 < P.tiles) {
-                            if (u == 0) {
-                                if (!wait(&B.full[sk], (q + 1) / NS)) break;
-                                tc_fence_after();
-                            }
-                            scores(u, sk);
-                            if (u == P.nu - 1) {
-                                mma_commit_w(&B.empty[sk]);
-                                if (j + 2 == P.tiles) mma_commit_w(&B.q_empty);
-                            }
-                        }
+                        if (j + 1 < P.tiles) scores(u, slot);
                     }
-                    q += j + 1 < P.tiles ? 2 : 1;
+                    mma_commit_w(&B.empty[slot]);
+                    if (j + 2 == P.tiles) mma_commit_w(&B.q_empty);
                 }
                 if (ok) mma_commit_w(&B.o_full);
             }
@@ -361,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int nt = 0, ni = 0;  // tiles of this unit, items
         bool ok = true;
         for (int k = 0; ok; ++k) {
-            const int it = item_of(k);
+            const int it = B.items.get(k, a.err, abort_flag, lane);
             if (it >= items) break;
             const Pair P = pair_of(a, it, per);
             if (P.tiles > 0) ++ni;
@@ -481,6 +524,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // memory, so a CTA has one unit, tiles of 64 keys, and two score buffers that
 // the tiles take in turn: the scores of the next tile are formed under this
 // tile's softmax.  Warp 0 copies, warp 1 issues, warps 4-7 are the softmax.
+// 24/8 heads of 256, 2048 tokens, causal: 64-66 us (790-800 TFLOP/s); with one
+// unit there is nothing to fill the gaps of its chain.
 constexpr int kWideKB = 4, kWideKeys = 64, kWideSlots = 4;
 constexpr int kWideThreads = 256;
 constexpr int kWideBlk = kWideKeys * 128;        // bytes of 64 rows of 64 columns
@@ -490,6 +535,7 @@ struct WideBars {
     uint64_t q_full, q_empty, o_full, o_empty, pv_done, drained;
     uint64_t s_full[2], p_ready[2];
     uint64_t full[kWideSlots], empty[kWideSlots];
+    Items items;
     uint32_t tmem;
     int abort;
 };
@@ -532,6 +578,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         mbar_init(&B.o_empty, 4);
         mbar_init(&B.pv_done, 1);
         mbar_init(&B.drained, 1);
+        B.items.init(5);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B.s_full[i], 1);
             mbar_init(&B.p_ready[i], 4);
@@ -561,8 +608,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                               &B.full[s]);
             ++q;
         };
-        for (int k = 0; ok; ++k) {
-            const int it = item_of(k);
+        int it = blockIdx.x;
+        for (int k = 0; ok; ++k, it = B.items.draw(items, a.err, lane)) {
+            if (!B.items.put(k, it, a.err, abort_flag, lane)) break;
             if (it >= items) break;
             const WideItem P = wide_item(a, it, per);
             if (P.tiles == 0) continue;
@@ -597,7 +645,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             mma_commit_w(&B.empty[slot]);
         };
         for (int k = 0; ok; ++k) {
-            const int it = item_of(k);
+            const int it = B.items.get(k, a.err, abort_flag, lane);
             if (it >= items) break;
             const WideItem P = wide_item(a, it, per);
             if (P.tiles == 0) continue;
@@ -652,7 +700,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         int nt = 0, ni = 0;
         bool ok = true;
         for (int k = 0; ok; ++k) {
-            const int it = item_of(k);
+            const int it = B.items.get(k, a.err, abort_flag, lane);
             if (it >= items) break;
             const WideItem P = wide_item(a, it, per);
             const int p0 = P.qt * kTile + a.len_k - a.len_q, p = p0 + row, n = P.rg.n;
@@ -802,7 +850,7 @@ template <int KB, bool BF>
 int launch_kb(const SinkArgs& a, int items, int per, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
               cudaStream_t st) {
     // the barriers, and up to 1023 bytes of alignment; Q and the ring; the output rows' stage
-    const int smem = 2048 + (2 + stages(KB)) * KB * kBlk + 8 * 4096;
+    const int smem = 2048 + (2 + 2 * stages(KB)) * KB * kBlk + 8 * 4096;
     if (cudaFuncSetAttribute(sink_tc_kernel<KB, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
