@@ -414,8 +414,11 @@ int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, int weight_st
  * p = i + len_k - len_q (len_q <= len_k; the first len_k - len_q keys are a
  * cached prefix) and sees key j <= p when window == 0, or j < sinks, or
  * j > p - window.  lens (nullable): device [batch], the valid keys of each
- * item of a padded batch; keys from lens[b] on are never read and query rows
- * at positions from lens[b] on are left as they were.
+ * item of a padded batch; keys from lens[b] on may hold anything and query rows
+ * at positions from lens[b] on are left as they were.  V of the keys before
+ * that must be finite: keys are taken by tiles, and an infinity or NaN in V
+ * may reach a query of the tile that does not see its key.  A NaN in K stays
+ * in the queries that see it.
  * Q: [batch][num_heads][len_q][dim_head], K, V: [batch][num_heads_kv][len_k]
  * [dim_head], O as Q, all of dtype (RKV_F32, RKV_BF16, RKV_F16; sums and
  * softmax in fp32), at the given strides (bytes, multiples of 16; NULL: rows,

@@ -9,6 +9,13 @@
 // shared memory, so they are read once, and the digit counts meet through
 // distributed shared memory.  Then the rows are copied, K and V by the same
 // threads, or moved in place.
+//
+// bf16, 8 KV heads of 128, to other pages, device time: 64 ragged sequences of
+// up to 3717 tokens to 1024, 90 us (481 MB), of which the selection takes 16
+// and the copy 74; 8 x 131072 tokens to 8192, 88 us (337 MB), 37 and 42; one of
+// 2112 tokens, 9.5 us.  Memory bounds the copies; chains of digit counts,
+// barriers and scans bound the selections (a weight is read from memory once
+// and, in a long cache, a second time from L2).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -375,7 +382,9 @@ __global__ void __launch_bounds__(1024) weight_shift_kernel(const WEvictArgs a) 
 constexpr int kMoveNT = 256;
 
 // Rows to other pages: 2^lg lanes per row (the row's vectors, rounded up),
-// K and V by the same thread, kCopyRows rows in flight per thread.
+// K and V by the same thread, kCopyRows rows in flight per thread (64 ragged
+// sequences / 8 x 131072 tokens, whole eviction: 102 / 90 us with 1, 90 / 89
+// with 2, 100 / 97 with 4, 127 / 117 with 8).
 constexpr int kCopyRows = 2;
 __global__ void __launch_bounds__(kMoveNT) weight_copy_kernel(const WEvictArgs a, int lg) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -414,44 +423,100 @@ __global__ void __launch_bounds__(kMoveNT) weight_copy_kernel(const WEvictArgs a
 // Rows within their own pages.  A kept list ascends and kept[i] >= i, so a
 // row is overwritten only by rows whose sources lie at or behind it: reading
 // a chunk's sources before writing any of its destinations keeps every
-// source.  One CTA walks the chunks of an (item, head) in order; the row is
-// cut into slices of slice_v vectors, and K and V are apart, so that several
-// CTAs share it.
-constexpr int kMoveVPT = 8;
+// source, and later chunks may be read earlier still.  One CTA walks the
+// chunks of an (item, head) in order, with the next kMoveAhead chunks' sources
+// on their way to shared memory (each thread's own vectors); the row is cut
+// into slices of slice_v vectors, and K and V are apart, so that several CTAs
+// share it.  Memory latency bounds it, a chunk after the other: the whole
+// eviction in place, bf16, 8 KV heads of 128: 64 x 3717 tokens to 1024 124 us,
+// 8 x 131072 to 8192 185, one of 2112 tokens to 1024 17.  2 vectors a thread
+// and 3 chunks ahead were best (64 / 8 sequences 138 / 185 us; 1 and 3 139 /
+// 248, 4 and 3 181 / 204, 2 and 5 163 / 263), and slices to 296 CTAs (124 /
+// 185 us; to 592 124 / 216, to 1184 132 / 216).
+constexpr int kMoveVPT = 2, kMoveAhead = 3;
+constexpr long long kMoveCTAs = 2 * 148;  // as many at least, if the row's slices allow it
+constexpr int kMoveSmem = (kMoveAhead + 1) * kMoveVPT * kMoveNT * 16;
 __global__ void __launch_bounds__(kMoveNT) weight_move_kernel(const WEvictArgs a, int slice_v) {
+    constexpr int S = kMoveAhead + 1, U = kMoveVPT;
+    extern __shared__ __align__(16) uint8_t smem[];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int unit = blockIdx.y, hk = unit % a.HK, b = unit / a.HK;
     const int n = paged_len(a.c, b, a.max_len), keep = min(n, a.budget);
     if (keep == n) return;
     const int* kept = a.kept + (size_t)unit * a.kept_stride;
+    const int* table = a.c.table + (size_t)b * a.c.table_stride;
+    const unsigned page = a.c.page_size;
     uint8_t* base = (blockIdx.x & 1) ? a.c.V : a.c.K;
     const int v0 = (blockIdx.x >> 1) * slice_v, nv = min(slice_v, a.vpr - v0);
-    const int rows = kMoveNT * kMoveVPT / nv;  // per chunk
-    for (int r0 = 0; r0 < keep; r0 += rows) {
-        uint4 x[kMoveVPT];
-        long long to[kMoveVPT];
+    const int rows = kMoveNT * U / nv;  // per chunk
+    const int chunks = (keep + rows - 1) / rows;
+    uint8_t* mine = smem + threadIdx.x * 16;
+    // A source's address takes two loads, its place in the list and its page; each is asked for a chunk before
+    // the next step needs it.
+    int row[U], vec[U];                 // of a chunk
+    int t2[U], t1[U], pf[U], pt[U];     // tokens of the chunk after the next; of the next, and its pages
+    long long to[S][U];
 #pragma unroll
-        for (int u = 0; u < kMoveVPT; ++u) {
-            const int g = threadIdx.x + u * kMoveNT;
-            const int r = g / nv, i = r0 + r, vec = v0 + g - r * nv;
-            to[u] = -1;
-            if (r < rows && i < keep) {
-                const int t = kept[i];
-                if (t != i) {
-                    const long long from = paged_offset(a.c, b, hk, t);
-                    if (from >= 0) to[u] = paged_offset(a.c, b, hk, i);
-                    if (to[u] >= 0) {
-                        to[u] += vec * 16;
-                        x[u] = *reinterpret_cast<const uint4*>(base + from + vec * 16);
-                    }
-                }
+    for (int u = 0; u < U; ++u) {
+        const int g = threadIdx.x + u * kMoveNT;
+        row[u] = g / nv;
+        vec[u] = (v0 + g - row[u] * nv) * 16;
+        if (row[u] >= rows) row[u] = 0x40000000;  // the chunk's remainder
+    }
+    auto place = [&](int c, int u) { return c < chunks && row[u] < keep - c * rows ? c * rows + row[u] : -1; };
+    auto tokens = [&](int c) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = place(c, u);
+            t2[u] = i >= 0 ? kept[i] : -1;
+        }
+    };
+    auto pages = [&](int c) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = place(c, u);
+            t1[u] = t2[u] == i ? -1 : t2[u];  // a row that is in its place stays
+            pf[u] = pt[u] = -1;
+            if (t1[u] >= 0) {
+                pf[u] = table[(unsigned)t1[u] / page];
+                pt[u] = table[(unsigned)i / page];
             }
         }
-        __syncthreads();  // every source of the chunk read before a destination is written
+    };
+    auto fetch = [&](int c, long long* dst, int s) {
 #pragma unroll
-        for (int u = 0; u < kMoveVPT; ++u)
-            if (to[u] >= 0) *reinterpret_cast<uint4*>(base + to[u]) = x[u];
-        __syncthreads();
+        for (int u = 0; u < U; ++u) {
+            dst[u] = -1;
+            if ((unsigned)pf[u] < (unsigned)a.c.num_pages && (unsigned)pt[u] < (unsigned)a.c.num_pages) {
+                const unsigned i = c * rows + row[u], t = t1[u];
+                dst[u] = pt[u] * a.c.page_stride + hk * a.c.head_stride + (long long)(i % page) * a.c.token_stride + vec[u];
+                const long long from = pf[u] * a.c.page_stride + hk * a.c.head_stride + (long long)(t % page) * a.c.token_stride + vec[u];
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(mine + (s * U + u) * kMoveNT * 16)),
+                             "l"(base + from)
+                             : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        pages(c + 1);
+        tokens(c + 2);
+    };
+    tokens(0);
+    pages(0);
+    tokens(1);
+#pragma unroll
+    for (int s = 0; s < kMoveAhead; ++s) fetch(s, to[s], s);
+    for (int c0 = 0; c0 < chunks; c0 += S) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            if (c0 + s >= chunks) break;
+            fetch(c0 + s + kMoveAhead, to[(s + kMoveAhead) % S], (s + kMoveAhead) % S);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kMoveAhead) : "memory");
+            __syncthreads();  // every source of the chunk read before a destination is written
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (to[s][u] >= 0)
+                    *reinterpret_cast<uint4*>(base + to[s][u]) = *reinterpret_cast<const uint4*>(mine + (s * U + u) * kMoveNT * 16);
+        }
     }
 }
 
@@ -550,11 +615,13 @@ extern "C" int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, in
         // no rows stay
     } else if (a.inplace) {
         int slices = 1, slice_v = a.vpr;
-        while (slices < 4 && slice_v % 2 == 0 && slice_v >= 4) {
+        while (units * 2 * slices < kMoveCTAs && slice_v % 2 == 0 && slice_v >= 4) {
             slices *= 2;
             slice_v /= 2;
         }
-        e = launch_pdl(weight_move_kernel, dim3(2 * slices, (unsigned)units), dim3(kMoveNT), 0, st, a, slice_v);
+        e = cudaFuncSetAttribute(weight_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoveSmem);
+        if (e == cudaSuccess)
+            e = launch_pdl(weight_move_kernel, dim3(2 * slices, (unsigned)units), dim3(kMoveNT), kMoveSmem, st, a, slice_v);
     } else {
         int lg = 0;
         while ((1 << lg) < a.vpr) ++lg;
