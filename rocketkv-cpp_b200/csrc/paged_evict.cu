@@ -12,8 +12,8 @@
 //
 // bf16, 8 KV heads of 128, to other pages, device time: 64 ragged sequences of
 // up to 3717 tokens to 1024, 90 us (481 MB), of which the selection takes 16
-// and the copy 74; 8 x 131072 tokens to 8192, 88 us (337 MB), 37 and 42; one of
-// 2112 tokens, 9.5 us.  Memory bounds the copies; chains of digit counts,
+// and the copy 74; 8 x 131072 tokens (fp16) to 4096, 88 us (337 MB), 37 and 42;
+// one of 2112 tokens to 2048, 9.5 us.  Memory bounds the copies; chains of digit counts,
 // barriers and scans bound the selections (a weight is read from memory once
 // and, in a long cache, a second time from L2).
 #include <cooperative_groups.h>

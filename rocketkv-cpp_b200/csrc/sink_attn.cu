@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(F32Shape<DP>::NT) sink_f32_kernel(const SinkAr
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t qs = smem_u32(smem), ks = qs + S::BM * S::ROW, vs = ks + kBN * S::ROW;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    if (blockIdx.x == 0 && tid == 0) *a.err = 0;  // nothing here waits
     long long id = blockIdx.x;
     const int part = (int)(id % a.parts);
     id /= a.parts;
@@ -440,7 +441,6 @@ extern "C" int rkv_sink_attention(const void* Q, const void* K, const void* V, i
     a.parts = plan.parts;
     a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.off_ml);
     a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.off_o);
-    if (cudaMemsetAsync(a.err, 0, (kSinkTicket + 1) * sizeof(int), st) != cudaSuccess) return RKV_ERR_CUDA;  // error word, ticket
     int done;
     if (dtype != RKV_F32)
         done = launch_sink_tc(a, dtype, batch, st);

@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&B.o_full, 1);
         mbar_init(&B.drained, 1);
         B.items.init(9);
+        if (blockIdx.x == 0 && items <= (int)gridDim.x) *a.err = 0;
         for (int u = 0; u < 2; ++u) {
             mbar_init(&B.s_full[u], 1);
             mbar_init(&B.p_half[u], 4);
@@ -579,6 +580,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         mbar_init(&B.pv_done, 1);
         mbar_init(&B.drained, 1);
         B.items.init(5);
+        if (blockIdx.x == 0 && items <= (int)gridDim.x) *a.err = 0;
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B.s_full[i], 1);
             mbar_init(&B.p_ready[i], 4);
@@ -846,9 +848,16 @@ bool encode(CUtensorMap* m, const void* base, bool bf, int D, int rows, int head
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Error word and ticket.  Where no ticket is drawn the kernel clears the error word itself: a wait gives up after
+// two seconds at the soonest, long after the first CTA's first instructions, and a memset costs a launch.
+bool clear_header(const SinkArgs& a, int items, cudaStream_t st) {
+    return items <= kSinkSms || cudaMemsetAsync(a.err, 0, (kSinkTicket + 1) * sizeof(int), st) == cudaSuccess;
+}
+
 template <int KB, bool BF>
 int launch_kb(const SinkArgs& a, int items, int per, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
               cudaStream_t st) {
+    if (!clear_header(a, items, st)) return RKV_ERR_CUDA;
     // the barriers, and up to 1023 bytes of alignment; Q and the ring; the output rows' stage
     const int smem = 2048 + (2 + 2 * stages(KB)) * KB * kBlk + 8 * 4096;
     if (cudaFuncSetAttribute(sink_tc_kernel<KB, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
@@ -862,6 +871,7 @@ int launch_kb(const SinkArgs& a, int items, int per, const CUtensorMap& tq, cons
 template <bool BF>
 int launch_wide(const SinkArgs& a, int items, int per, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                 cudaStream_t st) {
+    if (!clear_header(a, items, st)) return RKV_ERR_CUDA;
     if (cudaFuncSetAttribute(sink_wide_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem) != cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
