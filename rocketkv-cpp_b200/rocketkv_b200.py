@@ -484,6 +484,16 @@ def _launch(device, stream, what, fn, *args) -> None:
         raise RkvError(st, what)
 
 
+def _on_stream(device, stream):
+    """What a call allocates and fills belongs to its stream, not to the current one."""
+    import contextlib
+    import torch
+    if stream is None:
+        return contextlib.nullcontext()
+    h = int(stream)
+    return torch.cuda.stream(torch.cuda.ExternalStream(h, device=device) if h else torch.cuda.default_stream(device))
+
+
 def _int32(t, device, what):
     import torch
     if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
@@ -576,8 +586,9 @@ class PagedDecoder:
         self.max_len, self.batch, self.sinks, self.window = max_len, batch, sinks, window
         self.ws_bytes = b.value
         self.ws = _workspace(b.value, device)
-        self.O = torch.zeros((batch, num_heads, dim_head), dtype=torch.float32, device=device)
-        self.lse = torch.zeros((batch, num_heads), dtype=torch.float32, device=device)
+        # each call writes all of them; a fill on this stream could run after a call on another
+        self.O = torch.empty((batch, num_heads, dim_head), dtype=torch.float32, device=device)
+        self.lse = torch.empty((batch, num_heads), dtype=torch.float32, device=device)
 
     def __call__(self, Q, cache: PagedCache, weights=None, stream=None):
         """Q [B, H, D] of the cache's type.  weights (nullable): float32
@@ -619,8 +630,9 @@ class WeightEvictor:
         import torch
         self.num_heads_kv, self.max_len, self.batch = num_heads_kv, max_len, batch
         self.budget, self.sinks, self.recent = budget, sinks, recent
-        self.kept = torch.full((batch, num_heads_kv, max(0, min(budget, max_len))), -1, dtype=torch.int32, device=device)
-        self.new_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        # each call writes all of them; a fill on this stream could run after a call on another
+        self.kept = torch.empty((batch, num_heads_kv, max(0, min(budget, max_len))), dtype=torch.int32, device=device)
+        self.new_lens = torch.empty(batch, dtype=torch.int32, device=device)
 
     def __call__(self, cache: PagedCache, weights, out: PagedCache | None = None, weights_out=None, stream=None):
         """In place without out / weights_out.  Returns (kept [B, HK, min(budget,
@@ -674,7 +686,8 @@ class SinkAttention:
         if not (Q.device == K.device == V.device == self.ws.device):
             raise ValueError("Q, K, V and the workspace: one device")
         if out is None:
-            out = torch.zeros(Q.shape, dtype=Q.dtype, device=Q.device)
+            with _on_stream(Q.device, stream):
+                out = torch.zeros(Q.shape, dtype=Q.dtype, device=Q.device)
         if out.shape != Q.shape or out.dtype != Q.dtype or out.device != Q.device:
             raise ValueError("out: Q's shape, type and device")
         B, H, Lq, D = Q.shape
@@ -693,7 +706,8 @@ class SinkAttention:
                "rkv_sink_attention_workspace_size")
         if self.ws.numel() < need.value:
             self._outgrown.append(self.ws)  # calls in flight and captured graphs may still use it
-            self.ws = _workspace(need.value, Q.device)
+            with _on_stream(Q.device, stream):
+                self.ws = _workspace(need.value, Q.device)
         qs, ks, os_ = _row_strides(Q, "Q"), _row_strides(K, "K, V"), _row_strides(out, "out")
         _launch(Q.device, stream, "rkv_sink_attention", lib().rkv_sink_attention, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
                 dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(qs), ctypes.byref(ks), _ptr(lens), self.sinks,

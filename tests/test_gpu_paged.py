@@ -407,6 +407,25 @@ def test_evict_into_other_pages_of_the_same_pools(cuda):
     assert torch.equal(K, Ko) and torch.equal(V, Vo) and torch.equal(Wo, We)
 
 
+def test_fresh_objects_on_another_stream(cuda):
+    """A decoder and an evictor made and called on another stream while the
+    current one is busy: nothing of their making comes behind the calls."""
+    B, H, HK, D, page, n, budget = 2, 4, 2, 64, 16, 200, 64
+    c = _cache(101, B, HK, D, page, n, torch.bfloat16, cuda, lens=[n, 90])
+    out = _cache(102, B, HK, D, page, budget, torch.bfloat16, cuda, lens=[0, 0])
+    Q, W = _query(103, B, H, D, torch.bfloat16, cuda), _weights(104, B, HK, n, cuda)
+    want = rkv.PagedDecoder(H, HK, D, n, B, cuda)(Q, c)
+    kept0, new0 = rkv.WeightEvictor(HK, n, B, budget, cuda, sinks=2)(c, W, out=out, weights_out=torch.zeros_like(W))
+    Wo, s = torch.zeros_like(W), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(50_000_000)  # about 25 ms
+    dec, ev = rkv.PagedDecoder(H, HK, D, n, B, cuda), rkv.WeightEvictor(HK, n, B, budget, cuda, sinks=2)
+    dec(Q, c, stream=s.cuda_stream)
+    ev(c, W, out=out, weights_out=Wo, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(dec.O, want) and torch.equal(ev.kept, kept0) and torch.equal(ev.new_lens, new0)
+
+
 def test_generation_with_evictions(cuda):
     """Prompt rows appended, then 24 steps of append, decode with weights, and
     an eviction in place whenever the cache has grown 8 tokens over its budget;

@@ -147,6 +147,19 @@ def test_repeats_and_graph(cuda):
     assert all(torch.equal(o, want) for _, o, _ in both)
 
 
+def test_output_of_a_call_on_another_stream(cuda):
+    """What a call allocates is filled on its own stream: work queued on the
+    current one does not come behind the attention."""
+    Q, K, V = _inputs(21, 1, 4, 2, 200, 200, 64, torch.bfloat16, cuda)
+    att, s = rkv.SinkAttention(device=cuda), torch.cuda.Stream()
+    want = att(Q, K, V)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(50_000_000)  # about 25 ms
+    out = att(Q, K, V, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
 def test_prompt_through_prefill_eviction_and_decode(cuda):
     """A prompt's attention, stage 1 on its own Q and K, the kept rows put into
     pages, and the next token decoded over them: the decode equals plain
