@@ -359,7 +359,8 @@ typedef struct rkv_paged_cache {
  * i * src_token_stride + h * src_head_stride + d * element size, the cache's
  * dtype, strides in bytes and multiples of the element size (rows of a fused
  * projection are read in place).  The source must not overlap the pages, and
- * no two written tokens may share a row.  Asynchronous on `stream`. */
+ * no two written tokens may share a row.  batch: at most 65535.  Asynchronous
+ * on `stream`. */
 int rkv_paged_append(const rkv_paged_cache* cache, const void* k, const void* v, int n_rows, int batch,
                      long long src_item_stride, long long src_token_stride, long long src_head_stride,
                      const int* n_new, void* stream);
@@ -401,10 +402,12 @@ int rkv_paged_decode(const void* Q, long long q_item_stride, int num_heads, cons
  * them up to max_len set to zero.  out NULL (or the same pools and table):
  * in place; rows from new_lens[b] on keep what they held.  Otherwise `out` is
  * a cache of the same dtype, heads and dim_head whose pages the input's
- * sequences do not use (the same pools may hold them); only its first
- * min(budget, max_len) tokens per sequence are written and its lens is not
- * read.  weights_out NULL or weights: in place.  In place, no page may belong
- * to two sequences.  Asynchronous on `stream`; allocates nothing. */
+ * sequences do not use (the same pools may hold them), with room for
+ * min(budget, max_len) tokens of a sequence, or for all that the input's table
+ * holds; only those are written and its lens is not read.  weights_out NULL or
+ * weights: in place, otherwise the two must not overlap.  In place, no page
+ * may belong to two sequences.  batch * num_heads_kv: at most 65535.
+ * Asynchronous on `stream`; allocates nothing. */
 int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, int weight_stride, int max_len, int batch,
                      int budget, int sinks, int recent, const rkv_paged_cache* out, float* weights_out,
                      int* kept, int kept_stride, int* new_lens, void* stream);

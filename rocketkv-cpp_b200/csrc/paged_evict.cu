@@ -593,6 +593,9 @@ extern "C" int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, in
          out->head_stride != cache->head_stride || out->token_stride != cache->token_stride ||
          out->table_stride != cache->table_stride || out->num_pages != cache->num_pages))
         return RKV_ERR_INVALID_ARG;
+    // the rows that any sequence can keep have a place
+    const long long from = (long long)cache->table_stride * cache->page_size, most = list < from ? list : from;
+    if ((long long)a.o.table_stride * a.o.page_size < most) return RKV_ERR_INVALID_ARG;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Short lists: a CTA of 512 threads each, four to an SM.  Longer ones: CTAs of 1024 threads, one to an SM,
     // as many to a list as give every SM one (a second wave costs more than a longer slice).

@@ -136,3 +136,11 @@ def test_python_front_end_refuses_cpu_tensors():
         rkv.PagedCache(K, K, torch.zeros((1, 2), dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
     with pytest.raises(ValueError):
         rkv.PagedCache(K, K[:, :1], torch.zeros((1, 2), dtype=torch.int32), None)
+
+
+def test_evict_into_too_few_pages():
+    """A destination without room for the rows that stay is refused: they would
+    be lost while new_lens counts them."""
+    c = cache()  # 32 tokens of a sequence, 16 stay
+    assert evict(c, out=cache(K=2 * P, V=3 * P, table_stride=1, page_size=8, page_stride=2 * 8 * 128, head_stride=8 * 128)) == INV
+    assert evict(c, budget=100, kst=100, max_len=100, wst=100, out=cache(K=2 * P, V=3 * P, table_stride=1)) == INV
