@@ -86,6 +86,28 @@ def test_against_64_bits(case, token_major, cuda):
     _check(Q, K, V, sinks, window, lens, out, lse, O0, lse0)
 
 
+@pytest.mark.parametrize("D,window", [(64, 0), (128, 70), (256, 0)])
+def test_many_ragged_sequences(D, window, cuda):
+    """Several times as many items as SMs, of very different lengths and some
+    without a row, an odd number of query tiles per KV head; the same bits when
+    the calls run on two streams at once."""
+    B, H, HK, n = 60, 6, 2, 300
+    Q, K, V = _inputs(31, B, H, HK, n, n, D, torch.bfloat16, cuda)
+    lens = [(37 * b * b + 11 * b) % (n + 1) if b % 7 else 0 for b in range(B)]
+    lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    runs = [(rkv.SinkAttention(sinks=2, window=window, device=cuda), torch.full_like(Q, 3.0),
+             torch.full((B, H, n), 5.0, device=cuda), torch.cuda.Stream()) for _ in range(2)]
+    O0, lse0 = runs[0][1].clone(), runs[0][2].clone()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for att, out, lse, st in runs:
+            att(Q, K, V, lens=lt, out=out, lse=lse, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(att.status() == 0 for att, *_ in runs)
+    _check(Q, K, V, 2, window, lens, runs[0][1], runs[0][2], O0, lse0)
+    assert torch.equal(runs[0][1], runs[1][1]) and torch.equal(runs[0][2], runs[1][2])
+
+
 def test_large_scores(cuda):
     """Scores far apart, largest late or early in the row."""
     Q, K, V = _inputs(8, 1, 4, 2, 400, 400, 128, torch.bfloat16, cuda)
