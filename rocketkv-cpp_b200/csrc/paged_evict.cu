@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "paged.cuh"
+#include "weight_list.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -269,11 +270,7 @@ __global__ void __launch_bounds__(NT) weight_select_kernel(const WEvictArgs a) {
         }
         if (all) f = 0xFFFFu;
         if (m == 0) f = 0;
-        if (i0 < c0 || i0 + 16 > c1)  // sinks and recent tokens are listed, nothing behind the stretch
-            for (int e = 0; e < 16; ++e) {
-                const int i = i0 + e;
-                if (i < c0 || i >= c1 || i >= t1) f = i < t1 ? f | 1u << e : f & ~(1u << e);
-            }
+        f = listed_tokens(f, i0, c0, c1, t1);
         const int c = __popc(f);
         int inc = c;
 #pragma unroll
