@@ -281,11 +281,12 @@ __global__ void __launch_bounds__(256) sink_join_kernel(const SinkArgs a) {
     const long long rows = (long long)a.batch * a.H * a.len_q;
     const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (row >= rows) return;
     const int i = (int)(row % a.len_q), h = (int)(row / a.len_q % a.H), b = (int)(row / a.len_q / a.H);
-    const int n = a.lens ? min(max(a.lens[b], 0), a.len_k) : a.len_k;
-    if (i + a.len_k - a.len_q >= n) return;  // behind the sequence's end
+    const int n = a.lens && row < rows ? min(max(a.lens[b], 0), a.len_k) : a.len_k;
+    // Every thread waits, also those without a row: where no row exists the join would otherwise end before the
+    // attention, and the stream's next work would not be ordered behind that.
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (row >= rows || i + a.len_k - a.len_q >= n) return;  // or behind the sequence's end
     const float2 ml = lane < a.parts ? a.part_ml[lane * rows + row] : make_float2(-INFINITY, 0.0f);
     // a part without a visible key has l = 0, whatever its m
     float m = ml.y == 0.0f ? -INFINITY : ml.x;
