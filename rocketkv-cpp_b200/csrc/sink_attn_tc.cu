@@ -19,7 +19,8 @@
 // products take both operands in one type) and the output.  Scores, m, l and
 // the accumulator are fp32.  The accumulator is rescaled only when a row's
 // largest score has grown by more than 2^8 since its last rescale: P stays
-// below 2^8 then, which both types hold, and O and l carry the same factor.
+// below 2^8 then (2^15 in fp16, see kLift), which both types hold, and O and l
+// carry the same factor.
 //
 // What bounds it.  24/8 heads of 128, causal: 4096 tokens 104 us (994
 // TFLOP/s), 8192 tokens under a window of 2048 186 us (970).  A pair of tiles
@@ -49,6 +50,11 @@ constexpr int kTile = 128;            // queries of a unit, keys of a tile
 constexpr int kThreads = 384;
 constexpr int kBlk = kTile * 128;     // bytes of a 128-row block of 64 columns
 constexpr float kGrow = 8.0f;         // log2 growth of a row's maximum that is carried without a rescale
+// log2 of a factor on P, and so on l and O, which it leaves with O / l.  fp16's P is kept 2^7 larger: at most 2^15
+// then, and a weight is lost from 2^-32 of the row's largest on instead of 2^-25 (40000 weights of 2^-26 beside one
+// of 1 are 6e-4 of the sum, a half step of fp16 4.9e-4).  bf16 has fp32's exponents.
+template <bool BF>
+constexpr float kLift = BF ? 0.0f : 7.0f;
 
 __host__ __device__ constexpr int stages(int kb) { return kb == 1 ? 4 : 2; }  // of a V and a K tile
 
@@ -464,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                const float ms = (m == -INFINITY ? 0.0f : m) * a.scale2;
+                const float ms = (m == -INFINITY ? 0.0f : m) * a.scale2 - kLift<BF>;
                 const float2 nm = make_float2(-ms, -ms);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
@@ -501,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint8_t* so = stage_o + (warp - 4) * 4096;
             const uint32_t rows_ok = __ballot_sync(0xffffffffu, real);
             if (a.parts > 1) {
-                if (real) a.part_ml[prow] = make_float2((m == -INFINITY ? 0.0f : m) * a.scale2, l);
+                if (real) a.part_ml[prow] = make_float2((m == -INFINITY ? 0.0f : m) * a.scale2 - kLift<BF>, l);
 #pragma unroll
                 for (int kb = 0; kb < KB * 2; ++kb)
                     write_part(so, o + kb * 32, rows_ok, a.part_o + (prow - lane) * a.D, kb * 32, a.D, lane);
@@ -512,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 write_rows<BF>(so, o + kb * 64, inv, rows_ok, po, qt * kTile + q4 * 32, a.os.token, kb * 64, a.D, lane);
             if (real && a.lse)
                 a.lse[((size_t)P.b * a.H + h) * a.len_q + i] =
-                    l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) * a.scale2 + log2f(l)) * 0.693147180559945f;
+                    l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) * a.scale2 - kLift<BF> + log2f(l)) * 0.693147180559945f;
         }
         tc_fence_before();
     }
@@ -761,7 +767,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                         }
                     }
                 }
-                const float ms = (m == -INFINITY ? 0.0f : m) * a.scale2;
+                const float ms = (m == -INFINITY ? 0.0f : m) * a.scale2 - kLift<BF>;
                 const float2 nm = make_float2(-ms, -ms);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
@@ -805,12 +811,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 }
             }
             if (a.parts > 1) {
-                if (real) a.part_ml[prow] = make_float2((m == -INFINITY ? 0.0f : m) * a.scale2, l);
+                if (real) a.part_ml[prow] = make_float2((m == -INFINITY ? 0.0f : m) * a.scale2 - kLift<BF>, l);
                 continue;
             }
             if (real && a.lse)
                 a.lse[((size_t)P.b * a.H + P.h) * a.len_q + i] =
-                    l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) * a.scale2 + log2f(l)) * 0.693147180559945f;
+                    l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) * a.scale2 - kLift<BF> + log2f(l)) * 0.693147180559945f;
         }
         tc_fence_before();
     }

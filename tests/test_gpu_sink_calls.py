@@ -40,3 +40,39 @@ def test_nothing_to_join_then_a_call_on_the_same_workspace(dtype, D, cuda):
         assert bool((empty == 3.0).all()) and bool((empty_lse == 5.0).all())
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
     assert att.status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,q0,k0", [(64, 12.0, 12.0), (128, 12.0, 17.0), (256, 16.0, 18.0)])
+def test_many_small_weights_count(dtype, D, q0, k0, cuda):
+    """One key 18 above all others, whose V is 0: the output is what 40000
+    weights of e^-18 = 2^-26 add up to.  Against the formula in 64 bits: such a
+    weight as an fp16 number 2^7 larger is off by half of its fixed step, 2^-32,
+    or relative by half a step of the type; then the output by half a step
+    (fp32's own errors, 2^-24 a term at the most, are below both)."""
+    H, Lq, Lk = 40, 300, 40000  # every SM has queries, so the keys stay in one part
+    Q, K = torch.zeros((1, H, Lq, D), dtype=dtype, device=cuda), torch.zeros((1, H, Lk, D), dtype=dtype, device=cuda)
+    Q[..., 0], K[:, :, 0, 0] = q0, k0
+    g = torch.Generator(device=cuda).manual_seed(3)
+    V = (1 + torch.rand((1, H, Lk, D), generator=g, device=cuda)).to(dtype)
+    V[:, :, 0] = 0
+    out, lse = torch.zeros_like(Q), torch.zeros((1, H, Lq), device=cuda)
+    att = rkv.SinkAttention(device=cuda)
+    att(Q, K, V, out=out, lse=lse)
+    assert att.status() == 0
+    s, u = q0 * k0 / math.sqrt(D), R.unit(dtype)
+    w = math.exp(-s)
+    p = torch.arange(Lk - Lq, Lk, device=cuda, dtype=torch.float64)
+    total = 1 + p * w
+    for h in range(H):
+        add = V[0, h].double().cumsum(0)[Lk - Lq:]
+        want = add * w / total[:, None]
+        fixed = 2.0 ** -32 * p[:, None] * 2 if dtype == torch.float16 else 0.0  # V < 2
+        sums = R.EPS * (625 + 16 * s)
+        tol = want * (2 * u + sums) + fixed
+        off = float(((out[0, h] - want).abs() / tol).max())
+        assert off <= 1, (h, off)
+    # the weights' sum is rounded once a tile, and with equal terms always the same way: up to 625 tiles of 64 keys,
+    # 625 * 2^-24 of it; the exponent's largest term and lse itself a few times
+    off = float((lse[0].double() - s - total.log()).abs().max())
+    assert off <= R.EPS * (625 + 8 * s), off
