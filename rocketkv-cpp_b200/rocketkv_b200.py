@@ -667,12 +667,26 @@ def _row_strides(t, what):
 class SinkAttention:
     """Causal prefill attention over a sliding window and a few first tokens
     that stay visible (rkv_sink_attention); window 0: every key up to the
-    query.  Holds the workspace, which grows with the calls' sizes: calls that
-    may run at the same time need an object each."""
+    query.  Holds the workspace, which grows with the calls' sizes, at least to
+    twice what it was, so that what is kept of outgrown ones stays below the
+    largest: calls that may run at the same time need an object each."""
 
     def __init__(self, sinks: int = 0, window: int = 0, device="cuda"):
         self.sinks, self.window = sinks, window
         self.ws, self._outgrown = _workspace(0, device), []
+
+    def reserve(self, dtype: int, num_heads: int, num_heads_kv: int, dim_head: int, len_q: int, len_k: int, batch: int = 1,
+                stream=None) -> None:
+        """Makes room for calls of these sizes, under any sinks and window, as
+        each call does for its own.  Few queries take more than many: their keys
+        are split."""
+        need = _SZ(0)
+        _check(lib().rkv_sink_attention_workspace_size(dtype, len_q, len_k, batch, num_heads, num_heads_kv, dim_head,
+                                                       ctypes.byref(need)), "rkv_sink_attention_workspace_size")
+        if self.ws.numel() < need.value:
+            self._outgrown.append(self.ws)  # calls in flight and captured graphs may still use it
+            with _on_stream(self.ws.device, stream):
+                self.ws = _workspace(max(need.value, 2 * self.ws.numel()), self.ws.device)
 
     def __call__(self, Q, K, V, lens=None, out=None, lse=None, stream=None):
         """Q [B, H, len_q, D], K, V [B, HK, len_k, D] (float32, bfloat16 or
@@ -701,13 +715,7 @@ class SinkAttention:
             _int32(lens, Q.device, "lens")
             if lens.numel() != B:
                 raise ValueError("lens: one entry per item")
-        need = _SZ(0)
-        _check(lib().rkv_sink_attention_workspace_size(dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(need)),
-               "rkv_sink_attention_workspace_size")
-        if self.ws.numel() < need.value:
-            self._outgrown.append(self.ws)  # calls in flight and captured graphs may still use it
-            with _on_stream(Q.device, stream):
-                self.ws = _workspace(need.value, Q.device)
+        self.reserve(dt, H, K.shape[1], D, Lq, K.shape[2], B, stream)
         qs, ks, os_ = _row_strides(Q, "Q"), _row_strides(K, "K, V"), _row_strides(out, "out")
         _launch(Q.device, stream, "rkv_sink_attention", lib().rkv_sink_attention, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
                 dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(qs), ctypes.byref(ks), _ptr(lens), self.sinks,
