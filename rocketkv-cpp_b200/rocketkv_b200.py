@@ -674,6 +674,7 @@ class SinkAttention:
     def __init__(self, sinks: int = 0, window: int = 0, device="cuda"):
         self.sinks, self.window = sinks, window
         self.ws, self._outgrown = _workspace(0, device), []
+        self._ran = False  # a call with work to do has used ws (and each of _outgrown), and written its error word
 
     def reserve(self, dtype: int, num_heads: int, num_heads_kv: int, dim_head: int, len_q: int, len_k: int, batch: int = 1,
                 stream=None) -> None:
@@ -684,9 +685,11 @@ class SinkAttention:
         _check(lib().rkv_sink_attention_workspace_size(dtype, len_q, len_k, batch, num_heads, num_heads_kv, dim_head,
                                                        ctypes.byref(need)), "rkv_sink_attention_workspace_size")
         if self.ws.numel() < need.value:
-            self._outgrown.append(self.ws)  # calls in flight and captured graphs may still use it
+            if self._ran:
+                self._outgrown.append(self.ws)  # calls in flight and captured graphs may still use it
             with _on_stream(self.ws.device, stream):
                 self.ws = _workspace(max(need.value, 2 * self.ws.numel()), self.ws.device)
+            self._ran = False
 
     def __call__(self, Q, K, V, lens=None, out=None, lse=None, stream=None):
         """Q [B, H, len_q, D], K, V [B, HK, len_k, D] (float32, bfloat16 or
@@ -720,9 +723,16 @@ class SinkAttention:
         _launch(Q.device, stream, "rkv_sink_attention", lib().rkv_sink_attention, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
                 dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(qs), ctypes.byref(ks), _ptr(lens), self.sinks,
                 self.window, out.data_ptr(), ctypes.byref(os_), _ptr(lse), self.ws.data_ptr(), self.ws.numel())
+        self._ran |= B > 0 and Lq > 0
         return out
 
     def status(self, stream=None) -> int:
+        """Waits for `stream`; the first error that a call recorded in any
+        workspace since the last look, or RKV_OK."""
         import torch
+        found = RKV_OK
         with torch.cuda.device(self.ws.device):
-            return lib().rkv_workspace_status(_ptr(self.ws), _stream(stream))
+            for ws in self._outgrown + [self.ws] * self._ran:
+                st = lib().rkv_workspace_status(_ptr(ws), _stream(stream))
+                found = found or st
+        return found

@@ -76,3 +76,32 @@ def test_many_small_weights_count(dtype, D, q0, k0, cuda):
     # 625 * 2^-24 of it; the exponent's largest term and lse itself a few times
     off = float((lse[0].double() - s - total.log()).abs().max())
     assert off <= R.EPS * (625 + 8 * s), off
+
+
+def test_status_of_an_object_that_has_not_run(cuda):
+    """No error word is read that no call has written: neither of a new
+    object, in memory that held something else, nor after calls without work."""
+    for _ in range(8):  # blocks of the size a workspace has, given back full of ones
+        junk = [torch.full((256,), 255, dtype=torch.uint8, device=cuda) for _ in range(64)]
+        del junk
+        att = rkv.SinkAttention(device=cuda)
+        assert att.status() == 0
+        Q, K, V = _inputs(5, 0, 2, 1, 8, 8, 64, torch.bfloat16, cuda)
+        att(Q, K, V)
+        Q, K, V = _inputs(5, 1, 2, 1, 0, 8, 64, torch.bfloat16, cuda)
+        att(Q, K, V)
+        assert att.status() == 0
+
+
+def test_status_of_a_call_whose_workspace_was_outgrown(cuda):
+    """An error that a call recorded is found after the workspace has grown,
+    once, and whatever the other calls recorded."""
+    att = rkv.SinkAttention(device=cuda)
+    Q, K, V = _inputs(6, 1, 2, 1, 8, 8, 64, torch.bfloat16, cuda)
+    att(Q, K, V)
+    first = att.ws
+    att(*_inputs(6, 1, 2, 1, 8, 5000, 64, torch.bfloat16, cuda))
+    assert att.ws is not first and att.status() == 0
+    first[:4].view(torch.int32).fill_(rkv.RKV_ERR_DEVICE_TIMEOUT)  # as the kernel records it
+    assert att.status() == rkv.RKV_ERR_DEVICE_TIMEOUT
+    assert att.status() == 0
