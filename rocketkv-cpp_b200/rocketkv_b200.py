@@ -636,8 +636,9 @@ class WeightEvictor:
 
     def __call__(self, cache: PagedCache, weights, out: PagedCache | None = None, weights_out=None, stream=None):
         """In place without out / weights_out.  Returns (kept [B, HK, min(budget,
-        max_len)] int32 ascending with -1 behind, new_lens [B] int32): the
-        caller's next calls take new_lens (copied, or as the cache's lens)."""
+        max_len)] int32 ascending with -1 behind, new_lens [B] int32), which the
+        next call overwrites: copy new_lens to where the cache's lens is kept.
+        A cache whose lens is this evictor's new_lens is refused."""
         dev = cache.K.device
         if cache.batch != self.batch or cache.c.num_heads_kv != self.num_heads_kv or cache._lens is None or weights is None:
             raise ValueError("the evictor's batch and KV heads, lens and weights are needed")
@@ -645,6 +646,8 @@ class WeightEvictor:
             raise ValueError("out: the same batch, on the cache's device")
         if self.kept.device != dev:
             raise ValueError("the cache is not on the evictor's device")
+        if self.batch and cache.c.lens == self.new_lens.data_ptr():
+            raise ValueError("the cache's lens is this evictor's new_lens, which the call overwrites: copy it")
         ws = _check_weights(weights, self.batch, self.num_heads_kv, self.max_len, dev)
         if weights_out is not None and _check_weights(weights_out, self.batch, self.num_heads_kv, self.max_len, dev) != ws:
             raise ValueError("weights_out: the layout of weights")

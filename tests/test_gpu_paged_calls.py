@@ -1,0 +1,44 @@
+"""Calls of the paged-cache operators one after the other: lengths handed on
+from eviction to eviction, buffers on other streams, batches without a
+sequence."""
+import pytest
+import torch
+
+import pagedref as R
+import rocketkv_b200 as rkv
+
+pytestmark = pytest.mark.gpu
+
+
+def _cache(seed, B, hk, d, page, top, dtype, dev, lens):
+    per = max(1, -(-top // page))
+    K, V = R.pool(seed, B * per + 2, hk, page, d, dtype, dev)
+    return rkv.PagedCache(K, V, R.table(seed + 1, B, per, B * per + 2, dev), torch.tensor(lens, dtype=torch.int32, device=dev))
+
+
+def test_evictions_in_a_row_hand_their_lengths_on(cuda):
+    """new_lens is copied into the cache's lens before the next call; taken as
+    the cache's lens itself it is refused before anything is changed, since
+    the call would overwrite what it reads."""
+    B, HK, D, n = 2, 2, 64, 300
+    c = _cache(1, B, HK, D, 16, n, torch.bfloat16, cuda, [300, 150])
+    lens = c.lens
+    g = torch.Generator(device=cuda).manual_seed(3)
+    W = torch.rand((B, HK, n), generator=g, device=cuda)
+    first = rkv.WeightEvictor(HK, n, B, 200, cuda, sinks=2, recent=8)
+    second = rkv.WeightEvictor(HK, n, B, 120, cuda, sinks=2, recent=8)
+    _, new = first(c, W)
+    assert new.tolist() == [200, 150]
+    c.lens = new
+    before = [t.clone() for t in (c.K, c.V, W, new, first.kept)]
+    with pytest.raises(ValueError, match="copy"):
+        first(c, W)
+    assert all(torch.equal(a, b) for a, b in zip(before, (c.K, c.V, W, new, first.kept)))
+    second(c, W)  # another evictor's own lengths are no trouble
+    assert second.new_lens.tolist() == [120, 120] and new.tolist() == [200, 150]
+    c.lens = lens
+    lens.copy_(second.new_lens)
+    w0 = W.clone()
+    kept, new = rkv.WeightEvictor(HK, n, B, 50, cuda)(c, W)
+    assert new.tolist() == [50, 50]
+    assert kept[..., :50].tolist() == R.kept_lists(w0, [120, 120], 50, 0, 0)
