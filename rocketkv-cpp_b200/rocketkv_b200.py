@@ -698,8 +698,8 @@ class SinkAttention:
         """Q [B, H, len_q, D], K, V [B, HK, len_k, D] (float32, bfloat16 or
         float16; unit stride along D, K and V strided alike); lens (nullable) [B]
         int32: valid keys of each item, query rows at positions from lens[b] on
-        are left as they were.  out: as Q (allocated without); lse: float32
-        [B, H, len_q].  Returns out."""
+        are left as they were.  out: as Q (a fresh one without, 0 in the rows left
+        out); lse: float32 [B, H, len_q].  Returns out."""
         import torch
         if K.shape != V.shape or K.stride() != V.stride() or not (Q.dtype == K.dtype == V.dtype):
             raise ValueError("K and V: one shape and layout; Q, K, V: one type")
@@ -707,7 +707,8 @@ class SinkAttention:
             raise ValueError("Q, K, V and the workspace: one device")
         if out is None:
             with _on_stream(Q.device, stream):
-                out = torch.zeros(Q.shape, dtype=Q.dtype, device=Q.device)
+                # without lens every row is written
+                out = (torch.empty if lens is None else torch.zeros)(Q.shape, dtype=Q.dtype, device=Q.device)
         if out.shape != Q.shape or out.dtype != Q.dtype or out.device != Q.device:
             raise ValueError("out: Q's shape, type and device")
         B, H, Lq, D = Q.shape

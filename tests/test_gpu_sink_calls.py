@@ -105,3 +105,23 @@ def test_status_of_a_call_whose_workspace_was_outgrown(cuda):
     first[:4].view(torch.int32).fill_(rkv.RKV_ERR_DEVICE_TIMEOUT)  # as the kernel records it
     assert att.status() == rkv.RKV_ERR_DEVICE_TIMEOUT
     assert att.status() == 0
+
+
+def test_a_fresh_output_is_filled_only_where_rows_stay_unwritten(cuda, monkeypatch):
+    """Zeros behind the ends of padded sequences; without lens every row is
+    written and nothing else is launched."""
+    Q, K, V = _inputs(7, 2, 4, 2, 70, 90, 64, torch.bfloat16, cuda)
+    att = rkv.SinkAttention(device=cuda)
+    lens = torch.tensor([90, 33], dtype=torch.int32, device=cuda)
+    want = torch.zeros_like(Q)
+    att(Q, K, V, lens=lens, out=want)
+    assert torch.equal(att(Q, K, V, lens=lens), want) and bool((want[1, :, 13:] == 0).all())
+    att(Q, K, V, out=want)
+
+    def fill(*args, **kw):
+        raise AssertionError("an output was filled")
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "zeros", fill)
+        got = att(Q, K, V)
+    assert torch.equal(got, want)
