@@ -471,15 +471,32 @@ class HsaDecoder:
 # ---------------------------------------------------------------------------
 # Paged KV cache: append, dense decode, eviction by accumulated weight
 # ---------------------------------------------------------------------------
-def _launch(device, stream, what, fn, *args) -> None:
+def _handle(device, stream) -> int:
+    return _current_stream(device.index) if stream is None else int(stream)
+
+
+def _stream_object(device, handle: int):
+    import torch
+    return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+
+
+def _launch(device, stream, what, fn, *args, owner=None) -> None:
     """fn(*args, stream) with the tensors' device current (a stream belongs to one)."""
     import torch
-    i = device.index
-    if i == torch.cuda.current_device():
-        st = fn(*args, _current_stream(i) if stream is None else int(stream))
+    h = _handle(device, stream)
+    if owner is not None and h not in owner._streams:
+        # the object's buffers belong to the stream they were made on; dropped with it while this call runs on
+        # another one, they would be handed out again at once (the mark lasts, but not one set under a capture)
+        other = _stream_object(device, h)
+        for t in owner._buffers():
+            t.record_stream(other)
+        if not torch.cuda.is_current_stream_capturing():
+            owner._streams.add(h)
+    if device.index == torch.cuda.current_device():
+        st = fn(*args, h)
     else:
         with torch.cuda.device(device):
-            st = fn(*args, _current_stream(i) if stream is None else int(stream))
+            st = fn(*args, h)
     if st != RKV_OK:
         raise RkvError(st, what)
 
@@ -490,8 +507,7 @@ def _on_stream(device, stream):
     import torch
     if stream is None:
         return contextlib.nullcontext()
-    h = int(stream)
-    return torch.cuda.stream(torch.cuda.ExternalStream(h, device=device) if h else torch.cuda.default_stream(device))
+    return torch.cuda.stream(_stream_object(device, int(stream)))
 
 
 def _int32(t, device, what):
@@ -589,6 +605,10 @@ class PagedDecoder:
         # each call writes all of them; a fill on this stream could run after a call on another
         self.O = torch.empty((batch, num_heads, dim_head), dtype=torch.float32, device=device)
         self.lse = torch.empty((batch, num_heads), dtype=torch.float32, device=device)
+        self._streams = {_handle(self.ws.device, None)}  # whose work its buffers outlive
+
+    def _buffers(self):
+        return self.ws, self.O, self.lse
 
     def __call__(self, Q, cache: PagedCache, weights=None, stream=None):
         """Q [B, H, D] of the cache's type.  weights (nullable): float32
@@ -606,7 +626,7 @@ class PagedDecoder:
         _launch(dev, stream, "rkv_paged_decode", lib().rkv_paged_decode, Q.data_ptr(),
                 self.num_heads * self.dim_head * Q.element_size(), self.num_heads, cache.ref, self.max_len, self.batch,
                 self.sinks, self.window, self.O.data_ptr(), self.lse.data_ptr(), _ptr(weights), wstride,
-                self.ws.data_ptr(), self.ws_bytes)
+                self.ws.data_ptr(), self.ws_bytes, owner=self)
         return self.O
 
 
@@ -633,6 +653,10 @@ class WeightEvictor:
         # each call writes all of them; a fill on this stream could run after a call on another
         self.kept = torch.empty((batch, num_heads_kv, max(0, min(budget, max_len))), dtype=torch.int32, device=device)
         self.new_lens = torch.empty(batch, dtype=torch.int32, device=device)
+        self._streams = {_handle(self.kept.device, None)}
+
+    def _buffers(self):
+        return self.kept, self.new_lens
 
     def __call__(self, cache: PagedCache, weights, out: PagedCache | None = None, weights_out=None, stream=None):
         """In place without out / weights_out.  Returns (kept [B, HK, min(budget,
@@ -653,7 +677,7 @@ class WeightEvictor:
             raise ValueError("weights_out: the layout of weights")
         _launch(dev, stream, "rkv_weight_evict", lib().rkv_weight_evict, cache.ref, weights.data_ptr(), ws, self.max_len,
                 self.batch, self.budget, self.sinks, self.recent, out.ref if out is not None else None, _ptr(weights_out),
-                self.kept.data_ptr(), self.kept.shape[2], self.new_lens.data_ptr())
+                self.kept.data_ptr(), self.kept.shape[2], self.new_lens.data_ptr(), owner=self)
         return self.kept, self.new_lens
 
 
@@ -677,6 +701,7 @@ class SinkAttention:
     def __init__(self, sinks: int = 0, window: int = 0, device="cuda"):
         self.sinks, self.window = sinks, window
         self.ws, self._outgrown = _workspace(0, device), []
+        self._streams = {_handle(self.ws.device, None)}  # whose work its buffers outlive
         self._ran = False  # a call with work to do has used ws (and each of _outgrown), and written its error word
 
     def reserve(self, dtype: int, num_heads: int, num_heads_kv: int, dim_head: int, len_q: int, len_k: int, batch: int = 1,
@@ -692,7 +717,10 @@ class SinkAttention:
                 self._outgrown.append(self.ws)  # calls in flight and captured graphs may still use it
             with _on_stream(self.ws.device, stream):
                 self.ws = _workspace(max(need.value, 2 * self.ws.numel()), self.ws.device)
-            self._ran = False
+            self._streams, self._ran = {_handle(self.ws.device, stream)}, False
+
+    def _buffers(self):
+        return (self.ws,)
 
     def __call__(self, Q, K, V, lens=None, out=None, lse=None, stream=None):
         """Q [B, H, len_q, D], K, V [B, HK, len_k, D] (float32, bfloat16 or
@@ -726,7 +754,7 @@ class SinkAttention:
         qs, ks, os_ = _row_strides(Q, "Q"), _row_strides(K, "K, V"), _row_strides(out, "out")
         _launch(Q.device, stream, "rkv_sink_attention", lib().rkv_sink_attention, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
                 dt, Lq, K.shape[2], B, H, K.shape[1], D, ctypes.byref(qs), ctypes.byref(ks), _ptr(lens), self.sinks,
-                self.window, out.data_ptr(), ctypes.byref(os_), _ptr(lse), self.ws.data_ptr(), self.ws.numel())
+                self.window, out.data_ptr(), ctypes.byref(os_), _ptr(lse), self.ws.data_ptr(), self.ws.numel(), owner=self)
         self._ran |= B > 0 and Lq > 0
         return out
 

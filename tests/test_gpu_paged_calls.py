@@ -42,3 +42,44 @@ def test_evictions_in_a_row_hand_their_lengths_on(cuda):
     kept, new = rkv.WeightEvictor(HK, n, B, 50, cuda)(c, W)
     assert new.tolist() == [50, 50]
     assert kept[..., :50].tolist() == R.kept_lists(w0, [120, 120], 50, 0, 0)
+
+
+def _tensors(o):
+    return [t for t in vars(o).values() if isinstance(t, torch.Tensor)]
+
+
+@pytest.mark.parametrize("kind", ["decoder", "evictor", "prefill"])
+def test_buffers_outlive_their_object_while_a_call_on_another_stream_runs(kind, cuda):
+    """An object made here, called on another stream that is still busy, and
+    dropped: its workspace and outputs are not handed to new tensors (which are
+    only allocated here, never written) until the call has run."""
+    B, H, HK, D, n = 2, 4, 2, 64, 200
+    c = _cache(5, B, HK, D, 16, n, torch.bfloat16, cuda, [n, 90])
+    g = torch.Generator(device=cuda).manual_seed(6)
+    W = torch.rand((B, HK, n), generator=g, device=cuda)
+    Q, K, V = (torch.randn((B, h, n, D), generator=g, device=cuda).to(torch.bfloat16) for h in (H, HK, HK))
+    q, out = Q[:, :, 0].contiguous(), torch.zeros_like(Q)
+    s = torch.cuda.Stream()
+    for cycles in (1000, 200_000_000):  # first to load and allocate, which waits for the device; then about 100 ms
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(cycles)
+        if kind == "decoder":
+            o = rkv.PagedDecoder(H, HK, D, n, B, cuda, weights=True)
+            o(q, c, W, stream=s.cuda_stream)
+        elif kind == "evictor":
+            o = rkv.WeightEvictor(HK, n, B, 64, cuda)
+            o(c, W, stream=s.cuda_stream)
+        else:
+            o = rkv.SinkAttention(device=cuda)
+            o(Q, K, V, out=out, stream=s.cuda_stream)
+        mine = [(t.data_ptr(), t.numel() * t.element_size()) for t in _tensors(o)]
+        assert mine
+        del o
+        new = [torch.empty(size, dtype=torch.uint8, device=cuda) for _, size in mine for _ in range(4)]
+        busy = not s.query()
+    assert busy, "the call ended too early to show anything"
+    for t in new:
+        for at, size in mine:
+            assert t.data_ptr() + t.numel() <= at or at + size <= t.data_ptr()
+    torch.cuda.synchronize()

@@ -10,7 +10,8 @@ import rocketkv_b200 as rkv
 def launches(monkeypatch):
     """Arguments of the calls that would have been launched."""
     got = []
-    monkeypatch.setattr(rkv, "_launch", lambda device, stream, what, fn, *args: got.append(args))
+    monkeypatch.setattr(rkv, "_launch", lambda device, stream, what, fn, *args, **kw: got.append(args))
+    monkeypatch.setattr(rkv, "_current_stream", lambda index: 0)
     return got
 
 
