@@ -829,7 +829,7 @@ using namespace rkv;
 extern "C" int rkv_paged_append(const rkv_paged_cache* cache, const void* k, const void* v, int n_rows, int batch,
                                 long long src_item_stride, long long src_token_stride, long long src_head_stride,
                                 const int* n_new, void* stream) {
-    const int rc = paged_check(cache, true);
+    const int rc = paged_check(cache, true, batch);
     if (rc) return rc;
     if (n_rows < 0 || batch < 0) return RKV_ERR_INVALID_ARG;
     if (n_rows == 0 || batch == 0 || cache->num_pages == 0 || cache->table_stride == 0) return RKV_OK;
@@ -892,7 +892,7 @@ extern "C" int rkv_paged_decode_workspace_size(int num_heads, int num_heads_kv, 
 extern "C" int rkv_paged_decode(const void* Q, long long q_item_stride, int num_heads, const rkv_paged_cache* cache,
                                 int max_len, int batch, int sinks, int window, float* O, float* lse, float* weights,
                                 int weight_stride, void* workspace, size_t workspace_bytes, void* stream) {
-    int rc = paged_check(cache, true);
+    int rc = paged_check(cache, true, batch);
     if (!rc) rc = decode_shape_check(num_heads, cache->num_heads_kv, cache->dim_head, max_len, batch);
     if (rc) return rc;
     if (sinks < 0 || window < 0) return RKV_ERR_INVALID_ARG;

@@ -50,8 +50,9 @@ __device__ __forceinline__ long long paged_offset(const PagedView& c, int b, int
 inline bool paged_dtype(int dt) { return dt == RKV_F32 || dt == RKV_BF16 || dt == RKV_F16; }
 inline int elem_size(int dt) { return dt == RKV_F32 ? 4 : 2; }
 
-// Sizes, alignment and strides of a cache; lens_too: whether lens is read.
-inline int paged_check(const rkv_paged_cache* c, bool lens_too) {
+// Sizes, alignment and strides of a cache; lens_too: whether lens is read.  A batch without a sequence reads
+// neither lens nor the table.
+inline int paged_check(const rkv_paged_cache* c, bool lens_too, int batch) {
     if (!c || !paged_dtype(c->dtype)) return RKV_ERR_INVALID_ARG;
     if (c->num_heads_kv <= 0 || c->dim_head <= 0 || c->page_size <= 0 || c->num_pages < 0 || c->table_stride < 0)
         return RKV_ERR_INVALID_ARG;
@@ -63,6 +64,7 @@ inline int paged_check(const rkv_paged_cache* c, bool lens_too) {
         (c->num_pages > 1 && c->page_stride < rowb))
         return RKV_ERR_INVALID_ARG;
     if (c->num_pages > 0 && (!c->K || !c->V)) return RKV_ERR_INVALID_ARG;
+    if (batch == 0) return RKV_OK;
     if (c->table_stride > 0 && !c->block_table) return RKV_ERR_INVALID_ARG;
     if (lens_too && !c->lens) return RKV_ERR_INVALID_ARG;
     return RKV_OK;

@@ -550,13 +550,13 @@ using namespace rkv;
 extern "C" int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, int weight_stride, int max_len, int batch,
                                 int budget, int sinks, int recent, const rkv_paged_cache* out, float* weights_out,
                                 int* kept, int kept_stride, int* new_lens, void* stream) {
-    int rc = paged_check(cache, true);
+    int rc = paged_check(cache, true, batch);
     if (rc) return rc;
     if (max_len < 0 || batch < 0 || budget < 0 || sinks < 0 || recent < 0 || (long long)sinks + recent > budget)
         return RKV_ERR_INVALID_ARG;
     if (max_len > kMaxLen) return RKV_ERR_UNSUPPORTED;
     if (out) {
-        if ((rc = paged_check(out, false))) return rc;
+        if ((rc = paged_check(out, false, batch))) return rc;
         if (out->dtype != cache->dtype || out->num_heads_kv != cache->num_heads_kv || out->dim_head != cache->dim_head)
             return RKV_ERR_INVALID_ARG;
     }

@@ -83,3 +83,20 @@ def test_buffers_outlive_their_object_while_a_call_on_another_stream_runs(kind, 
         for at, size in mine:
             assert t.data_ptr() + t.numel() <= at or at + size <= t.data_ptr()
     torch.cuda.synchronize()
+
+
+def test_a_batch_without_a_sequence(cuda):
+    """Every call of the paged cache takes an empty batch and does nothing."""
+    H, HK, D, n = 4, 2, 64, 50
+    K, V = R.pool(8, 6, HK, 16, D, torch.bfloat16, cuda)
+    K0 = K.clone()
+    c = rkv.PagedCache(K, V, torch.empty((0, 4), dtype=torch.int32, device=cuda), torch.empty(0, dtype=torch.int32, device=cuda))
+    k = torch.empty((0, 3, HK, D), dtype=torch.bfloat16, device=cuda)
+    rkv.paged_append(c, k, k)
+    W = torch.empty((0, HK, n), device=cuda)
+    assert rkv.PagedDecoder(H, HK, D, n, 0, cuda, weights=True)(k[:, 0].repeat(1, 2, 1), c, W).shape == (0, H, D)
+    kept, new = rkv.WeightEvictor(HK, n, 0, 20, cuda)(c, W)
+    assert kept.shape == (0, HK, 20) and new.shape == (0,)
+    assert rkv.SinkAttention(device=cuda)(*(torch.empty((0, h, 8, D), dtype=torch.bfloat16, device=cuda) for h in (H, HK, HK))).shape[0] == 0
+    torch.cuda.synchronize()
+    assert torch.equal(K, K0)
