@@ -336,7 +336,8 @@ int rkv_evict_compact(const void* Q, const void* K, const void* V, int dtype, in
  * of sequence b; it is read on the device and clamped to
  * [0, min(max_len, table_stride * page_size)].  Pages may be shared between
  * sequences that only read them.  A page index outside [0, num_pages) is
- * never followed: its tokens are left out (not read, not written). */
+ * never followed: its tokens are left out (not read, not written).  A batch
+ * of 0 has nothing to do and needs neither table nor lens. */
 typedef struct rkv_paged_cache {
     void* K;
     void* V;
@@ -379,7 +380,17 @@ int rkv_paged_append(const rkv_paged_cache* cache, const void* k, const void* v,
  * what rkv_weight_evict ranks by.  max_len: host bound on lens (it fixes the
  * launch, so a captured call serves every length up to it).  The split of the
  * cache over CTAs does not depend on what lens holds and the parts are joined
- * in a fixed order: results repeat bit for bit.
+ * in a fixed order: results repeat bit for bit.  The price: a few sequences far
+ * below max_len run on the few CTAs that their part of it has (24/8 heads of
+ * 128, bf16: one sequence of 2048 tokens 7 us under max_len 2048, 11 under
+ * 8192, 35 under 131072; from 64 sequences on it makes no difference), so
+ * capture calls for some lengths, not for the largest alone.
+ * Sums and the softmax are fp32; products of 16-bit types are exact, with the
+ * weights in two (fp16) or three (bf16) 16-bit parts, and fp32 operands enter
+ * as two tf32 parts each, without the product of the two smaller ones (2^-22
+ * or so of a product).  A NaN or infinity in a visible row of K reaches its KV
+ * head's outputs, one in V its column of them, as a NaN also where the formula
+ * gives an infinity (or, for fp32 K, a weight of 0).
  * Workspace: device, 16-byte aligned, not shared with a call that may run at
  * the same time; with_weights: whether weights will be passed.  Asynchronous
  * on `stream`; allocates nothing. */
@@ -420,18 +431,25 @@ int rkv_weight_evict(const rkv_paged_cache* cache, float* weights, int weight_st
  * item of a padded batch; keys from lens[b] on may hold anything and query rows
  * at positions from lens[b] on are left as they were.  V of the keys before
  * that must be finite: keys are taken by tiles, and an infinity or NaN in V
- * may reach a query of the tile that does not see its key.  A NaN in K stays
- * in the queries that see it.
+ * may reach a query of the tile that does not see its key.  A NaN or infinity
+ * in K stays in the queries that see it.
  * Q: [batch][num_heads][len_q][dim_head], K, V: [batch][num_heads_kv][len_k]
- * [dim_head], O as Q, all of dtype (RKV_F32, RKV_BF16, RKV_F16; sums and
- * softmax in fp32), at the given strides (bytes, multiples of 16; NULL: rows,
- * heads and items back to back).  dim_head: a multiple of 8, at most 256;
- * num_heads a multiple of num_heads_kv.  lse (nullable):
- * [batch][num_heads][len_q] fp32.  O must not overlap the inputs.
+ * [dim_head], O as Q, all of dtype (RKV_F32, RKV_BF16, RKV_F16), at the given
+ * strides (bytes, multiples of 16; NULL: rows, heads and items back to back).
+ * dim_head: a multiple of 8, at most 256; num_heads a multiple of num_heads_kv.
+ * lse (nullable): [batch][num_heads][len_q] fp32.  O must not overlap the
+ * inputs.
+ * Scores, the softmax's maxima and sums, and the output's sums are fp32.  With
+ * 16-bit types each weight is rounded to the type before it meets V (half a
+ * step of the type; in fp16 a fixed 2^-32 of the row's largest below 2^-21 of
+ * it) and the output once more; fp32 operands enter as two tf32 parts each,
+ * without the product of the two smaller ones.
  * Workspace: device, 16-byte aligned, not shared with a call that may run at
  * the same time; the size serves every sinks and window.  It begins with the
- * error word that rkv_workspace_status reads, and holds the parts of the keys
- * where few queries meet many.  Asynchronous on `stream`; allocates nothing. */
+ * error word that rkv_workspace_status reads, which every call with a query
+ * sets anew, and holds the parts of the keys where few queries meet many (at
+ * most as many parts as there are SMs, so fewer queries may need more).
+ * Asynchronous on `stream`; allocates nothing. */
 typedef struct rkv_row_strides {
     long long item, head, token;
 } rkv_row_strides;

@@ -100,3 +100,27 @@ def test_a_batch_without_a_sequence(cuda):
     assert rkv.SinkAttention(device=cuda)(*(torch.empty((0, h, 8, D), dtype=torch.bfloat16, device=cuda) for h in (H, HK, HK))).shape[0] == 0
     torch.cuda.synchronize()
     assert torch.equal(K, K0)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.bfloat16, 128), (torch.float16, 256)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_decode_keeps_non_finite_values_where_they_are(dtype, D, bad, cuda):
+    """In a visible row of V: in its column of its KV head's outputs, nowhere
+    else.  In a visible row of K: in its KV head's outputs."""
+    B, H, HK, n = 1, 6, 3, 700
+    c = _cache(11, B, HK, D, 16, n, dtype, cuda, [n])
+    g = torch.Generator(device=cuda).manual_seed(12)
+    q = torch.randn((B, H, D), generator=g, device=cuda).to(dtype)
+    dec, ref = (rkv.PagedDecoder(H, HK, D, n, B, cuda) for _ in range(2))
+    ref(q, c)
+    at, row = c.block_table[0, 20].long(), 7
+    c.V[at, 1, row, 5] = bad
+    dec(q, c)
+    hit = torch.zeros_like(dec.O, dtype=torch.bool)
+    hit[0, 2:4, 5] = True
+    assert not bool(dec.O[hit].isfinite().any()) and torch.equal(dec.O[~hit], ref.O[~hit]) and torch.equal(dec.lse, ref.lse)
+    c.V[at, 1, row, 5] = 1.0
+    ref(q, c)
+    c.K[at, 1, row, 5] = bad
+    dec(q, c)
+    assert torch.equal(dec.O[0, :2], ref.O[0, :2]) and torch.equal(dec.O[0, 4:], ref.O[0, 4:])

@@ -125,3 +125,26 @@ def test_a_fresh_output_is_filled_only_where_rows_stay_unwritten(cuda, monkeypat
         m.setattr(torch, "zeros", fill)
         got = att(Q, K, V)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.bfloat16, 128), (torch.float16, 256)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("Lq,Lk", [(600, 600), (40, 6000)])
+def test_a_non_finite_key_stays_in_the_queries_that_see_it(dtype, D, bad, Lq, Lk, cuda):
+    """Queries before it and those whose window has passed it keep their bits,
+    though their tiles hold it, and so do other KV heads' queries."""
+    H, HK, window = 4, 2, 17
+    Q, K, V = _inputs(8, 1, H, HK, Lq, Lk, D, dtype, cuda)
+    j = Lk - Lq + 20
+    ref, got = (torch.zeros_like(Q) for _ in range(2))
+    lse0, lse = (torch.zeros((1, H, Lq), device=cuda) for _ in range(2))
+    att = rkv.SinkAttention(sinks=3, window=window, device=cuda)
+    att(Q, K, V, out=ref, lse=lse0)
+    K[0, 1, j, 2] = bad
+    att(Q, K, V, out=got, lse=lse)
+    p = torch.arange(Lk - Lq, Lk, device=cuda)
+    sees = torch.zeros((1, H, Lq), dtype=torch.bool, device=cuda)
+    sees[0, H // HK:] = (p >= j) & (p < j + window)
+    assert torch.equal(got[~sees], ref[~sees]) and torch.equal(lse[~sees], lse0[~sees])
+    if math.isnan(bad):
+        assert bool(got[sees].isnan().all())
