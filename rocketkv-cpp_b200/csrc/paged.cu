@@ -13,10 +13,10 @@
 // Memory bounds it: K and V are read once, 4 G flops per row of K and V of D
 // 16-bit values for G heads that share it.  bf16, 24/8 heads of 128, device
 // time: 8 x 131072 tokens 641 us (6.7 TB/s), 64 ragged sequences of up to 8192
-// 182 us (6.3), 16 x 3717 with weights 50.6 us (4.9); fp32, 8 x 32768 tokens,
-// 327 us (6.6).  Where there is little to read it is two launches: 1 x 2048
-// tokens 7.3 us, an fp32 window of 1024 tokens 10.0 us.  Not kept: the parts of
-// a head joined in a cluster's shared memory (64 ragged 201 us -> 301: parts
+// 182 us (6.3), 16 x 3717 with weights 50-55 us (5.0-4.5); fp32, 8 x 32768
+// tokens, 327 us (6.6).  Where there is little to read it is two launches:
+// 1 x 2048 tokens 7.3 us, an fp32 window of 1024 tokens 10-14 us.  Not kept: the
+// parts of a head joined in a cluster's shared memory (64 ragged 201 us -> 301: parts
 // without tokens hold their SM until the longest ends), and by the last CTA to
 // arrive in place of the second kernel (182 -> 187, 1 x 2048 7.3 -> 8.4).
 #include "paged.cuh"
@@ -275,9 +275,9 @@ struct Shape {
 // different banks.
 //
 // 16 bit: fragments by ldmatrix; P's fragment is the transpose of the scores'.
-// P keeps fp32's precision: it enters as a sum of 16-bit parts (three for
-// bf16, two for fp16), one product each, which costs little here, since the
-// kernel is bound by its reads.  fp32: tf32 products, each operand as its top
+// P keeps 22 bits or more: it enters as a sum of 16-bit parts (three for bf16,
+// two for fp16), one product each, which costs little here, since the kernel is
+// bound by its reads.  fp32: tf32 products, each operand as its top
 // 19 bits and the rest, three products (hi hi + lo hi + hi lo); the columns a
 // lane needs for four steps are one 16-byte chunk, since the order in which a
 // product sums its columns (or tokens) is free.

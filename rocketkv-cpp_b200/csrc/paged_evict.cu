@@ -15,7 +15,8 @@
 // and the copy 74; 8 x 131072 tokens (fp16) to 4096, 88 us (337 MB), 37 and 42;
 // one of 2112 tokens to 2048, 9.5 us.  Memory bounds the copies; chains of digit counts,
 // barriers and scans bound the selections (a weight is read from memory once
-// and, in a long cache, a second time from L2).
+// and, in a long cache, a second time from L2; the zeros behind the kept weights
+// are written in between).
 #include <cooperative_groups.h>
 
 #include <type_traits>

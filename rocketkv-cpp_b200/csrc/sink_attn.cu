@@ -16,9 +16,10 @@ constexpr int kBN = 64;  // keys of a tile
 // fp32 inputs: tf32 products of each operand as its top 19 bits and the rest,
 // three per product (hi hi + lo hi + hi lo), summed by the matrix units over a
 // tile or less and then added (their sums cut instead of rounding).  The rate
-// of these products bounds it: 24/8 heads of 128, 2048 tokens, causal, run at
-// 40 TFLOP/s, which is 120 of products.  One CTA per BM queries of
-// a head, a warp per 16 of them, 64 keys at a time; V arrives under the scores
+// of mma.sync bounds it: 24/8 heads of 128, 2048 tokens, causal, 642 us, 40
+// TFLOP/s, which is 120 of products (tcgen05 would allow some 275; not built).
+// Spills at 128 and 256 columns: 56 and 248 bytes a thread.  One CTA per BM
+// queries of a head, a warp per 16 of them, 64 keys at a time; V arrives under the scores
 // and the next K under the output's products.
 //
 // S = Q K^T has the queries on the rows; its fragment is P's fragment for

@@ -16,25 +16,28 @@
 //   warps 4-7, 8-11   softmax of unit 0, 1, and their output rows
 //
 // Two roundings to 16 bits: P (relative half a step of the type, as the
-// products take both operands in one type) and the output.  Scores, m, l and
-// the accumulator are fp32.  The accumulator is rescaled only when a row's
-// largest score has grown by more than 2^8 since its last rescale: P stays
-// below 2^8 then (2^15 in fp16, see kLift), which both types hold, and O and l
-// carry the same factor.
+// products take both operands in one type; two parts of P would double P V) and
+// the output.  Error against 64 bits, bf16: 2.1e-3, 1.6e-3 with the output's
+// rounding alone.  Scores, m, l and the accumulator are fp32.  The accumulator
+// is rescaled only when a row's largest score has grown by more than 2^8 since
+// its last rescale: P stays below 2^8 then (2^15 in fp16, see kLift), which both
+// types hold, and O and l carry the same factor.
 //
 // What bounds it.  24/8 heads of 128, causal: 4096 tokens 104 us (994
-// TFLOP/s), 8192 tokens under a window of 2048 186 us (970).  A pair of tiles
-// takes 3300 cycles, 2048 of them products at their full rate: a unit's
-// chain is 2100 of softmax, then 1200 of its last products with P and its next
-// scores, and the two units fill each other's gaps only in part.  Power bounds
-// it too: some milliseconds of it bring the GPU to its 1000 W cap (1.74 GHz
-// sampled, of 1.97), where the 186 us become 210, and shortening one part of
-// the chain gives little: leaving out the maximum or the exponentials (wrong
-// results, to see) makes it 3 and 9 % faster.  Measured and not kept, on the
-// 186 us: 64 keys a tile with two score buffers 237 (200 with a second
-// issuing warp for P V); one thread that issues everything 224; two issuing
-// warps 213; 16 softmax warps 197; P handed over whole 197; the maximum taken
-// under the first half's exponentials 203.
+// TFLOP/s), 8192 tokens under a window of 2048 185-200 us (900-970) cold and
+// 213 in loops of seconds.  A pair of tiles takes 3300 cycles, 2048 of them
+// products at their full rate: a unit's chain is 2100 of softmax, then 1200 of
+// its last products with P and its next scores, and the two units fill each
+// other's gaps only in part (the tensor and the exponentials' pipe are both
+// active 55 % of the time).  Power comes on top: some milliseconds of it bring
+// the GPU to its 1000 W cap (1.74 GHz sampled, of 1.97).  Shortening one part
+// of the chain gives little: leaving out the maximum or the exponentials (wrong
+// results, to see) makes it 3 and 9 % faster.  With 128 columns the kernel
+// spills 76 bytes a thread.  Measured and not kept, beside 186 us: 64 keys a
+// tile with two score buffers 237 (200 with a second issuing warp for P V); one
+// thread that issues everything 224; two issuing warps 213; 16 softmax warps
+// 197; P handed over whole 197; the maximum taken under the first half's
+// exponentials 203.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
