@@ -461,6 +461,57 @@ int rkv_sink_attention(const void* Q, const void* K, const void* V, int dtype, i
                        const rkv_row_strides* o_strides, float* lse, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* ---- rotary positions ---------------------------------------------------------
+ * Rows of Q and K turned by their positions, with one or several axes (time,
+ * height and width of images and video).  Pair i < pairs of a row, columns
+ * (i, i + pairs) or, interleaved, (2 i, 2 i + 1), holds (x, y) and becomes
+ * (x cos t - y sin t, x sin t + y cos t), t = f_i p in radians, with p the row's
+ * position on axis axes[i]; columns from 2 pairs on are copied.  The reference
+ * takes rows that its model has turned already.
+ * freqs: device [pairs], 8-byte aligned, f_i as turns per position in units of
+ * 2^-64, as rkv_rotary_frequencies makes them (so that angles of far positions
+ * lose nothing: they are off by 2^-25 half turns at most); axes: device
+ * [pairs], NULL for axis 0 throughout; a pair of an axis >= num_axes is copied.
+ * num_axes: at most 256.  Positions are 32-bit, negative ones turn back: the
+ * gradient of a rotation is the rotation of the gradient by -p.  Sines,
+ * cosines, products and sums are fp32, each result is rounded to the type once. */
+typedef struct rkv_rotary {
+    const unsigned long long* freqs;
+    const unsigned char* axes;
+    int pairs;        /* >= 1, at most dim_head / 2 */
+    int num_axes;     /* >= 1                        */
+    int interleaved;
+} rkv_rotary;
+
+/* Host: freqs[i] for radians[i] radians per position; both host arrays. */
+int rkv_rotary_frequencies(const double* radians, int pairs, unsigned long long* freqs);
+
+/* q: [batch][num_heads][len][dim_head], k: [batch][num_heads_kv][len][dim_head]
+ * of dtype (RKV_F32, RKV_BF16, RKV_F16) to q_out and k_out, all at the given
+ * strides (bytes, multiples of the element size; NULL: rows, heads and items
+ * back to back); no heads: q, or k, is left out.  positions: device
+ * [num_axes][batch][len].  In place where q_out == q (k_out == k) with the same
+ * strides, otherwise outputs overlap nothing.  dim_head: a multiple of 8, at
+ * most 256; batch: at most 65535.  Asynchronous on `stream`. */
+int rkv_rotate(const rkv_rotary* rotary, const int* positions, const void* q, void* q_out, int num_heads,
+               const void* k, void* k_out, int num_heads_kv, int dtype, int dim_head, int len, int batch,
+               const rkv_row_strides* q_strides, const rkv_row_strides* q_out_strides,
+               const rkv_row_strides* k_strides, const rkv_row_strides* k_out_strides, void* stream);
+
+/* rkv_paged_append with the rows of k turned on the way into the pages, v
+ * copied, and the rows of q (num_heads > 0) turned to q_out in the same launch:
+ * the step of a server between its projection and rkv_paged_decode.  positions:
+ * device [num_axes][batch][n_rows], or NULL: every axis of a row is at its
+ * token's index lens[b] - n + i (which is its position as long as nothing was
+ * evicted).  Rows i < n = n_new[b] of q are turned, also where their token has
+ * no place in the table; the rows of q_out behind them are left as they were.
+ * k and v share kv_strides; strides, n_new and the other rules as in rkv_rotate
+ * and rkv_paged_append. */
+int rkv_paged_append_rotated(const rkv_paged_cache* cache, const rkv_rotary* rotary, const int* positions,
+                             const void* k, const void* v, const rkv_row_strides* kv_strides, int n_rows,
+                             int batch, const int* n_new, const void* q, const rkv_row_strides* q_strides,
+                             void* q_out, const rkv_row_strides* q_out_strides, int num_heads, void* stream);
+
 /* ---- errors raised inside kernels ----------------------------------------
  * Kernels record a failed bounded wait in the workspace.  This synchronises
  * `stream`, returns RKV_OK or the recorded status, and clears it. */

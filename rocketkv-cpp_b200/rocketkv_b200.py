@@ -39,7 +39,8 @@ EXPORTS = [
     "rkv_selftest_wait_timeout", "rkv_compact_kv", "rkv_hsa_summary_size", "rkv_hsa_build_summary",
     "rkv_hsa_decode_summary", "rkv_capture_rows", "rkv_evict_compact", "rkv_paged_append",
     "rkv_paged_decode_workspace_size", "rkv_paged_decode", "rkv_weight_evict",
-    "rkv_sink_attention_workspace_size", "rkv_sink_attention",
+    "rkv_sink_attention_workspace_size", "rkv_sink_attention", "rkv_rotary_frequencies", "rkv_rotate",
+    "rkv_paged_append_rotated",
 ]
 
 
@@ -71,6 +72,11 @@ class _PagedCache(ctypes.Structure):
 
 class _RowStrides(ctypes.Structure):
     _fields_ = [(n, ctypes.c_longlong) for n in ("item", "head", "token")]
+
+
+class _Rotary(ctypes.Structure):
+    _fields_ = ([("freqs", ctypes.c_void_p), ("axes", ctypes.c_void_p)]
+                + [(n, ctypes.c_int) for n in ("pairs", "num_axes", "interleaved")])
 
 
 @dataclass
@@ -115,6 +121,7 @@ _SZ = ctypes.c_size_t
 _CFGP = ctypes.POINTER(_Config)
 _PCP = ctypes.POINTER(_PagedCache)
 _RSP = ctypes.POINTER(_RowStrides)
+_ROP = ctypes.POINTER(_Rotary)
 
 
 def lib() -> ctypes.CDLL:
@@ -164,6 +171,9 @@ def lib() -> ctypes.CDLL:
         "rkv_sink_attention_workspace_size": ([_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)], _I),
         "rkv_sink_attention": ([_VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _RSP, _RSP, _VP, _I, _I, _VP, _RSP, _VP,
                                 _VP, _SZ, _VP], _I),
+        "rkv_rotary_frequencies": ([_VP, _I, _VP], _I),
+        "rkv_rotate": ([_ROP, _VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _RSP, _RSP, _RSP, _RSP, _VP], _I),
+        "rkv_paged_append_rotated": ([_PCP, _ROP, _VP, _VP, _VP, _RSP, _I, _I, _VP, _VP, _RSP, _VP, _RSP, _I, _VP], _I),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -768,3 +778,138 @@ class SinkAttention:
                 st = lib().rkv_workspace_status(_ptr(ws), _stream(stream))
                 found = found or st
         return found
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions, alone and on the way into the paged cache
+# ---------------------------------------------------------------------------
+class Rotary:
+    """How rows are turned by their positions (rkv_rotary): inv_freq, radians
+    per position of each pair (taken in 64 bits); axes (nullable), the axis of
+    each pair, num_axes of them (one more than the largest without);
+    interleaved: pairs are neighbouring columns, not columns of the two halves
+    of the first 2 pairs.  Holds device tensors: it may serve any number of
+    calls, on any stream, at the same time."""
+
+    def __init__(self, inv_freq, dim_head: int, axes=None, num_axes: int | None = None, interleaved: bool = False, device="cuda"):
+        import torch
+        radians = torch.as_tensor(inv_freq, dtype=torch.float64).cpu().contiguous()
+        if radians.dim() != 1 or not 1 <= len(radians) <= dim_head // 2:
+            raise ValueError("inv_freq: one entry per pair, at most dim_head / 2 of them")
+        freqs = torch.empty(len(radians), dtype=torch.int64)
+        _check(lib().rkv_rotary_frequencies(radians.data_ptr(), len(radians), freqs.data_ptr()), "rkv_rotary_frequencies")
+        self.axes = None
+        if axes is not None:
+            axes = torch.as_tensor(axes).cpu().long()
+            if axes.shape != radians.shape or int(axes.min()) < 0 or int(axes.max()) > 255:
+                raise ValueError("axes: one entry per pair, 0 .. 255")
+            num_axes = int(axes.max()) + 1 if num_axes is None else num_axes
+            if not int(axes.max()) < num_axes <= 256:
+                raise ValueError("axes: below num_axes, which is at most 256")
+            self.axes = axes.to(torch.uint8).to(device)
+        self.freqs = freqs.to(device)
+        self.dim_head, self.num_axes, self.interleaved = dim_head, 1 if num_axes is None else num_axes, bool(interleaved)
+        self.c = _Rotary(_ptr(self.freqs), _ptr(self.axes), len(radians), self.num_axes, int(self.interleaved))
+        self.ref = ctypes.byref(self.c)
+        self._streams = {_handle(self.freqs.device, None)}  # whose work its buffers outlive
+
+    def _buffers(self):
+        return (self.freqs,) if self.axes is None else (self.freqs, self.axes)
+
+
+def _check_positions(positions, rotary, batch, n, device):
+    _int32(positions, device, "positions")
+    if positions.numel() != rotary.num_axes * batch * n or tuple(positions.shape)[-2:] != (batch, n):
+        raise ValueError("positions: [num_axes, B, rows], or [B, rows] for one axis")
+
+
+def _rotated_out(x, out, what):
+    """out, or a fresh one; its strides."""
+    import torch
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"{what}: the rows' shape, type and device")
+    return out, _row_strides(out, what)
+
+
+def rotate(q, k, positions, rotary: Rotary, q_out=None, k_out=None, stream=None):
+    """Rows turned by their positions (rkv_rotate): q [B, H, len, D] and k
+    [B, HK, len, D] (either may be None; float32, bfloat16 or float16, unit
+    stride along D), positions int32 [num_axes, B, len] ([B, len] for one axis),
+    to q_out and k_out (fresh ones without; q and k themselves to turn in
+    place).  Returns (q_out, k_out)."""
+    some = q if q is not None else k
+    if some is None:
+        raise ValueError("q or k is needed")
+    dev, dt = some.device, _dtype_of(some)
+    for x in (q, k):
+        if x is not None and (x.dim() != 4 or x.shape[0] != some.shape[0] or x.shape[2:] != some.shape[2:] or x.dtype != some.dtype
+                              or x.device != dev):
+            raise ValueError("q and k: [B, heads, len, D], of one batch, length, D, type and device")
+    if rotary.freqs.device != dev or rotary.dim_head != some.shape[3]:
+        raise ValueError("the rows are not of the rotary's device or dim_head")
+    B, _, n, D = some.shape
+    _check_positions(positions, rotary, B, n, dev)
+    args = []
+    with _on_stream(dev, stream):
+        for x, out, what in ((q, q_out, "q_out"), (k, k_out, "k_out")):
+            if x is None:
+                args.append((None, None, 0, None, None))
+                continue
+            out, so = _rotated_out(x, out, what)
+            args.append((x, out, x.shape[1], _row_strides(x, what[0]), so))
+    (q, q_out, H, qs, qo), (k, k_out, HK, ks, ko) = args
+    ref = lambda s: None if s is None else ctypes.byref(s)  # noqa: E731
+    _launch(dev, stream, "rkv_rotate", lib().rkv_rotate, rotary.ref, _ptr(positions), _ptr(q), _ptr(q_out), H, _ptr(k), _ptr(k_out), HK,
+            dt, D, n, B, ref(qs), ref(qo), ref(ks), ref(ko), owner=rotary)
+    return q_out, k_out
+
+
+def paged_append_rotated(cache: PagedCache, k, v, rotary: Rotary, q=None, q_out=None, positions=None, n_new=None, stream=None):
+    """paged_append with the rows of k turned by their positions on the way, and
+    those of q to q_out in the same launch (rkv_paged_append_rotated).  k, v
+    [B, n_rows, HK, D] and q [B, n_rows, H, D] (or [B, heads, D] for one row)
+    of the cache's type; positions int32 [num_axes, B, n_rows] ([B, n_rows], or
+    [B] for one row, where there is one axis), each row's token index without.
+    q_out: as q; a fresh one without, 0 in the rows behind n_new.  Returns it
+    (None without q)."""
+    import torch
+    one = k.dim() == 3
+    if one:
+        k, v = k[:, None], v[:, None]
+        q, q_out = (None if x is None else x[:, None] for x in (q, q_out))
+    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != cache.K.dtype or v.dtype != k.dtype or k.dim() != 4:
+        raise ValueError("k and v: one shape, layout and the cache's type")
+    dev = cache.K.device
+    B, n, hk, d = k.shape
+    if B != cache.batch or hk != cache.K.shape[1] or d != cache.K.shape[3] or (d > 1 and k.stride(3) != 1):
+        raise ValueError("k, v: [B, n_rows, HK, D] of the cache's geometry, unit stride along D")
+    if k.device != dev or v.device != dev or rotary.freqs.device != dev or rotary.dim_head != d:
+        raise ValueError("k, v and the rotary: on the cache's device, of its dim_head")
+    if B and cache._lens is None:
+        raise ValueError("the cache's lens are needed")
+    if n_new is not None:
+        _int32(n_new, dev, "n_new")
+        if n_new.numel() != B:
+            raise ValueError("n_new: one entry per sequence")
+    if positions is not None:
+        _check_positions(positions[..., None] if one and positions.shape[-1:] == (B,) and positions.dim() <= 2 else positions, rotary, B, n, dev)
+    H, qs, qo = 0, None, None
+    if q is not None:
+        if q.dim() != 4 or q.shape[0] != B or q.shape[1] != n or q.shape[3] != d or q.dtype != k.dtype or q.device != dev:
+            raise ValueError("q: [B, n_rows, H, D] of the cache's type, on its device")
+        H = q.shape[2]
+        if q_out is None:
+            with _on_stream(dev, stream):
+                # without n_new every row is written
+                q_out = (torch.empty if n_new is None else torch.zeros)(q.shape, dtype=q.dtype, device=dev)
+        q_out, qo = _rotated_out(q.transpose(1, 2), q_out.transpose(1, 2), "q_out")
+        qs, q_out = _row_strides(q.transpose(1, 2), "q"), q_out.transpose(1, 2)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    ks = _row_strides(k.transpose(1, 2), "k")
+    ref = lambda s: None if s is None else ctypes.byref(s)  # noqa: E731
+    _launch(dev, stream, "rkv_paged_append_rotated", lib().rkv_paged_append_rotated, cache.ref, rotary.ref, _ptr(positions), _ptr(k),
+            _ptr(v), ref(ks), n, B, _ptr(n_new), _ptr(q), ref(qs), _ptr(q_out), ref(qo), H, owner=rotary)
+    return q_out[:, 0] if one and q_out is not None else q_out
