@@ -512,6 +512,37 @@ int rkv_paged_append_rotated(const rkv_paged_cache* cache, const rkv_rotary* rot
                              int batch, const int* n_new, const void* q, const rkv_row_strides* q_strides,
                              void* q_out, const rkv_row_strides* q_out_strides, int num_heads, void* stream);
 
+/* ---- decode of sequences that share leading tokens ------------------------------
+ * rkv_paged_decode (without a window or weights) for a batch whose sequences
+ * share the pages of their first tokens, group by group: a group's shared rows
+ * of K and V meet the queries of all its sequences at once and are read once.
+ * Group g is the sequences group_starts[g] .. group_starts[g + 1] - 1 and shares
+ * its first group_tokens[g] tokens (device arrays [num_groups + 1], ascending,
+ * and [num_groups]; read on the device, starts clamped to [0, batch], tokens to
+ * what a sequence can hold).  Sequences of no group, and those shorter than
+ * their group's shared tokens (idle slots of a padded batch), are attended on
+ * their own.  The shared rows are read through the table row of the group's first
+ * sequence that holds them all; the others' entries for them are not looked at,
+ * so any number of shared tokens is taken, whole pages or not, as long as the
+ * rows are equal.  O: [batch][num_heads][dim_head] in the cache's dtype (as
+ * rkv_sink_attention's; rkv_paged_decode's is fp32), 16-byte aligned; lse
+ * (nullable) fp32.  max_len, pages outside the pool, non-finite values, sequences
+ * without a token and the rest as in rkv_paged_decode.
+ * Scores, the softmax's maxima and sums and the outputs' sums are fp32.  Where
+ * the shared tokens of a 16-bit cache meet many queries, each of their weights is
+ * rounded to the type before it meets V (half a step of the type; in fp16 a fixed
+ * 2^-32 of the row's largest below 2^-21 of it); O is rounded to the type once.
+ * The split over CTAs depends on the lengths on the device, not on timing:
+ * results repeat bit for bit.
+ * Workspace: device, 16-byte aligned, not shared with a call that may run at
+ * the same time; it begins with the error word that rkv_workspace_status reads.
+ * Asynchronous on `stream`; allocates nothing. */
+int rkv_prefix_decode_workspace_size(int dtype, int num_heads, int num_heads_kv, int dim_head, int max_len,
+                                     int batch, int num_groups, size_t* bytes);
+int rkv_prefix_decode(const void* Q, long long q_item_stride, int num_heads, const rkv_paged_cache* cache,
+                      int max_len, int batch, const int* group_starts, const int* group_tokens, int num_groups,
+                      void* O, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- errors raised inside kernels ----------------------------------------
  * Kernels record a failed bounded wait in the workspace.  This synchronises
  * `stream`, returns RKV_OK or the recorded status, and clears it. */

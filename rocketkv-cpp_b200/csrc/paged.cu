@@ -20,6 +20,7 @@
 // without tokens hold their SM until the longest ends), and by the last CTA to
 // arrive in place of the second kernel (182 -> 187, 1 x 2048 7.3 -> 8.4).
 #include "paged.cuh"
+#include "prefix.cuh"
 #include "tf32.cuh"
 
 namespace rkv {
@@ -109,6 +110,9 @@ struct DecodeArgs {
     float* scores;       // [batch][H][vmax], base-2 scores (with weights)
     long long o_blocks;  // join: CTAs that join O; the others add weights
     int w_blocks;        // join: CTAs per (item, KV head) that add weights
+    Groups gr;           // the passes of a batch that shares leading tokens
+    int slots, slot0;    // their parts of a row, and the first of this pass
+    int units;           // prefix pass: row groups of all groups at most
 };
 
 // The visible tokens are numbered 0 .. nvis - 1: the sinks, then the window.
@@ -137,13 +141,17 @@ __device__ __forceinline__ float warp_sum(float x) {
     for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
+// What a launch of the decode kernel attends: all tokens of every sequence; or, of a batch that shares leading tokens,
+// every sequence's own, or every group's shared ones with the rows of all its sequences.
+enum { PASS_ALL = 0, PASS_OWN = 1, PASS_SHARED = 2 };
+
 // 0 in place of -inf, so that a set with nothing in it subtracts no infinities.
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 
 // Joins the warps' (m, l, o) of ng heads from shared memory (ms, ls [warps][rows], os [warps][rows][pitch])
 // and writes the part, or the output where there is one part.
-template <int W>
-__device__ __forceinline__ void merge_warps(const DecodeArgs& a, size_t head0, int ng, int split, const float* ms,
+template <int W, int PASS, typename Head>
+__device__ __forceinline__ void merge_warps(const DecodeArgs& a, Head head_of, int ng, int split, const float* ms,
                                             const float* ls, const float* os, int rows, int pitch) {
     const int D = a.D;
     for (int i = threadIdx.x; i < ng * D; i += W * 32) {
@@ -159,7 +167,13 @@ __device__ __forceinline__ void merge_warps(const DecodeArgs& a, size_t head0, i
             ll = fmaf(ls[w * rows + g], c, ll);
             oo = fmaf(os[(w * rows + g) * pitch + d], c, oo);
         }
-        const size_t head = head0 + g;
+        const size_t head = head_of(g);
+        if (PASS != PASS_ALL) {
+            const size_t part = head * a.slots + a.slot0 + split;
+            a.part_o[part * D + d] = oo;
+            if (d == 0) a.part_ml[part] = make_float2(mm, ll);
+            continue;
+        }
         if (a.splits == 1) {
             a.O[head * D + d] = ll == 0.0f ? 0.0f : oo / ll;
             if (d == 0 && a.lse) a.lse[head] = ll == 0.0f ? -INFINITY : (mf + log2f(ll)) * 0.693147180559945f;
@@ -289,7 +303,13 @@ struct Shape {
 // A row's maximum is raised only when a score exceeds it by more than 2^8
 // (all types hold P then); fp16's P is kept 2^7 larger, away from the type's
 // smallest numbers.
-template <typename S>
+//
+// The passes of a batch that shares leading tokens (PASS) differ in which rows
+// and tokens a CTA has: own tokens begin behind the shared ones; a group's
+// shared tokens take the rows (sequence, head) of all its sequences, 8 NT at a
+// time, the row groups of one stretch of tokens side by side, so that the L2
+// cache serves all but the first.
+template <typename S, int PASS>
 __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const DecodeArgs a) {
     constexpr int KIND = S::KIND, DP = S::DP, NT = S::NT, W = S::W, SLOTS = S::SLOTS;
     constexpr bool F32 = KIND == KIND_F32, BF = KIND == KIND_BF16;
@@ -306,16 +326,71 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
     const int D = a.D, chunks = D * S::SIZE / 16;
 
     long long id = blockIdx.x;
-    const int split = (int)(id % a.splits);
-    id /= a.splits;
-    const int grp = (int)(id % a.ngroups);
-    id /= a.ngroups;
-    const int hk = (int)(id % a.HK), b = (int)(id / a.HK);
-    const Visible vis = visible(a, b);
-    const long long v_lo = (long long)split * a.chunk;
-    if (split > 0 && v_lo >= vis.nvis) return;  // the join takes the parts that hold tokens
-    const int v0 = (int)v_lo, v1 = (int)min((long long)vis.nvis, v_lo + a.chunk);
-    const int h0 = hk * a.G + grp * 8 * NT, ng = min(8 * NT, a.G - grp * 8 * NT);
+    int split, b, hk, h0, ng, first = 0;  // b: whose table row; first: the first row's sequence, among the group's rows
+    Visible vis;
+    int chunk = a.chunk;
+    if (PASS == PASS_SHARED) {
+        const int unit = (int)(id % a.units);
+        id /= a.units;
+        hk = (int)(id % a.HK);
+        split = (int)(id / a.HK);
+        // the group of this row group
+        int g = -1, before = 0;
+        for (int g0 = 0; g0 < a.gr.n && g < 0; g0 += 32) {
+            const int mine = g0 + lane < a.gr.n ? (a.gr.size(g0 + lane) * a.G + 8 * NT - 1) / (8 * NT) : 0;
+            int sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += y;
+            }
+            const unsigned hits = __ballot_sync(0xffffffffu, unit < before + sum);
+            if (hits) {
+                const int l = __ffs(hits) - 1;
+                g = g0 + l;
+                before += __shfl_sync(0xffffffffu, sum - mine, l);
+            } else {
+                before += __shfl_sync(0xffffffffu, sum, 31);
+            }
+        }
+        vis.n = vis.nvis = g < 0 ? 0 : a.gr.shared(a.c, g);
+        vis.sinks = vis.gap = 0;
+        first = g < 0 ? 0 : a.gr.start(g);
+        h0 = (unit - before) * 8 * NT;  // row of the group
+        ng = g < 0 ? 0 : min(8 * NT, a.gr.size(g) * a.G - h0);
+        b = g < 0 ? 0 : leader_of(a.gr, a.c, g, vis.n);
+        chunk = part_tokens(vis.n, a.splits);
+    } else {
+        split = (int)(id % a.splits);
+        id /= a.splits;
+        const int grp = (int)(id % a.ngroups);
+        id /= a.ngroups;
+        hk = (int)(id % a.HK);
+        b = (int)(id / a.HK);
+        vis = visible(a, b);
+        if (PASS == PASS_OWN) {
+            const int shared = member_of(a.gr, a.c, b, vis.n).tokens;
+            vis.sinks = 0;
+            vis.gap = shared;
+            vis.nvis = vis.n - shared;
+            chunk = part_tokens(vis.nvis, a.splits);
+        }
+        h0 = hk * a.G + grp * 8 * NT;
+        ng = min(8 * NT, a.G - grp * 8 * NT);
+    }
+    const long long v_lo = (long long)split * chunk;
+    if ((PASS != PASS_ALL || split > 0) && v_lo >= vis.nvis) {
+        // the join takes the parts that hold tokens
+        if (PASS != PASS_ALL) asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
+    const int v0 = (int)v_lo, v1 = (int)min((long long)vis.nvis, v_lo + chunk);
+    // row i of the CTA: its query head among all sequences', and its query
+    auto head_of = [&](int i) -> size_t {
+        if (PASS != PASS_SHARED) return (size_t)b * a.H + h0 + i;
+        const unsigned r = (unsigned)(h0 + i), s = r / (unsigned)a.G;
+        return (size_t)(first + s) * a.H + hk * a.G + (r - s * a.G);
+    };
 
     uint8_t* qsm = smem;
     const uint32_t ring = smem_u32(smem + S::QBYTES) + warp * SLOTS * S::SLOT;
@@ -358,13 +433,18 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
 
     // q^T fragments
     const uint8_t* qb = a.Q + (size_t)b * a.q_stride;
+    auto query_of = [&](int i) -> const uint8_t* {
+        if (PASS != PASS_SHARED) return qb + (size_t)(h0 + i) * D * S::SIZE;
+        const unsigned r = (unsigned)(h0 + i), s = r / (unsigned)a.G;
+        return a.Q + (size_t)(first + s) * a.q_stride + (size_t)(hk * a.G + (r - s * a.G)) * D * S::SIZE;
+    };
     uint32_t q[S::QS ? 1 : NT][S::QS ? 1 : DP / 16][2];
     if (F32) {
         // step (blk, e): columns 32 blk + 4 t + e and 16 further of head g, as hi, hi, lo, lo
         for (int i = warp; i < DP / 8 * NT; i += W) {
             const int n = i / (DP / 8), st = i % (DP / 8), d = (st >> 2) * 32 + 4 * t + (st & 3);
             const bool have = n * 8 + g < ng;
-            const float* row = reinterpret_cast<const float*>(qb) + (size_t)(h0 + n * 8 + g) * D;
+            const float* row = reinterpret_cast<const float*>(query_of(n * 8 + g));
             const uint32_t b0 = have && d < D ? __float_as_uint(__ldg(row + d)) : 0u;
             const uint32_t b1 = have && d + 16 < D ? __float_as_uint(__ldg(row + d + 16)) : 0u;
             uint4 f;
@@ -378,7 +458,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
         auto frag = [&](int n, int k, int e) {
             const int d = k * 16 + e * 8 + 2 * t;
             return n * 8 + g < ng && d < D
-                       ? __ldg(reinterpret_cast<const uint32_t*>(qb + ((size_t)(h0 + n * 8 + g) * D + d) * 2))
+                       ? __ldg(reinterpret_cast<const uint32_t*>(query_of(n * 8 + g) + d * 2))
                        : 0u;
         };
         if (S::QS) {
@@ -489,7 +569,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
             s[n][2] = r1 ? s[n][2] * a.scale2 : -INFINITY;
             s[n][3] = r1 ? s[n][3] * a.scale2 : -INFINITY;
             need |= fmaxf(s[n][0], s[n][2]) > m[n][0] + kGrow || fmaxf(s[n][1], s[n][3]) > m[n][1] + kGrow;
-            if (a.scores) {
+            if (PASS == PASS_ALL && a.scores) {
                 const int v = v0 + tile * kKeys + g;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -631,7 +711,8 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
             }
         }
     __syncthreads();
-    merge_warps<W>(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, 8 * NT, S::PITCH);
+    merge_warps<W, PASS>(a, head_of, ng, split, ms, ls, os, 8 * NT, S::PITCH);
+    if (PASS != PASS_ALL) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // m and l of all parts of a head (one warp): the same order whatever the grid.
@@ -800,28 +881,92 @@ DecodePlan decode_plan(int dtype, int H, int HK, int D, long long visible_max, i
     return p;
 }
 
-template <int KIND, int DP, int NT>
-int launch_shape(const DecodeArgs& a, long long blocks, cudaStream_t st) {
+template <int KIND, int DP, int NT, int PASS>
+int launch_shape(const DecodeArgs& a, long long blocks, bool dependent, cudaStream_t st) {
     using S = Shape<KIND, DP, NT>;
     static_assert(S::SMEM * S::CTAS + 1024 * S::CTAS <= 228 * 1024, "the CTAs of an SM fit in its shared memory");
-    if (cudaFuncSetAttribute(paged_decode_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
+    if (cudaFuncSetAttribute(paged_decode_kernel<S, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
-    paged_decode_kernel<S><<<(unsigned)blocks, S::W * 32, S::SMEM, st>>>(a);
+    if (PASS != PASS_ALL && dependent) {
+        const cudaError_t e = launch_pdl(paged_decode_kernel<S, PASS>, dim3((unsigned)blocks), dim3(S::W * 32), S::SMEM, st, a);
+        if (e != cudaSuccess) (void)cudaGetLastError();
+        return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
+    }
+    paged_decode_kernel<S, PASS><<<(unsigned)blocks, S::W * 32, S::SMEM, st>>>(a);
     return launched();
 }
-template <int KIND>
-int launch_kind(const DecodeArgs& a, int gt, long long blocks, cudaStream_t st) {
+template <int KIND, int PASS>
+int launch_kind(const DecodeArgs& a, int gt, long long blocks, bool dependent, cudaStream_t st) {
     if constexpr (KIND != KIND_F32) {
-        if (gt == 16) return a.D <= 64 ? launch_shape<KIND, 64, 2>(a, blocks, st) : launch_shape<KIND, 128, 2>(a, blocks, st);
+        if (gt == 16)
+            return a.D <= 64 ? launch_shape<KIND, 64, 2, PASS>(a, blocks, dependent, st) : launch_shape<KIND, 128, 2, PASS>(a, blocks, dependent, st);
     }
-    if (a.D <= 64) return launch_shape<KIND, 64, 1>(a, blocks, st);
-    if (a.D <= 128) return launch_shape<KIND, 128, 1>(a, blocks, st);
-    return launch_shape<KIND, 256, 1>(a, blocks, st);
+    if (a.D <= 64) return launch_shape<KIND, 64, 1, PASS>(a, blocks, dependent, st);
+    if (a.D <= 128) return launch_shape<KIND, 128, 1, PASS>(a, blocks, dependent, st);
+    return launch_shape<KIND, 256, 1, PASS>(a, blocks, dependent, st);
 }
+template <int PASS>
+int launch_pass(const DecodeArgs& a, int dtype, int gt, long long blocks, bool dependent, cudaStream_t st) {
+    if (blocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
+    switch (dtype) {
+        case RKV_F32: return launch_kind<KIND_F32, PASS>(a, gt, blocks, dependent, st);
+        case RKV_BF16: return launch_kind<KIND_BF16, PASS>(a, gt, blocks, dependent, st);
+        default: return launch_kind<KIND_F16, PASS>(a, gt, blocks, dependent, st);
+    }
+}
+// Rows of a group that one CTA of the prefix pass takes.
+int shared_rows(int dtype, int D, int H, int HK, int batch, int groups) {
+    return head_group(dtype, (int)(((long long)batch * (H / HK) + groups - 1) / groups > 8 ? 9 : 1), D);
+}
+long long shared_units(int rows, int H, int HK, int batch, int groups) { return groups + (long long)batch * (H / HK) / rows; }
 
 }  // namespace
+
+int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch) {
+    return (int)decode_parts(dtype, H, HK, D, max_len, batch);
+}
+// As many as give two waves of CTAs, each of 128 tokens or more.
+int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
+    const int rows = shared_rows(dtype, D, H, HK, batch, groups);
+    const long long each = ((long long)batch * (H / HK) + groups * (long long)rows - 1) / (groups * (long long)rows);  // of a group of mean size
+    long long p = 2LL * decode_slots(dtype, D) / (each * groups * HK);
+    const long long most = ((long long)max_len + kMinChunk - 1) / kMinChunk;
+    if (p > most) p = most;
+    if (p > 256) p = 256;
+    return p < 1 ? 1 : (int)p;
+}
+int launch_shared_pass(const SharedArgs& s, bool prefix, bool dependent, cudaStream_t st) {
+    DecodeArgs a{};
+    a.c = s.c;
+    a.Q = s.Q;
+    a.q_stride = s.q_stride;
+    a.H = s.H;
+    a.HK = s.HK;
+    a.G = s.H / s.HK;
+    a.D = s.D;
+    a.max_len = s.gr.max_len;
+    a.scale2 = 1.4426950408889634f / sqrtf((float)s.D);
+    a.part_o = s.part_o;
+    a.part_ml = s.part_ml;
+    a.gr = s.gr;
+    a.slots = s.slots;
+    if (prefix) {
+        const int rows = shared_rows(s.dtype, s.D, s.H, s.HK, s.batch, s.gr.n);
+        const long long units = shared_units(rows, s.H, s.HK, s.batch, s.gr.n);
+        if (units > 0x7FFFFFF) return RKV_ERR_UNSUPPORTED;
+        a.units = (int)units;
+        a.slot0 = s.own;
+        a.splits = s.slots - s.own;
+        return launch_pass<PASS_SHARED>(a, s.dtype, rows, units * s.HK * a.splits, dependent, st);
+    }
+    const int gt = head_group(s.dtype, a.G, s.D);
+    a.ngroups = (a.G + gt - 1) / gt;
+    a.splits = s.own;
+    return launch_pass<PASS_OWN>(a, s.dtype, gt, (long long)s.batch * s.HK * a.ngroups * a.splits, dependent, st);
+}
+
 }  // namespace rkv
 
 using namespace rkv;
@@ -939,11 +1084,7 @@ extern "C" int rkv_paged_decode(const void* Q, long long q_item_stride, int num_
     a.w_blocks = weights ? (int)((vis + kJoinTokens - 1) / kJoinTokens) : 0;
     const long long jblocks = a.o_blocks + (long long)batch * a.HK * a.w_blocks;
     if (blocks > 0x7FFFFFFFLL || jblocks > 0x7FFFFFFFLL) return RKV_ERR_UNSUPPORTED;
-    switch (cache->dtype) {
-        case RKV_F32: rc = launch_kind<KIND_F32>(a, p.gt, blocks, st); break;
-        case RKV_BF16: rc = launch_kind<KIND_BF16>(a, p.gt, blocks, st); break;
-        default: rc = launch_kind<KIND_F16>(a, p.gt, blocks, st); break;
-    }
+    rc = launch_pass<PASS_ALL>(a, cache->dtype, p.gt, blocks, false, st);
     if (rc || !join || jblocks == 0) return rc;
     size_t smem = (size_t)p.splits * sizeof(float);
     if (weights && smem < (size_t)a.G * sizeof(float2)) smem = (size_t)a.G * sizeof(float2);

@@ -1,0 +1,189 @@
+// prefix.cu -- one token per sequence attended over a paged cache whose
+// sequences share leading tokens, group by group.
+//
+// The softmax of a row (sequence, query head) is split between the tokens that
+// its group shares and its own: parts with disjoint tokens, each (m, l, o) =
+// (largest score, sum 2^(x - m), sum 2^(x - m) v) with x = q k log2(e) / sqrt(D),
+// join as (M, sum l 2^(m - M), sum o 2^(m - M)).  A group's shared rows of K and V
+// meet the queries of all its sequences at once, so they are read once and
+// not once per sequence.  Three kernels: the shared tokens, every sequence's own
+// (both of paged.cu, or the former on the tcgen05 tensor cores, prefix_tc.cu),
+// and the join.
+#include "prefix.cuh"
+
+namespace rkv {
+namespace {
+
+struct JoinArgs {
+    SharedArgs s;
+    void* O;
+    float* lse;
+    int* clear;  // the error word, where no kernel before this one has cleared it
+};
+
+template <typename T>
+__device__ __forceinline__ void put4(T* o, const float4& v);
+template <>
+__device__ __forceinline__ void put4(float* o, const float4& v) { *reinterpret_cast<float4*>(o) = v; }
+template <>
+__device__ __forceinline__ void put4(__nv_bfloat16* o, const float4& v) {
+    reinterpret_cast<__nv_bfloat162*>(o)[0] = __floats2bfloat162_rn(v.x, v.y);
+    reinterpret_cast<__nv_bfloat162*>(o)[1] = __floats2bfloat162_rn(v.z, v.w);
+}
+template <>
+__device__ __forceinline__ void put4(__half* o, const float4& v) {
+    reinterpret_cast<__half2*>(o)[0] = __floats2half2_rn(v.x, v.y);
+    reinterpret_cast<__half2*>(o)[1] = __floats2half2_rn(v.z, v.w);
+}
+
+constexpr int kJoinRows = 4;  // rows of a CTA, a warp each
+
+// Joins the parts of a row: those of its own tokens, then those of the shared
+// ones, in their order whatever the grid.  O is rounded to Q's type, once.
+template <typename T>
+__global__ void __launch_bounds__(kJoinRows * 32) prefix_join_kernel(const JoinArgs a) {
+    const SharedArgs& s = a.s;
+    const int lane = threadIdx.x & 31;
+    const long long rows = (long long)s.batch * s.H, row = (long long)blockIdx.x * kJoinRows + (threadIdx.x >> 5);
+    const int b = row < rows ? (int)(row / s.H) : 0;
+    const int n = paged_len(s.c, b, s.gr.max_len);
+    const Member m = member_of(s.gr, s.c, b, n);
+    const int mine = n - m.tokens;
+    const int own = mine > 0 ? (mine + part_tokens(mine, s.own) - 1) / part_tokens(mine, s.own) : 0;
+    int shared = 0;
+    if (m.tokens > 0) {
+        const int t = part_tokens(m.tokens, s.slots - s.own);
+        shared = (m.tokens + t - 1) / t;
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.clear = 0;
+    if (row >= rows) return;
+    const float2* ml = s.part_ml + row * s.slots;
+    const float* po = s.part_o + row * s.slots * s.D;
+    // part i: own ones in the slots from 0, shared ones in those from s.own
+    const int parts = own + shared;
+    auto slot = [&](int i) { return i < own ? i : s.own + (i - own); };
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml[slot(i)].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f;
+    float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    const int c0 = lane * 4, c1 = c0 + 128;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        float w = 0.0f;
+        if (i0 + lane < parts) {
+            const float2 x = ml[slot(i0 + lane)];
+            w = exp2f(x.x - base);
+            l = fmaf(x.y, w, l);
+        }
+        const int here = min(32, parts - i0);
+#pragma unroll 4
+        for (int i = 0; i < here; ++i) {
+            const float f = __shfl_sync(0xffffffffu, w, i);
+            const float* p = po + (size_t)slot(i0 + i) * s.D;
+            if (c0 < s.D) {
+                const float4 v = *reinterpret_cast<const float4*>(p + c0);
+                o[0] = make_float4(fmaf(v.x, f, o[0].x), fmaf(v.y, f, o[0].y), fmaf(v.z, f, o[0].z), fmaf(v.w, f, o[0].w));
+            }
+            if (c1 < s.D) {
+                const float4 v = *reinterpret_cast<const float4*>(p + c1);
+                o[1] = make_float4(fmaf(v.x, f, o[1].x), fmaf(v.y, f, o[1].y), fmaf(v.z, f, o[1].z), fmaf(v.w, f, o[1].w));
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(a.O) + row * s.D;
+    if (c0 < s.D) put4(out + c0, make_float4(o[0].x * inv, o[0].y * inv, o[0].z * inv, o[0].w * inv));
+    if (c1 < s.D) put4(out + c1, make_float4(o[1].x * inv, o[1].y * inv, o[1].z * inv, o[1].w * inv));
+    if (lane == 0 && a.lse) a.lse[row] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945f;
+}
+
+template <typename T>
+int launch_join(const JoinArgs& a, cudaStream_t st) {
+    const long long blocks = ((long long)a.s.batch * a.s.H + kJoinRows - 1) / kJoinRows;
+    const cudaError_t e = launch_pdl(prefix_join_kernel<T>, dim3((unsigned)blocks), dim3(kJoinRows * 32), 0, st, a);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
+}
+
+int prefix_check(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
+    if (!paged_dtype(dtype) || H <= 0 || HK <= 0 || H % HK != 0 || D <= 0 || max_len < 0 || batch < 0 || groups < 0)
+        return RKV_ERR_INVALID_ARG;
+    if (D % 8 != 0 || D > 256 || H / HK > 1024 || max_len > kMaxLen) return RKV_ERR_UNSUPPORTED;
+    if ((long long)batch * H > 0x3FFFFFFFLL || groups > (1 << 24)) return RKV_ERR_UNSUPPORTED;
+    return RKV_OK;
+}
+
+struct PrefixPlan {
+    int own, slots;
+    size_t off_ml, off_o, bytes;
+};
+PrefixPlan prefix_plan(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
+    PrefixPlan p{};
+    p.own = shared_own_parts(dtype, H, HK, D, max_len, batch);
+    p.slots = p.own + (groups > 0 && batch > 0 ? shared_prefix_parts(dtype, H, HK, D, max_len, batch, groups) : 0);
+    const size_t rows = (size_t)batch * H * p.slots;
+    size_t off = kWorkspaceHeader;
+    p.off_ml = off;
+    off = align_up(off + rows * sizeof(float2), kWorkspaceAlign);
+    p.off_o = off;
+    off = align_up(off + rows * D * sizeof(float), kWorkspaceAlign);
+    p.bytes = off;
+    return p;
+}
+
+}  // namespace
+}  // namespace rkv
+
+using namespace rkv;
+
+extern "C" int rkv_prefix_decode_workspace_size(int dtype, int num_heads, int num_heads_kv, int dim_head, int max_len, int batch,
+                                                int num_groups, size_t* bytes) {
+    const int rc = prefix_check(dtype, num_heads, num_heads_kv, dim_head, max_len, batch, num_groups);
+    if (rc || !bytes) return rc ? rc : (int)RKV_ERR_INVALID_ARG;
+    *bytes = prefix_plan(dtype, num_heads, num_heads_kv, dim_head, max_len, batch, num_groups).bytes;
+    return RKV_OK;
+}
+
+extern "C" int rkv_prefix_decode(const void* Q, long long q_item_stride, int num_heads, const rkv_paged_cache* cache, int max_len,
+                                 int batch, const int* group_starts, const int* group_tokens, int num_groups, void* O, float* lse,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = paged_check(cache, true, batch);
+    if (!rc) rc = prefix_check(cache->dtype, num_heads, cache->num_heads_kv, cache->dim_head, max_len, batch, num_groups);
+    if (rc) return rc;
+    if (batch == 0) return RKV_OK;
+    const int D = cache->dim_head, es = elem_size(cache->dtype);
+    if (!Q || !O || ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(O)) & 15)) return RKV_ERR_INVALID_ARG;
+    if (batch > 1 && (q_item_stride < (long long)num_heads * D * es || (q_item_stride & 15))) return RKV_ERR_INVALID_ARG;
+    if (num_groups > 0 && (!group_starts || !group_tokens)) return RKV_ERR_INVALID_ARG;
+    const PrefixPlan p = prefix_plan(cache->dtype, num_heads, cache->num_heads_kv, D, max_len, batch, num_groups);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < p.bytes) return RKV_ERR_WORKSPACE;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    JoinArgs a{};
+    SharedArgs& s = a.s;
+    s.c = paged_view(*cache);
+    s.gr = Groups{group_starts, group_tokens, num_groups, batch, max_len};
+    s.Q = static_cast<const uint8_t*>(Q);
+    s.q_stride = q_item_stride;
+    s.dtype = cache->dtype;
+    s.H = num_heads;
+    s.HK = cache->num_heads_kv;
+    s.D = D;
+    s.batch = batch;
+    s.own = p.own;
+    s.slots = p.slots;
+    s.part_ml = reinterpret_cast<float2*>(ws + p.off_ml);
+    s.part_o = reinterpret_cast<float*>(ws + p.off_o);
+    a.O = O;
+    a.lse = lse;
+    a.clear = static_cast<int*>(workspace);
+    if (num_groups > 0) rc = launch_shared_pass(s, true, false, st);
+    if (!rc) rc = launch_shared_pass(s, false, num_groups > 0, st);
+    if (rc) return rc;
+    return s.dtype == RKV_F32 ? launch_join<float>(a, st) : s.dtype == RKV_BF16 ? launch_join<__nv_bfloat16>(a, st) : launch_join<__half>(a, st);
+}

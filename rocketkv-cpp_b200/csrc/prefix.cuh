@@ -1,0 +1,140 @@
+// prefix.cuh -- decode of a batch whose sequences share leading tokens: the groups, and the passes over them.
+#pragma once
+
+#include "paged.cuh"
+
+namespace rkv {
+
+// Groups of sequences: group g is starts[g] .. starts[g + 1] - 1 and shares its first tokens[g] tokens.
+struct Groups {
+    const int* starts;  // [n + 1], ascending
+    const int* tokens;  // [n]
+    int n, batch, max_len;
+
+    __device__ __forceinline__ int start(int g) const { return min(max(starts[g], 0), batch); }
+    __device__ __forceinline__ int size(int g) const { return max(0, start(g + 1) - start(g)); }
+    // Shared tokens of group g: at most what a sequence can hold.
+    __device__ __forceinline__ int shared(const PagedView& c, int g) const {
+        const long long cap = (long long)c.table_stride * c.page_size;
+        const int n = min(tokens[g], max_len);
+        return max(0, cap < n ? (int)cap : n);
+    }
+};
+
+// Shared tokens that sequence b of n tokens takes from its group: all of the
+// group's, or none where the sequence is shorter (it is attended on its own
+// then, so that every row of a shared tile sees all of it).  A whole warp calls.
+struct Member {
+    int group, tokens;  // -1, 0: of none
+};
+__device__ __forceinline__ Member member_of(const Groups& gr, const PagedView& c, int b, int n) {
+    const int lane = threadIdx.x & 31;
+    Member m{-1, 0};
+    for (int g0 = 0; g0 < gr.n; g0 += 32) {
+        const int g = g0 + lane;
+        const bool hit = g < gr.n && gr.start(g) <= b && b < gr.start(g + 1);
+        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+        if (hits) {
+            m.group = g0 + __ffs(hits) - 1;
+            break;
+        }
+    }
+    if (m.group >= 0) {
+        const int p = gr.shared(c, m.group);
+        if (p <= n) m.tokens = p;
+    }
+    return m;
+}
+// The sequence through whose table row a group's shared tokens are read: the first that holds them all.  A whole
+// warp calls.
+__device__ __forceinline__ int leader_of(const Groups& gr, const PagedView& c, int g, int shared) {
+    const int lane = threadIdx.x & 31, s0 = gr.start(g), s1 = gr.start(g + 1);
+    for (int b0 = s0; b0 < s1; b0 += 32) {
+        const int b = b0 + lane;
+        const unsigned hits = __ballot_sync(0xffffffffu, b < s1 && paged_len(c, b, gr.max_len) >= shared);
+        if (hits) return b0 + __ffs(hits) - 1;
+    }
+    return s0;
+}
+
+// A part of a pass: tokens of one part where `tokens` are taken in at most `splits` parts.
+constexpr int kPartMin = 128;
+__host__ __device__ __forceinline__ int part_tokens(int tokens, int splits) {
+    const int c = ((tokens + splits - 1) / splits + 31) / 32 * 32;
+    return c < kPartMin ? kPartMin : c;
+}
+
+// What the passes leave: part s of row (sequence b, query head h) at ((b H + h) slots + s), o [D] not divided by l,
+// and (m, l) in base 2.  Own tokens take the slots 0 .. own - 1, shared ones the others (where the matrix-instruction
+// kernel of paged.cu attends them).
+struct SharedArgs {
+    PagedView c;
+    Groups gr;
+    const uint8_t* Q;
+    long long q_stride;
+    int dtype, H, HK, D, batch;
+    int own, slots;
+    float* part_o;
+    float2* part_ml;
+};
+// Parts of every sequence's own tokens, and of every group's shared ones for the matrix-instruction kernel.
+int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch);
+int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups);
+// One pass: prefix, the groups' shared tokens; else every sequence's own.  dependent: launched while the kernel
+// before it still runs.
+int launch_shared_pass(const SharedArgs& s, bool prefix, bool dependent, cudaStream_t st);
+
+// The shared tokens on the tcgen05 tensor cores (prefix_tc.cu): 16-bit types.  The tiles of all units -- a unit is up
+// to 256 rows (128 above 128 columns) of one group and KV head -- are cut into equal stretches, one per CTA.  A unit's first
+// stretch leaves its rows in `first` (row b H + h), a stretch that begins inside a unit in `later` (256 rows per CTA).
+struct TcParts {
+    float* first_o;
+    float2* first_ml;
+    float* later_o;
+    float2* later_ml;
+    int* err;
+};
+constexpr int kTcSms = 148;
+constexpr int kTcKeys = 128;
+constexpr int kTcRows = 256;
+constexpr int kTcMinTiles = 2;  // of a stretch
+
+// Tiles of all units, and the CTAs that take them.
+struct TcCut {
+    long long tiles;
+    int ctas;
+    __device__ __forceinline__ long long begin(int c) const { return tiles * c / ctas; }
+};
+// Rows of a group and KV head, its units and the tiles of one.
+struct TcGroup {
+    int rows, units, tiles;
+};
+__device__ __forceinline__ TcGroup tc_group(const Groups& gr, const PagedView& c, int g, int G, int unit_rows) {
+    TcGroup t;
+    t.rows = gr.size(g) * G;
+    t.units = (t.rows + unit_rows - 1) / unit_rows;
+    t.tiles = (gr.shared(c, g) + kTcKeys - 1) / kTcKeys;
+    return t;
+}
+// Tiles of the groups before g (all: g = gr.n).  A whole warp calls.
+__device__ __forceinline__ long long tc_tiles(const Groups& gr, const PagedView& c, int g, int G, int HK, int unit_rows) {
+    const int lane = threadIdx.x & 31;
+    long long n = 0;
+    for (int i = lane; i < g; i += 32) {
+        const TcGroup t = tc_group(gr, c, i, G, unit_rows);
+        n += (long long)t.units * t.tiles * HK;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+}
+__device__ __forceinline__ TcCut tc_cut(long long tiles, int most) {
+    TcCut k;
+    k.tiles = tiles;
+    const long long n = (tiles + kTcMinTiles - 1) / kTcMinTiles;
+    k.ctas = n < most ? (n < 1 ? 1 : (int)n) : most;
+    return k;
+}
+int launch_prefix_tc(const SharedArgs& s, const TcParts& p, cudaStream_t st);
+
+}  // namespace rkv

@@ -40,7 +40,7 @@ EXPORTS = [
     "rkv_hsa_decode_summary", "rkv_capture_rows", "rkv_evict_compact", "rkv_paged_append",
     "rkv_paged_decode_workspace_size", "rkv_paged_decode", "rkv_weight_evict",
     "rkv_sink_attention_workspace_size", "rkv_sink_attention", "rkv_rotary_frequencies", "rkv_rotate",
-    "rkv_paged_append_rotated",
+    "rkv_paged_append_rotated", "rkv_prefix_decode_workspace_size", "rkv_prefix_decode",
 ]
 
 
@@ -171,6 +171,8 @@ def lib() -> ctypes.CDLL:
         "rkv_sink_attention_workspace_size": ([_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)], _I),
         "rkv_sink_attention": ([_VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _RSP, _RSP, _VP, _I, _I, _VP, _RSP, _VP,
                                 _VP, _SZ, _VP], _I),
+        "rkv_prefix_decode_workspace_size": ([_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)], _I),
+        "rkv_prefix_decode": ([_VP, _LL, _I, _PCP, _I, _I, _VP, _VP, _I, _VP, _VP, _VP, _SZ, _VP], _I),
         "rkv_rotary_frequencies": ([_VP, _I, _VP], _I),
         "rkv_rotate": ([_ROP, _VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _RSP, _RSP, _RSP, _RSP, _VP], _I),
         "rkv_paged_append_rotated": ([_PCP, _ROP, _VP, _VP, _VP, _RSP, _I, _I, _VP, _VP, _RSP, _VP, _RSP, _I, _VP], _I),
@@ -638,6 +640,63 @@ class PagedDecoder:
                 self.sinks, self.window, self.O.data_ptr(), self.lse.data_ptr(), _ptr(weights), wstride,
                 self.ws.data_ptr(), self.ws_bytes, owner=self)
         return self.O
+
+
+class PrefixDecoder:
+    """PagedDecoder for a batch whose sequences share leading tokens, group by
+    group (rkv_prefix_decode): what a group shares is read once for all its
+    sequences.  dtype: the cache's, and that of the output O [B, H, D]; lse
+    [B, H] float32; both and the workspace are the object's, so calls that may
+    run at the same time need an object each."""
+
+    def __init__(self, num_heads: int, num_heads_kv: int, dim_head: int, max_len: int, batch: int, dtype, device, num_groups: int = 1):
+        import torch
+        b = _SZ(0)
+        self.O = torch.empty((batch, num_heads, dim_head), dtype=dtype, device=device)
+        _check(lib().rkv_prefix_decode_workspace_size(_dtype_of(self.O), num_heads, num_heads_kv, dim_head, max_len, batch, num_groups,
+                                                      ctypes.byref(b)), "rkv_prefix_decode_workspace_size")
+        self.num_heads, self.num_heads_kv, self.dim_head = num_heads, num_heads_kv, dim_head
+        self.max_len, self.batch, self.num_groups = max_len, batch, num_groups
+        self.ws_bytes = b.value
+        self.ws = _workspace(b.value, device)
+        self.lse = torch.empty((batch, num_heads), dtype=torch.float32, device=device)
+        self._streams = {_handle(self.ws.device, None)}  # whose work its buffers outlive
+        self._ran = False  # a call has written the workspace's error word
+
+    def _buffers(self):
+        return self.ws, self.O, self.lse
+
+    def __call__(self, Q, cache: PagedCache, group_starts, group_tokens, stream=None):
+        """Q [B, H, D] of the cache's type; group g is the sequences
+        group_starts[g] .. group_starts[g + 1] - 1, whose first group_tokens[g]
+        tokens are the same (int32 on the device, [num_groups + 1] and
+        [num_groups]).  Returns O."""
+        if Q.shape != self.O.shape or not Q.is_contiguous():
+            raise ValueError("Q: contiguous [B, H, D] of the decoder's sizes")
+        dev = Q.device
+        if (Q.dtype != cache.K.dtype or Q.dtype != self.O.dtype or dev != cache.K.device or dev != self.ws.device
+                or cache.batch != self.batch or cache._lens is None):
+            raise ValueError("Q, the cache and the decoder: one type, device and batch, and the cache's lens set")
+        if (cache.c.num_heads_kv, cache.c.dim_head) != (self.num_heads_kv, self.dim_head):
+            raise ValueError("the cache's heads are not the decoder's")
+        _int32(group_starts, dev, "group_starts")
+        _int32(group_tokens, dev, "group_tokens")
+        if group_tokens.numel() != self.num_groups or group_starts.numel() != self.num_groups + 1:
+            raise ValueError("group_starts, group_tokens: num_groups + 1 and num_groups entries")
+        _launch(dev, stream, "rkv_prefix_decode", lib().rkv_prefix_decode, Q.data_ptr(),
+                self.num_heads * self.dim_head * Q.element_size(), self.num_heads, cache.ref, self.max_len, self.batch,
+                group_starts.data_ptr(), group_tokens.data_ptr(), self.num_groups, self.O.data_ptr(), self.lse.data_ptr(),
+                self.ws.data_ptr(), self.ws_bytes, owner=self)
+        self._ran |= self.batch > 0
+        return self.O
+
+    def status(self, stream=None) -> int:
+        """Waits for `stream`; the first error that a call recorded since the last look, or RKV_OK."""
+        import torch
+        if not self._ran:
+            return RKV_OK
+        with torch.cuda.device(self.ws.device):
+            return lib().rkv_workspace_status(_ptr(self.ws), _stream(stream))
 
 
 def _check_weights(w, batch, heads, max_len, device) -> int:
