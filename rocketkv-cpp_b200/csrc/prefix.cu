@@ -16,6 +16,7 @@ namespace {
 
 struct JoinArgs {
     SharedArgs s;
+    TcParts tc;  // where the shared tokens' parts are those of the tcgen05 kernel
     void* O;
     float* lse;
     int* clear;  // the error word, where no kernel before this one has cleared it
@@ -40,7 +41,7 @@ constexpr int kJoinRows = 4;  // rows of a CTA, a warp each
 
 // Joins the parts of a row: those of its own tokens, then those of the shared
 // ones, in their order whatever the grid.  O is rounded to Q's type, once.
-template <typename T>
+template <typename T, bool TC>
 __global__ void __launch_bounds__(kJoinRows * 32) prefix_join_kernel(const JoinArgs a) {
     const SharedArgs& s = a.s;
     const int lane = threadIdx.x & 31;
@@ -51,20 +52,38 @@ __global__ void __launch_bounds__(kJoinRows * 32) prefix_join_kernel(const JoinA
     const int mine = n - m.tokens;
     const int own = mine > 0 ? (mine + part_tokens(mine, s.own) - 1) / part_tokens(mine, s.own) : 0;
     int shared = 0;
-    if (m.tokens > 0) {
+    long long later = 0;  // TC: the row of the second part
+    if (m.tokens > 0 && !TC) {
         const int t = part_tokens(m.tokens, s.slots - s.own);
         shared = (m.tokens + t - 1) / t;
+    }
+    if (m.tokens > 0 && TC) {
+        // the CTAs whose stretches hold tiles of this row's unit: one has the first, the others begin inside the unit
+        const int G = s.H / s.HK, h = (int)(row % s.H);
+        const TcGroup t = tc_group(s.gr, s.c, m.group, G, kTcRows);
+        const int r = (b - s.gr.start(m.group)) * G + h % G;
+        const long long t0 = tc_tiles(s.gr, s.c, m.group, G, s.HK, kTcRows) + ((long long)(h / G) * t.units + r / kTcRows) * t.tiles;
+        const TcCut k = tc_cut(tc_tiles(s.gr, s.c, s.gr.n, G, s.HK, kTcRows), kTcSms);
+        // CTA c begins at floor(tiles c / ctas)
+        const long long c0 = ((t0 + 1) * k.ctas + k.tiles - 1) / k.tiles, c1 = ((t0 + t.tiles) * k.ctas + k.tiles - 1) / k.tiles;
+        shared = 1 + (int)(c1 - c0);
+        later = c0 * kTcRows + r % kTcRows;
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (a.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.clear = 0;
     if (row >= rows) return;
-    const float2* ml = s.part_ml + row * s.slots;
-    const float* po = s.part_o + row * s.slots * s.D;
-    // part i: own ones in the slots from 0, shared ones in those from s.own
+    // part i: own ones in the slots from 0; shared ones in those from s.own, or where the tcgen05 kernel leaves them
     const int parts = own + shared;
-    auto slot = [&](int i) { return i < own ? i : s.own + (i - own); };
+    auto ml_of = [&](int i) -> float2 {
+        if (i < own || !TC) return s.part_ml[row * s.slots + (i < own ? i : s.own + (i - own))];
+        return i == own ? a.tc.first_ml[row] : a.tc.later_ml[later + (long long)(i - own - 1) * kTcRows];
+    };
+    auto o_of = [&](int i) -> const float* {
+        if (i < own || !TC) return s.part_o + (row * s.slots + (i < own ? i : s.own + (i - own))) * s.D;
+        return i == own ? a.tc.first_o + row * s.D : a.tc.later_o + (later + (long long)(i - own - 1) * kTcRows) * s.D;
+    };
     float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml[slot(i)].x);
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml_of(i).x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float base = top == -INFINITY ? 0.0f : top;
@@ -74,7 +93,7 @@ __global__ void __launch_bounds__(kJoinRows * 32) prefix_join_kernel(const JoinA
     for (int i0 = 0; i0 < parts; i0 += 32) {
         float w = 0.0f;
         if (i0 + lane < parts) {
-            const float2 x = ml[slot(i0 + lane)];
+            const float2 x = ml_of(i0 + lane);
             w = exp2f(x.x - base);
             l = fmaf(x.y, w, l);
         }
@@ -82,7 +101,7 @@ __global__ void __launch_bounds__(kJoinRows * 32) prefix_join_kernel(const JoinA
 #pragma unroll 4
         for (int i = 0; i < here; ++i) {
             const float f = __shfl_sync(0xffffffffu, w, i);
-            const float* p = po + (size_t)slot(i0 + i) * s.D;
+            const float* p = o_of(i0 + i);
             if (c0 < s.D) {
                 const float4 v = *reinterpret_cast<const float4*>(p + c0);
                 o[0] = make_float4(fmaf(v.x, f, o[0].x), fmaf(v.y, f, o[0].y), fmaf(v.z, f, o[0].z), fmaf(v.w, f, o[0].w));
@@ -105,7 +124,8 @@ __global__ void __launch_bounds__(kJoinRows * 32) prefix_join_kernel(const JoinA
 template <typename T>
 int launch_join(const JoinArgs& a, cudaStream_t st) {
     const long long blocks = ((long long)a.s.batch * a.s.H + kJoinRows - 1) / kJoinRows;
-    const cudaError_t e = launch_pdl(prefix_join_kernel<T>, dim3((unsigned)blocks), dim3(kJoinRows * 32), 0, st, a);
+    const cudaError_t e = a.tc.first_o ? launch_pdl(prefix_join_kernel<T, true>, dim3((unsigned)blocks), dim3(kJoinRows * 32), 0, st, a)
+                                       : launch_pdl(prefix_join_kernel<T, false>, dim3((unsigned)blocks), dim3(kJoinRows * 32), 0, st, a);
     if (e != cudaSuccess) (void)cudaGetLastError();
     return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }
@@ -118,20 +138,35 @@ int prefix_check(int dtype, int H, int HK, int D, int max_len, int batch, int gr
     return RKV_OK;
 }
 
+// The shared tokens on the tcgen05 tensor cores: 16-bit types where a group of mean size has more rows of a KV head
+// than two CTAs of the matrix-instruction kernel take.
+bool on_tc(int dtype, int H, int HK, int D, int batch, int groups) {
+    return dtype != RKV_F32 && D <= 128 && (long long)batch * (H / HK) > 16LL * groups;
+}
+
 struct PrefixPlan {
+    bool tc;
     int own, slots;
-    size_t off_ml, off_o, bytes;
+    size_t off_ml, off_o, off_first_ml, off_first_o, off_later_ml, off_later_o, bytes;
 };
 PrefixPlan prefix_plan(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
     PrefixPlan p{};
+    const bool any = groups > 0 && batch > 0;
+    p.tc = any && on_tc(dtype, H, HK, D, batch, groups);
     p.own = shared_own_parts(dtype, H, HK, D, max_len, batch);
-    p.slots = p.own + (groups > 0 && batch > 0 ? shared_prefix_parts(dtype, H, HK, D, max_len, batch, groups) : 0);
-    const size_t rows = (size_t)batch * H * p.slots;
+    p.slots = p.own + (any && !p.tc ? shared_prefix_parts(dtype, H, HK, D, max_len, batch, groups) : 0);
     size_t off = kWorkspaceHeader;
-    p.off_ml = off;
-    off = align_up(off + rows * sizeof(float2), kWorkspaceAlign);
-    p.off_o = off;
-    off = align_up(off + rows * D * sizeof(float), kWorkspaceAlign);
+    auto take = [&](size_t& ml, size_t& o, size_t rows) {
+        ml = off;
+        off = align_up(off + rows * sizeof(float2), kWorkspaceAlign);
+        o = off;
+        off = align_up(off + rows * D * sizeof(float), kWorkspaceAlign);
+    };
+    take(p.off_ml, p.off_o, (size_t)batch * H * p.slots);
+    if (p.tc) {
+        take(p.off_first_ml, p.off_first_o, (size_t)batch * H);
+        take(p.off_later_ml, p.off_later_o, (size_t)kTcSms * kTcRows);
+    }
     p.bytes = off;
     return p;
 }
@@ -181,8 +216,17 @@ extern "C" int rkv_prefix_decode(const void* Q, long long q_item_stride, int num
     s.part_o = reinterpret_cast<float*>(ws + p.off_o);
     a.O = O;
     a.lse = lse;
-    a.clear = static_cast<int*>(workspace);
-    if (num_groups > 0) rc = launch_shared_pass(s, true, false, st);
+    if (p.tc) {
+        a.tc.first_ml = reinterpret_cast<float2*>(ws + p.off_first_ml);
+        a.tc.first_o = reinterpret_cast<float*>(ws + p.off_first_o);
+        a.tc.later_ml = reinterpret_cast<float2*>(ws + p.off_later_ml);
+        a.tc.later_o = reinterpret_cast<float*>(ws + p.off_later_o);
+        a.tc.err = static_cast<int*>(workspace);
+        rc = launch_prefix_tc(s, a.tc, st);
+    } else {
+        a.clear = static_cast<int*>(workspace);
+        if (num_groups > 0) rc = launch_shared_pass(s, true, false, st);
+    }
     if (!rc) rc = launch_shared_pass(s, false, num_groups > 0, st);
     if (rc) return rc;
     return s.dtype == RKV_F32 ? launch_join<float>(a, st) : s.dtype == RKV_BF16 ? launch_join<__nv_bfloat16>(a, st) : launch_join<__half>(a, st);

@@ -1,0 +1,487 @@
+// prefix_tc.cu -- the shared tokens of a group of sequences against all of the
+// group's queries on the tcgen05 tensor cores: 16-bit types, dim_head <= 128.
+//
+// Rows are (sequence, query head of the KV head), 128 to an accumulator; a unit
+// is up to 256 of them, two accumulators, so that both use every K and V tile
+// that is loaded.  A unit of 128 rows or fewer takes the tiles in turn
+// instead, the even ones to the first accumulator and the odd ones to the
+// second, and joins the two at the end: either way one accumulator's softmax
+// runs while the tensor cores work on the other's products.  128 keys at a
+// time: S = Q K^T into tensor memory, P = 2^(S - m) rounded to the inputs' type
+// back into tensor memory in S's place, O += P V.
+//
+//   warps 0-3    copy Q's rows and K's and V's, which lie in pages of any size, by 16-byte
+//                asynchronous copies into the swizzled tiles
+//   warp 4       issues the products
+//   warps 8-11, 12-15   softmax of the first accumulator, of the second, and their rows
+//
+// The tiles of all units are one long list that is cut into equal stretches, one
+// per CTA: whatever the groups' sizes and lengths, every SM has the same work.
+// Each stretch leaves (m, l, O) of its rows, not divided by l, for the join.
+//
+// P is rounded to 16 bits (half a step of the type, as the products take both
+// operands in one type); scores, m, l and the accumulators are fp32.  Every
+// row of a tile sees all of its keys, but for those behind the shared tokens
+// and on pages outside the pool, which a mask of a bit per key leaves out.
+#include "attn_tc.cuh"
+#include "prefix.cuh"
+
+namespace rkv {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kBlk = 128 * 128;  // bytes of a 128-row block of 64 columns
+constexpr int kMasks = 16;       // tiles whose masks are kept: more than the copies are ahead of the softmax
+constexpr int kLag = 2;          // ring slots whose copies are on their way when the next is begun
+
+__host__ __device__ constexpr int ring_slots(int kb) { return kb == 1 ? 8 : 4; }  // of a K or a V tile
+
+struct Args {
+    SharedArgs s;
+    TcParts p;
+    int G;
+    float scale2;  // log2(e) / sqrt(D)
+};
+
+struct Bars {
+    uint64_t q_empty, o_full, o_empty, drained;
+    uint64_t s_full[2], p_half[2], p_ready[2];  // of an accumulator
+    uint64_t full[8], empty[8];
+    uint32_t mask[kMasks][4];
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(Bars) <= 1024, "the barriers' part of shared memory");
+
+// A CTA's part of a unit: rows row0 .. row0 + rows - 1 of group g (whose first sequence is s0) and KV head hk, and
+// `tiles` tiles from tile j0 on of its `shared` tokens.
+struct Stretch {
+    int g, hk, s0, row0, rows, shared, j0, tiles;
+};
+// The stretches of CTA c, which every warp of it walks on its own.
+struct Walk {
+    long long at, end;
+    __device__ __forceinline__ Walk(const Args& a) {
+        const TcCut k = tc_cut(tc_tiles(a.s.gr, a.s.c, a.s.gr.n, a.G, a.s.HK, kTcRows), gridDim.x);
+        const int c = blockIdx.x;
+        at = end = 0;
+        if (c < k.ctas) at = k.begin(c), end = k.begin(c + 1);
+    }
+    __device__ __forceinline__ bool next(const Args& a, Stretch& x) {
+        if (at >= end) return false;
+        const int lane = threadIdx.x & 31;
+        long long base = 0;
+        for (int g0 = 0; g0 < a.s.gr.n; g0 += 32) {
+            TcGroup t{0, 0, 0};
+            if (g0 + lane < a.s.gr.n) t = tc_group(a.s.gr, a.s.c, g0 + lane, a.G, kTcRows);
+            const long long mine = (long long)t.units * t.tiles * a.s.HK;
+            long long sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += y;
+            }
+            const unsigned hits = __ballot_sync(0xffffffffu, at < base + sum);
+            if (hits) {
+                const int l = __ffs(hits) - 1;
+                x.g = g0 + l;
+                base += __shfl_sync(0xffffffffu, sum - mine, l);
+                const int units = __shfl_sync(0xffffffffu, t.units, l), tiles = __shfl_sync(0xffffffffu, t.tiles, l);
+                const int rows = __shfl_sync(0xffffffffu, t.rows, l);
+                const long long off = at - base;
+                const int unit = (int)(off / tiles);  // the units of a KV head side by side: they read the same tiles
+                x.j0 = (int)(off - (long long)unit * tiles);
+                x.hk = unit / units;
+                x.row0 = (unit - x.hk * units) * kTcRows;
+                x.rows = min(kTcRows, rows - x.row0);
+                x.tiles = (int)min((long long)(tiles - x.j0), end - at);
+                x.s0 = a.s.gr.start(x.g);
+                x.shared = a.s.gr.shared(a.s.c, x.g);
+                at += x.tiles;
+                return true;
+            }
+            base += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        return false;
+    }
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+// A warp's 32 rows of KB blocks of 64 columns into a swizzled tile at dst (this warp's first row): off is this lane's
+// row's offset from src, or -1 for a row of zeros; columns from `chunks` 16-byte chunks on are zeros.
+template <int KB>
+__device__ __forceinline__ void copy_rows(uint32_t dst, const uint8_t* src, long long off, int chunks, int lane) {
+    constexpr int LPR = KB * 8, RPI = 32 / LPR;  // lanes of a row, rows of an instruction
+    const int c = lane % LPR, r0 = lane / LPR;
+#pragma unroll
+    for (int i = 0; i < 32 / RPI; ++i) {
+        const int r = i * RPI + r0;
+        const long long o = __shfl_sync(0xffffffffu, off, r);
+        const bool real = o >= 0 && c < chunks;
+        copy16(dst + (c >> 3) * kBlk + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (real ? o + c * 16 : 0), real);
+    }
+}
+
+// 32 fp32 columns of a warp's 32 rows (a row per lane in o) to the rows' places (place: this lane's row's, in
+// floats, or -1), through 4 KB of shared memory so that eight lanes write 128 bytes of a row.
+__device__ __forceinline__ void write_cols(uint8_t* so, const uint32_t* o, float* dst, long long place, int col0, int D, int lane) {
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+        *reinterpret_cast<uint4*>(so + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        const int r = x * 4 + (lane >> 3), v = lane & 7;
+        const uint4 y = *reinterpret_cast<const uint4*>(so + r * 128 + ((v ^ (r & 7)) << 4));
+        const long long at = __shfl_sync(0xffffffffu, place, r);
+        if (at >= 0 && col0 + v * 4 < D) *reinterpret_cast<uint4*>(dst + at + col0 + v * 4) = y;
+    }
+    __syncwarp();
+}
+
+template <int KB, bool BF>
+__global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
+    constexpr int NS = ring_slots(KB);
+    constexpr uint32_t kOne = KB * kBlk;
+    constexpr uint32_t kColO = 256;  // tensor memory: S0, S1 (128 columns each), O0, O1 (64 KB each)
+    extern __shared__ uint8_t smem_raw[];
+    asm volatile("griddepcontrol.launch_dependents;");  // the passes behind may be scheduled (they wait for this grid)
+    uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    Bars& B = *reinterpret_cast<Bars*>(sm);
+    volatile int* abort_flag = &B.abort;
+    int* err = a.p.err;
+    uint8_t* sq = sm + 1024;
+    uint8_t* ring = sq + 2 * kOne;
+    uint8_t* stage = ring + NS * kOne;  // 4 KB per softmax warp
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        mbar_init(&B.q_empty, 1);
+        mbar_init(&B.o_full, 1);
+        mbar_init(&B.o_empty, 8);
+        mbar_init(&B.drained, 1);
+        for (int u = 0; u < 2; ++u) {
+            mbar_init(&B.s_full[u], 1);
+            mbar_init(&B.p_half[u], 4);
+            mbar_init(&B.p_ready[u], 4);
+        }
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&B.full[i], 4);
+            mbar_init(&B.empty[i], 1);
+        }
+        *abort_flag = 0;
+        // a wait gives up after two seconds at the soonest, long after this
+        if (blockIdx.x == 0) *err = 0;
+        fence_mbar_init();
+    }
+    if (warp == 4) tmem_alloc(&B.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = B.tmem;
+    Walk walk(a);
+    Stretch x;
+
+    // (48 + 48 + 208 + 208) * 128 registers are the 128 * 512 of the launch
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        const int chunks = a.s.D / 8;
+        int q = 0, nq = 0, nk = 0, open = 0;  // slots, stretches, tiles; slots begun whose copies are not known to have landed
+        bool ok = true;
+        auto landed = [&](int pending) {  // all but the last `pending` slots
+            while (open > pending) {
+                if (open == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+                else if (open == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+                else asm volatile("cp.async.wait_group 0;" ::: "memory");
+                fence_proxy_async();  // the products read what was copied through another proxy
+                __syncwarp();
+                if (lane == 0) mbar_arrive1(&B.full[(q - open) % NS]);
+                --open;
+            }
+        };
+        auto slot = [&](const uint8_t* base, long long off) {
+            const int s = q % NS;
+            if (q >= NS && !(ok = warp_wait(&B.empty[s], (uint32_t)((q / NS - 1) & 1), err, abort_flag))) return;
+            copy_rows<KB>(smem_u32(ring) + s * kOne + warp * 4096, base, off, chunks, lane);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ++q;
+            ++open;
+            landed(kLag);
+        };
+        while (ok && walk.next(a, x)) {
+            const int leader = leader_of(a.s.gr, a.s.c, x.g, x.shared);
+            if (nq > 0 && !(ok = warp_wait(&B.q_empty, (uint32_t)((nq - 1) & 1), err, abort_flag))) break;
+            ++nq;
+            // Q's rows go with the first K tile
+            for (int u = 0; u < (x.rows > 128 ? 2 : 1); ++u) {
+                const int r = u * 128 + warp * 32 + lane;
+                const unsigned row = x.row0 + r, sq_ = row / (unsigned)a.G;
+                const long long off = r < x.rows ? (long long)(x.s0 + (int)sq_) * a.s.q_stride +
+                                                       (long long)(x.hk * a.G + (int)(row - sq_ * a.G)) * a.s.D * 2
+                                                 : -1;
+                copy_rows<KB>(smem_u32(sq) + u * kOne + warp * 4096, a.s.Q, off, chunks, lane);
+            }
+            for (int j = x.j0; j < x.j0 + x.tiles && ok; ++j, ++nk) {
+                const int t = j * kTcKeys + warp * 32 + lane;
+                const long long off = t < x.shared ? paged_offset(a.s.c, leader, x.hk, t) : -1;
+                const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0);
+                if (lane == 0) B.mask[nk % kMasks][warp] = mask;
+                slot(a.s.c.K, off);
+                if (ok) slot(a.s.c.V, off);
+            }
+            if (ok) landed(0);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 4) {
+            const uint32_t ids = mma_idesc(BF ? 1u : 0u, kTcKeys);
+            const uint32_t idv = mma_idesc(BF ? 1u : 0u, KB * 64) | (1u << 16);  // B with N contiguous
+            const uint64_t qd = mma_desc_sw128(smem_u32(sq)), kd = mma_desc_sw128(smem_u32(ring));
+            const uint64_t vd = v_desc(smem_u32(ring), kBlk);
+            int q = 0, nq = 0;
+            uint32_t steps = 0;  // a bit per accumulator: parity of its steps
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, int n) { return ok = warp_wait(bar, (uint32_t)(n & 1), err, abort_flag); };
+            while (ok && walk.next(a, x)) {
+                // step k: accumulator k & 1 and the next tile, or both accumulators one after the other with each tile
+                const bool both = x.rows > 128;
+                const int n = both ? 2 * x.tiles : x.tiles;
+                auto scores = [&](int k) {
+                    const int u = k & 1, at = q + 2 * (both ? k >> 1 : k), s = at % NS;
+                    if (!(both && u) && !wait(&B.full[s], at / NS)) return;
+                    tc_fence_after();
+                    const uint64_t da = qd + (uint32_t)((both ? u : 0) * (kOne >> 4)), db = kd + (uint32_t)(s * (kOne >> 4));
+#pragma unroll
+                    for (int ks = 0; ks < KB * 4; ++ks) {
+                        const uint32_t o = ((ks >> 2) * kBlk + (ks & 3) * 32) >> 4;
+                        mma_ss(tbase + u * 128, da + o, db + o, ids, ks > 0);
+                    }
+                    mma_commit_w(&B.s_full[u]);
+                    if (!both || u) mma_commit_w(&B.empty[s]);
+                    if (k == n - 1) mma_commit_w(&B.q_empty);
+                };
+                scores(0);
+                if (ok && n > 1) scores(1);
+                if (ok && nq > 0) wait(&B.o_empty, nq - 1);  // the rows of the stretch before have been read
+                ++nq;
+                for (int k = 0; k < n && ok; ++k) {
+                    const int u = k & 1, at = q + 2 * (both ? k >> 1 : k) + 1, s = at % NS;
+                    if (!(both && u) && !wait(&B.full[s], at / NS)) break;
+                    const uint64_t db = vd + (uint32_t)(s * (kOne >> 4));
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (!wait(half ? &B.p_ready[u] : &B.p_half[u], (int)(steps >> u))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int ks = half * 4; ks < half * 4 + 4; ++ks)
+                            mma_ts(tbase + kColO + u * (KB * 64), tbase + u * 128 + ks * 8, db + ks * 128, idv, k > 1 || ks > 0);
+                    }
+                    if (!ok) break;
+                    steps ^= 1u << u;
+                    if (!both || u) mma_commit_w(&B.empty[s]);
+                    if (k + 2 < n) scores(k + 2);
+                }
+                if (ok) mma_commit_w(&B.o_full);
+                q += 2 * x.tiles;
+            }
+            // the products have ended before the tensor memory is freed
+            mma_commit_w(&B.drained);
+            mbar_wait_bounded(&B.drained, 0, err);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int u = (warp >> 2) - 2, q4 = warp & 3, row = q4 * 32 + lane;
+        const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+        const uint32_t ts = tbase + u * 128 + lane_off, to = tbase + kColO + lane_off;
+        uint8_t* so = stage + (warp - 8) * 4096;
+        const float2 sc = make_float2(a.scale2, a.scale2);
+        int nt = 0, nk = 0, nq = 0;  // steps of this accumulator; tiles, stretches
+        bool ok = true;
+        while (ok && walk.next(a, x)) {
+            const bool both = x.rows > 128;
+            const int n = both ? x.tiles : (x.tiles + 1 - u) >> 1;
+            const int r = (both ? u * 128 : 0) + row;
+            const bool some = (both ? u * 128 : 0) + q4 * 32 < x.rows;  // this warp has rows
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < n; ++j, ++nt) {
+                if (!(ok = warp_wait(&B.s_full[u], (uint32_t)(nt & 1), err, abort_flag))) break;
+                if (!some) {
+                    if (lane == 0) {
+                        mbar_arrive1(&B.p_half[u]);
+                        mbar_arrive1(&B.p_ready[u]);
+                    }
+                    continue;
+                }
+                tc_fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) ld32_async(ts + c * 32, s + c * 32);
+                const uint4 mask = *reinterpret_cast<const uint4*>(B.mask[(nk + (both ? j : 2 * j + u)) % kMasks]);
+                wait_ld();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) pin32(s + c * 32);
+                if ((mask.x & mask.y & mask.z & mask.w) != 0xFFFFFFFFu) {
+                    const uint32_t see[4] = {mask.x, mask.y, mask.z, mask.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (!(see[w] & (1u << c))) s[32 * w + c] = 0xFF800000u;  // -inf
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 128; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool need = (mt - m) * a.scale2 > kGrow;  // true for a row's first key, false while it has none
+                if (__any_sync(0xffffffffu, need)) {
+                    const float corr = need ? ex2_approx((m - mt) * a.scale2) : 1.0f;
+                    l *= corr;
+                    if (need) m = mt;
+                    if (j > 0) {  // the products up to here are complete: this tile's scores were issued behind them
+#pragma unroll 1
+                        for (int c = 0; c < KB * 2; ++c) {
+                            uint32_t o[32];
+                            ld32_async(to + u * (KB * 64) + c * 32, o);
+                            wait_ld();
+                            pin32(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                            st32(to + u * (KB * 64) + c * 32, o);
+                        }
+                    }
+                }
+                const float ms = (m == -INFINITY ? 0.0f : m) * a.scale2 - kLift<BF>;
+                const float2 nm = make_float2(-ms, -ms);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {  // the products of the first 64 keys start under the second's exponentials
+#pragma unroll
+                    for (int c = half * 32; c < half * 32 + 32; ++c) {
+                        float2 e = __ffma2_rn(make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc, nm);
+                        e.x = ex2_approx(e.x);
+                        e.y = ex2_approx(e.y);
+                        sum[c & 1] = __fadd2_rn(sum[c & 1], e);
+                        s[c] = pack2<BF>(e.x, e.y);
+                    }
+                    st32(ts + half * 32, s + half * 32);
+                    wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive1(half ? &B.p_ready[u] : &B.p_half[u]);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            }
+            if (!ok || !(ok = warp_wait(&B.o_full, (uint32_t)(nq & 1), err, abort_flag))) break;
+            tc_fence_after();
+            const bool first = x.j0 == 0;
+            nk += x.tiles;
+            ++nq;
+            if (!some) {
+                tc_fence_before();
+                if (lane == 0) mbar_arrive1(&B.o_empty);
+                continue;
+            }
+            // this row's place
+            long long at = -1;
+            if (r < x.rows) {
+                const unsigned of = x.row0 + r, sq_ = of / (unsigned)a.G;
+                at = first ? (long long)(x.s0 + (int)sq_) * a.s.H + x.hk * a.G + (int)(of - sq_ * a.G) : (long long)blockIdx.x * kTcRows + r;
+            }
+            float* po = first ? a.p.first_o : a.p.later_o;
+            float2* pml = first ? a.p.first_ml : a.p.later_ml;
+            float2 ml = make_float2(m == -INFINITY ? -INFINITY : m * a.scale2 - kLift<BF>, l);
+            if (both) {
+                uint32_t o[KB * 64];
+#pragma unroll
+                for (int c = 0; c < KB * 2; ++c) ld32_async(to + u * (KB * 64) + c * 32, o + c * 32);
+                wait_ld();
+#pragma unroll
+                for (int c = 0; c < KB * 2; ++c) pin32(o + c * 32);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive1(&B.o_empty);
+                if (at >= 0) pml[at] = ml;
+                const long long place = at >= 0 ? at * a.s.D : -1;
+#pragma unroll
+                for (int c = 0; c < KB * 2; ++c) write_cols(so, o + c * 32, po, place, c * 32, a.s.D, lane);
+                continue;
+            }
+            // the two accumulators hold the same rows: each softmax takes half of the columns of their sum
+            float2* mine = reinterpret_cast<float2*>(so);
+            const float2* others = reinterpret_cast<const float2*>(stage + ((warp - 8) ^ 4) * 4096);
+            mine[lane] = ml;
+            group_sync(1 + q4, 64);
+            const float2 ot = others[lane];
+            group_sync(1 + q4, 64);  // the stage's other use begins
+            const float top = fmaxf(ml.x, ot.x), base = top == -INFINITY ? 0.0f : top;
+            const float fm = exp2f(ml.x - base), fo = exp2f(ot.x - base);
+            const float f0 = u ? fo : fm, f1 = u ? fm : fo;
+            if (u == 0 && at >= 0) pml[at] = make_float2(top, ml.y * fm + ot.y * fo);
+            const long long place = at >= 0 ? at * a.s.D : -1;
+#pragma unroll
+            for (int c = 0; c < KB; ++c) {
+                const int col = (u * KB + c) * 32;
+                uint32_t o[32], p[32];
+                ld32_async(to + col, o);
+                ld32_async(to + KB * 64 + col, p);
+                wait_ld();
+                pin32(o);
+                pin32(p);
+                if (c == KB - 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive1(&B.o_empty);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    // an accumulator without a tile holds anything
+                    const float y = x.tiles > 1 ? __uint_as_float(p[i]) * f1 : 0.0f;
+                    o[i] = __float_as_uint(fmaf(__uint_as_float(o[i]), f0, y));
+                }
+                write_cols(so, o, po, place, col, a.s.D, lane);
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 4) tmem_dealloc(tbase, 512);
+}
+
+template <int KB, bool BF>
+int launch(const Args& a, cudaStream_t st) {
+    // the barriers, and up to 1023 bytes of alignment; Q and the ring; the rows' stage
+    const int smem = 2048 + (2 + ring_slots(KB)) * KB * kBlk + 8 * 4096;
+    // the split of the registers is the launch's only where the kernel was compiled to 128 a thread
+    static const bool fits = [] {
+        cudaFuncAttributes f;
+        if (cudaFuncGetAttributes(&f, prefix_tc_kernel<KB, BF>) == cudaSuccess) return f.numRegs == 128;
+        (void)cudaGetLastError();
+        return false;
+    }();
+    if (!fits) return RKV_ERR_CUDA;
+    if (cudaFuncSetAttribute(prefix_tc_kernel<KB, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return RKV_ERR_CUDA;
+    }
+    prefix_tc_kernel<KB, BF><<<kTcSms, kThreads, smem, st>>>(a);
+    return launched();
+}
+
+}  // namespace
+
+int launch_prefix_tc(const SharedArgs& s, const TcParts& p, cudaStream_t st) {
+    Args a{};
+    a.s = s;
+    a.p = p;
+    a.G = s.H / s.HK;
+    a.scale2 = 1.4426950408889634f / sqrtf((float)s.D);
+    const bool bf = s.dtype == RKV_BF16;
+    if (s.D <= 64) return bf ? launch<1, true>(a, st) : launch<1, false>(a, st);
+    return bf ? launch<2, true>(a, st) : launch<2, false>(a, st);
+}
+
+}  // namespace rkv
