@@ -113,6 +113,8 @@ struct DecodeArgs {
     Groups gr;           // the passes of a batch that shares leading tokens
     int slots, slot0;    // their parts of a row, and the first of this pass
     int units;           // prefix pass: row groups of all groups at most
+    int2* info;          // pass over own tokens: what each row's parts are
+    int prefix_parts;    // of the prefix pass at most, 0 where it is not this kernel's
 };
 
 // The visible tokens are numbered 0 .. nvis - 1: the sinks, then the window.
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
     const int D = a.D, chunks = D * S::SIZE / 16;
 
     long long id = blockIdx.x;
-    int split, b, hk, h0, ng, first = 0;  // b: whose table row; first: the first row's sequence, among the group's rows
+    int split, b, hk, h0, ng, first = 0;  // b: whose table row; first: the group's first sequence
     Visible vis;
     int chunk = a.chunk;
     if (PASS == PASS_SHARED) {
@@ -374,6 +376,11 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
             vis.gap = shared;
             vis.nvis = vis.n - shared;
             chunk = part_tokens(vis.nvis, a.splits);
+            if (split == 0 && tid < min(8 * NT, a.G - grp * 8 * NT)) {
+                const int t = part_tokens(shared, a.prefix_parts > 0 ? a.prefix_parts : 1);
+                const int parts = shared == 0 ? 0 : a.prefix_parts > 0 ? (shared + t - 1) / t : 1;
+                a.info[(size_t)b * a.H + hk * a.G + grp * 8 * NT + tid] = make_int2((vis.nvis + chunk - 1) / chunk, parts);
+            }
         }
         h0 = hk * a.G + grp * 8 * NT;
         ng = min(8 * NT, a.G - grp * 8 * NT);
@@ -952,6 +959,8 @@ int launch_shared_pass(const SharedArgs& s, bool prefix, bool dependent, cudaStr
     a.part_ml = s.part_ml;
     a.gr = s.gr;
     a.slots = s.slots;
+    a.info = s.info;
+    a.prefix_parts = s.slots - s.own;
     if (prefix) {
         const int rows = shared_rows(s.dtype, s.D, s.H, s.HK, s.batch, s.gr.n);
         const long long units = shared_units(rows, s.H, s.HK, s.batch, s.gr.n);

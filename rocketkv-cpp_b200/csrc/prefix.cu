@@ -6,9 +6,9 @@
 // (largest score, sum 2^(x - m), sum 2^(x - m) v) with x = q k log2(e) / sqrt(D),
 // join as (M, sum l 2^(m - M), sum o 2^(m - M)).  A group's shared rows of K and V
 // meet the queries of all its sequences at once, so they are read once and
-// not once per sequence.  Three kernels: the shared tokens, every sequence's own
-// (both of paged.cu, or the former on the tcgen05 tensor cores, prefix_tc.cu),
-// and the join.
+// not once per sequence.  Three kernels: every sequence's own tokens, the
+// shared ones (both of paged.cu, or the latter on the tcgen05 tensor cores,
+// prefix_tc.cu) and the join, each begun while the one before still runs.
 #include "prefix.cuh"
 
 namespace rkv {
@@ -37,41 +37,29 @@ __device__ __forceinline__ void put4(__half* o, const float4& v) {
     reinterpret_cast<__half2*>(o)[1] = __floats2half2_rn(v.z, v.w);
 }
 
-constexpr int kJoinRows = 4;  // rows of a CTA, a warp each
+constexpr int kJoinWarps = 8;  // of a CTA, which joins one row
+constexpr int kJoinAhead = 4;  // parts of a warp that are on their way together
 
 // Joins the parts of a row: those of its own tokens, then those of the shared
 // ones, in their order whatever the grid.  O is rounded to Q's type, once.
 template <typename T, bool TC>
-__global__ void __launch_bounds__(kJoinRows * 32) prefix_join_kernel(const JoinArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const JoinArgs a) {
     const SharedArgs& s = a.s;
-    const int lane = threadIdx.x & 31;
-    const long long rows = (long long)s.batch * s.H, row = (long long)blockIdx.x * kJoinRows + (threadIdx.x >> 5);
-    const int b = row < rows ? (int)(row / s.H) : 0;
-    const int n = paged_len(s.c, b, s.gr.max_len);
-    const Member m = member_of(s.gr, s.c, b, n);
-    const int mine = n - m.tokens;
-    const int own = mine > 0 ? (mine + part_tokens(mine, s.own) - 1) / part_tokens(mine, s.own) : 0;
-    int shared = 0;
-    long long later = 0;  // TC: the row of the second part
-    if (m.tokens > 0 && !TC) {
-        const int t = part_tokens(m.tokens, s.slots - s.own);
-        shared = (m.tokens + t - 1) / t;
-    }
-    if (m.tokens > 0 && TC) {
-        // the CTAs whose stretches hold tiles of this row's unit: one has the first, the others begin inside the unit
-        const int G = s.H / s.HK, h = (int)(row % s.H);
-        const TcGroup t = tc_group(s.gr, s.c, m.group, G, kTcRows);
-        const int r = (b - s.gr.start(m.group)) * G + h % G;
-        const long long t0 = tc_tiles(s.gr, s.c, m.group, G, s.HK, kTcRows) + ((long long)(h / G) * t.units + r / kTcRows) * t.tiles;
-        const TcCut k = tc_cut(tc_tiles(s.gr, s.c, s.gr.n, G, s.HK, kTcRows), kTcSms);
-        // CTA c begins at floor(tiles c / ctas)
-        const long long c0 = ((t0 + 1) * k.ctas + k.tiles - 1) / k.tiles, c1 = ((t0 + t.tiles) * k.ctas + k.tiles - 1) / k.tiles;
-        shared = 1 + (int)(c1 - c0);
-        later = c0 * kTcRows + r % kTcRows;
-    }
+    constexpr int W = kJoinWarps, U = kJoinAhead;
+    __shared__ float4 sums[W][64];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long row = blockIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (a.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.clear = 0;
-    if (row >= rows) return;
+    const int2 info = s.info[row];
+    const int own = info.x;
+    int shared = info.y;
+    long long later = 0;  // TC: the row of the second part
+    if (TC) {
+        const int2 x = a.tc.first_later[row];  // not written where the row has no shared tokens
+        if (shared > 0) shared += x.x;
+        later = x.y;
+    }
     // part i: own ones in the slots from 0; shared ones in those from s.own, or where the tcgen05 kernel leaves them
     const int parts = own + shared;
     auto ml_of = [&](int i) -> float2 {
@@ -82,50 +70,67 @@ __global__ void __launch_bounds__(kJoinRows * 32) prefix_join_kernel(const JoinA
         if (i < own || !TC) return s.part_o + (row * s.slots + (i < own ? i : s.own + (i - own))) * s.D;
         return i == own ? a.tc.first_o + row * s.D : a.tc.later_o + (later + (long long)(i - own - 1) * kTcRows) * s.D;
     };
+    // warp w takes the parts w, w + W, ...; its first rows are on their way while the weights are formed
+    const int c0 = lane * 4, c1 = c0 + 128;
+    float4 x[U], y[U];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * W;
+            x[u] = y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i < parts) {
+                const float* p = o_of(i);
+                if (c0 < s.D) x[u] = *reinterpret_cast<const float4*>(p + c0);
+                if (c1 < s.D) y[u] = *reinterpret_cast<const float4*>(p + c1);
+            }
+        }
+    };
+    fetch(warp);
     float top = -INFINITY;
     for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml_of(i).x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float base = top == -INFINITY ? 0.0f : top;
     float l = 0.0f;
-    float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-    const int c0 = lane * 4, c1 = c0 + 128;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-        float w = 0.0f;
-        if (i0 + lane < parts) {
-            const float2 x = ml_of(i0 + lane);
-            w = exp2f(x.x - base);
-            l = fmaf(x.y, w, l);
-        }
-        const int here = min(32, parts - i0);
-#pragma unroll 4
-        for (int i = 0; i < here; ++i) {
-            const float f = __shfl_sync(0xffffffffu, w, i);
-            const float* p = o_of(i0 + i);
-            if (c0 < s.D) {
-                const float4 v = *reinterpret_cast<const float4*>(p + c0);
-                o[0] = make_float4(fmaf(v.x, f, o[0].x), fmaf(v.y, f, o[0].y), fmaf(v.z, f, o[0].z), fmaf(v.w, f, o[0].w));
-            }
-            if (c1 < s.D) {
-                const float4 v = *reinterpret_cast<const float4*>(p + c1);
-                o[1] = make_float4(fmaf(v.x, f, o[1].x), fmaf(v.y, f, o[1].y), fmaf(v.z, f, o[1].z), fmaf(v.w, f, o[1].w));
-            }
-        }
+    for (int i = lane; i < parts; i += 32) {
+        const float2 v = ml_of(i);
+        l = fmaf(v.y, exp2f(v.x - base), l);
     }
 #pragma unroll
-    for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* out = static_cast<T*>(a.O) + row * s.D;
-    if (c0 < s.D) put4(out + c0, make_float4(o[0].x * inv, o[0].y * inv, o[0].z * inv, o[0].w * inv));
-    if (c1 < s.D) put4(out + c1, make_float4(o[1].x * inv, o[1].y * inv, o[1].z * inv, o[1].w * inv));
-    if (lane == 0 && a.lse) a.lse[row] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945f;
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    float4 o0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o1 = o0;
+    for (int i0 = warp; i0 < parts; i0 += U * W) {
+        if (i0 != warp) fetch(i0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * W;
+            const float f = i < parts ? exp2f(ml_of(i).x - base) : 0.0f;
+            o0 = make_float4(fmaf(x[u].x, f, o0.x), fmaf(x[u].y, f, o0.y), fmaf(x[u].z, f, o0.z), fmaf(x[u].w, f, o0.w));
+            o1 = make_float4(fmaf(y[u].x, f, o1.x), fmaf(y[u].y, f, o1.y), fmaf(y[u].z, f, o1.z), fmaf(y[u].w, f, o1.w));
+        }
+    }
+    sums[warp][lane] = o0;
+    sums[warp][lane + 32] = o1;
+    __syncthreads();
+    const int c = threadIdx.x * 4;
+    if (c < s.D) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        float4 o = sums[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            const float4 v = sums[w][threadIdx.x];
+            o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+        }
+        put4(static_cast<T*>(a.O) + row * s.D + c, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    }
+    if (threadIdx.x == 0 && a.lse) a.lse[row] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945f;
 }
 
 template <typename T>
 int launch_join(const JoinArgs& a, cudaStream_t st) {
-    const long long blocks = ((long long)a.s.batch * a.s.H + kJoinRows - 1) / kJoinRows;
-    const cudaError_t e = a.tc.first_o ? launch_pdl(prefix_join_kernel<T, true>, dim3((unsigned)blocks), dim3(kJoinRows * 32), 0, st, a)
-                                       : launch_pdl(prefix_join_kernel<T, false>, dim3((unsigned)blocks), dim3(kJoinRows * 32), 0, st, a);
+    const dim3 grid((unsigned)(a.s.batch * a.s.H)), block(kJoinWarps * 32);
+    const cudaError_t e = a.tc.first_o ? launch_pdl(prefix_join_kernel<T, true>, grid, block, 0, st, a)
+                                       : launch_pdl(prefix_join_kernel<T, false>, grid, block, 0, st, a);
     if (e != cudaSuccess) (void)cudaGetLastError();
     return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }
@@ -140,19 +145,20 @@ int prefix_check(int dtype, int H, int HK, int D, int max_len, int batch, int gr
 
 // The shared tokens on the tcgen05 tensor cores: 16-bit types where a group of mean size has more rows of a KV head
 // than two CTAs of the matrix-instruction kernel take.
-bool on_tc(int dtype, int H, int HK, int D, int batch, int groups) {
-    return dtype != RKV_F32 && D <= 128 && (long long)batch * (H / HK) > 16LL * groups;
+bool on_tc(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
+    const double tiles = ((double)groups + (double)batch * (H / HK) / kTcRows) * HK * ((double)max_len / kTcKeys + 1);
+    return dtype != RKV_F32 && D <= 128 && (long long)batch * (H / HK) > 16LL * groups && tiles < 1e9;  // counted in 32 bits
 }
 
 struct PrefixPlan {
     bool tc;
     int own, slots;
-    size_t off_ml, off_o, off_first_ml, off_first_o, off_later_ml, off_later_o, bytes;
+    size_t off_ml, off_o, off_info, off_first, off_first_ml, off_first_o, off_later_ml, off_later_o, bytes;
 };
 PrefixPlan prefix_plan(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
     PrefixPlan p{};
     const bool any = groups > 0 && batch > 0;
-    p.tc = any && on_tc(dtype, H, HK, D, batch, groups);
+    p.tc = any && on_tc(dtype, H, HK, D, max_len, batch, groups);
     p.own = shared_own_parts(dtype, H, HK, D, max_len, batch);
     p.slots = p.own + (any && !p.tc ? shared_prefix_parts(dtype, H, HK, D, max_len, batch, groups) : 0);
     size_t off = kWorkspaceHeader;
@@ -163,7 +169,11 @@ PrefixPlan prefix_plan(int dtype, int H, int HK, int D, int max_len, int batch, 
         off = align_up(off + rows * D * sizeof(float), kWorkspaceAlign);
     };
     take(p.off_ml, p.off_o, (size_t)batch * H * p.slots);
+    p.off_info = off;
+    off = align_up(off + (size_t)batch * H * sizeof(int2), kWorkspaceAlign);
     if (p.tc) {
+        p.off_first = off;
+        off = align_up(off + (size_t)batch * H * sizeof(int2), kWorkspaceAlign);
         take(p.off_first_ml, p.off_first_o, (size_t)batch * H);
         take(p.off_later_ml, p.off_later_o, (size_t)kTcSms * kTcRows);
     }
@@ -214,20 +224,22 @@ extern "C" int rkv_prefix_decode(const void* Q, long long q_item_stride, int num
     s.slots = p.slots;
     s.part_ml = reinterpret_cast<float2*>(ws + p.off_ml);
     s.part_o = reinterpret_cast<float*>(ws + p.off_o);
+    s.info = reinterpret_cast<int2*>(ws + p.off_info);
     a.O = O;
     a.lse = lse;
+    rc = launch_shared_pass(s, false, false, st);
     if (p.tc) {
+        a.tc.first_later = reinterpret_cast<int2*>(ws + p.off_first);
         a.tc.first_ml = reinterpret_cast<float2*>(ws + p.off_first_ml);
         a.tc.first_o = reinterpret_cast<float*>(ws + p.off_first_o);
         a.tc.later_ml = reinterpret_cast<float2*>(ws + p.off_later_ml);
         a.tc.later_o = reinterpret_cast<float*>(ws + p.off_later_o);
         a.tc.err = static_cast<int*>(workspace);
-        rc = launch_prefix_tc(s, a.tc, st);
+        if (!rc) rc = launch_prefix_tc(s, a.tc, st);
     } else {
         a.clear = static_cast<int*>(workspace);
-        if (num_groups > 0) rc = launch_shared_pass(s, true, false, st);
+        if (!rc && num_groups > 0) rc = launch_shared_pass(s, true, true, st);
     }
-    if (!rc) rc = launch_shared_pass(s, false, num_groups > 0, st);
     if (rc) return rc;
     return s.dtype == RKV_F32 ? launch_join<float>(a, st) : s.dtype == RKV_BF16 ? launch_join<__nv_bfloat16>(a, st) : launch_join<__half>(a, st);
 }

@@ -32,17 +32,17 @@ __device__ __forceinline__ Member member_of(const Groups& gr, const PagedView& c
     Member m{-1, 0};
     for (int g0 = 0; g0 < gr.n; g0 += 32) {
         const int g = g0 + lane;
-        const bool hit = g < gr.n && gr.start(g) <= b && b < gr.start(g + 1);
-        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+        const bool some = g < gr.n;
+        const int lo = some ? gr.start(g) : 0, hi = some ? gr.start(g + 1) : 0, p = some ? gr.shared(c, g) : 0;
+        const unsigned hits = __ballot_sync(0xffffffffu, lo <= b && b < hi);
         if (hits) {
-            m.group = g0 + __ffs(hits) - 1;
+            const int l = __ffs(hits) - 1;
+            m.group = g0 + l;
+            m.tokens = __shfl_sync(0xffffffffu, p, l);
             break;
         }
     }
-    if (m.group >= 0) {
-        const int p = gr.shared(c, m.group);
-        if (p <= n) m.tokens = p;
-    }
+    if (m.tokens > n) m.tokens = 0;
     return m;
 }
 // The sequence through whose table row a group's shared tokens are read: the first that holds them all.  A whole
@@ -66,7 +66,7 @@ __host__ __device__ __forceinline__ int part_tokens(int tokens, int splits) {
 
 // What the passes leave: part s of row (sequence b, query head h) at ((b H + h) slots + s), o [D] not divided by l,
 // and (m, l) in base 2.  Own tokens take the slots 0 .. own - 1, shared ones the others (where the matrix-instruction
-// kernel of paged.cu attends them).
+// kernel of paged.cu attends them).  info[row]: its parts of own tokens, and of shared ones (tcgen05: 1 for any).
 struct SharedArgs {
     PagedView c;
     Groups gr;
@@ -76,20 +76,23 @@ struct SharedArgs {
     int own, slots;
     float* part_o;
     float2* part_ml;
+    int2* info;
 };
 // Parts of every sequence's own tokens, and of every group's shared ones for the matrix-instruction kernel.
 int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch);
 int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups);
-// One pass: prefix, the groups' shared tokens; else every sequence's own.  dependent: launched while the kernel
-// before it still runs.
+// One pass: prefix, the groups' shared tokens; else every sequence's own.  dependent: launched while the pass before
+// it still runs, which it waits for at its end only.
 int launch_shared_pass(const SharedArgs& s, bool prefix, bool dependent, cudaStream_t st);
 
-// The shared tokens on the tcgen05 tensor cores (prefix_tc.cu): 16-bit types.  The tiles of all units -- a unit is up
-// to 256 rows (128 above 128 columns) of one group and KV head -- are cut into equal stretches, one per CTA.  A unit's first
-// stretch leaves its rows in `first` (row b H + h), a stretch that begins inside a unit in `later` (256 rows per CTA).
+// The shared tokens on the tcgen05 tensor cores (prefix_tc.cu): 16-bit types.  A unit is up to 256 rows of one group
+// and KV head; the tiles of the units are cut into stretches, one or more per CTA.  A unit's first stretch leaves its
+// rows in first (row b H + h), a stretch that begins inside a unit in later (256 rows per CTA).  first_later[row]: how
+// many stretches follow the first one, and the row of the first of them in later; the others' are 256 further each.
 struct TcParts {
     float* first_o;
     float2* first_ml;
+    int2* first_later;
     float* later_o;
     float2* later_ml;
     int* err;
@@ -97,44 +100,6 @@ struct TcParts {
 constexpr int kTcSms = 148;
 constexpr int kTcKeys = 128;
 constexpr int kTcRows = 256;
-constexpr int kTcMinTiles = 2;  // of a stretch
-
-// Tiles of all units, and the CTAs that take them.
-struct TcCut {
-    long long tiles;
-    int ctas;
-    __device__ __forceinline__ long long begin(int c) const { return tiles * c / ctas; }
-};
-// Rows of a group and KV head, its units and the tiles of one.
-struct TcGroup {
-    int rows, units, tiles;
-};
-__device__ __forceinline__ TcGroup tc_group(const Groups& gr, const PagedView& c, int g, int G, int unit_rows) {
-    TcGroup t;
-    t.rows = gr.size(g) * G;
-    t.units = (t.rows + unit_rows - 1) / unit_rows;
-    t.tiles = (gr.shared(c, g) + kTcKeys - 1) / kTcKeys;
-    return t;
-}
-// Tiles of the groups before g (all: g = gr.n).  A whole warp calls.
-__device__ __forceinline__ long long tc_tiles(const Groups& gr, const PagedView& c, int g, int G, int HK, int unit_rows) {
-    const int lane = threadIdx.x & 31;
-    long long n = 0;
-    for (int i = lane; i < g; i += 32) {
-        const TcGroup t = tc_group(gr, c, i, G, unit_rows);
-        n += (long long)t.units * t.tiles * HK;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    return n;
-}
-__device__ __forceinline__ TcCut tc_cut(long long tiles, int most) {
-    TcCut k;
-    k.tiles = tiles;
-    const long long n = (tiles + kTcMinTiles - 1) / kTcMinTiles;
-    k.ctas = n < most ? (n < 1 ? 1 : (int)n) : most;
-    return k;
-}
 int launch_prefix_tc(const SharedArgs& s, const TcParts& p, cudaStream_t st);
 
 }  // namespace rkv

@@ -15,8 +15,8 @@
 //   warp 4       issues the products
 //   warps 8-11, 12-15   softmax of the first accumulator, of the second, and their rows
 //
-// The tiles of all units are one long list that is cut into equal stretches, one
-// per CTA: whatever the groups' sizes and lengths, every SM has the same work.
+// The tiles of the units are cut into stretches so that, whatever the groups'
+// sizes and lengths, every SM has about the same work.
 // Each stretch leaves (m, l, O) of its rows, not divided by l, for the join.
 //
 // P is rounded to 16 bits (half a step of the type, as the products take both
@@ -32,9 +32,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kBlk = 128 * 128;  // bytes of a 128-row block of 64 columns
 constexpr int kMasks = 16;       // tiles whose masks are kept: more than the copies are ahead of the softmax
-constexpr int kLag = 2;          // ring slots whose copies are on their way when the next is begun
 
-__host__ __device__ constexpr int ring_slots(int kb) { return kb == 1 ? 8 : 4; }  // of a K or a V tile
+__host__ __device__ constexpr int ring_slots(int kb) { return kb == 1 ? 8 : 5; }  // of a K or a V tile
 
 struct Args {
     SharedArgs s;
@@ -44,7 +43,7 @@ struct Args {
 };
 
 struct Bars {
-    uint64_t q_empty, o_full, o_empty, drained;
+    uint64_t o_full, o_empty, written, drained;
     uint64_t s_full[2], p_half[2], p_ready[2];  // of an accumulator
     uint64_t full[8], empty[8];
     uint32_t mask[kMasks][4];
@@ -54,50 +53,116 @@ struct Bars {
 static_assert(sizeof(Bars) <= 1024, "the barriers' part of shared memory");
 
 // A CTA's part of a unit: rows row0 .. row0 + rows - 1 of group g (whose first sequence is s0) and KV head hk, and
-// `tiles` tiles from tile j0 on of its `shared` tokens.
+// `tiles` tiles from tile j0 on of its `shared` tokens; from tile 0: how many CTAs behind this one have the others.
 struct Stretch {
-    int g, hk, s0, row0, rows, shared, j0, tiles;
+    int g, hk, s0, row0, rows, shared, j0, tiles, behind;
 };
-// The stretches of CTA c, which every warp of it walks on its own.
+// Rows of a group and KV head, the group's units (of all KV heads) and the tiles of one.
+struct Group {
+    int rows, per_head, units, tiles;
+};
+__device__ __forceinline__ Group group_of(const Args& a, int g) {
+    Group t{0, 0, 0, 0};
+    if (g < a.s.gr.n) {
+        t.rows = a.s.gr.size(g) * a.G;
+        t.per_head = (t.rows + kTcRows - 1) / kTcRows;
+        t.units = t.per_head * a.s.HK;
+        t.tiles = (a.s.gr.shared(a.s.c, g) + kTcKeys - 1) / kTcKeys;
+    }
+    return t;
+}
+// The stretches of this CTA, which every warp of it walks on its own.  Either each unit is cut into as many equal
+// stretches as its share of the tiles is worth CTAs, one per CTA; or, where that needs more CTAs than there are or
+// leaves one kAligned tiles more to do than an equal share, the tiles of all units are one list that is cut into
+// equal stretches: a CTA whose stretch spans two units pays the ends of a unit (4 us) twice.
+constexpr int kAligned = 3;
+constexpr int kMinTiles = 2;  // of a stretch
 struct Walk {
-    long long at, end;
+    int total, ctas;  // tiles, CTAs that take them
+    int at, end;      // this CTA's; aligned: one stretch
+    bool aligned;
+
+    __device__ __forceinline__ int parts(const Group& t) const {  // aligned: of a unit
+        return max(1, min((int)((unsigned)ctas * t.tiles / (unsigned)total), t.tiles / kMinTiles));
+    }
     __device__ __forceinline__ Walk(const Args& a) {
-        const TcCut k = tc_cut(tc_tiles(a.s.gr, a.s.c, a.s.gr.n, a.G, a.s.HK, kTcRows), gridDim.x);
-        const int c = blockIdx.x;
+        const int lane = threadIdx.x & 31;
+        int n = 0;
+        for (int g = lane; g < a.s.gr.n; g += 32) {
+            const Group t = group_of(a, g);
+            n += t.units * t.tiles;
+        }
+        total = __reduce_add_sync(0xffffffffu, n);
+        ctas = gridDim.x;
         at = end = 0;
-        if (c < k.ctas) at = k.begin(c), end = k.begin(c + 1);
+        aligned = true;
+        if (total > 0) {
+            int need = 0, most = 0;
+            for (int g = lane; g < a.s.gr.n; g += 32) {
+                const Group t = group_of(a, g);
+                if (t.units > 0 && t.tiles > 0) {
+                    const int p = parts(t);
+                    need += t.units * p;
+                    most = max(most, (t.tiles + p - 1) / p);
+                }
+            }
+            need = __reduce_add_sync(0xffffffffu, need);
+            most = __reduce_max_sync(0xffffffffu, most);
+            aligned = need <= ctas && (most <= kMinTiles + 1 || most <= (total + ctas - 1) / ctas + kAligned);
+            const int c = blockIdx.x;
+            if (aligned) {
+                end = c < need;
+            } else {
+                ctas = min(ctas, (total + kMinTiles - 1) / kMinTiles);
+                if (c < ctas) at = begin(c), end = begin(c + 1);
+            }
+        }
+    }
+    // One list: the first total % ctas CTAs have a tile more than the others.
+    __device__ __forceinline__ int begin(int c) const { return total / ctas * c + min(c, total % ctas); }
+    __device__ __forceinline__ int cta_of(int tile) const {
+        const int q = total / ctas, r = total % ctas, cut = (q + 1) * r;
+        return tile < cut ? tile / (q + 1) : r + (tile - cut) / q;
     }
     __device__ __forceinline__ bool next(const Args& a, Stretch& x) {
         if (at >= end) return false;
-        const int lane = threadIdx.x & 31;
-        long long base = 0;
+        const int lane = threadIdx.x & 31, want = aligned ? (int)blockIdx.x : at;
+        int base = 0;
         for (int g0 = 0; g0 < a.s.gr.n; g0 += 32) {
-            TcGroup t{0, 0, 0};
-            if (g0 + lane < a.s.gr.n) t = tc_group(a.s.gr, a.s.c, g0 + lane, a.G, kTcRows);
-            const long long mine = (long long)t.units * t.tiles * a.s.HK;
-            long long sum = mine;
+            const Group t = group_of(a, g0 + lane);
+            const int p = aligned && t.units > 0 && t.tiles > 0 ? parts(t) : 0;
+            const int mine = t.units * (aligned ? p : t.tiles);
+            int sum = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+                const int y = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += y;
             }
-            const unsigned hits = __ballot_sync(0xffffffffu, at < base + sum);
+            const unsigned hits = __ballot_sync(0xffffffffu, want < base + sum);
             if (hits) {
                 const int l = __ffs(hits) - 1;
                 x.g = g0 + l;
-                base += __shfl_sync(0xffffffffu, sum - mine, l);
-                const int units = __shfl_sync(0xffffffffu, t.units, l), tiles = __shfl_sync(0xffffffffu, t.tiles, l);
-                const int rows = __shfl_sync(0xffffffffu, t.rows, l);
-                const long long off = at - base;
-                const int unit = (int)(off / tiles);  // the units of a KV head side by side: they read the same tiles
-                x.j0 = (int)(off - (long long)unit * tiles);
-                x.hk = unit / units;
-                x.row0 = (unit - x.hk * units) * kTcRows;
+                const int off = want - base - __shfl_sync(0xffffffffu, sum - mine, l);
+                const int per_head = __shfl_sync(0xffffffffu, t.per_head, l), tiles = __shfl_sync(0xffffffffu, t.tiles, l);
+                const int rows = __shfl_sync(0xffffffffu, t.rows, l), parts = __shfl_sync(0xffffffffu, p, l);
+                const int unit = off / (aligned ? parts : tiles);  // the units of a KV head side by side: they read the same tiles
+                const int in = off - unit * (aligned ? parts : tiles);
+                x.hk = unit / per_head;
+                x.row0 = (unit - x.hk * per_head) * kTcRows;
                 x.rows = min(kTcRows, rows - x.row0);
-                x.tiles = (int)min((long long)(tiles - x.j0), end - at);
                 x.s0 = a.s.gr.start(x.g);
                 x.shared = a.s.gr.shared(a.s.c, x.g);
-                at += x.tiles;
+                if (aligned) {
+                    x.j0 = (int)((unsigned)tiles * in / (unsigned)parts);
+                    x.tiles = (int)((unsigned)tiles * (in + 1) / (unsigned)parts) - x.j0;
+                    x.behind = parts - 1;
+                    at = end;
+                } else {
+                    x.j0 = in;
+                    x.tiles = min(tiles - in, end - at);
+                    x.behind = in == 0 ? cta_of(at + tiles - 1) - (int)blockIdx.x : 0;
+                    at += x.tiles;
+                }
                 return true;
             }
             base += __shfl_sync(0xffffffffu, sum, 31);
@@ -109,18 +174,38 @@ struct Walk {
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
+// Whether the phase has ended, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // A warp's 32 rows of KB blocks of 64 columns into a swizzled tile at dst (this warp's first row): off is this lane's
 // row's offset from src, or -1 for a row of zeros; columns from `chunks` 16-byte chunks on are zeros.
 template <int KB>
 __device__ __forceinline__ void copy_rows(uint32_t dst, const uint8_t* src, long long off, int chunks, int lane) {
     constexpr int LPR = KB * 8, RPI = 32 / LPR;  // lanes of a row, rows of an instruction
     const int c = lane % LPR, r0 = lane / LPR;
+    constexpr int U = 8;  // rows whose places are asked for together
+    src += c * 16;
+    dst += (c >> 3) * kBlk + r0 * 128;
 #pragma unroll
-    for (int i = 0; i < 32 / RPI; ++i) {
-        const int r = i * RPI + r0;
-        const long long o = __shfl_sync(0xffffffffu, off, r);
-        const bool real = o >= 0 && c < chunks;
-        copy16(dst + (c >> 3) * kBlk + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (real ? o + c * 16 : 0), real);
+    for (int i0 = 0; i0 < 32 / RPI; i0 += U) {
+        long long o[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) o[i] = __shfl_sync(0xffffffffu, off, (i0 + i) * RPI + r0);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int r = (i0 + i) * RPI;
+            const bool real = o[i] >= 0 && c < chunks;
+            copy16(dst + r * 128 + (((c & 7) ^ ((r + r0) & 7)) << 4), src + (real ? o[i] : -16 * c), real);
+        }
     }
 }
 
@@ -147,20 +232,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
     constexpr uint32_t kOne = KB * kBlk;
     constexpr uint32_t kColO = 256;  // tensor memory: S0, S1 (128 columns each), O0, O1 (64 KB each)
     extern __shared__ uint8_t smem_raw[];
-    asm volatile("griddepcontrol.launch_dependents;");  // the passes behind may be scheduled (they wait for this grid)
+    asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled (it waits for this grid)
     uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     Bars& B = *reinterpret_cast<Bars*>(sm);
     volatile int* abort_flag = &B.abort;
     int* err = a.p.err;
     uint8_t* sq = sm + 1024;
     uint8_t* ring = sq + 2 * kOne;
-    uint8_t* stage = ring + NS * kOne;  // 4 KB per softmax warp
+    uint8_t* stage = sq + 2 * kOne - 8 * 4096;  // 4 KB per softmax warp, in Q's place once its products have ended
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        mbar_init(&B.q_empty, 1);
         mbar_init(&B.o_full, 1);
         mbar_init(&B.o_empty, 8);
+        mbar_init(&B.written, 8);
         mbar_init(&B.drained, 1);
         for (int u = 0; u < 2; ++u) {
             mbar_init(&B.s_full[u], 1);
@@ -184,35 +269,46 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
     Walk walk(a);
     Stretch x;
 
-    // (48 + 48 + 208 + 208) * 128 registers are the 128 * 512 of the launch
+    // (56 + 40 + 208 + 208) * 128 registers are the 128 * 512 of the launch
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         const int chunks = a.s.D / 8;
         int q = 0, nq = 0, nk = 0, open = 0;  // slots, stretches, tiles; slots begun whose copies are not known to have landed
         bool ok = true;
-        auto landed = [&](int pending) {  // all but the last `pending` slots
-            while (open > pending) {
-                if (open == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-                else if (open == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-                else asm volatile("cp.async.wait_group 0;" ::: "memory");
-                fence_proxy_async();  // the products read what was copied through another proxy
-                __syncwarp();
-                if (lane == 0) mbar_arrive1(&B.full[(q - open) % NS]);
-                --open;
+        auto landed = [&]() {  // the oldest slot
+            switch (open) {
+                case 8: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
+                case 7: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
+                case 6: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+                case 5: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+                case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+                case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+                case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+                default: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
             }
+            fence_proxy_async();  // the products read what was copied through another proxy
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(&B.full[(q - open) % NS]);
+            --open;
         };
         auto slot = [&](const uint8_t* base, long long off) {
             const int s = q % NS;
-            if (q >= NS && !(ok = warp_wait(&B.empty[s], (uint32_t)((q / NS - 1) & 1), err, abort_flag))) return;
-            copy_rows<KB>(smem_u32(ring) + s * kOne + warp * 4096, base, off, chunks, lane);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            ++q;
-            ++open;
-            landed(kLag);
+            if (q >= NS) {
+                // while the slot is not free, those on their way are handed over as they land
+                const uint32_t parity = (uint32_t)((q / NS - 1) & 1);
+                while (open > 0 && !__all_sync(0xffffffffu, mbar_test(&B.empty[s], parity))) landed();
+                ok = warp_wait(&B.empty[s], parity, err, abort_flag);
+            }
+            if (ok) {
+                copy_rows<KB>(smem_u32(ring) + s * kOne + warp * 4096, base, off, chunks, lane);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                ++q;
+                ++open;
+            }
         };
         while (ok && walk.next(a, x)) {
             const int leader = leader_of(a.s.gr, a.s.c, x.g, x.shared);
-            if (nq > 0 && !(ok = warp_wait(&B.q_empty, (uint32_t)((nq - 1) & 1), err, abort_flag))) break;
+            if (nq > 0 && !(ok = warp_wait(&B.written, (uint32_t)((nq - 1) & 1), err, abort_flag))) break;
             ++nq;
             // Q's rows go with the first K tile
             for (int u = 0; u < (x.rows > 128 ? 2 : 1); ++u) {
@@ -231,11 +327,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
                 slot(a.s.c.K, off);
                 if (ok) slot(a.s.c.V, off);
             }
-            if (ok) landed(0);
+            while (ok && open > 0) landed();
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 4) {
             const uint32_t ids = mma_idesc(BF ? 1u : 0u, kTcKeys);
             const uint32_t idv = mma_idesc(BF ? 1u : 0u, KB * 64) | (1u << 16);  // B with N contiguous
@@ -244,24 +340,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
             int q = 0, nq = 0;
             uint32_t steps = 0;  // a bit per accumulator: parity of its steps
             bool ok = true;
-            auto wait = [&](uint64_t* bar, int n) { return ok = warp_wait(bar, (uint32_t)(n & 1), err, abort_flag); };
+            auto wait = [&](uint64_t* bar, int n) { ok = ok && warp_wait(bar, (uint32_t)(n & 1), err, abort_flag); };
             while (ok && walk.next(a, x)) {
                 // step k: accumulator k & 1 and the next tile, or both accumulators one after the other with each tile
                 const bool both = x.rows > 128;
                 const int n = both ? 2 * x.tiles : x.tiles;
                 auto scores = [&](int k) {
                     const int u = k & 1, at = q + 2 * (both ? k >> 1 : k), s = at % NS;
-                    if (!(both && u) && !wait(&B.full[s], at / NS)) return;
-                    tc_fence_after();
-                    const uint64_t da = qd + (uint32_t)((both ? u : 0) * (kOne >> 4)), db = kd + (uint32_t)(s * (kOne >> 4));
+                    if (!(both && u)) wait(&B.full[s], at / NS);
+                    if (ok) {
+                        tc_fence_after();
+                        const uint64_t da = qd + (uint32_t)((both ? u : 0) * (kOne >> 4)), db = kd + (uint32_t)(s * (kOne >> 4));
 #pragma unroll
-                    for (int ks = 0; ks < KB * 4; ++ks) {
-                        const uint32_t o = ((ks >> 2) * kBlk + (ks & 3) * 32) >> 4;
-                        mma_ss(tbase + u * 128, da + o, db + o, ids, ks > 0);
+                        for (int ks = 0; ks < KB * 4; ++ks) {
+                            const uint32_t o = ((ks >> 2) * kBlk + (ks & 3) * 32) >> 4;
+                            mma_ss(tbase + u * 128, da + o, db + o, ids, ks > 0);
+                        }
+                        mma_commit_w(&B.s_full[u]);
+                        if (!both || u) mma_commit_w(&B.empty[s]);
                     }
-                    mma_commit_w(&B.s_full[u]);
-                    if (!both || u) mma_commit_w(&B.empty[s]);
-                    if (k == n - 1) mma_commit_w(&B.q_empty);
                 };
                 scores(0);
                 if (ok && n > 1) scores(1);
@@ -269,11 +366,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
                 ++nq;
                 for (int k = 0; k < n && ok; ++k) {
                     const int u = k & 1, at = q + 2 * (both ? k >> 1 : k) + 1, s = at % NS;
-                    if (!(both && u) && !wait(&B.full[s], at / NS)) break;
+                    if (!(both && u)) wait(&B.full[s], at / NS);
                     const uint64_t db = vd + (uint32_t)(s * (kOne >> 4));
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        if (!wait(half ? &B.p_ready[u] : &B.p_half[u], (int)(steps >> u))) break;
+                        wait(half ? &B.p_ready[u] : &B.p_half[u], (int)(steps >> u));
+                        if (!ok) break;
                         tc_fence_after();
 #pragma unroll
                         for (int ks = half * 4; ks < half * 4 + 4; ++ks)
@@ -377,11 +475,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
             if (!ok || !(ok = warp_wait(&B.o_full, (uint32_t)(nq & 1), err, abort_flag))) break;
             tc_fence_after();
             const bool first = x.j0 == 0;
+            if (first && r < x.rows && (both || u == 0)) {
+                const unsigned of = x.row0 + r, sq_ = of / (unsigned)a.G;
+                a.p.first_later[(long long)(x.s0 + (int)sq_) * a.s.H + x.hk * a.G + (int)(of - sq_ * a.G)] =
+                    make_int2(x.behind, (int)(blockIdx.x + 1) * kTcRows + r);
+            }
             nk += x.tiles;
             ++nq;
             if (!some) {
                 tc_fence_before();
-                if (lane == 0) mbar_arrive1(&B.o_empty);
+                if (lane == 0) {
+                    mbar_arrive1(&B.o_empty);
+                    mbar_arrive1(&B.written);
+                }
                 continue;
             }
             // this row's place
@@ -407,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
                 const long long place = at >= 0 ? at * a.s.D : -1;
 #pragma unroll
                 for (int c = 0; c < KB * 2; ++c) write_cols(so, o + c * 32, po, place, c * 32, a.s.D, lane);
+                if (lane == 0) mbar_arrive1(&B.written);
                 continue;
             }
             // the two accumulators hold the same rows: each softmax takes half of the columns of their sum
@@ -443,18 +550,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
                 }
                 write_cols(so, o, po, place, col, a.s.D, lane);
             }
+            if (lane == 0) mbar_arrive1(&B.written);
         }
         tc_fence_before();
     }
     __syncthreads();
     tc_fence_after();
     if (warp == 4) tmem_dealloc(tbase, 512);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the pass before has ended too once this one has
 }
 
 template <int KB, bool BF>
 int launch(const Args& a, cudaStream_t st) {
-    // the barriers, and up to 1023 bytes of alignment; Q and the ring; the rows' stage
-    const int smem = 2048 + (2 + ring_slots(KB)) * KB * kBlk + 8 * 4096;
+    // the barriers, and up to 1023 bytes of alignment; Q and the ring
+    const int smem = 2048 + (2 + ring_slots(KB)) * KB * kBlk;
     // the split of the registers is the launch's only where the kernel was compiled to 128 a thread
     static const bool fits = [] {
         cudaFuncAttributes f;
@@ -467,8 +576,9 @@ int launch(const Args& a, cudaStream_t st) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
-    prefix_tc_kernel<KB, BF><<<kTcSms, kThreads, smem, st>>>(a);
-    return launched();
+    const cudaError_t e = launch_pdl(prefix_tc_kernel<KB, BF>, dim3(kTcSms), dim3(kThreads), smem, st, a);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }
 
 }  // namespace
