@@ -152,8 +152,8 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 
 // Joins the warps' (m, l, o) of ng heads from shared memory (ms, ls [warps][rows], os [warps][rows][pitch])
 // and writes the part, or the output where there is one part.
-template <int W, int PASS, typename Head>
-__device__ __forceinline__ void merge_warps(const DecodeArgs& a, Head head_of, int ng, int split, const float* ms,
+template <int W>
+__device__ __forceinline__ void merge_warps(const DecodeArgs& a, size_t head0, int ng, int split, const float* ms,
                                             const float* ls, const float* os, int rows, int pitch) {
     const int D = a.D;
     for (int i = threadIdx.x; i < ng * D; i += W * 32) {
@@ -169,13 +169,7 @@ __device__ __forceinline__ void merge_warps(const DecodeArgs& a, Head head_of, i
             ll = fmaf(ls[w * rows + g], c, ll);
             oo = fmaf(os[(w * rows + g) * pitch + d], c, oo);
         }
-        const size_t head = head_of(g);
-        if (PASS != PASS_ALL) {
-            const size_t part = head * a.slots + a.slot0 + split;
-            a.part_o[part * D + d] = oo;
-            if (d == 0) a.part_ml[part] = make_float2(mm, ll);
-            continue;
-        }
+        const size_t head = head0 + g;
         if (a.splits == 1) {
             a.O[head * D + d] = ll == 0.0f ? 0.0f : oo / ll;
             if (d == 0 && a.lse) a.lse[head] = ll == 0.0f ? -INFINITY : (mf + log2f(ll)) * 0.693147180559945f;
@@ -184,6 +178,38 @@ __device__ __forceinline__ void merge_warps(const DecodeArgs& a, Head head_of, i
             if (a.splits > 1) a.part_o[(head * a.splits + split) * D + d] = oo;
             if (d == 0) a.part_ml[head * a.splits + split] = make_float2(mm, ll);
         }
+    }
+}
+
+// The same for a part of a pass: a warp's share of a row is formed once (in fs [warps][rows]), four columns at a time.
+template <int W, typename Head>
+__device__ __forceinline__ void merge_part(const DecodeArgs& a, Head head_of, int ng, int split, const float* ms, const float* ls,
+                                           const float* os, float* fs, int rows, int pitch) {
+    for (int i = threadIdx.x; i < W * ng; i += W * 32) {
+        const int w = i / ng, g = i - w * ng;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < W; ++v) mm = fmaxf(mm, ms[v * rows + g]);
+        fs[w * rows + g] = exp2f(ms[w * rows + g] - finite_max(mm));
+        if (w == 0) {
+            float ll = 0.0f;
+#pragma unroll
+            for (int v = 0; v < W; ++v) ll = fmaf(ls[v * rows + g], exp2f(ms[v * rows + g] - finite_max(mm)), ll);
+            a.part_ml[head_of(g) * a.slots + a.slot0 + split] = make_float2(mm, ll);
+        }
+    }
+    __syncthreads();
+    const int per = a.D / 4;
+    for (int i = threadIdx.x; i < ng * per; i += W * 32) {
+        const int g = i / per, d = (i - g * per) * 4;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float c = fs[w * rows + g];
+            const float4 v = *reinterpret_cast<const float4*>(os + (w * rows + g) * pitch + d);
+            o = make_float4(fmaf(v.x, c, o.x), fmaf(v.y, c, o.y), fmaf(v.z, c, o.z), fmaf(v.w, c, o.w));
+        }
+        *reinterpret_cast<float4*>(a.part_o + (head_of(g) * a.slots + a.slot0 + split) * a.D + d) = o;
     }
 }
 
@@ -361,7 +387,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
         h0 = (unit - before) * 8 * NT;  // row of the group
         ng = g < 0 ? 0 : min(8 * NT, a.gr.size(g) * a.G - h0);
         b = g < 0 ? 0 : leader_of(a.gr, a.c, g, vis.n);
-        chunk = part_tokens(vis.n, a.splits);
+        chunk = part_tokens(vis.n, a.splits, kSharedLeast);
     } else {
         split = (int)(id % a.splits);
         id /= a.splits;
@@ -375,9 +401,9 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
             vis.sinks = 0;
             vis.gap = shared;
             vis.nvis = vis.n - shared;
-            chunk = part_tokens(vis.nvis, a.splits);
+            chunk = part_tokens(vis.nvis, a.splits, kOwnLeast);
             if (split == 0 && tid < min(8 * NT, a.G - grp * 8 * NT)) {
-                const int t = part_tokens(shared, a.prefix_parts > 0 ? a.prefix_parts : 1);
+                const int t = part_tokens(shared, a.prefix_parts > 0 ? a.prefix_parts : 1, kSharedLeast);
                 const int parts = shared == 0 ? 0 : a.prefix_parts > 0 ? (shared + t - 1) / t : 1;
                 a.info[(size_t)b * a.H + hk * a.G + grp * 8 * NT + tid] = make_int2((vis.nvis + chunk - 1) / chunk, parts);
             }
@@ -718,8 +744,13 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
             }
         }
     __syncthreads();
-    merge_warps<W, PASS>(a, head_of, ng, split, ms, ls, os, 8 * NT, S::PITCH);
-    if (PASS != PASS_ALL) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (PASS == PASS_ALL) {
+        merge_warps<W>(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, 8 * NT, S::PITCH);
+    } else {
+        static_assert(S::MERGE + W * 8 * NT * 4 <= S::RING, "the shares lie in the ring too");
+        merge_part<W>(a, head_of, ng, split, ms, ls, os, os + W * 8 * NT * S::PITCH, 8 * NT, S::PITCH);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    }
 }
 
 // m and l of all parts of a head (one warp): the same order whatever the grid.
@@ -931,8 +962,15 @@ long long shared_units(int rows, int H, int HK, int batch, int groups) { return 
 
 }  // namespace
 
+constexpr int kOwnWaves = 2;
+// How many own tokens there are is known on the device alone; sequences with few leave their CTAs behind the first
+// without work, so that these are kOwnWaves waves at most.
 int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch) {
-    return (int)decode_parts(dtype, H, HK, D, max_len, batch);
+    const long long units = decode_units(dtype, H, HK, D, batch), most = ((long long)max_len + kOwnLeast - 1) / kOwnLeast;
+    long long p = units > 0 ? kOwnWaves * decode_slots(dtype, D) / units : 1;
+    if (p > most) p = most;
+    if (p > kMaxSplits) p = kMaxSplits;
+    return p < 1 ? 1 : (int)p;
 }
 // As many as give two waves of CTAs, each of 128 tokens or more.
 int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {

@@ -37,16 +37,16 @@ __device__ __forceinline__ void put4(__half* o, const float4& v) {
     reinterpret_cast<__half2*>(o)[1] = __floats2half2_rn(v.z, v.w);
 }
 
-constexpr int kJoinWarps = 8;  // of a CTA, which joins one row
+constexpr int kJoinWarps = 4;  // of a CTA, which joins one row
 constexpr int kJoinAhead = 4;  // parts of a warp that are on their way together
 
 // Joins the parts of a row: those of its own tokens, then those of the shared
 // ones, in their order whatever the grid.  O is rounded to Q's type, once.
-template <typename T, bool TC>
+template <typename T, bool TC, bool WIDE>
 __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const JoinArgs a) {
     const SharedArgs& s = a.s;
     constexpr int W = kJoinWarps, U = kJoinAhead;
-    __shared__ float4 sums[W][64];
+    __shared__ float4 sums[W][WIDE ? 64 : 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long row = blockIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const Join
             if (i < parts) {
                 const float* p = o_of(i);
                 if (c0 < s.D) x[u] = *reinterpret_cast<const float4*>(p + c0);
-                if (c1 < s.D) y[u] = *reinterpret_cast<const float4*>(p + c1);
+                if (WIDE && c1 < s.D) y[u] = *reinterpret_cast<const float4*>(p + c1);
             }
         }
     };
@@ -106,11 +106,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const Join
             const int i = i0 + u * W;
             const float f = i < parts ? exp2f(ml_of(i).x - base) : 0.0f;
             o0 = make_float4(fmaf(x[u].x, f, o0.x), fmaf(x[u].y, f, o0.y), fmaf(x[u].z, f, o0.z), fmaf(x[u].w, f, o0.w));
-            o1 = make_float4(fmaf(y[u].x, f, o1.x), fmaf(y[u].y, f, o1.y), fmaf(y[u].z, f, o1.z), fmaf(y[u].w, f, o1.w));
+            if (WIDE) o1 = make_float4(fmaf(y[u].x, f, o1.x), fmaf(y[u].y, f, o1.y), fmaf(y[u].z, f, o1.z), fmaf(y[u].w, f, o1.w));
         }
     }
     sums[warp][lane] = o0;
-    sums[warp][lane + 32] = o1;
+    if (WIDE) sums[warp][lane + 32] = o1;
     __syncthreads();
     const int c = threadIdx.x * 4;
     if (c < s.D) {
@@ -129,8 +129,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const Join
 template <typename T>
 int launch_join(const JoinArgs& a, cudaStream_t st) {
     const dim3 grid((unsigned)(a.s.batch * a.s.H)), block(kJoinWarps * 32);
-    const cudaError_t e = a.tc.first_o ? launch_pdl(prefix_join_kernel<T, true>, grid, block, 0, st, a)
-                                       : launch_pdl(prefix_join_kernel<T, false>, grid, block, 0, st, a);
+    const bool wide = a.s.D > 128;
+    const cudaError_t e = a.tc.first_o && wide ? launch_pdl(prefix_join_kernel<T, true, true>, grid, block, 0, st, a)
+                          : a.tc.first_o       ? launch_pdl(prefix_join_kernel<T, true, false>, grid, block, 0, st, a)
+                          : wide               ? launch_pdl(prefix_join_kernel<T, false, true>, grid, block, 0, st, a)
+                                               : launch_pdl(prefix_join_kernel<T, false, false>, grid, block, 0, st, a);
     if (e != cudaSuccess) (void)cudaGetLastError();
     return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }

@@ -57,11 +57,11 @@ __device__ __forceinline__ int leader_of(const Groups& gr, const PagedView& c, i
     return s0;
 }
 
-// A part of a pass: tokens of one part where `tokens` are taken in at most `splits` parts.
-constexpr int kPartMin = 128;
-__host__ __device__ __forceinline__ int part_tokens(int tokens, int splits) {
+// Tokens of a part where `tokens` are taken in at most `splits` parts of `least` tokens or more.
+constexpr int kOwnLeast = 256, kSharedLeast = 128;
+__host__ __device__ __forceinline__ int part_tokens(int tokens, int splits, int least) {
     const int c = ((tokens + splits - 1) / splits + 31) / 32 * 32;
-    return c < kPartMin ? kPartMin : c;
+    return c < least ? least : c;
 }
 
 // What the passes leave: part s of row (sequence b, query head h) at ((b H + h) slots + s), o [D] not divided by l,

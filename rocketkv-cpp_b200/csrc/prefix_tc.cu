@@ -10,8 +10,9 @@
 // time: S = Q K^T into tensor memory, P = 2^(S - m) rounded to the inputs' type
 // back into tensor memory in S's place, O += P V.
 //
-//   warps 0-3    copy Q's rows and K's and V's, which lie in pages of any size, by 16-byte
-//                asynchronous copies into the swizzled tiles
+//   warps 0-3    copy Q's rows by 16-byte asynchronous copies into the swizzled tiles, and K's and V's,
+//                in pages of any size, likewise; where pages are multiples of 8 tokens
+//                warp 0 has those copied as boxes of a tensor map
 //   warp 4       issues the products
 //   warps 8-11, 12-15   softmax of the first accumulator, of the second, and their rows
 //
@@ -39,14 +40,15 @@ struct Args {
     SharedArgs s;
     TcParts p;
     int G;
+    int box;       // tokens of a box, a power of two that divides the page size; 0: none, copies by 16 bytes
     float scale2;  // log2(e) / sqrt(D)
 };
 
 struct Bars {
-    uint64_t o_full, o_empty, written, drained;
+    uint64_t q_full, o_full, o_empty, written, drained;
     uint64_t s_full[2], p_half[2], p_ready[2];  // of an accumulator
     uint64_t full[8], empty[8];
-    uint32_t mask[kMasks][4];
+    alignas(16) uint32_t mask[kMasks][4];
     uint32_t tmem;
     int abort;
 };
@@ -174,17 +176,9 @@ struct Walk {
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
-// Whether the phase has ended, without waiting for it.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
+// Arrives on `bar` once the copies that this thread has begun have landed.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // A warp's 32 rows of KB blocks of 64 columns into a swizzled tile at dst (this warp's first row): off is this lane's
 // row's offset from src, or -1 for a row of zeros; columns from `chunks` 16-byte chunks on are zeros.
@@ -226,8 +220,9 @@ __device__ __forceinline__ void write_cols(uint8_t* so, const uint32_t* o, float
     __syncwarp();
 }
 
-template <int KB, bool BF>
-__global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
+template <int KB, bool BF, bool BOXES>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix_tc_kernel(const Args a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
     constexpr int NS = ring_slots(KB);
     constexpr uint32_t kOne = KB * kBlk;
     constexpr uint32_t kColO = 256;  // tensor memory: S0, S1 (128 columns each), O0, O1 (64 KB each)
@@ -242,7 +237,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
     uint8_t* stage = sq + 2 * kOne - 8 * 4096;  // 4 KB per softmax warp, in Q's place once its products have ended
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    Walk walk(a);
     if (tid == 0) {
+        mbar_init(&B.q_full, 128);
         mbar_init(&B.o_full, 1);
         mbar_init(&B.o_empty, 8);
         mbar_init(&B.written, 8);
@@ -253,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
             mbar_init(&B.p_ready[u], 4);
         }
         for (int i = 0; i < NS; ++i) {
-            mbar_init(&B.full[i], 4);
+            mbar_init(&B.full[i], BOXES ? 1 : 4 * 33);  // 33: a copying warp's lanes' copies, and its word of the mask
             mbar_init(&B.empty[i], 1);
         }
         *abort_flag = 0;
@@ -266,51 +263,28 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tbase = B.tmem;
-    Walk walk(a);
     Stretch x;
 
     // (56 + 40 + 208 + 208) * 128 registers are the 128 * 512 of the launch
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         const int chunks = a.s.D / 8;
-        int q = 0, nq = 0, nk = 0, open = 0;  // slots, stretches, tiles; slots begun whose copies are not known to have landed
+        int q = 0, nq = 0, nk = 0;  // slots, stretches, tiles
         bool ok = true;
-        auto landed = [&]() {  // the oldest slot
-            switch (open) {
-                case 8: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
-                case 7: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-                case 6: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-                case 5: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-                case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-                case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-                case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-                default: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-            }
-            fence_proxy_async();  // the products read what was copied through another proxy
-            __syncwarp();
-            if (lane == 0) mbar_arrive1(&B.full[(q - open) % NS]);
-            --open;
-        };
         auto slot = [&](const uint8_t* base, long long off) {
             const int s = q % NS;
-            if (q >= NS) {
-                // while the slot is not free, those on their way are handed over as they land
-                const uint32_t parity = (uint32_t)((q / NS - 1) & 1);
-                while (open > 0 && !__all_sync(0xffffffffu, mbar_test(&B.empty[s], parity))) landed();
-                ok = warp_wait(&B.empty[s], parity, err, abort_flag);
-            }
+            if (q >= NS) ok = warp_wait(&B.empty[s], (uint32_t)((q / NS - 1) & 1), err, abort_flag);
             if (ok) {
                 copy_rows<KB>(smem_u32(ring) + s * kOne + warp * 4096, base, off, chunks, lane);
-                asm volatile("cp.async.commit_group;" ::: "memory");
+                copies_arrive(&B.full[s]);
+                if (lane == 0) mbar_arrive1(&B.full[s]);
                 ++q;
-                ++open;
             }
         };
         while (ok && walk.next(a, x)) {
             const int leader = leader_of(a.s.gr, a.s.c, x.g, x.shared);
             if (nq > 0 && !(ok = warp_wait(&B.written, (uint32_t)((nq - 1) & 1), err, abort_flag))) break;
             ++nq;
-            // Q's rows go with the first K tile
             for (int u = 0; u < (x.rows > 128 ? 2 : 1); ++u) {
                 const int r = u * 128 + warp * 32 + lane;
                 const unsigned row = x.row0 + r, sq_ = row / (unsigned)a.G;
@@ -318,6 +292,38 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
                                                        (long long)(x.hk * a.G + (int)(row - sq_ * a.G)) * a.s.D * 2
                                                  : -1;
                 copy_rows<KB>(smem_u32(sq) + u * kOne + warp * 4096, a.s.Q, off, chunks, lane);
+            }
+            copies_arrive(&B.q_full);
+            if (BOXES) {
+                for (int j = x.j0; j < x.j0 + x.tiles && ok && warp == 0; ++j, ++nk) {
+                    // lane i has box i; one of a page outside the pool begins behind it and is filled with zeros
+                    const int t = j * kTcKeys + lane * a.box;
+                    int page = a.s.c.num_pages, row = 0;
+                    if (lane * a.box < kTcKeys && t < x.shared) {
+                        const unsigned n = (unsigned)t / (unsigned)a.s.c.page_size;
+                        const int p = a.s.c.table[(size_t)leader * a.s.c.table_stride + n];
+                        if ((unsigned)p < (unsigned)page) page = p, row = t - (int)n * a.s.c.page_size;
+                    }
+                    const uint32_t have = __ballot_sync(0xffffffffu, page < a.s.c.num_pages);
+                    uint32_t mask[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int k = w * 32 + lane;
+                        mask[w] = __ballot_sync(0xffffffffu, ((have >> (k / a.box)) & 1u) && j * kTcKeys + k < x.shared);
+                    }
+                    if (lane == 0) *reinterpret_cast<uint4*>(B.mask[nk % kMasks]) = make_uint4(mask[0], mask[1], mask[2], mask[3]);
+                    for (int v = 0; v < 2 && ok; ++v, ++q) {
+                        const int s = q % NS;
+                        if (q >= NS) ok = warp_wait(&B.empty[s], (uint32_t)((q / NS - 1) & 1), err, abort_flag);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(&B.full[s], kOne);
+                        __syncwarp();
+                        if (lane * a.box < kTcKeys)
+                            for (int kb = 0; kb < KB; ++kb)
+                                tma_load_4d(ring + s * kOne + kb * kBlk + lane * a.box * 128, v ? &tv : &tk, kb * 64, row, x.hk, page, &B.full[s]);
+                    }
+                }
+                continue;
             }
             for (int j = x.j0; j < x.j0 + x.tiles && ok; ++j, ++nk) {
                 const int t = j * kTcKeys + warp * 32 + lane;
@@ -327,9 +333,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
                 slot(a.s.c.K, off);
                 if (ok) slot(a.s.c.V, off);
             }
-            while (ok && open > 0) landed();
         }
+        // every copy has landed before the CTA may end
         asm volatile("cp.async.wait_all;" ::: "memory");
+        if (BOXES && warp == 0)
+            for (int s = 0; s < min(q, NS); ++s) mbar_wait_bounded(&B.full[s], (uint32_t)(((q - 1 - s) / NS) & 1), err);
     } else if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 4) {
@@ -347,7 +355,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
                 const int n = both ? 2 * x.tiles : x.tiles;
                 auto scores = [&](int k) {
                     const int u = k & 1, at = q + 2 * (both ? k >> 1 : k), s = at % NS;
-                    if (!(both && u)) wait(&B.full[s], at / NS);
+                    if (!(both && u)) {
+                        wait(&B.full[s], at / NS);
+                        fence_proxy_async();  // what the copies wrote is read through another proxy
+                    }
                     if (ok) {
                         tc_fence_after();
                         const uint64_t da = qd + (uint32_t)((both ? u : 0) * (kOne >> 4)), db = kd + (uint32_t)(s * (kOne >> 4));
@@ -360,13 +371,28 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
                         if (!both || u) mma_commit_w(&B.empty[s]);
                     }
                 };
+                wait(&B.q_full, nq);
+                fence_proxy_async();
                 scores(0);
                 if (ok && n > 1) scores(1);
                 if (ok && nq > 0) wait(&B.o_empty, nq - 1);  // the rows of the stretch before have been read
                 ++nq;
                 for (int k = 0; k < n && ok; ++k) {
                     const int u = k & 1, at = q + 2 * (both ? k >> 1 : k) + 1, s = at % NS;
-                    if (!(both && u)) wait(&B.full[s], at / NS);
+                    if (!(both && u)) {
+                        wait(&B.full[s], at / NS);
+                        fence_proxy_async();
+                    }
+                    const int real = x.shared - (x.j0 + (both ? k >> 1 : k)) * kTcKeys;  // of the tile's rows
+                    if (BOXES && ok && real < kTcKeys && !(both && u)) {
+                        // a box holds what lies behind the shared tokens too, which may be anything, and 0 * NaN is NaN
+                        for (int e = lane; e < (kTcKeys - real) * 8; e += 32)
+#pragma unroll
+                            for (int kb = 0; kb < KB; ++kb)
+                                *reinterpret_cast<uint4*>(ring + s * kOne + kb * kBlk + real * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
                     const uint64_t db = vd + (uint32_t)(s * (kOne >> 4));
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
@@ -560,25 +586,50 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const Args a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the pass before has ended too once this one has
 }
 
-template <int KB, bool BF>
-int launch(const Args& a, cudaStream_t st) {
+// [pages][heads][tokens of a page][D] with the cache's strides; boxes of 64 columns x box tokens of a page and
+// head, 128-byte swizzle, zeros outside.  A stride of a dimension of one entry is not used and set to a valid value.
+bool encode(CUtensorMap* m, const uint8_t* base, const SharedArgs& s, int box) {
+    auto enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t rowb = (cuuint64_t)s.D * 2;
+    const cuuint64_t dims[4] = {(cuuint64_t)s.D, (cuuint64_t)s.c.page_size, (cuuint64_t)s.HK, (cuuint64_t)s.c.num_pages};
+    const cuuint64_t st[3] = {s.c.page_size > 1 ? (cuuint64_t)s.c.token_stride : rowb, s.HK > 1 ? (cuuint64_t)s.c.head_stride : rowb,
+                              s.c.num_pages > 1 ? (cuuint64_t)s.c.page_stride : rowb};
+    const cuuint32_t sizes[4] = {64u, (cuuint32_t)box, 1u, 1u}, one[4] = {1u, 1u, 1u, 1u};
+    return enc(m, s.dtype == RKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint8_t*>(base),
+               dims, st, sizes, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int KB, bool BF, bool BOXES>
+int launch_kernel(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
     // the barriers, and up to 1023 bytes of alignment; Q and the ring
     const int smem = 2048 + (2 + ring_slots(KB)) * KB * kBlk;
     // the split of the registers is the launch's only where the kernel was compiled to 128 a thread
     static const bool fits = [] {
         cudaFuncAttributes f;
-        if (cudaFuncGetAttributes(&f, prefix_tc_kernel<KB, BF>) == cudaSuccess) return f.numRegs == 128;
+        if (cudaFuncGetAttributes(&f, prefix_tc_kernel<KB, BF, BOXES>) == cudaSuccess) return f.numRegs == 128;
         (void)cudaGetLastError();
         return false;
     }();
     if (!fits) return RKV_ERR_CUDA;
-    if (cudaFuncSetAttribute(prefix_tc_kernel<KB, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    if (cudaFuncSetAttribute(prefix_tc_kernel<KB, BF, BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
-    const cudaError_t e = launch_pdl(prefix_tc_kernel<KB, BF>, dim3(kTcSms), dim3(kThreads), smem, st, a);
+    const cudaError_t e = launch_pdl(prefix_tc_kernel<KB, BF, BOXES>, dim3(kTcSms), dim3(kThreads), smem, st, a, tk, tv);
     if (e != cudaSuccess) (void)cudaGetLastError();
     return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
+}
+template <int KB, bool BF>
+int launch(Args& a, cudaStream_t st) {
+    CUtensorMap tk{}, tv{};
+    const int page = a.s.c.page_size & -a.s.c.page_size;  // the largest power of two that divides it
+    a.box = page < 8 ? 0 : page < kTcKeys ? page : kTcKeys;
+    // strides and sizes of a tensor map are bounded; where it cannot be made the copies need none
+    if (a.box && a.s.c.num_pages > 0 && encode(&tk, a.s.c.K, a.s, a.box) && encode(&tv, a.s.c.V, a.s, a.box))
+        return launch_kernel<KB, BF, true>(a, tk, tv, st);
+    return launch_kernel<KB, BF, false>(a, tk, tv, st);
 }
 
 }  // namespace

@@ -38,11 +38,6 @@
 // thread that issues everything 224; two issuing warps 213; 16 softmax warps
 // 197; P handed over whole 197; the maximum taken under the first half's
 // exponentials 203.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include <mutex>
-
 #include "attn_tc.cuh"
 #include "sink_attn.cuh"
 
@@ -745,19 +740,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     __syncthreads();
     tc_fence_after();
     if (warp == 1) tmem_dealloc(tbase, 512);
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    });
-    return fn;
 }
 
 // [batch][heads][rows][D] with byte strides; boxes of 64 columns x box_rows rows, 128-byte swizzle, zeros
