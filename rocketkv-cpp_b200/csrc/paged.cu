@@ -90,6 +90,7 @@ constexpr int kMinChunk = 128;  // visible tokens per CTA at least
 constexpr int kMaxSplits = 1024;
 constexpr int kSms = 148;
 constexpr int kMaxWaves = 8;       // of CTAs that a cache is split into at most
+constexpr int kJoinAhead = 16;     // parts of a column that the joins read before the shares are known
 constexpr int kStartTokens = 128;  // what a CTA costs before and behind its tokens, in tokens
 
 struct DecodeArgs {
@@ -110,11 +111,13 @@ struct DecodeArgs {
     float* scores;       // [batch][H][vmax], base-2 scores (with weights)
     long long o_blocks;  // join: CTAs that join O; the others add weights
     int w_blocks;        // join: CTAs per (item, KV head) that add weights
-    Groups gr;           // the passes of a batch that shares leading tokens
-    int slots, slot0;    // their parts of a row, and the first of this pass
-    int units;           // prefix pass: row groups of all groups at most
-    int2* info;          // pass over own tokens: what each row's parts are
-    int prefix_parts;    // of the prefix pass at most, 0 where it is not this kernel's
+    // the passes of a batch that shares leading tokens
+    SharedArgs sh;
+    TcParts tc;
+    Result res;
+    int slot0;         // of a row's parts, the first of this pass
+    int units;         // shared tokens: row groups of all groups at most
+    int prefix_parts;  // of the shared tokens at most, 0 where they are not this kernel's
 };
 
 // The visible tokens are numbered 0 .. nvis - 1: the sinks, then the window.
@@ -144,8 +147,11 @@ __device__ __forceinline__ float warp_sum(float x) {
     return x;
 }
 // What a launch of the decode kernel attends: all tokens of every sequence; or, of a batch that shares leading tokens,
-// every sequence's own, or every group's shared ones with the rows of all its sequences.
-enum { PASS_ALL = 0, PASS_OWN = 1, PASS_SHARED = 2 };
+// every sequence's own, every group's shared ones with the rows of all its sequences, or the own ones last, joined with
+// the others' parts.
+enum { PASS_ALL = 0, PASS_OWN = 1, PASS_SHARED = 2, PASS_LAST = 3 };
+
+enum { KIND_F16 = 0, KIND_BF16 = 1, KIND_F32 = 2 };
 
 // 0 in place of -inf, so that a set with nothing in it subtracts no infinities.
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
@@ -195,7 +201,7 @@ __device__ __forceinline__ void merge_part(const DecodeArgs& a, Head head_of, in
             float ll = 0.0f;
 #pragma unroll
             for (int v = 0; v < W; ++v) ll = fmaf(ls[v * rows + g], exp2f(ms[v * rows + g] - finite_max(mm)), ll);
-            a.part_ml[head_of(g) * a.slots + a.slot0 + split] = make_float2(mm, ll);
+            a.part_ml[head_of(g) * a.sh.slots + a.slot0 + split] = make_float2(mm, ll);
         }
     }
     __syncthreads();
@@ -209,7 +215,94 @@ __device__ __forceinline__ void merge_part(const DecodeArgs& a, Head head_of, in
             const float4 v = *reinterpret_cast<const float4*>(os + (w * rows + g) * pitch + d);
             o = make_float4(fmaf(v.x, c, o.x), fmaf(v.y, c, o.y), fmaf(v.z, c, o.z), fmaf(v.w, c, o.w));
         }
-        *reinterpret_cast<float4*>(a.part_o + (head_of(g) * a.slots + a.slot0 + split) * a.D + d) = o;
+        *reinterpret_cast<float4*>(a.part_o + (head_of(g) * a.sh.slots + a.slot0 + split) * a.D + d) = o;
+    }
+}
+
+// The two values as a 16-bit pair.
+template <bool BF>
+__device__ __forceinline__ uint32_t round2(float x, float y) {
+    if (BF) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Parts of a sequence's shared tokens; the tcgen05 kernel's: 1 for any, whose number it leaves itself.
+__device__ __forceinline__ int shared_parts(const DecodeArgs& a, int shared) {
+    if (shared == 0 || a.prefix_parts == 0) return shared > 0;
+    const int t = part_tokens(shared, a.prefix_parts, kSharedLeast);
+    return (shared + t - 1) / t;
+}
+
+// The end of the last pass: the warps' (m, l, o) and the parts of the shared tokens, joined; o [warps][rows][pitch],
+// then room for fs [warps][rows], [rows] 1 / l and the parts' shares [rows][kMaxShared].
+template <int KIND, int W, typename Head>
+__device__ __forceinline__ void merge_last(const DecodeArgs& a, Head head_of, int ng, int shared, const float* ms, const float* ls,
+                                           const float* os, float* fs, int rows, int pitch) {
+    float* inv = fs + W * rows;
+    float* share = inv + rows;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the shared tokens' parts are there
+    if (a.res.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.res.clear = 0;
+    const int own_parts = shared_parts(a, shared);
+    for (int g = warp; g < ng; g += W) {
+        const size_t row = head_of(g);
+        int2 x = make_int2(0, 0);
+        if (a.tc.first_o && own_parts > 0) x = a.tc.first_later[row];
+        const int parts = own_parts + x.x;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, ms[w * rows + g]);
+        for (int p = lane; p < parts; p += 32) top = fmaxf(top, shared_ml(a.sh, a.tc, row, x, p).x);
+        const float base = finite_max(warp_max(top));
+        float l = lane < W ? ls[lane * rows + g] * exp2f(ms[lane * rows + g] - base) : 0.0f;
+        if (lane < W) fs[lane * rows + g] = exp2f(ms[lane * rows + g] - base);
+        for (int p = lane; p < parts; p += 32) {
+            const float2 v = shared_ml(a.sh, a.tc, row, x, p);
+            const float f = exp2f(v.x - base);
+            share[g * kMaxShared + p] = f;
+            l = fmaf(v.y, f, l);
+        }
+        l = warp_sum(l);
+        if (lane == 0) {
+            inv[g] = l == 0.0f ? 0.0f : 1.0f / l;
+            if (a.res.lse) a.res.lse[row] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945f;
+        }
+    }
+    __syncthreads();
+    const int per = a.D / 4;
+    for (int i = threadIdx.x; i < ng * per; i += W * 32) {
+        const int g = i / per, d = (i - g * per) * 4;
+        const size_t row = head_of(g);
+        int2 x = make_int2(0, 0);
+        if (a.tc.first_o && own_parts > 0) x = a.tc.first_later[row];
+        const int parts = own_parts + x.x;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        auto add = [&](const float4& v, float c) {
+            o = make_float4(fmaf(v.x, c, o.x), fmaf(v.y, c, o.y), fmaf(v.z, c, o.z), fmaf(v.w, c, o.w));
+        };
+#pragma unroll
+        for (int w = 0; w < W; ++w) add(*reinterpret_cast<const float4*>(os + (w * rows + g) * pitch + d), fs[w * rows + g]);
+        constexpr int U = 8;  // parts on their way together
+        for (int p0 = 0; p0 < parts; p0 += U) {
+            float4 v[U];
+#pragma unroll
+            for (int p = 0; p < U; ++p)
+                v[p] = p0 + p < parts ? *reinterpret_cast<const float4*>(shared_o(a.sh, a.tc, row, x, p0 + p) + d) : make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int p = 0; p < U; ++p)
+                if (p0 + p < parts) add(v[p], share[g * kMaxShared + p0 + p]);
+        }
+        const float f = inv[g];
+        o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+        if (KIND == KIND_F32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(a.res.O) + row * a.D + d) = o;
+        } else {
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.res.O) + (row * a.D + d) * 2) =
+                make_uint2(round2<KIND == KIND_BF16>(o.x, o.y), round2<KIND == KIND_BF16>(o.z, o.w));
+        }
     }
 }
 
@@ -217,8 +310,6 @@ __device__ __forceinline__ void merge_part(const DecodeArgs& a, Head head_of, in
 // The decode kernel: matrix instructions on tiles of 16 tokens
 // ---------------------------------------------------------------------------
 constexpr int kKeys = 16;  // tokens of a tile
-
-enum { KIND_F16 = 0, KIND_BF16 = 1, KIND_F32 = 2 };
 
 template <int KIND>
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -287,16 +378,17 @@ __device__ __forceinline__ uint32_t split2(float& x, float& y) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 // Shapes of the kernel: DP columns (dim_head rounded up), 8 NT query heads, W warps, ring slots of a warp,
-// CTAs of an SM.
-template <int KIND_, int DP_, int NT_>
+// CTAs of an SM.  SHORT: for stretches of a few hundred tokens, whose begin and end take longer than their tokens: CTAs
+// of half the warps and twice as many of them, so that some read while others begin or end.
+template <int KIND_, int DP_, int NT_, bool SHORT = false>
 struct Shape {
     static constexpr int KIND = KIND_, DP = DP_, NT = NT_;
     static constexpr int SIZE = KIND == KIND_F32 ? 4 : 2;
     static constexpr int ROW = DP * SIZE;             // bytes of a row in shared memory
     static constexpr int SLOT = kKeys * ROW;          // 16 rows of K or of V
-    static constexpr int W = ROW > 512 ? 4 : 8;
+    static constexpr int W = (ROW > 512 ? 4 : 8) / (SHORT ? 2 : 1);
     static constexpr int SLOTS = ROW > 128 ? 3 : 5;   // odd: K and V take the slots in turn
-    static constexpr int CTAS = ROW > 256 ? 1 : 2;
+    static constexpr int CTAS = (ROW > 256 ? 1 : 2) * (SHORT ? 2 : 1);
     static constexpr bool QS = KIND == KIND_F32 || NT > 1;  // q in shared memory, else in registers
     static constexpr int QBYTES = !QS ? 0 : KIND == KIND_F32 ? DP / 8 * NT * 512 : DP / 16 * NT * 256;
     static constexpr int RING = W * SLOTS * SLOT;
@@ -354,7 +446,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
     const int D = a.D, chunks = D * S::SIZE / 16;
 
     long long id = blockIdx.x;
-    int split, b, hk, h0, ng, first = 0;  // b: whose table row; first: the group's first sequence
+    int split, b, hk, h0, ng, first = 0, shared = 0;  // b: whose table row; first: the group's first sequence
     Visible vis;
     int chunk = a.chunk;
     if (PASS == PASS_SHARED) {
@@ -364,8 +456,8 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
         split = (int)(id / a.HK);
         // the group of this row group
         int g = -1, before = 0;
-        for (int g0 = 0; g0 < a.gr.n && g < 0; g0 += 32) {
-            const int mine = g0 + lane < a.gr.n ? (a.gr.size(g0 + lane) * a.G + 8 * NT - 1) / (8 * NT) : 0;
+        for (int g0 = 0; g0 < a.sh.gr.n && g < 0; g0 += 32) {
+            const int mine = g0 + lane < a.sh.gr.n ? (a.sh.gr.size(g0 + lane) * a.G + 8 * NT - 1) / (8 * NT) : 0;
             int sum = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -381,12 +473,12 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
                 before += __shfl_sync(0xffffffffu, sum, 31);
             }
         }
-        vis.n = vis.nvis = g < 0 ? 0 : a.gr.shared(a.c, g);
+        vis.n = vis.nvis = g < 0 ? 0 : a.sh.gr.shared(a.c, g);
         vis.sinks = vis.gap = 0;
-        first = g < 0 ? 0 : a.gr.start(g);
+        first = g < 0 ? 0 : a.sh.gr.start(g);
         h0 = (unit - before) * 8 * NT;  // row of the group
-        ng = g < 0 ? 0 : min(8 * NT, a.gr.size(g) * a.G - h0);
-        b = g < 0 ? 0 : leader_of(a.gr, a.c, g, vis.n);
+        ng = g < 0 ? 0 : min(8 * NT, a.sh.gr.size(g) * a.G - h0);
+        b = g < 0 ? 0 : leader_of(a.sh.gr, a.c, g, vis.n);
         chunk = part_tokens(vis.n, a.splits, kSharedLeast);
     } else {
         split = (int)(id % a.splits);
@@ -396,23 +488,22 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
         hk = (int)(id % a.HK);
         b = (int)(id / a.HK);
         vis = visible(a, b);
-        if (PASS == PASS_OWN) {
-            const int shared = member_of(a.gr, a.c, b, vis.n).tokens;
+        if (PASS == PASS_OWN || PASS == PASS_LAST) {
+            shared = member_of(a.sh.gr, a.c, b, vis.n).tokens;
             vis.sinks = 0;
             vis.gap = shared;
             vis.nvis = vis.n - shared;
-            chunk = part_tokens(vis.nvis, a.splits, kOwnLeast);
-            if (split == 0 && tid < min(8 * NT, a.G - grp * 8 * NT)) {
-                const int t = part_tokens(shared, a.prefix_parts > 0 ? a.prefix_parts : 1, kSharedLeast);
-                const int parts = shared == 0 ? 0 : a.prefix_parts > 0 ? (shared + t - 1) / t : 1;
-                a.info[(size_t)b * a.H + hk * a.G + grp * 8 * NT + tid] = make_int2((vis.nvis + chunk - 1) / chunk, parts);
+            chunk = PASS == PASS_LAST ? vis.nvis : part_tokens(vis.nvis, a.splits, kOwnLeast);
+            if (PASS == PASS_OWN && split == 0 && tid < min(8 * NT, a.G - grp * 8 * NT)) {
+                a.sh.info[(size_t)b * a.H + hk * a.G + grp * 8 * NT + tid] =
+                    make_int2((vis.nvis + chunk - 1) / chunk, shared_parts(a, shared));
             }
         }
         h0 = hk * a.G + grp * 8 * NT;
         ng = min(8 * NT, a.G - grp * 8 * NT);
     }
     const long long v_lo = (long long)split * chunk;
-    if ((PASS != PASS_ALL || split > 0) && v_lo >= vis.nvis) {
+    if (PASS != PASS_LAST && (PASS != PASS_ALL || split > 0) && v_lo >= vis.nvis) {
         // the join takes the parts that hold tokens
         if (PASS != PASS_ALL) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
@@ -746,8 +837,10 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
     __syncthreads();
     if (PASS == PASS_ALL) {
         merge_warps<W>(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, 8 * NT, S::PITCH);
+    } else if (PASS == PASS_LAST) {
+        static_assert(S::MERGE + (W + 1 + kMaxShared) * 8 * NT * 4 <= S::RING, "the shares lie in the ring too");
+        merge_last<KIND, W>(a, head_of, ng, shared, ms, ls, os, os + W * 8 * NT * S::PITCH, 8 * NT, S::PITCH);
     } else {
-        static_assert(S::MERGE + W * 8 * NT * 4 <= S::RING, "the shares lie in the ring too");
         merge_part<W>(a, head_of, ng, split, ms, ls, os, os + W * 8 * NT * S::PITCH, 8 * NT, S::PITCH);
         asm volatile("griddepcontrol.wait;" ::: "memory");
     }
@@ -767,7 +860,6 @@ __device__ __forceinline__ float2 join_ml(const float2* ml, int parts, int lane)
 }
 
 constexpr int kJoinTokens = 512;  // tokens whose weights one CTA of the join adds
-constexpr int kJoinAhead = 16;    // parts of a column read before the shares are known
 
 // Joins the parts.  The first o_blocks CTAs take one query head each; the
 // others add the weights of a stretch of tokens of one KV head.  Launched
@@ -921,7 +1013,7 @@ DecodePlan decode_plan(int dtype, int H, int HK, int D, long long visible_max, i
 
 template <int KIND, int DP, int NT, int PASS>
 int launch_shape(const DecodeArgs& a, long long blocks, bool dependent, cudaStream_t st) {
-    using S = Shape<KIND, DP, NT>;
+    using S = Shape<KIND, DP, NT, PASS == PASS_OWN || PASS == PASS_LAST>;
     static_assert(S::SMEM * S::CTAS + 1024 * S::CTAS <= 228 * 1024, "the CTAs of an SM fit in its shared memory");
     if (cudaFuncSetAttribute(paged_decode_kernel<S, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
         (void)cudaGetLastError();
@@ -962,12 +1054,12 @@ long long shared_units(int rows, int H, int HK, int batch, int groups) { return 
 
 }  // namespace
 
-constexpr int kOwnWaves = 2;
+constexpr int kOwnWaves = 1;
 // How many own tokens there are is known on the device alone; sequences with few leave their CTAs behind the first
 // without work, so that these are kOwnWaves waves at most.
 int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch) {
     const long long units = decode_units(dtype, H, HK, D, batch), most = ((long long)max_len + kOwnLeast - 1) / kOwnLeast;
-    long long p = units > 0 ? kOwnWaves * decode_slots(dtype, D) / units : 1;
+    long long p = units > 0 ? kOwnWaves * 2 * decode_slots(dtype, D) / units : 1;
     if (p > most) p = most;
     if (p > kMaxSplits) p = kMaxSplits;
     return p < 1 ? 1 : (int)p;
@@ -979,10 +1071,10 @@ int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch,
     long long p = 2LL * decode_slots(dtype, D) / (each * groups * HK);
     const long long most = ((long long)max_len + kMinChunk - 1) / kMinChunk;
     if (p > most) p = most;
-    if (p > 256) p = 256;
+    if (p > 128) p = 128;  // of kMaxShared
     return p < 1 ? 1 : (int)p;
 }
-int launch_shared_pass(const SharedArgs& s, bool prefix, bool dependent, cudaStream_t st) {
+int launch_shared_pass(const SharedArgs& s, SharedPass pass, const TcParts& t, const Result& r, bool dependent, cudaStream_t st) {
     DecodeArgs a{};
     a.c = s.c;
     a.Q = s.Q;
@@ -995,23 +1087,25 @@ int launch_shared_pass(const SharedArgs& s, bool prefix, bool dependent, cudaStr
     a.scale2 = 1.4426950408889634f / sqrtf((float)s.D);
     a.part_o = s.part_o;
     a.part_ml = s.part_ml;
-    a.gr = s.gr;
-    a.slots = s.slots;
-    a.info = s.info;
+    a.sh = s;
+    a.tc = t;
+    a.res = r;
     a.prefix_parts = s.slots - s.own;
-    if (prefix) {
+    if (pass == SHARED_TOKENS) {
         const int rows = shared_rows(s.dtype, s.D, s.H, s.HK, s.batch, s.gr.n);
         const long long units = shared_units(rows, s.H, s.HK, s.batch, s.gr.n);
         if (units > 0x7FFFFFF) return RKV_ERR_UNSUPPORTED;
         a.units = (int)units;
         a.slot0 = s.own;
-        a.splits = s.slots - s.own;
+        a.splits = a.prefix_parts;
         return launch_pass<PASS_SHARED>(a, s.dtype, rows, units * s.HK * a.splits, dependent, st);
     }
     const int gt = head_group(s.dtype, a.G, s.D);
     a.ngroups = (a.G + gt - 1) / gt;
-    a.splits = s.own;
-    return launch_pass<PASS_OWN>(a, s.dtype, gt, (long long)s.batch * s.HK * a.ngroups * a.splits, dependent, st);
+    a.splits = pass == OWN_AND_JOIN ? 1 : s.own;
+    const long long blocks = (long long)s.batch * s.HK * a.ngroups * a.splits;
+    return pass == OWN_AND_JOIN ? launch_pass<PASS_LAST>(a, s.dtype, gt, blocks, dependent, st)
+                                : launch_pass<PASS_OWN>(a, s.dtype, gt, blocks, dependent, st);
 }
 
 }  // namespace rkv

@@ -8,7 +8,9 @@
 // meet the queries of all its sequences at once, so they are read once and
 // not once per sequence.  Three kernels: every sequence's own tokens, the
 // shared ones (both of paged.cu, or the latter on the tcgen05 tensor cores,
-// prefix_tc.cu) and the join, each begun while the one before still runs.
+// prefix_tc.cu) and the join; or, where the sequences alone fill the GPU, the
+// shared tokens and the own ones with the join.  Each is begun while the one
+// before still runs.
 #include "prefix.cuh"
 
 namespace rkv {
@@ -17,9 +19,7 @@ namespace {
 struct JoinArgs {
     SharedArgs s;
     TcParts tc;  // where the shared tokens' parts are those of the tcgen05 kernel
-    void* O;
-    float* lse;
-    int* clear;  // the error word, where no kernel before this one has cleared it
+    Result r;
 };
 
 template <typename T>
@@ -50,38 +50,31 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const Join
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long row = blockIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (a.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.clear = 0;
+    if (a.r.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.r.clear = 0;
     const int2 info = s.info[row];
     const int own = info.x;
     int shared = info.y;
-    long long later = 0;  // TC: the row of the second part
-    if (TC) {
-        const int2 x = a.tc.first_later[row];  // not written where the row has no shared tokens
-        if (shared > 0) shared += x.x;
-        later = x.y;
+    int2 x = make_int2(0, 0);
+    if (TC && shared > 0) {
+        x = a.tc.first_later[row];
+        shared += x.x;
     }
-    // part i: own ones in the slots from 0; shared ones in those from s.own, or where the tcgen05 kernel leaves them
+    // own parts, then shared ones
     const int parts = own + shared;
-    auto ml_of = [&](int i) -> float2 {
-        if (i < own || !TC) return s.part_ml[row * s.slots + (i < own ? i : s.own + (i - own))];
-        return i == own ? a.tc.first_ml[row] : a.tc.later_ml[later + (long long)(i - own - 1) * kTcRows];
-    };
-    auto o_of = [&](int i) -> const float* {
-        if (i < own || !TC) return s.part_o + (row * s.slots + (i < own ? i : s.own + (i - own))) * s.D;
-        return i == own ? a.tc.first_o + row * s.D : a.tc.later_o + (later + (long long)(i - own - 1) * kTcRows) * s.D;
-    };
+    auto ml_of = [&](int i) { return i < own ? s.part_ml[row * s.slots + i] : shared_ml(s, a.tc, row, x, i - own); };
+    auto o_of = [&](int i) { return i < own ? s.part_o + (row * s.slots + i) * s.D : shared_o(s, a.tc, row, x, i - own); };
     // warp w takes the parts w, w + W, ...; its first rows are on their way while the weights are formed
     const int c0 = lane * 4, c1 = c0 + 128;
-    float4 x[U], y[U];
+    float4 v0[U], v1[U];
     auto fetch = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * W;
-            x[u] = y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            v0[u] = v1[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (i < parts) {
                 const float* p = o_of(i);
-                if (c0 < s.D) x[u] = *reinterpret_cast<const float4*>(p + c0);
-                if (WIDE && c1 < s.D) y[u] = *reinterpret_cast<const float4*>(p + c1);
+                if (c0 < s.D) v0[u] = *reinterpret_cast<const float4*>(p + c0);
+                if (WIDE && c1 < s.D) v1[u] = *reinterpret_cast<const float4*>(p + c1);
             }
         }
     };
@@ -105,8 +98,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const Join
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * W;
             const float f = i < parts ? exp2f(ml_of(i).x - base) : 0.0f;
-            o0 = make_float4(fmaf(x[u].x, f, o0.x), fmaf(x[u].y, f, o0.y), fmaf(x[u].z, f, o0.z), fmaf(x[u].w, f, o0.w));
-            if (WIDE) o1 = make_float4(fmaf(y[u].x, f, o1.x), fmaf(y[u].y, f, o1.y), fmaf(y[u].z, f, o1.z), fmaf(y[u].w, f, o1.w));
+            o0 = make_float4(fmaf(v0[u].x, f, o0.x), fmaf(v0[u].y, f, o0.y), fmaf(v0[u].z, f, o0.z), fmaf(v0[u].w, f, o0.w));
+            if (WIDE) o1 = make_float4(fmaf(v1[u].x, f, o1.x), fmaf(v1[u].y, f, o1.y), fmaf(v1[u].z, f, o1.z), fmaf(v1[u].w, f, o1.w));
         }
     }
     sums[warp][lane] = o0;
@@ -121,9 +114,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const Join
             const float4 v = sums[w][threadIdx.x];
             o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
         }
-        put4(static_cast<T*>(a.O) + row * s.D + c, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        put4(static_cast<T*>(a.r.O) + row * s.D + c, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
-    if (threadIdx.x == 0 && a.lse) a.lse[row] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945f;
+    if (threadIdx.x == 0 && a.r.lse) a.r.lse[row] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945f;
 }
 
 template <typename T>
@@ -228,9 +221,7 @@ extern "C" int rkv_prefix_decode(const void* Q, long long q_item_stride, int num
     s.part_ml = reinterpret_cast<float2*>(ws + p.off_ml);
     s.part_o = reinterpret_cast<float*>(ws + p.off_o);
     s.info = reinterpret_cast<int2*>(ws + p.off_info);
-    a.O = O;
-    a.lse = lse;
-    rc = launch_shared_pass(s, false, false, st);
+    a.r = Result{O, lse, nullptr};
     if (p.tc) {
         a.tc.first_later = reinterpret_cast<int2*>(ws + p.off_first);
         a.tc.first_ml = reinterpret_cast<float2*>(ws + p.off_first_ml);
@@ -238,11 +229,21 @@ extern "C" int rkv_prefix_decode(const void* Q, long long q_item_stride, int num
         a.tc.later_ml = reinterpret_cast<float2*>(ws + p.off_later_ml);
         a.tc.later_o = reinterpret_cast<float*>(ws + p.off_later_o);
         a.tc.err = static_cast<int*>(workspace);
-        if (!rc) rc = launch_prefix_tc(s, a.tc, st);
     } else {
-        a.clear = static_cast<int*>(workspace);
-        if (!rc && num_groups > 0) rc = launch_shared_pass(s, true, true, st);
+        a.r.clear = static_cast<int*>(workspace);
     }
+    auto shared = [&](bool dependent) {
+        return p.tc             ? launch_prefix_tc(s, a.tc, dependent, st)
+               : num_groups > 0 ? launch_shared_pass(s, SHARED_TOKENS, a.tc, a.r, dependent, st)
+                                : (int)RKV_OK;
+    };
+    if (p.own == 1) {
+        // as many sequences as there is room for CTAs: each takes its own tokens in one part and joins the others' to it
+        rc = shared(false);
+        return rc ? rc : launch_shared_pass(s, OWN_AND_JOIN, a.tc, a.r, num_groups > 0, st);
+    }
+    rc = launch_shared_pass(s, OWN_TOKENS, a.tc, a.r, false, st);
+    if (!rc) rc = shared(true);
     if (rc) return rc;
     return s.dtype == RKV_F32 ? launch_join<float>(a, st) : s.dtype == RKV_BF16 ? launch_join<__nv_bfloat16>(a, st) : launch_join<__half>(a, st);
 }

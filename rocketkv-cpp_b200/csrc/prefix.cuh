@@ -81,10 +81,6 @@ struct SharedArgs {
 // Parts of every sequence's own tokens, and of every group's shared ones for the matrix-instruction kernel.
 int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch);
 int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups);
-// One pass: prefix, the groups' shared tokens; else every sequence's own.  dependent: launched while the pass before
-// it still runs, which it waits for at its end only.
-int launch_shared_pass(const SharedArgs& s, bool prefix, bool dependent, cudaStream_t st);
-
 // The shared tokens on the tcgen05 tensor cores (prefix_tc.cu): 16-bit types.  A unit is up to 256 rows of one group
 // and KV head; the tiles of the units are cut into stretches, one or more per CTA.  A unit's first stretch leaves its
 // rows in first (row b H + h), a stretch that begins inside a unit in later (256 rows per CTA).  first_later[row]: how
@@ -100,6 +96,31 @@ struct TcParts {
 constexpr int kTcSms = 148;
 constexpr int kTcKeys = 128;
 constexpr int kTcRows = 256;
-int launch_prefix_tc(const SharedArgs& s, const TcParts& p, cudaStream_t st);
+// Parts of a row's shared tokens at most.
+constexpr int kMaxShared = 152;
+static_assert(kMaxShared >= kTcSms, "a unit may have a stretch per CTA");
+// Part p of row's shared tokens, wherever the pass over them left it; x: first_later[row].
+__device__ __forceinline__ float2 shared_ml(const SharedArgs& s, const TcParts& t, long long row, int2 x, int p) {
+    return !t.first_o ? s.part_ml[row * s.slots + s.own + p] : p == 0 ? t.first_ml[row] : t.later_ml[x.y + (p - 1) * kTcRows];
+}
+__device__ __forceinline__ const float* shared_o(const SharedArgs& s, const TcParts& t, long long row, int2 x, int p) {
+    return !t.first_o ? s.part_o + (row * s.slots + s.own + p) * s.D
+           : p == 0   ? t.first_o + row * s.D
+                      : t.later_o + (long long)(x.y + (p - 1) * kTcRows) * s.D;
+}
+// Where the last pass leaves its rows, and the error word, where no pass before it has cleared it.
+struct Result {
+    void* O;  // [batch][H][D] of the cache's type
+    float* lse;
+    int* clear;
+};
+
+// The passes of the matrix-instruction kernel: every sequence's own tokens; the groups' shared ones; or the own ones
+// in one part, joined with the parts of the shared ones that the launch before has left.
+enum SharedPass { OWN_TOKENS, SHARED_TOKENS, OWN_AND_JOIN };
+// dependent: launched while the kernel before it still runs, which it waits for at its end only.
+int launch_shared_pass(const SharedArgs& s, SharedPass pass, const TcParts& t, const Result& r, bool dependent, cudaStream_t st);
+// dependent as above.
+int launch_prefix_tc(const SharedArgs& s, const TcParts& p, bool dependent, cudaStream_t st);
 
 }  // namespace rkv

@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t kOne = KB * kBlk;
     constexpr uint32_t kColO = 256;  // tensor memory: S0, S1 (128 columns each), O0, O1 (64 KB each)
     extern __shared__ uint8_t smem_raw[];
-    asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled (it waits for this grid)
+    asm volatile("griddepcontrol.launch_dependents;");  // the kernel behind may be scheduled (it waits for this grid)
     uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     Bars& B = *reinterpret_cast<Bars*>(sm);
     volatile int* abort_flag = &B.abort;
@@ -265,9 +265,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tbase = B.tmem;
     Stretch x;
 
-    // (56 + 40 + 208 + 208) * 128 registers are the 128 * 512 of the launch
+    // (56 + 56 + 200 + 200) * 128 registers are the 128 * 512 of the launch
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(56));
         const int chunks = a.s.D / 8;
         int q = 0, nq = 0, nk = 0;  // slots, stretches, tiles
         bool ok = true;
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (BOXES && warp == 0)
             for (int s = 0; s < min(q, NS); ++s) mbar_wait_bounded(&B.full[s], (uint32_t)(((q - 1 - s) / NS) & 1), err);
     } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(56));
         if (warp == 4) {
             const uint32_t ids = mma_idesc(BF ? 1u : 0u, kTcKeys);
             const uint32_t idv = mma_idesc(BF ? 1u : 0u, KB * 64) | (1u << 16);  // B with N contiguous
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int u = k & 1, at = q + 2 * (both ? k >> 1 : k), s = at % NS;
                     if (!(both && u)) {
                         wait(&B.full[s], at / NS);
-                        fence_proxy_async();  // what the copies wrote is read through another proxy
+                        if (!BOXES) fence_proxy_async();  // what 16-byte copies wrote is read through another proxy
                     }
                     if (ok) {
                         tc_fence_after();
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int u = k & 1, at = q + 2 * (both ? k >> 1 : k) + 1, s = at % NS;
                     if (!(both && u)) {
                         wait(&B.full[s], at / NS);
-                        fence_proxy_async();
+                        if (!BOXES) fence_proxy_async();
                     }
                     const int real = x.shared - (x.j0 + (both ? k >> 1 : k)) * kTcKeys;  // of the tile's rows
                     if (BOXES && ok && real < kTcKeys && !(both && u)) {
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_wait_bounded(&B.drained, 0, err);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(200));
         const int u = (warp >> 2) - 2, q4 = warp & 3, row = q4 * 32 + lane;
         const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
         const uint32_t ts = tbase + u * 128 + lane_off, to = tbase + kColO + lane_off;
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     if (warp == 4) tmem_dealloc(tbase, 512);
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the pass before has ended too once this one has
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the pass before, where there is one, has ended too once this one has
 }
 
 // [pages][heads][tokens of a page][D] with the cache's strides; boxes of 64 columns x box tokens of a page and
@@ -602,7 +602,7 @@ bool encode(CUtensorMap* m, const uint8_t* base, const SharedArgs& s, int box) {
 }
 
 template <int KB, bool BF, bool BOXES>
-int launch_kernel(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
+int launch_kernel(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, bool dependent, cudaStream_t st) {
     // the barriers, and up to 1023 bytes of alignment; Q and the ring
     const int smem = 2048 + (2 + ring_slots(KB)) * KB * kBlk;
     // the split of the registers is the launch's only where the kernel was compiled to 128 a thread
@@ -617,32 +617,36 @@ int launch_kernel(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, c
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
     }
+    if (!dependent) {
+        prefix_tc_kernel<KB, BF, BOXES><<<kTcSms, kThreads, smem, st>>>(a, tk, tv);
+        return launched();
+    }
     const cudaError_t e = launch_pdl(prefix_tc_kernel<KB, BF, BOXES>, dim3(kTcSms), dim3(kThreads), smem, st, a, tk, tv);
     if (e != cudaSuccess) (void)cudaGetLastError();
     return e == cudaSuccess ? RKV_OK : RKV_ERR_CUDA;
 }
 template <int KB, bool BF>
-int launch(Args& a, cudaStream_t st) {
+int launch(Args& a, bool dependent, cudaStream_t st) {
     CUtensorMap tk{}, tv{};
     const int page = a.s.c.page_size & -a.s.c.page_size;  // the largest power of two that divides it
     a.box = page < 8 ? 0 : page < kTcKeys ? page : kTcKeys;
     // strides and sizes of a tensor map are bounded; where it cannot be made the copies need none
     if (a.box && a.s.c.num_pages > 0 && encode(&tk, a.s.c.K, a.s, a.box) && encode(&tv, a.s.c.V, a.s, a.box))
-        return launch_kernel<KB, BF, true>(a, tk, tv, st);
-    return launch_kernel<KB, BF, false>(a, tk, tv, st);
+        return launch_kernel<KB, BF, true>(a, tk, tv, dependent, st);
+    return launch_kernel<KB, BF, false>(a, tk, tv, dependent, st);
 }
 
 }  // namespace
 
-int launch_prefix_tc(const SharedArgs& s, const TcParts& p, cudaStream_t st) {
+int launch_prefix_tc(const SharedArgs& s, const TcParts& p, bool dependent, cudaStream_t st) {
     Args a{};
     a.s = s;
     a.p = p;
     a.G = s.H / s.HK;
     a.scale2 = 1.4426950408889634f / sqrtf((float)s.D);
     const bool bf = s.dtype == RKV_BF16;
-    if (s.D <= 64) return bf ? launch<1, true>(a, st) : launch<1, false>(a, st);
-    return bf ? launch<2, true>(a, st) : launch<2, false>(a, st);
+    if (s.D <= 64) return bf ? launch<1, true>(a, dependent, st) : launch<1, false>(a, dependent, st);
+    return bf ? launch<2, true>(a, dependent, st) : launch<2, false>(a, dependent, st);
 }
 
 }  // namespace rkv
