@@ -870,26 +870,31 @@ class Rotary:
         self.dim_head, self.num_axes, self.interleaved = dim_head, 1 if num_axes is None else num_axes, bool(interleaved)
         self.c = _Rotary(_ptr(self.freqs), _ptr(self.axes), len(radians), self.num_axes, int(self.interleaved))
         self.ref = ctypes.byref(self.c)
+        self.device, self._int32, self._empty, self._zeros = self.freqs.device, torch.int32, torch.empty, torch.zeros
         self._streams = {_handle(self.freqs.device, None)}  # whose work its buffers outlive
 
     def _buffers(self):
         return (self.freqs,) if self.axes is None else (self.freqs, self.axes)
 
 
-def _check_positions(positions, rotary, batch, n, device):
-    _int32(positions, device, "positions")
-    if positions.numel() != rotary.num_axes * batch * n or tuple(positions.shape)[-2:] != (batch, n):
-        raise ValueError("positions: [num_axes, B, rows], or [B, rows] for one axis")
+_row_refs: dict = {}
 
 
-def _rotated_out(x, out, what):
-    """out, or a fresh one; its strides."""
-    import torch
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-        raise ValueError(f"{what}: the rows' shape, type and device")
-    return out, _row_strides(out, what)
+def _rows_of(t, what, token_major=False):
+    """_row_strides of [B, heads, len, D] (token_major: [B, len, heads, D]) by reference, formed once for a shape, its
+    strides and type."""
+    key = (t.shape, t.stride(), t.dtype, token_major)
+    ref = _row_refs.get(key)
+    if ref is None:
+        if len(_row_refs) >= 4096:
+            _row_refs.clear()
+        ref = _row_refs[key] = ctypes.byref(_row_strides(t.transpose(1, 2) if token_major else t, what))
+    return ref
+
+
+def _positions_ok(positions, rotary, batch, n) -> bool:
+    return (positions.dtype is rotary._int32 and positions.device == rotary.device and positions.is_contiguous()
+            and positions.shape in (((rotary.num_axes, batch, n), (batch, n)) if rotary.num_axes == 1 else ((rotary.num_axes, batch, n),)))
 
 
 def rotate(q, k, positions, rotary: Rotary, q_out=None, k_out=None, stream=None):
@@ -901,27 +906,32 @@ def rotate(q, k, positions, rotary: Rotary, q_out=None, k_out=None, stream=None)
     some = q if q is not None else k
     if some is None:
         raise ValueError("q or k is needed")
-    dev, dt = some.device, _dtype_of(some)
-    for x in (q, k):
-        if x is not None and (x.dim() != 4 or x.shape[0] != some.shape[0] or x.shape[2:] != some.shape[2:] or x.dtype != some.dtype
-                              or x.device != dev):
-            raise ValueError("q and k: [B, heads, len, D], of one batch, length, D, type and device")
-    if rotary.freqs.device != dev or rotary.dim_head != some.shape[3]:
-        raise ValueError("the rows are not of the rotary's device or dim_head")
+    if some.dim() != 4:
+        raise ValueError("q and k: [B, heads, len, D]")
+    dev, dtype = rotary.device, some.dtype
     B, _, n, D = some.shape
-    _check_positions(positions, rotary, B, n, dev)
+    if some.device != dev or D != rotary.dim_head:
+        raise ValueError("the rows are not of the rotary's device or dim_head")
+    if q is not None and k is not None and (k.dim() != 4 or k.shape[0] != B or k.shape[2:] != some.shape[2:] or k.dtype is not dtype
+                                            or k.device != dev):
+        raise ValueError("q and k: one batch, length, D, type and device")
+    if not _positions_ok(positions, rotary, B, n):
+        raise ValueError("positions: contiguous int32 [num_axes, B, len], or [B, len] for one axis, on the rows' device")
+    if (q is not None and q_out is None) or (k is not None and k_out is None):
+        with _on_stream(dev, stream):
+            q_out = rotary._empty(q.shape, dtype=dtype, device=dev) if q is not None and q_out is None else q_out
+            k_out = rotary._empty(k.shape, dtype=dtype, device=dev) if k is not None and k_out is None else k_out
     args = []
-    with _on_stream(dev, stream):
-        for x, out, what in ((q, q_out, "q_out"), (k, k_out, "k_out")):
-            if x is None:
-                args.append((None, None, 0, None, None))
-                continue
-            out, so = _rotated_out(x, out, what)
-            args.append((x, out, x.shape[1], _row_strides(x, what[0]), so))
-    (q, q_out, H, qs, qo), (k, k_out, HK, ks, ko) = args
-    ref = lambda s: None if s is None else ctypes.byref(s)  # noqa: E731
-    _launch(dev, stream, "rkv_rotate", lib().rkv_rotate, rotary.ref, _ptr(positions), _ptr(q), _ptr(q_out), H, _ptr(k), _ptr(k_out), HK,
-            dt, D, n, B, ref(qs), ref(qo), ref(ks), ref(ko), owner=rotary)
+    for x, out in ((q, q_out), (k, k_out)):
+        if x is None:
+            args.append((None, None, 0, None, None))
+            continue
+        if out.shape != x.shape or out.dtype is not dtype or out.device != dev:
+            raise ValueError("q_out and k_out: the rows' shape, type and device")
+        args.append((x.data_ptr(), out.data_ptr(), x.shape[1], _rows_of(x, "q and k"), _rows_of(out, "q_out and k_out")))
+    (qp, qo, H, qs, qos), (kp, ko, HK, ks, kos) = args
+    _launch(dev, stream, "rkv_rotate", lib().rkv_rotate, rotary.ref, positions.data_ptr(), qp, qo, H, kp, ko, HK, _dtype_of(some), D, n, B,
+            qs, qos, ks, kos, owner=rotary)
     return q_out, k_out
 
 
@@ -933,42 +943,43 @@ def paged_append_rotated(cache: PagedCache, k, v, rotary: Rotary, q=None, q_out=
     [B] for one row, where there is one axis), each row's token index without.
     q_out: as q; a fresh one without, 0 in the rows behind n_new.  Returns it
     (None without q)."""
-    import torch
     one = k.dim() == 3
     if one:
         k, v = k[:, None], v[:, None]
         q, q_out = (None if x is None else x[:, None] for x in (q, q_out))
-    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != cache.K.dtype or v.dtype != k.dtype or k.dim() != 4:
+        if positions is not None and positions.dim() == 1:
+            positions = positions[:, None]
+    K, dev = cache.K, rotary.device
+    strides, dtype = k.stride(), k.dtype
+    if k.shape != v.shape or strides != v.stride() or dtype is not K.dtype or v.dtype is not dtype or len(strides) != 4:
         raise ValueError("k and v: one shape, layout and the cache's type")
-    dev = cache.K.device
     B, n, hk, d = k.shape
-    if B != cache.batch or hk != cache.K.shape[1] or d != cache.K.shape[3] or (d > 1 and k.stride(3) != 1):
+    if B != cache.batch or hk != K.shape[1] or d != K.shape[3] or (d > 1 and strides[3] != 1):
         raise ValueError("k, v: [B, n_rows, HK, D] of the cache's geometry, unit stride along D")
-    if k.device != dev or v.device != dev or rotary.freqs.device != dev or rotary.dim_head != d:
+    if k.device != dev or v.device != dev or K.device != dev or rotary.dim_head != d:
         raise ValueError("k, v and the rotary: on the cache's device, of its dim_head")
     if B and cache._lens is None:
         raise ValueError("the cache's lens are needed")
-    if n_new is not None:
-        _int32(n_new, dev, "n_new")
-        if n_new.numel() != B:
-            raise ValueError("n_new: one entry per sequence")
-    if positions is not None:
-        _check_positions(positions[..., None] if one and positions.shape[-1:] == (B,) and positions.dim() <= 2 else positions, rotary, B, n, dev)
-    H, qs, qo = 0, None, None
+    if n_new is not None and (n_new.dtype is not rotary._int32 or n_new.device != dev or n_new.numel() != B or not n_new.is_contiguous()):
+        raise ValueError("n_new: contiguous int32, one entry per sequence, on the cache's device")
+    if positions is not None and not _positions_ok(positions, rotary, B, n):
+        raise ValueError("positions: contiguous int32 [num_axes, B, n_rows], or [B, n_rows] for one axis, on the cache's device")
+    H = qp = qo = 0
+    qs = qos = None
     if q is not None:
-        if q.dim() != 4 or q.shape[0] != B or q.shape[1] != n or q.shape[3] != d or q.dtype != k.dtype or q.device != dev:
+        if q.dim() != 4 or q.shape[0] != B or q.shape[1] != n or q.shape[3] != d or q.dtype is not dtype or q.device != dev:
             raise ValueError("q: [B, n_rows, H, D] of the cache's type, on its device")
-        H = q.shape[2]
         if q_out is None:
             with _on_stream(dev, stream):
                 # without n_new every row is written
-                q_out = (torch.empty if n_new is None else torch.zeros)(q.shape, dtype=q.dtype, device=dev)
-        q_out, qo = _rotated_out(q.transpose(1, 2), q_out.transpose(1, 2), "q_out")
-        qs, q_out = _row_strides(q.transpose(1, 2), "q"), q_out.transpose(1, 2)
+                q_out = (rotary._empty if n_new is None else rotary._zeros)(q.shape, dtype=dtype, device=dev)
+        if q_out.shape != q.shape or q_out.dtype is not dtype or q_out.device != dev:
+            raise ValueError("q_out: q's shape, type and device")
+        H, qp, qo = q.shape[2], q.data_ptr(), q_out.data_ptr()
+        qs, qos = _rows_of(q, "q", True), _rows_of(q_out, "q_out", True)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    ks = _row_strides(k.transpose(1, 2), "k")
-    ref = lambda s: None if s is None else ctypes.byref(s)  # noqa: E731
-    _launch(dev, stream, "rkv_paged_append_rotated", lib().rkv_paged_append_rotated, cache.ref, rotary.ref, _ptr(positions), _ptr(k),
-            _ptr(v), ref(ks), n, B, _ptr(n_new), _ptr(q), ref(qs), _ptr(q_out), ref(qo), H, owner=rotary)
+    _launch(dev, stream, "rkv_paged_append_rotated", lib().rkv_paged_append_rotated, cache.ref, rotary.ref,
+            None if positions is None else positions.data_ptr(), k.data_ptr(), v.data_ptr(), _rows_of(k, "k", True), n, B,
+            None if n_new is None else n_new.data_ptr(), qp, qs, qo, qos, H, owner=rotary)
     return q_out[:, 0] if one and q_out is not None else q_out
