@@ -142,8 +142,8 @@ int prefix_check(int dtype, int H, int HK, int D, int max_len, int batch, int gr
 // The shared tokens on the tcgen05 tensor cores: 16-bit types where a group of mean size has more rows of a KV head
 // than two CTAs of the matrix-instruction kernel take.
 bool on_tc(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
-    const double tiles = ((double)groups + (double)batch * (H / HK) / kTcRows) * HK * ((double)max_len / kTcKeys + 1);
-    return dtype != RKV_F32 && D <= 128 && (long long)batch * (H / HK) > 16LL * groups && tiles < 1e9;  // counted in 32 bits
+    const double tiles = ((double)groups + (double)batch * (H / HK) / 128) * HK * ((double)max_len / 64 + 1);
+    return dtype != RKV_F32 && (long long)batch * (H / HK) > 16LL * groups && tiles < 1e9;  // counted in 32 bits
 }
 
 struct PrefixPlan {

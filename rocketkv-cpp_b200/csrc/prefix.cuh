@@ -81,8 +81,8 @@ struct SharedArgs {
 // Parts of every sequence's own tokens, and of every group's shared ones for the matrix-instruction kernel.
 int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch);
 int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups);
-// The shared tokens on the tcgen05 tensor cores (prefix_tc.cu): 16-bit types.  A unit is up to 256 rows of one group
-// and KV head; the tiles of the units are cut into stretches, one or more per CTA.  A unit's first stretch leaves its
+// The shared tokens on the tcgen05 tensor cores (prefix_tc.cu): 16-bit types.  A unit is up to 256 rows (128 above 128
+// columns) of one group and KV head; the tiles of the units are cut into stretches, one or more per CTA.  A unit's first stretch leaves its
 // rows in first (row b H + h), a stretch that begins inside a unit in later (256 rows per CTA).  first_later[row]: how
 // many stretches follow the first one, and the row of the first of them in later; the others' are 256 further each.
 struct TcParts {
@@ -94,7 +94,6 @@ struct TcParts {
     int* err;
 };
 constexpr int kTcSms = 148;
-constexpr int kTcKeys = 128;
 constexpr int kTcRows = 256;
 // Parts of a row's shared tokens at most.
 constexpr int kMaxShared = 152;
