@@ -115,7 +115,7 @@ struct DecodeArgs {
     SharedArgs sh;
     TcParts tc;
     Result res;
-    int slot0;         // of a row's parts, the first of this pass
+    int shared_blocks;  // CTAs of shared tokens, before those of own ones
     int units;         // shared tokens: row groups of all groups at most
     int prefix_parts;  // of the shared tokens at most, 0 where they are not this kernel's
 };
@@ -147,9 +147,9 @@ __device__ __forceinline__ float warp_sum(float x) {
     return x;
 }
 // What a launch of the decode kernel attends: all tokens of every sequence; or, of a batch that shares leading tokens,
-// every sequence's own, every group's shared ones with the rows of all its sequences, or the own ones last, joined with
-// the others' parts.
-enum { PASS_ALL = 0, PASS_OWN = 1, PASS_SHARED = 2, PASS_LAST = 3 };
+// parts of every group's shared ones with the rows of all its sequences, and of every sequence's own; or the own ones
+// last, joined with the others' parts.
+enum { PASS_ALL = 0, PASS_PARTS = 1, PASS_LAST = 2 };
 
 enum { KIND_F16 = 0, KIND_BF16 = 1, KIND_F32 = 2 };
 
@@ -189,7 +189,7 @@ __device__ __forceinline__ void merge_warps(const DecodeArgs& a, size_t head0, i
 
 // The same for a part of a pass: a warp's share of a row is formed once (in fs [warps][rows]), four columns at a time.
 template <int W, typename Head>
-__device__ __forceinline__ void merge_part(const DecodeArgs& a, Head head_of, int ng, int split, const float* ms, const float* ls,
+__device__ __forceinline__ void merge_part(const DecodeArgs& a, Head head_of, int ng, int slot, const float* ms, const float* ls,
                                            const float* os, float* fs, int rows, int pitch) {
     for (int i = threadIdx.x; i < W * ng; i += W * 32) {
         const int w = i / ng, g = i - w * ng;
@@ -201,7 +201,7 @@ __device__ __forceinline__ void merge_part(const DecodeArgs& a, Head head_of, in
             float ll = 0.0f;
 #pragma unroll
             for (int v = 0; v < W; ++v) ll = fmaf(ls[v * rows + g], exp2f(ms[v * rows + g] - finite_max(mm)), ll);
-            a.part_ml[head_of(g) * a.sh.slots + a.slot0 + split] = make_float2(mm, ll);
+            a.part_ml[head_of(g) * a.sh.slots + slot] = make_float2(mm, ll);
         }
     }
     __syncthreads();
@@ -215,7 +215,7 @@ __device__ __forceinline__ void merge_part(const DecodeArgs& a, Head head_of, in
             const float4 v = *reinterpret_cast<const float4*>(os + (w * rows + g) * pitch + d);
             o = make_float4(fmaf(v.x, c, o.x), fmaf(v.y, c, o.y), fmaf(v.z, c, o.z), fmaf(v.w, c, o.w));
         }
-        *reinterpret_cast<float4*>(a.part_o + (head_of(g) * a.sh.slots + a.slot0 + split) * a.D + d) = o;
+        *reinterpret_cast<float4*>(a.part_o + (head_of(g) * a.sh.slots + slot) * a.D + d) = o;
     }
 }
 
@@ -424,11 +424,11 @@ struct Shape {
 // (all types hold P then); fp16's P is kept 2^7 larger, away from the type's
 // smallest numbers.
 //
-// The passes of a batch that shares leading tokens (PASS) differ in which rows
-// and tokens a CTA has: own tokens begin behind the shared ones; a group's
-// shared tokens take the rows (sequence, head) of all its sequences, 8 NT at a
-// time, the row groups of one stretch of tokens side by side, so that the L2
-// cache serves all but the first.
+// For a batch that shares leading tokens (PASS) it differs in which rows and
+// tokens a CTA has: own tokens begin behind the shared ones; a group's shared
+// tokens take the rows (sequence, head) of all its sequences, 8 NT at a time,
+// the row groups of one stretch of tokens side by side, so that the L2 cache
+// serves all but the first.
 template <typename S, int PASS>
 __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const DecodeArgs a) {
     constexpr int KIND = S::KIND, DP = S::DP, NT = S::NT, W = S::W, SLOTS = S::SLOTS;
@@ -449,7 +449,14 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
     int split, b, hk, h0, ng, first = 0, shared = 0;  // b: whose table row; first: the group's first sequence
     Visible vis;
     int chunk = a.chunk;
-    if (PASS == PASS_SHARED) {
+    bool rows_of_group = false;  // the CTA's rows are of a group's sequences, not of one
+    int parts = a.splits;
+    if (PASS == PASS_PARTS) {
+        rows_of_group = id < a.shared_blocks;
+        if (rows_of_group) parts = a.prefix_parts;
+        else id -= a.shared_blocks;
+    }
+    if (PASS == PASS_PARTS && rows_of_group) {
         const int unit = (int)(id % a.units);
         id /= a.units;
         hk = (int)(id % a.HK);
@@ -479,7 +486,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
         h0 = (unit - before) * 8 * NT;  // row of the group
         ng = g < 0 ? 0 : min(8 * NT, a.sh.gr.size(g) * a.G - h0);
         b = g < 0 ? 0 : leader_of(a.sh.gr, a.c, g, vis.n);
-        chunk = part_tokens(vis.n, a.splits, kSharedLeast);
+        chunk = part_tokens(vis.n, parts, kSharedLeast);
     } else {
         split = (int)(id % a.splits);
         id /= a.splits;
@@ -488,13 +495,13 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
         hk = (int)(id % a.HK);
         b = (int)(id / a.HK);
         vis = visible(a, b);
-        if (PASS == PASS_OWN || PASS == PASS_LAST) {
+        if (PASS != PASS_ALL) {
             shared = member_of(a.sh.gr, a.c, b, vis.n).tokens;
             vis.sinks = 0;
             vis.gap = shared;
             vis.nvis = vis.n - shared;
             chunk = PASS == PASS_LAST ? vis.nvis : part_tokens(vis.nvis, a.splits, kOwnLeast);
-            if (PASS == PASS_OWN && split == 0 && tid < min(8 * NT, a.G - grp * 8 * NT)) {
+            if (PASS == PASS_PARTS && split == 0 && tid < min(8 * NT, a.G - grp * 8 * NT)) {
                 a.sh.info[(size_t)b * a.H + hk * a.G + grp * 8 * NT + tid] =
                     make_int2((vis.nvis + chunk - 1) / chunk, shared_parts(a, shared));
             }
@@ -511,7 +518,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
     const int v0 = (int)v_lo, v1 = (int)min((long long)vis.nvis, v_lo + chunk);
     // row i of the CTA: its query head among all sequences', and its query
     auto head_of = [&](int i) -> size_t {
-        if (PASS != PASS_SHARED) return (size_t)b * a.H + h0 + i;
+        if (!(PASS == PASS_PARTS && rows_of_group)) return (size_t)b * a.H + h0 + i;
         const unsigned r = (unsigned)(h0 + i), s = r / (unsigned)a.G;
         return (size_t)(first + s) * a.H + hk * a.G + (r - s * a.G);
     };
@@ -558,7 +565,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
     // q^T fragments
     const uint8_t* qb = a.Q + (size_t)b * a.q_stride;
     auto query_of = [&](int i) -> const uint8_t* {
-        if (PASS != PASS_SHARED) return qb + (size_t)(h0 + i) * D * S::SIZE;
+        if (!(PASS == PASS_PARTS && rows_of_group)) return qb + (size_t)(h0 + i) * D * S::SIZE;
         const unsigned r = (unsigned)(h0 + i), s = r / (unsigned)a.G;
         return a.Q + (size_t)(first + s) * a.q_stride + (size_t)(hk * a.G + (r - s * a.G)) * D * S::SIZE;
     };
@@ -841,7 +848,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
         static_assert(S::MERGE + (W + 1 + kMaxShared) * 8 * NT * 4 <= S::RING, "the shares lie in the ring too");
         merge_last<KIND, W>(a, head_of, ng, shared, ms, ls, os, os + W * 8 * NT * S::PITCH, 8 * NT, S::PITCH);
     } else {
-        merge_part<W>(a, head_of, ng, split, ms, ls, os, os + W * 8 * NT * S::PITCH, 8 * NT, S::PITCH);
+        merge_part<W>(a, head_of, ng, rows_of_group ? a.sh.own + split : split, ms, ls, os, os + W * 8 * NT * S::PITCH, 8 * NT, S::PITCH);
         asm volatile("griddepcontrol.wait;" ::: "memory");
     }
 }
@@ -1013,7 +1020,7 @@ DecodePlan decode_plan(int dtype, int H, int HK, int D, long long visible_max, i
 
 template <int KIND, int DP, int NT, int PASS>
 int launch_shape(const DecodeArgs& a, long long blocks, bool dependent, cudaStream_t st) {
-    using S = Shape<KIND, DP, NT, PASS == PASS_OWN || PASS == PASS_LAST>;
+    using S = Shape<KIND, DP, NT, PASS != PASS_ALL>;
     static_assert(S::SMEM * S::CTAS + 1024 * S::CTAS <= 228 * 1024, "the CTAs of an SM fit in its shared memory");
     if (cudaFuncSetAttribute(paged_decode_kernel<S, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
         (void)cudaGetLastError();
@@ -1068,8 +1075,8 @@ int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch) {
 int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
     const int rows = shared_rows(dtype, D, H, HK, batch, groups);
     const long long each = ((long long)batch * (H / HK) + groups * (long long)rows - 1) / (groups * (long long)rows);  // of a group of mean size
-    long long p = 2LL * decode_slots(dtype, D) / (each * groups * HK);
-    const long long most = ((long long)max_len + kMinChunk - 1) / kMinChunk;
+    long long p = 2LL * 2 * decode_slots(dtype, D) / (each * groups * HK);
+    const long long most = ((long long)max_len + kSharedLeast - 1) / kSharedLeast;
     if (p > most) p = most;
     if (p > 128) p = 128;  // of kMaxShared
     return p < 1 ? 1 : (int)p;
@@ -1091,21 +1098,22 @@ int launch_shared_pass(const SharedArgs& s, SharedPass pass, const TcParts& t, c
     a.tc = t;
     a.res = r;
     a.prefix_parts = s.slots - s.own;
-    if (pass == SHARED_TOKENS) {
+    const bool shared = pass == SHARED_TOKENS || pass == ALL_TOKENS, own = pass != SHARED_TOKENS;
+    int gt = 8;
+    if (own) gt = head_group(s.dtype, a.G, s.D);
+    if (shared) {
         const int rows = shared_rows(s.dtype, s.D, s.H, s.HK, s.batch, s.gr.n);
-        const long long units = shared_units(rows, s.H, s.HK, s.batch, s.gr.n);
-        if (units > 0x7FFFFFF) return RKV_ERR_UNSUPPORTED;
+        if (rows > gt) gt = rows;
+        const long long units = shared_units(gt, s.H, s.HK, s.batch, s.gr.n), blocks = units * s.HK * a.prefix_parts;
+        if (blocks > 0x3FFFFFFF) return RKV_ERR_UNSUPPORTED;
         a.units = (int)units;
-        a.slot0 = s.own;
-        a.splits = a.prefix_parts;
-        return launch_pass<PASS_SHARED>(a, s.dtype, rows, units * s.HK * a.splits, dependent, st);
+        a.shared_blocks = (int)blocks;
     }
-    const int gt = head_group(s.dtype, a.G, s.D);
     a.ngroups = (a.G + gt - 1) / gt;
     a.splits = pass == OWN_AND_JOIN ? 1 : s.own;
-    const long long blocks = (long long)s.batch * s.HK * a.ngroups * a.splits;
+    const long long blocks = a.shared_blocks + (own ? (long long)s.batch * s.HK * a.ngroups * a.splits : 0);
     return pass == OWN_AND_JOIN ? launch_pass<PASS_LAST>(a, s.dtype, gt, blocks, dependent, st)
-                                : launch_pass<PASS_OWN>(a, s.dtype, gt, blocks, dependent, st);
+                                : launch_pass<PASS_PARTS>(a, s.dtype, gt, blocks, dependent, st);
 }
 
 }  // namespace rkv

@@ -6,11 +6,11 @@
 // (largest score, sum 2^(x - m), sum 2^(x - m) v) with x = q k log2(e) / sqrt(D),
 // join as (M, sum l 2^(m - M), sum o 2^(m - M)).  A group's shared rows of K and V
 // meet the queries of all its sequences at once, so they are read once and
-// not once per sequence.  Three kernels: every sequence's own tokens, the
-// shared ones (both of paged.cu, or the latter on the tcgen05 tensor cores,
-// prefix_tc.cu) and the join; or, where the sequences alone fill the GPU, the
-// shared tokens and the own ones with the join.  Each is begun while the one
-// before still runs.
+// not once per sequence.  Two or three kernels: every sequence's own tokens
+// with the shared ones (paged.cu), or before them where these run on the
+// tcgen05 tensor cores (prefix_tc.cu), then the join; or, where the sequences
+// alone fill the GPU, the shared tokens, then the own ones with the join.  Each
+// is begun while the one before still runs.
 #include "prefix.cuh"
 
 namespace rkv {
@@ -232,18 +232,14 @@ extern "C" int rkv_prefix_decode(const void* Q, long long q_item_stride, int num
     } else {
         a.r.clear = static_cast<int*>(workspace);
     }
-    auto shared = [&](bool dependent) {
-        return p.tc             ? launch_prefix_tc(s, a.tc, dependent, st)
-               : num_groups > 0 ? launch_shared_pass(s, SHARED_TOKENS, a.tc, a.r, dependent, st)
-                                : (int)RKV_OK;
-    };
     if (p.own == 1) {
         // as many sequences as there is room for CTAs: each takes its own tokens in one part and joins the others' to it
-        rc = shared(false);
+        if (p.tc) rc = launch_prefix_tc(s, a.tc, false, st);
+        else if (num_groups > 0) rc = launch_shared_pass(s, SHARED_TOKENS, a.tc, a.r, false, st);
         return rc ? rc : launch_shared_pass(s, OWN_AND_JOIN, a.tc, a.r, num_groups > 0, st);
     }
-    rc = launch_shared_pass(s, OWN_TOKENS, a.tc, a.r, false, st);
-    if (!rc) rc = shared(true);
+    rc = launch_shared_pass(s, num_groups > 0 && !p.tc ? ALL_TOKENS : OWN_TOKENS, a.tc, a.r, false, st);
+    if (!rc && p.tc) rc = launch_prefix_tc(s, a.tc, true, st);
     if (rc) return rc;
     return s.dtype == RKV_F32 ? launch_join<float>(a, st) : s.dtype == RKV_BF16 ? launch_join<__nv_bfloat16>(a, st) : launch_join<__half>(a, st);
 }

@@ -114,9 +114,9 @@ struct Result {
     int* clear;
 };
 
-// The passes of the matrix-instruction kernel: every sequence's own tokens; the groups' shared ones; or the own ones
-// in one part, joined with the parts of the shared ones that the launch before has left.
-enum SharedPass { OWN_TOKENS, SHARED_TOKENS, OWN_AND_JOIN };
+// Passes of the matrix-instruction kernel: the groups' shared tokens, every sequence's own, or both; or the own ones in
+// one part, joined with the parts of the shared ones that the launch before has left.
+enum SharedPass { SHARED_TOKENS, OWN_TOKENS, ALL_TOKENS, OWN_AND_JOIN };
 // dependent: launched while the kernel before it still runs, which it waits for at its end only.
 int launch_shared_pass(const SharedArgs& s, SharedPass pass, const TcParts& t, const Result& r, bool dependent, cudaStream_t st);
 // dependent as above.
