@@ -119,7 +119,7 @@ struct Result {
 enum SharedPass { SHARED_TOKENS, OWN_TOKENS, ALL_TOKENS, OWN_AND_JOIN };
 // dependent: launched while the kernel before it still runs, which it waits for at its end only.
 int launch_shared_pass(const SharedArgs& s, SharedPass pass, const TcParts& t, const Result& r, bool dependent, cudaStream_t st);
-// dependent as above.
-int launch_prefix_tc(const SharedArgs& s, const TcParts& p, bool dependent, cudaStream_t st);
+// spare: CTAs of the kernel before that hold an SM each; dependent as above.
+int launch_prefix_tc(const SharedArgs& s, const TcParts& p, int spare, bool dependent, cudaStream_t st);
 
 }  // namespace rkv

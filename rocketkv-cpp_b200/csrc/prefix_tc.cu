@@ -50,6 +50,7 @@ struct Args {
     TcParts p;
     int G;
     int box;       // tokens of a box, a power of two that divides the page size; 0: none, copies by 16 bytes
+    int spare;     // SMs that may be left to the kernel before, at most half of all
     float scale2;  // log2(e) / sqrt(D)
 };
 
@@ -121,7 +122,8 @@ __device__ __forceinline__ Group group_of(const Args& a, int g) {
 // more to do than an equal share, the tiles of all units are one list that is cut into equal stretches: a CTA whose
 // stretch spans two units pays the ends of a unit (4 us) twice.
 constexpr int kAligned = 3;
-constexpr int kMinTiles = 2;  // of a stretch
+constexpr int kSpare = 4;  // tiles more of a CTA at most for SMs that are left to the own tokens' CTAs
+__host__ __device__ constexpr int min_tiles(int kb) { return 128 / tile_keys(kb); }  // of a stretch
 template <int KB>
 struct Walk {
     int total, ctas;  // tiles, CTAs that take them
@@ -131,7 +133,7 @@ struct Walk {
 
     __device__ __forceinline__ Group group(const Args& a, int g0, int lane) const { return g0 == 0 ? mine : group_of<KB>(a, g0 + lane); }
     __device__ __forceinline__ int parts(const Group& t) const {  // aligned: of a unit
-        return max(1, min((int)((unsigned)ctas * t.tiles / (unsigned)total), t.tiles / kMinTiles));
+        return max(1, min((int)((unsigned)ctas * t.tiles / (unsigned)total), t.tiles / min_tiles(KB)));
     }
     __device__ __forceinline__ void begin_walk(const Args& a, int lane) {
         mine = group_of<KB>(a, lane);
@@ -141,7 +143,9 @@ struct Walk {
             n += t.units * t.tiles;
         }
         total = __reduce_add_sync(0xffffffffu, n);
-        ctas = gridDim.x;
+        // the own tokens' CTAs, begun before, hold their SMs for about as long as four tiles take
+        const int all = gridDim.x, few = all - a.spare;
+        ctas = (total + few - 1) / few <= (total + all - 1) / all + kSpare ? few : all;
         at = end = 0;
         aligned = true;
         if (total > 0) {
@@ -156,12 +160,12 @@ struct Walk {
             }
             need = __reduce_add_sync(0xffffffffu, need);
             most = __reduce_max_sync(0xffffffffu, most);
-            aligned = need <= ctas && (most <= kMinTiles + 1 || most <= (total + ctas - 1) / ctas + kAligned);
+            aligned = need <= ctas && (most <= min_tiles(KB) + 1 || most <= (total + ctas - 1) / ctas + kAligned);
             const int c = blockIdx.x;
             if (aligned) {
                 end = c < need;
             } else {
-                ctas = min(ctas, (total + kMinTiles - 1) / kMinTiles);
+                ctas = min(ctas, (total + min_tiles(KB) - 1) / min_tiles(KB));
                 if (c < ctas) at = begin(c), end = begin(c + 1);
             }
         }
@@ -720,11 +724,12 @@ int launch(Args& a, bool dependent, cudaStream_t st) {
 
 }  // namespace
 
-int launch_prefix_tc(const SharedArgs& s, const TcParts& p, bool dependent, cudaStream_t st) {
+int launch_prefix_tc(const SharedArgs& s, const TcParts& p, int spare, bool dependent, cudaStream_t st) {
     Args a{};
     a.s = s;
     a.p = p;
     a.G = s.H / s.HK;
+    a.spare = spare < kTcSms / 2 ? spare : kTcSms / 2;
     a.scale2 = 1.4426950408889634f / sqrtf((float)s.D);
     const bool bf = s.dtype == RKV_BF16;
     if (s.D <= 64) return bf ? launch<1, true>(a, dependent, st) : launch<1, false>(a, dependent, st);
