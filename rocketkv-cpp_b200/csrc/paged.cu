@@ -237,60 +237,80 @@ __device__ __forceinline__ int shared_parts(const DecodeArgs& a, int shared) {
 }
 
 // The end of the last pass: the warps' (m, l, o) and the parts of the shared tokens, joined; o [warps][rows][pitch],
-// then room for fs [warps][rows], [rows] 1 / l and the parts' shares [rows][kMaxShared].
+// then room for fs [warps][rows], [rows] 1 / l, [rows] where the parts are and their shares [rows][kMaxShared].  A
+// thread's first part rows are on their way while half a warp per row forms the shares.
 template <int KIND, int W, typename Head>
 __device__ __forceinline__ void merge_last(const DecodeArgs& a, Head head_of, int ng, int shared, const float* ms, const float* ls,
                                            const float* os, float* fs, int rows, int pitch) {
+    constexpr int U = 12;  // parts on their way together
     float* inv = fs + W * rows;
-    float* share = inv + rows;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int2* xs = reinterpret_cast<int2*>(inv + rows);
+    float* share = inv + 3 * rows;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the shared tokens' parts are there
     if (a.res.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.res.clear = 0;
-    const int own_parts = shared_parts(a, shared);
-    for (int g = warp; g < ng; g += W) {
+    const int some = shared_parts(a, shared);
+    if ((int)threadIdx.x < ng) xs[threadIdx.x] = a.tc.first_o && some > 0 ? a.tc.first_later[head_of(threadIdx.x)] : make_int2(0, 0);
+    __syncthreads();
+    const int per = a.D / 4;
+    float4 v[U];
+    auto load = [&](int i, int p0) {
+        const int g = i / per, d = (i - g * per) * 4;
+        const int2 x = xs[g];
         const size_t row = head_of(g);
-        int2 x = make_int2(0, 0);
-        if (a.tc.first_o && own_parts > 0) x = a.tc.first_later[row];
-        const int parts = own_parts + x.x;
-        float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < W; ++w) top = fmaxf(top, ms[w * rows + g]);
-        for (int p = lane; p < parts; p += 32) top = fmaxf(top, shared_ml(a.sh, a.tc, row, x, p).x);
-        const float base = finite_max(warp_max(top));
-        float l = lane < W ? ls[lane * rows + g] * exp2f(ms[lane * rows + g] - base) : 0.0f;
-        if (lane < W) fs[lane * rows + g] = exp2f(ms[lane * rows + g] - base);
-        for (int p = lane; p < parts; p += 32) {
-            const float2 v = shared_ml(a.sh, a.tc, row, x, p);
-            const float f = exp2f(v.x - base);
-            share[g * kMaxShared + p] = f;
-            l = fmaf(v.y, f, l);
+        for (int p = 0; p < U; ++p)
+            v[p] = p0 + p < some + x.x ? *reinterpret_cast<const float4*>(shared_o(a.sh, a.tc, row, x, p0 + p) + d) : make_float4(0, 0, 0, 0);
+    };
+    if ((int)threadIdx.x < ng * per) load(threadIdx.x, 0);
+    const int l16 = threadIdx.x & 15;
+    for (int g0 = 0; g0 < ng; g0 += W * 2) {
+        const int g = g0 + (threadIdx.x >> 4);
+        const bool have = g < ng;
+        const int2 x = have ? xs[g] : make_int2(0, 0);
+        const size_t row = have ? head_of(g) : 0;
+        const int parts = have ? some + x.x : 0;
+        const float2 none = make_float2(-INFINITY, 0.0f);
+        const float2 own = have && l16 < W ? make_float2(ms[l16 * rows + g], ls[l16 * rows + g]) : none;
+        float2 ml[2];  // the first 32 parts'
+#pragma unroll
+        for (int k = 0; k < 2; ++k) ml[k] = l16 + 16 * k < parts ? shared_ml(a.sh, a.tc, row, x, l16 + 16 * k) : none;
+        float top = fmaxf(own.x, fmaxf(ml[0].x, ml[1].x));
+        for (int p = l16 + 32; p < parts; p += 16) top = fmaxf(top, shared_ml(a.sh, a.tc, row, x, p).x);
+#pragma unroll
+        for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float base = finite_max(top);
+        float l = 0.0f;
+        if (have && l16 < W) {
+            const float f = exp2f(own.x - base);
+            fs[l16 * rows + g] = f;
+            l = own.y * f;
         }
-        l = warp_sum(l);
-        if (lane == 0) {
+        for (int p = l16; p < parts; p += 16) {
+            const float2 m = p == l16 ? ml[0] : p == l16 + 16 ? ml[1] : shared_ml(a.sh, a.tc, row, x, p);
+            const float f = exp2f(m.x - base);
+            share[g * kMaxShared + p] = f;
+            l = fmaf(m.y, f, l);
+        }
+#pragma unroll
+        for (int o = 8; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (have && l16 == 0) {
             inv[g] = l == 0.0f ? 0.0f : 1.0f / l;
             if (a.res.lse) a.res.lse[row] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945f;
         }
     }
     __syncthreads();
-    const int per = a.D / 4;
     for (int i = threadIdx.x; i < ng * per; i += W * 32) {
-        const int g = i / per, d = (i - g * per) * 4;
+        const int g = i / per, d = (i - g * per) * 4, parts = some + xs[g].x;
         const size_t row = head_of(g);
-        int2 x = make_int2(0, 0);
-        if (a.tc.first_o && own_parts > 0) x = a.tc.first_later[row];
-        const int parts = own_parts + x.x;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        auto add = [&](const float4& v, float c) {
-            o = make_float4(fmaf(v.x, c, o.x), fmaf(v.y, c, o.y), fmaf(v.z, c, o.z), fmaf(v.w, c, o.w));
+        auto add = [&](const float4& y, float c) {
+            o = make_float4(fmaf(y.x, c, o.x), fmaf(y.y, c, o.y), fmaf(y.z, c, o.z), fmaf(y.w, c, o.w));
         };
+        if (i != (int)threadIdx.x) load(i, 0);
 #pragma unroll
         for (int w = 0; w < W; ++w) add(*reinterpret_cast<const float4*>(os + (w * rows + g) * pitch + d), fs[w * rows + g]);
-        constexpr int U = 8;  // parts on their way together
         for (int p0 = 0; p0 < parts; p0 += U) {
-            float4 v[U];
-#pragma unroll
-            for (int p = 0; p < U; ++p)
-                v[p] = p0 + p < parts ? *reinterpret_cast<const float4*>(shared_o(a.sh, a.tc, row, x, p0 + p) + d) : make_float4(0, 0, 0, 0);
+            if (p0 > 0) load(i, p0);
 #pragma unroll
             for (int p = 0; p < U; ++p)
                 if (p0 + p < parts) add(v[p], share[g * kMaxShared + p0 + p]);
@@ -845,7 +865,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
     if (PASS == PASS_ALL) {
         merge_warps<W>(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, 8 * NT, S::PITCH);
     } else if (PASS == PASS_LAST) {
-        static_assert(S::MERGE + (W + 1 + kMaxShared) * 8 * NT * 4 <= S::RING, "the shares lie in the ring too");
+        static_assert(S::MERGE + (W + 3 + kMaxShared) * 8 * NT * 4 <= S::RING, "the shares lie in the ring too");
         merge_last<KIND, W>(a, head_of, ng, shared, ms, ls, os, os + W * 8 * NT * S::PITCH, 8 * NT, S::PITCH);
     } else {
         merge_part<W>(a, head_of, ng, rows_of_group ? a.sh.own + split : split, ms, ls, os, os + W * 8 * NT * S::PITCH, 8 * NT, S::PITCH);
