@@ -862,9 +862,9 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
             }
         }
     __syncthreads();
-    if (PASS == PASS_ALL) {
+    if constexpr (PASS == PASS_ALL) {
         merge_warps<W>(a, (size_t)b * a.H + h0, ng, split, ms, ls, os, 8 * NT, S::PITCH);
-    } else if (PASS == PASS_LAST) {
+    } else if constexpr (PASS == PASS_LAST) {
         static_assert(S::MERGE + (W + 3 + kMaxShared) * 8 * NT * 4 <= S::RING, "the shares lie in the ring too");
         merge_last<KIND, W>(a, head_of, ng, shared, ms, ls, os, os + W * 8 * NT * S::PITCH, 8 * NT, S::PITCH);
     } else {
@@ -1040,7 +1040,7 @@ DecodePlan decode_plan(int dtype, int H, int HK, int D, long long visible_max, i
 
 template <int KIND, int DP, int NT, int PASS>
 int launch_shape(const DecodeArgs& a, long long blocks, bool dependent, cudaStream_t st) {
-    using S = Shape<KIND, DP, NT, PASS != PASS_ALL>;
+    using S = Shape<KIND, DP, NT, PASS != PASS_ALL && NT < 4>;
     static_assert(S::SMEM * S::CTAS + 1024 * S::CTAS <= 228 * 1024, "the CTAs of an SM fit in its shared memory");
     if (cudaFuncSetAttribute(paged_decode_kernel<S, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
         (void)cudaGetLastError();
@@ -1059,6 +1059,9 @@ int launch_kind(const DecodeArgs& a, int gt, long long blocks, bool dependent, c
     if constexpr (KIND != KIND_F32) {
         if (gt == 16)
             return a.D <= 64 ? launch_shape<KIND, 64, 2, PASS>(a, blocks, dependent, st) : launch_shape<KIND, 128, 2, PASS>(a, blocks, dependent, st);
+    } else if constexpr (PASS == PASS_PARTS) {
+        if (gt == 32)
+            return launch_shape<KIND, 128, 4, PASS>(a, blocks, dependent, st);
     }
     if (a.D <= 64) return launch_shape<KIND, 64, 1, PASS>(a, blocks, dependent, st);
     if (a.D <= 128) return launch_shape<KIND, 128, 1, PASS>(a, blocks, dependent, st);
@@ -1073,10 +1076,16 @@ int launch_pass(const DecodeArgs& a, int dtype, int gt, long long blocks, bool d
         default: return launch_kind<KIND_F16, PASS>(a, gt, blocks, dependent, st);
     }
 }
-// Rows of a group that one CTA of the prefix pass takes.
+}  // namespace
+// Rows of a group that one CTA takes: as many as a group of mean size has, up to what fits in the registers.  fp32's
+// operands are split once for all of them: 20 sequences behind 56208 tokens, 24/8 heads of 128, 395 us with 32 rows and
+// 503 with 8; with 64 columns 42 and 36, with 256 columns there is room for 8 alone.
 int shared_rows(int dtype, int D, int H, int HK, int batch, int groups) {
-    return head_group(dtype, (int)(((long long)batch * (H / HK) + groups - 1) / groups > 8 ? 9 : 1), D);
+    const long long rows = ((long long)batch * (H / HK) + groups - 1) / groups;
+    if (dtype == RKV_F32) return rows > 16 && D > 64 && D <= 128 ? 32 : 8;
+    return head_group(dtype, rows > 8 ? 9 : 1, D);
 }
+namespace {
 long long shared_units(int rows, int H, int HK, int batch, int groups) { return groups + (long long)batch * (H / HK) / rows; }
 
 }  // namespace

@@ -238,7 +238,10 @@ extern "C" int rkv_prefix_decode(const void* Q, long long q_item_stride, int num
         else if (num_groups > 0) rc = launch_shared_pass(s, SHARED_TOKENS, a.tc, a.r, false, st);
         return rc ? rc : launch_shared_pass(s, OWN_AND_JOIN, a.tc, a.r, num_groups > 0, st);
     }
-    rc = launch_shared_pass(s, num_groups > 0 && !p.tc ? ALL_TOKENS : OWN_TOKENS, a.tc, a.r, false, st);
+    // side by side in one launch where both take CTAs of few rows
+    const bool few = num_groups > 0 && !p.tc && shared_rows(s.dtype, D, num_heads, s.HK, batch, num_groups) <= 16;
+    rc = launch_shared_pass(s, few ? ALL_TOKENS : OWN_TOKENS, a.tc, a.r, false, st);
+    if (!rc && num_groups > 0 && !p.tc && !few) rc = launch_shared_pass(s, SHARED_TOKENS, a.tc, a.r, true, st);
     if (!rc && p.tc) rc = launch_prefix_tc(s, a.tc, batch * s.HK, true, st);
     if (rc) return rc;
     return s.dtype == RKV_F32 ? launch_join<float>(a, st) : s.dtype == RKV_BF16 ? launch_join<__nv_bfloat16>(a, st) : launch_join<__half>(a, st);

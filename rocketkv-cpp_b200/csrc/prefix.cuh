@@ -78,6 +78,8 @@ struct SharedArgs {
     float2* part_ml;
     int2* info;
 };
+// Rows of a group that one CTA of the matrix-instruction kernel takes.
+int shared_rows(int dtype, int D, int H, int HK, int batch, int groups);
 // Parts of every sequence's own tokens, and of every group's shared ones for the matrix-instruction kernel.
 int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch);
 int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups);
