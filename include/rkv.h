@@ -471,7 +471,8 @@ int rkv_sink_attention(const void* Q, const void* K, const void* V, int dtype, i
  * freqs: device [pairs], 8-byte aligned, f_i as turns per position in units of
  * 2^-64, as rkv_rotary_frequencies makes them (so that angles of far positions
  * lose nothing: they are off by 2^-25 half turns at most); axes: device
- * [pairs], NULL for axis 0 throughout; a pair of an axis >= num_axes is copied.
+ * [pairs], NULL for axis 0 throughout; a pair of an axis >= num_axes stays at
+ * position 0.
  * num_axes: at most 256.  Positions are 32-bit, negative ones turn back: the
  * gradient of a rotation is the rotation of the gradient by -p.  Sines,
  * cosines, products and sums are fp32, each result is rounded to the type once. */

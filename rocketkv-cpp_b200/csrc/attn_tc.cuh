@@ -92,7 +92,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
     return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, err, abort));
 }
 
-// The driver's tensor-map encoder.
+// cuTensorMapEncodeTiled, looked up once.
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;

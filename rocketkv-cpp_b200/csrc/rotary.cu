@@ -116,7 +116,8 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(const RotArgs a)
     using V = Vec<T, VEC>;
     constexpr int U = kRotAhead;
     extern __shared__ float2 table[];  // [tile][pairs], cosine and sine
-    const int b = blockIdx.z, tid = threadIdx.x, i0 = blockIdx.x * a.tile;
+    const int b = blockIdx.z, tid = threadIdx.x;
+    const long long i0 = (long long)blockIdx.x * a.tile;
     int n = a.rows, first = 0;  // rows of this item; token of row 0
     if (PAGED) {
         if (a.n_new) n = min(max(a.n_new[b], 0), n);
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(const RotArgs a)
         const int axis = a.axes ? a.axes[pair] : 0;
         float2 t = make_float2(1.0f, 0.0f);
         if (i0 + row < n && axis < a.num_axes) {
-            const int p = PAGED && !a.positions ? first + i0 + row : a.positions[((size_t)axis * a.batch + b) * a.rows + i0 + row];
+            const int p = PAGED && !a.positions ? (int)(first + i0 + row) : a.positions[((size_t)axis * a.batch + b) * a.rows + i0 + row];
             const unsigned long long ph = (unsigned long long)(long long)p * a.freqs[pair];
             sincospif((float)(int)(ph >> 32) * 0x1p-31f, &t.y, &t.x);
         }
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(const RotArgs a)
     for (int e = 0; e < VEC; ++e) {
         // neighbouring columns: half of a chunk's pairs lie in each vector
         const int pair = INTER && VEC > 1 ? (e < VEC / 2 ? lo / 2 + e : hi / 2 + e - VEC / 2) : chunk * VEC + e;
-        const float2 t = turn ? table[(i - i0) * a.pairs + pair] : make_float2(1.0f, 0.0f);
+        const float2 t = turn ? table[(int)(i - i0) * a.pairs + pair] : make_float2(1.0f, 0.0f);
         cs[e] = t.x;
         sn[e] = t.y;
     }

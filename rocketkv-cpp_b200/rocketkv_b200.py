@@ -492,11 +492,23 @@ def _stream_object(device, handle: int):
     return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
 
 
+_raw_device = None
+
+
+def _current_device() -> int:
+    global _raw_device
+    if _raw_device is None:
+        import torch
+        torch.cuda.init()
+        _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    return _raw_device()
+
+
 def _launch(device, stream, what, fn, *args, owner=None) -> None:
     """fn(*args, stream) with the tensors' device current (a stream belongs to one)."""
-    import torch
     h = _handle(device, stream)
     if owner is not None and h not in owner._streams:
+        import torch
         # the object's buffers belong to the stream they were made on; dropped with it while this call runs on
         # another one, they would be handed out again at once (the mark lasts, but not one set under a capture)
         other = _stream_object(device, h)
@@ -504,9 +516,10 @@ def _launch(device, stream, what, fn, *args, owner=None) -> None:
             t.record_stream(other)
         if not torch.cuda.is_current_stream_capturing():
             owner._streams.add(h)
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():
         st = fn(*args, h)
     else:
+        import torch
         with torch.cuda.device(device):
             st = fn(*args, h)
     if st != RKV_OK:
@@ -867,10 +880,13 @@ class Rotary:
                 raise ValueError("axes: below num_axes, which is at most 256")
             self.axes = axes.to(torch.uint8).to(device)
         self.freqs = freqs.to(device)
+        if not self.freqs.is_cuda:
+            raise TypeError("device: a CUDA device")
         self.dim_head, self.num_axes, self.interleaved = dim_head, 1 if num_axes is None else num_axes, bool(interleaved)
         self.c = _Rotary(_ptr(self.freqs), _ptr(self.axes), len(radians), self.num_axes, int(self.interleaved))
         self.ref = ctypes.byref(self.c)
         self.device, self._int32, self._empty, self._zeros = self.freqs.device, torch.int32, torch.empty, torch.zeros
+        self._types = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
         self._streams = {_handle(self.freqs.device, None)}  # whose work its buffers outlive
 
     def _buffers(self):
@@ -910,8 +926,9 @@ def rotate(q, k, positions, rotary: Rotary, q_out=None, k_out=None, stream=None)
         raise ValueError("q and k: [B, heads, len, D]")
     dev, dtype = rotary.device, some.dtype
     B, _, n, D = some.shape
-    if some.device != dev or D != rotary.dim_head:
-        raise ValueError("the rows are not of the rotary's device or dim_head")
+    kind = rotary._types.get(dtype)
+    if some.device != dev or D != rotary.dim_head or kind is None:
+        raise ValueError("the rows are not of the rotary's device or dim_head, or of no type that is turned")
     if q is not None and k is not None and (k.dim() != 4 or k.shape[0] != B or k.shape[2:] != some.shape[2:] or k.dtype is not dtype
                                             or k.device != dev):
         raise ValueError("q and k: one batch, length, D, type and device")
@@ -930,7 +947,7 @@ def rotate(q, k, positions, rotary: Rotary, q_out=None, k_out=None, stream=None)
             raise ValueError("q_out and k_out: the rows' shape, type and device")
         args.append((x.data_ptr(), out.data_ptr(), x.shape[1], _rows_of(x, "q and k"), _rows_of(out, "q_out and k_out")))
     (qp, qo, H, qs, qos), (kp, ko, HK, ks, kos) = args
-    _launch(dev, stream, "rkv_rotate", lib().rkv_rotate, rotary.ref, positions.data_ptr(), qp, qo, H, kp, ko, HK, _dtype_of(some), D, n, B,
+    _launch(dev, stream, "rkv_rotate", lib().rkv_rotate, rotary.ref, positions.data_ptr(), qp, qo, H, kp, ko, HK, kind, D, n, B,
             qs, qos, ks, kos, owner=rotary)
     return q_out, k_out
 
