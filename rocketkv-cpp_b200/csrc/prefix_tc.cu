@@ -30,6 +30,15 @@
 // operands in one type); scores, m, l and the accumulators are fp32.  Every
 // row of a tile sees all of its keys, but for those behind the shared tokens
 // and on pages outside the pool, which a mask of a bit per key leaves out.
+//
+// What bounds it.  Long prefixes and few rows: HBM, 8 sequences behind 131072
+// tokens (24/8 heads of 128, bf16) 87 us, 6.2 TB/s.  Many rows: a pair of tiles
+// takes 2.5 us, of which the products are 1.1 at their full rate and the
+// exponentials 1.1 at theirs; an accumulator's chain of scores, softmax and
+// products is covered by the other's in part.  Short ones: begin and end, 64
+// sequences behind 8192 tokens 21 us, 4 until the first scores, 4 tiles, 2 for
+// the rows.  Not kept: a wait of the copying warps before each hand-over (103 us
+// -> 119 at 131072 tokens), K and V by 16-byte copies where boxes can be (110).
 #include "attn_tc.cuh"
 #include "prefix.cuh"
 
