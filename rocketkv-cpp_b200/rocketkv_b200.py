@@ -570,6 +570,7 @@ class PagedCache:
                              _ptr(block_table), None)
         self.ref = ctypes.byref(self.c)
         self.batch = block_table.shape[0]
+        self._geometry = (self.batch, hk, d, K.dtype)
         self.lens = lens
 
     @property
@@ -893,24 +894,44 @@ class Rotary:
         return (self.freqs,) if self.axes is None else (self.freqs, self.axes)
 
 
-_row_refs: dict = {}
+_layouts: dict = {}
 
 
-def _rows_of(t, what, token_major=False):
-    """_row_strides of [B, heads, len, D] (token_major: [B, len, heads, D]) by reference, formed once for a shape, its
-    strides and type."""
-    key = (t.shape, t.stride(), t.dtype, token_major)
-    ref = _row_refs.get(key)
-    if ref is None:
-        if len(_row_refs) >= 4096:
-            _row_refs.clear()
-        ref = _row_refs[key] = ctypes.byref(_row_strides(t.transpose(1, 2) if token_major else t, what))
-    return ref
+def _remember(key, plan):
+    """A call's layout that was found right, by its shapes, strides and types."""
+    if len(_layouts) >= 4096:
+        _layouts.clear()
+    _layouts[key] = plan
+    return plan
 
 
-def _positions_ok(positions, rotary, batch, n) -> bool:
-    return (positions.dtype is rotary._int32 and positions.device == rotary.device and positions.is_contiguous()
-            and positions.shape in (((rotary.num_axes, batch, n), (batch, n)) if rotary.num_axes == 1 else ((rotary.num_axes, batch, n),)))
+def _rows_of(t, what):
+    return None if t is None else ctypes.byref(_row_strides(t, what))
+
+
+def _check_positions(positions, rotary, batch, n):
+    if (positions.dtype is not rotary._int32 or not positions.is_contiguous()
+            or tuple(positions.shape) not in (((rotary.num_axes, batch, n), (batch, n)) if rotary.num_axes == 1 else ((rotary.num_axes, batch, n),))):
+        raise ValueError("positions: contiguous int32 [num_axes, B, rows], or [B, rows] for one axis")
+
+
+def _rotate_layout(key, q, k, positions, rotary, q_out, k_out):
+    some = q if q is not None else k
+    if some.dim() != 4:
+        raise ValueError("q and k: [B, heads, len, D]")
+    B, _, n, D = some.shape
+    kind = rotary._types.get(some.dtype)
+    if D != rotary.dim_head or kind is None:
+        raise ValueError("the rows are not of the rotary's dim_head, or of no type that is turned")
+    for x, out in ((q, q_out), (k, k_out)):
+        if x is not None and (x.dim() != 4 or x.shape[0] != B or x.shape[2:] != some.shape[2:] or x.dtype is not some.dtype):
+            raise ValueError("q and k: one batch, length, D and type")
+        if x is not None and (out.shape != x.shape or out.dtype is not x.dtype):
+            raise ValueError("q_out and k_out: the rows' shape and type")
+    _check_positions(positions, rotary, B, n)
+    return _remember(key, (0 if q is None else q.shape[1], 0 if k is None else k.shape[1], kind, D, n, B, _rows_of(q, "q"),
+                           _rows_of(q_out if q is not None else None, "q_out"), _rows_of(k, "k"),
+                           _rows_of(k_out if k is not None else None, "k_out")))
 
 
 def rotate(q, k, positions, rotary: Rotary, q_out=None, k_out=None, stream=None):
@@ -919,37 +940,50 @@ def rotate(q, k, positions, rotary: Rotary, q_out=None, k_out=None, stream=None)
     stride along D), positions int32 [num_axes, B, len] ([B, len] for one axis),
     to q_out and k_out (fresh ones without; q and k themselves to turn in
     place).  Returns (q_out, k_out)."""
-    some = q if q is not None else k
-    if some is None:
+    if q is None and k is None:
         raise ValueError("q or k is needed")
-    if some.dim() != 4:
-        raise ValueError("q and k: [B, heads, len, D]")
-    dev, dtype = rotary.device, some.dtype
-    B, _, n, D = some.shape
-    kind = rotary._types.get(dtype)
-    if some.device != dev or D != rotary.dim_head or kind is None:
-        raise ValueError("the rows are not of the rotary's device or dim_head, or of no type that is turned")
-    if q is not None and k is not None and (k.dim() != 4 or k.shape[0] != B or k.shape[2:] != some.shape[2:] or k.dtype is not dtype
-                                            or k.device != dev):
-        raise ValueError("q and k: one batch, length, D, type and device")
-    if not _positions_ok(positions, rotary, B, n):
-        raise ValueError("positions: contiguous int32 [num_axes, B, len], or [B, len] for one axis, on the rows' device")
+    dev = rotary.device
     if (q is not None and q_out is None) or (k is not None and k_out is None):
         with _on_stream(dev, stream):
-            q_out = rotary._empty(q.shape, dtype=dtype, device=dev) if q is not None and q_out is None else q_out
-            k_out = rotary._empty(k.shape, dtype=dtype, device=dev) if k is not None and k_out is None else k_out
-    args = []
-    for x, out in ((q, q_out), (k, k_out)):
+            q_out = rotary._empty(q.shape, dtype=q.dtype, device=dev) if q is not None and q_out is None else q_out
+            k_out = rotary._empty(k.shape, dtype=k.dtype, device=dev) if k is not None and k_out is None else k_out
+    key = [rotary.num_axes, rotary.dim_head]
+    at = []
+    for x in (q, q_out if q is not None else None, k, k_out if k is not None else None, positions):
         if x is None:
-            args.append((None, None, 0, None, None))
+            key.append(None)
+            at.append(None)
             continue
-        if out.shape != x.shape or out.dtype is not dtype or out.device != dev:
-            raise ValueError("q_out and k_out: the rows' shape, type and device")
-        args.append((x.data_ptr(), out.data_ptr(), x.shape[1], _rows_of(x, "q and k"), _rows_of(out, "q_out and k_out")))
-    (qp, qo, H, qs, qos), (kp, ko, HK, ks, kos) = args
-    _launch(dev, stream, "rkv_rotate", lib().rkv_rotate, rotary.ref, positions.data_ptr(), qp, qo, H, kp, ko, HK, kind, D, n, B,
+        if x.device != dev:
+            raise ValueError("the rows and the positions: on the rotary's device")
+        key += (x.shape, x.stride(), x.dtype)
+        at.append(x.data_ptr())
+    key = tuple(key)
+    H, HK, kind, D, n, B, qs, qos, ks, kos = _layouts.get(key) or _rotate_layout(key, q, k, positions, rotary, q_out, k_out)
+    _launch(dev, stream, "rkv_rotate", lib().rkv_rotate, rotary.ref, at[4], at[0], at[1], H, at[2], at[3], HK, kind, D, n, B,
             qs, qos, ks, kos, owner=rotary)
     return q_out, k_out
+
+
+def _append_layout(key, cache, k, v, rotary, q, q_out, positions, n_new):
+    if k.shape != v.shape or k.stride() != v.stride() or k.dtype is not cache.K.dtype or v.dtype is not k.dtype or k.dim() != 4:
+        raise ValueError("k and v: one shape, layout and the cache's type")
+    B, n, hk, d = k.shape
+    if (B, hk, d) != cache._geometry[:3] or (d > 1 and k.stride(3) != 1):
+        raise ValueError("k, v: [B, n_rows, HK, D] of the cache's geometry, unit stride along D")
+    if rotary.dim_head != d:
+        raise ValueError("the rows are not of the rotary's dim_head")
+    if n_new is not None and (n_new.dtype is not rotary._int32 or n_new.numel() != B or not n_new.is_contiguous()):
+        raise ValueError("n_new: contiguous int32, one entry per sequence")
+    if positions is not None:
+        _check_positions(positions, rotary, B, n)
+    if q is not None:
+        if q.dim() != 4 or q.shape[0] != B or q.shape[1] != n or q.shape[3] != d or q.dtype is not k.dtype:
+            raise ValueError("q: [B, n_rows, H, D] of the cache's type")
+        if q_out.shape != q.shape or q_out.dtype is not q.dtype:
+            raise ValueError("q_out: q's shape and type")
+    heads = lambda x, what: None if x is None else _rows_of(x.transpose(1, 2), what)  # noqa: E731
+    return _remember(key, (n, B, 0 if q is None else q.shape[2], heads(k, "k"), heads(q, "q"), heads(q_out, "q_out")))
 
 
 def paged_append_rotated(cache: PagedCache, k, v, rotary: Rotary, q=None, q_out=None, positions=None, n_new=None, stream=None):
@@ -966,37 +1000,31 @@ def paged_append_rotated(cache: PagedCache, k, v, rotary: Rotary, q=None, q_out=
         q, q_out = (None if x is None else x[:, None] for x in (q, q_out))
         if positions is not None and positions.dim() == 1:
             positions = positions[:, None]
-    K, dev = cache.K, rotary.device
-    strides, dtype = k.stride(), k.dtype
-    if k.shape != v.shape or strides != v.stride() or dtype is not K.dtype or v.dtype is not dtype or len(strides) != 4:
-        raise ValueError("k and v: one shape, layout and the cache's type")
-    B, n, hk, d = k.shape
-    if B != cache.batch or hk != K.shape[1] or d != K.shape[3] or (d > 1 and strides[3] != 1):
-        raise ValueError("k, v: [B, n_rows, HK, D] of the cache's geometry, unit stride along D")
-    if k.device != dev or v.device != dev or K.device != dev or rotary.dim_head != d:
-        raise ValueError("k, v and the rotary: on the cache's device, of its dim_head")
-    if B and cache._lens is None:
+    dev = rotary.device
+    if cache.K.device != dev:
+        raise ValueError("the cache: on the rotary's device")
+    if cache.batch and cache._lens is None:
         raise ValueError("the cache's lens are needed")
-    if n_new is not None and (n_new.dtype is not rotary._int32 or n_new.device != dev or n_new.numel() != B or not n_new.is_contiguous()):
-        raise ValueError("n_new: contiguous int32, one entry per sequence, on the cache's device")
-    if positions is not None and not _positions_ok(positions, rotary, B, n):
-        raise ValueError("positions: contiguous int32 [num_axes, B, n_rows], or [B, n_rows] for one axis, on the cache's device")
-    H = qp = qo = 0
-    qs = qos = None
-    if q is not None:
-        if q.dim() != 4 or q.shape[0] != B or q.shape[1] != n or q.shape[3] != d or q.dtype is not dtype or q.device != dev:
-            raise ValueError("q: [B, n_rows, H, D] of the cache's type, on its device")
-        if q_out is None:
-            with _on_stream(dev, stream):
-                # without n_new every row is written
-                q_out = (rotary._empty if n_new is None else rotary._zeros)(q.shape, dtype=dtype, device=dev)
-        if q_out.shape != q.shape or q_out.dtype is not dtype or q_out.device != dev:
-            raise ValueError("q_out: q's shape, type and device")
-        H, qp, qo = q.shape[2], q.data_ptr(), q_out.data_ptr()
-        qs, qos = _rows_of(q, "q", True), _rows_of(q_out, "q_out", True)
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    _launch(dev, stream, "rkv_paged_append_rotated", lib().rkv_paged_append_rotated, cache.ref, rotary.ref,
-            None if positions is None else positions.data_ptr(), k.data_ptr(), v.data_ptr(), _rows_of(k, "k", True), n, B,
-            None if n_new is None else n_new.data_ptr(), qp, qs, qo, qos, H, owner=rotary)
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out without q")
+    elif q_out is None:
+        with _on_stream(dev, stream):
+            # without n_new every row is written
+            q_out = (rotary._empty if n_new is None else rotary._zeros)(q.shape, dtype=q.dtype, device=dev)
+    key = [rotary.num_axes, rotary.dim_head, cache._geometry]
+    at = []
+    for x in (k, v, q, q_out, positions, n_new):
+        if x is None:
+            key.append(None)
+            at.append(None)
+            continue
+        if x.device != dev:
+            raise ValueError("k, v, q, positions and n_new: on the cache's device")
+        key += (x.shape, x.stride(), x.dtype)
+        at.append(x.data_ptr())
+    key = tuple(key)
+    n, B, H, ks, qs, qos = _layouts.get(key) or _append_layout(key, cache, k, v, rotary, q, q_out, positions, n_new)
+    _launch(dev, stream, "rkv_paged_append_rotated", lib().rkv_paged_append_rotated, cache.ref, rotary.ref, at[4], at[0], at[1], ks, n, B,
+            at[5], at[2], qs, at[3], qos, H, owner=rotary)
     return q_out[:, 0] if one and q_out is not None else q_out
