@@ -412,3 +412,44 @@ def test_refused_calls(cuda):
     with pytest.raises(rkv.RkvError):
         rkv.PrefixDecoder(4, 3, 64, 200, 2, torch.float16, cuda)
     assert bool((dec.O == 7.0).all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_large_batches_without_tokens_or_pages(D, cuda):
+    B = 40
+    K, V = R.pool(8, 6, 2, 16, D, torch.bfloat16, cuda)
+    q = _query(9, B, 4, D, torch.bfloat16, cuda)
+    starts, shared = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in ([0, B], [20]))
+    tab = torch.zeros((B, 4), dtype=torch.int32, device=cuda)
+    for cache, top in ((rkv.PagedCache(K, V, tab, torch.zeros(B, dtype=torch.int32, device=cuda)), 60),
+                       (rkv.PagedCache(K, V, tab, torch.full((B,), 30, dtype=torch.int32, device=cuda)), 0),
+                       (rkv.PagedCache(K[:0], V[:0], tab, torch.full((B,), 30, dtype=torch.int32, device=cuda)), 60),
+                       (rkv.PagedCache(K, V, tab[:, :0], torch.full((B,), 30, dtype=torch.int32, device=cuda)), 60)):
+        dec = _decoder(q, cache, shared, top)
+        dec(q, cache, starts, shared)
+        assert dec.status() == rkv.RKV_OK
+        assert bool((dec.O == 0).all()) and bool((dec.lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("seed", range(36))
+def test_random_batches(seed, cuda):
+    """Groups, lengths, pages, heads and layouts drawn together."""
+    import random
+    r = random.Random(seed)
+    kind = r.choice(["bf16", "f16", "f32"])
+    D = r.choice([8, 32, 64, 72, 96, 128, 128, 136, 200, 256])
+    HK, G = r.choice([1, 2, 3]), r.choice([1, 2, 5, 8, 12])
+    page, layout = r.choice([1, 3, 8, 16, 24, 64, 128, 200]), r.choice(["hnd", "nhd", "mixed"])
+    groups = []
+    for _ in range(r.randint(1, 5)):
+        p = r.choice([0, r.randint(1, 300), r.randint(100, 900)])
+        groups.append((p, [r.choice([p, p + r.randint(0, 400), p + 1, max(0, p - r.randint(0, 60)), 0]) for _ in range(r.randint(0, 20))]))
+    alone = [r.randint(0, 300) for _ in range(r.randint(0, 3))]
+    if not any(x[1] for x in groups) and not alone:
+        alone = [5]
+    dt = TYPES[kind]
+    cache, starts, shared = _setup(200 + seed, HK, D, page, groups, dt, cuda, layout, alone)
+    Q = _query(300 + seed, cache.batch, HK * G, D, dt, cuda)
+    dec = _decoder(Q, cache, shared, max(1, int(cache.lens.max())) + r.choice([0, 100, 5000]))
+    dec(Q, cache, starts, shared)
+    _check(dec, Q, cache)
