@@ -232,7 +232,7 @@ __device__ __forceinline__ uint32_t round2(float x, float y) {
 // Parts of a sequence's shared tokens; the tcgen05 kernel's: 1 for any, whose number it leaves itself.
 __device__ __forceinline__ int shared_parts(const DecodeArgs& a, int shared) {
     if (shared == 0 || a.prefix_parts == 0) return shared > 0;
-    const int t = part_tokens(shared, a.prefix_parts, kSharedLeast);
+    const int t = part_tokens(shared, a.prefix_parts);
     return (shared + t - 1) / t;
 }
 
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
         h0 = (unit - before) * 8 * NT;  // row of the group
         ng = g < 0 ? 0 : min(8 * NT, a.sh.gr.size(g) * a.G - h0);
         b = g < 0 ? 0 : leader_of(a.sh.gr, a.c, g, vis.n);
-        chunk = part_tokens(vis.n, parts, kSharedLeast);
+        chunk = part_tokens(vis.n, parts);
     } else {
         split = (int)(id % a.splits);
         id /= a.splits;
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(S::W * 32, S::CTAS) paged_decode_kernel(const 
             vis.sinks = 0;
             vis.gap = shared;
             vis.nvis = vis.n - shared;
-            chunk = PASS == PASS_LAST ? vis.nvis : part_tokens(vis.nvis, a.splits, kOwnLeast);
+            chunk = PASS == PASS_LAST ? vis.nvis : part_tokens(vis.nvis, a.splits);
             if (PASS == PASS_PARTS && split == 0 && tid < min(8 * NT, a.G - grp * 8 * NT)) {
                 a.sh.info[(size_t)b * a.H + hk * a.G + grp * 8 * NT + tid] =
                     make_int2((vis.nvis + chunk - 1) / chunk, shared_parts(a, shared));
@@ -1094,7 +1094,7 @@ constexpr int kOwnWaves = 1;
 // How many own tokens there are is known on the device alone; sequences with few leave their CTAs behind the first
 // without work, so that these are kOwnWaves waves at most.
 int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch) {
-    const long long units = decode_units(dtype, H, HK, D, batch), most = ((long long)max_len + kOwnLeast - 1) / kOwnLeast;
+    const long long units = decode_units(dtype, H, HK, D, batch), most = ((long long)max_len + kPartLeast - 1) / kPartLeast;
     long long p = units > 0 ? kOwnWaves * 2 * decode_slots(dtype, D) / units : 1;
     if (p > most) p = most;
     if (p > kMaxSplits) p = kMaxSplits;
@@ -1105,7 +1105,7 @@ int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch,
     const int rows = shared_rows(dtype, D, H, HK, batch, groups);
     const long long each = ((long long)batch * (H / HK) + groups * (long long)rows - 1) / (groups * (long long)rows);  // of a group of mean size
     long long p = 2LL * 2 * decode_slots(dtype, D) / (each * groups * HK);
-    const long long most = ((long long)max_len + kSharedLeast - 1) / kSharedLeast;
+    const long long most = ((long long)max_len + kPartLeast - 1) / kPartLeast;
     if (p > most) p = most;
     if (p > 128) p = 128;  // of kMaxShared
     return p < 1 ? 1 : (int)p;

@@ -42,7 +42,7 @@ __device__ __forceinline__ void put4(__half* o, const float4& v) {
     reinterpret_cast<__half2*>(o)[1] = __floats2half2_rn(v.z, v.w);
 }
 
-constexpr int kJoinWarps = 4;  // of a CTA, which joins one row
+constexpr int kJoinWarps = 8;  // of a CTA, which joins one row
 constexpr int kJoinAhead = 4;  // parts of a warp that are on their way together
 
 // Joins the parts of a row: those of its own tokens, then those of the shared
