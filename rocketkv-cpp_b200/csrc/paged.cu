@@ -1090,12 +1090,16 @@ long long shared_units(int rows, int H, int HK, int batch, int groups) { return 
 
 }  // namespace
 
-constexpr int kOwnWaves = 1;
-// How many own tokens there are is known on the device alone; sequences with few leave their CTAs behind the first
-// without work, so that these are kOwnWaves waves at most.
-int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch) {
+// How many own tokens there are is known on the device alone, and they are few beside the shared ones as a rule;
+// sequences with few leave their CTAs behind the first without work, so that these are one wave at most, but for
+// kOwnMost tokens of max_len each: one of 64 sequences with 65536 own tokens (8 KV heads of 128, bf16) would take one CTA
+// 1745 us.  Where nothing is shared, as many as the decode of all tokens takes.
+constexpr int kOwnMost = 12288;
+int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
     const long long units = decode_units(dtype, H, HK, D, batch), most = ((long long)max_len + kPartLeast - 1) / kPartLeast;
-    long long p = units > 0 ? kOwnWaves * 2 * decode_slots(dtype, D) / units : 1;
+    long long p = units > 0 ? 2 * decode_slots(dtype, D) / units : 1;
+    if (p < (max_len + kOwnMost - 1) / kOwnMost) p = (max_len + kOwnMost - 1) / kOwnMost;
+    if (groups == 0) p = decode_parts(dtype, H, HK, D, max_len, batch);
     if (p > most) p = most;
     if (p > kMaxSplits) p = kMaxSplits;
     return p < 1 ? 1 : (int)p;

@@ -13,7 +13,7 @@
 // is begun while the one before still runs.
 //
 // 24/8 heads of 128, bf16: 2 sequences behind 1024 tokens 11 us, 64 behind 8192
-// with up to 512 of their own 43, 8 behind 131072 102 (0.82 of a copy's rate; 640
+// with up to 512 of their own 43, 8 behind 131072 99 (0.85 of a copy's rate; 640
 // without sharing).  Not kept: the shared tokens first where a join follows (45 us
 // -> 47), and the last CTA to arrive as the join (34 -> 42 for 24 sequences).
 #include "prefix.cuh"
@@ -160,7 +160,7 @@ PrefixPlan prefix_plan(int dtype, int H, int HK, int D, int max_len, int batch, 
     PrefixPlan p{};
     const bool any = groups > 0 && batch > 0;
     p.tc = any && on_tc(dtype, H, HK, D, max_len, batch, groups);
-    p.own = shared_own_parts(dtype, H, HK, D, max_len, batch);
+    p.own = shared_own_parts(dtype, H, HK, D, max_len, batch, groups);
     p.slots = p.own + (any && !p.tc ? shared_prefix_parts(dtype, H, HK, D, max_len, batch, groups) : 0);
     size_t off = kWorkspaceHeader;
     auto take = [&](size_t& ml, size_t& o, size_t rows) {

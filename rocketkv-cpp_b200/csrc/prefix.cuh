@@ -86,12 +86,13 @@ struct SharedArgs {
 // Rows of a group that one CTA of the matrix-instruction kernel takes.
 int shared_rows(int dtype, int D, int H, int HK, int batch, int groups);
 // Parts of every sequence's own tokens, and of every group's shared ones for the matrix-instruction kernel.
-int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch);
+int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups);
 int shared_prefix_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups);
 // The shared tokens on the tcgen05 tensor cores (prefix_tc.cu): 16-bit types.  A unit is up to 256 rows (128 above 128
-// columns) of one group and KV head; the tiles of the units are cut into stretches, one or more per CTA.  A unit's first stretch leaves its
-// rows in first (row b H + h), a stretch that begins inside a unit in later (256 rows per CTA).  first_later[row]: how
-// many stretches follow the first one, and the row of the first of them in later; the others' are 256 further each.
+// columns) of one group and KV head; the tiles of the units are cut into stretches, one or more per CTA.  A unit's
+// first stretch leaves its rows in first (row b H + h), a stretch that begins inside a unit in later (256 rows per
+// CTA).  first_later[row]: how many stretches follow the first one, and the row of the first of them in later; the
+// others' are 256 further each.
 struct TcParts {
     float* first_o;
     float2* first_ml;
