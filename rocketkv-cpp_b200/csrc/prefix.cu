@@ -13,8 +13,8 @@
 // is begun while the one before still runs.
 //
 // 24/8 heads of 128, bf16: 2 sequences behind 1024 tokens 11 us, 64 behind 8192
-// with up to 512 of their own 43, 8 behind 131072 99 (0.85 of a copy's rate; 640
-// without sharing).  Not kept: the shared tokens first where a join follows (45 us
+// with up to 512 of their own 43, 8 behind 131072 107, 99 over one cache (0.78, 0.85
+// of a copy's rate; 640 without sharing).  Not kept: the shared tokens first where a join follows (45 us
 // -> 47), and the last CTA to arrive as the join (34 -> 42 for 24 sequences).
 #include "prefix.cuh"
 
