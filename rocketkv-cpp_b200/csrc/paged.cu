@@ -1098,7 +1098,8 @@ constexpr int kOwnMost = 12288;
 int shared_own_parts(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
     const long long units = decode_units(dtype, H, HK, D, batch), most = ((long long)max_len + kPartLeast - 1) / kPartLeast;
     long long p = units > 0 ? 2 * decode_slots(dtype, D) / units : 1;
-    if (p < (max_len + kOwnMost - 1) / kOwnMost) p = (max_len + kOwnMost - 1) / kOwnMost;
+    const long long many = ((long long)max_len + kOwnMost - 1) / kOwnMost;
+    if (p < many) p = many < 64 ? many : 64;  // the workspace holds them all
     if (groups == 0) p = decode_parts(dtype, H, HK, D, max_len, batch);
     if (p > most) p = most;
     if (p > kMaxSplits) p = kMaxSplits;
