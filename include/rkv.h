@@ -529,10 +529,11 @@ int rkv_paged_append_rotated(const rkv_paged_cache* cache, const rkv_rotary* rot
  * rkv_sink_attention's; rkv_paged_decode's is fp32), 16-byte aligned; lse
  * (nullable) fp32.  max_len, pages outside the pool, non-finite values, sequences
  * without a token and the rest as in rkv_paged_decode.
- * Scores, the softmax's maxima and sums and the outputs' sums are fp32.  Where
- * the shared tokens of a 16-bit cache meet many queries, each of their weights is
- * rounded to the type before it meets V (half a step of the type; in fp16 a fixed
- * 2^-32 of the row's largest below 2^-21 of it); O is rounded to the type once.
+ * Scores, the softmax's maxima and sums and the outputs' sums are fp32; weights
+ * enter as in rkv_paged_decode, but that where the shared tokens of a bf16 cache
+ * meet many queries they are two bf16 parts, not three (off by 2^-16 of a weight
+ * at most); in fp16 they are off by 2^-22, or by 2^-32 of the row's largest where
+ * that is more.  O is rounded to the type once.
  * The split over CTAs depends on the lengths on the device, not on timing:
  * results repeat bit for bit.  It is made for own tokens that are few beside the
  * shared ones and alike: a sequence with far more of them than the others runs

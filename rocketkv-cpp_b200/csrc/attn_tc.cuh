@@ -81,6 +81,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+// x - the two values of a pair (fp16: the product's form spills 48-68 bytes a thread in prefix_tc_kernel, this none).
+template <bool BF>
+__device__ __forceinline__ float2 minus2(float2 x, uint32_t w) {
+    if (BF) return __ffma2_rn(make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)), make_float2(-1.0f, -1.0f), x);
+    w ^= 0x80008000u;
+    return __fadd2_rn(x, __half22float2(*reinterpret_cast<const __half2*>(&w)));
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

@@ -7,8 +7,8 @@
 // instead, the even ones to the first accumulator and the odd ones to the
 // second, and joins the two at the end: either way one accumulator's softmax
 // runs while the tensor cores work on the other's products.  128 keys at a
-// time: S = Q K^T into tensor memory, P = 2^(S - m) rounded to the inputs' type
-// back into tensor memory in S's place, O += P V.
+// time: S = Q K^T into tensor memory, P = 2^(S - m) as a sum of two 16-bit parts
+// back into tensor memory in S's place, O += P V, a product for each part.
 //
 // Above 128 columns the accumulator of 128 rows takes half of the tensor memory:
 // a unit is 128 rows then, tiles are 64 keys, and two score buffers take the
@@ -26,8 +26,14 @@
 // sizes and lengths, every SM has about the same work.
 // Each stretch leaves (m, l, O) of its rows, not divided by l, for the join.
 //
-// P is rounded to 16 bits (half a step of the type, as the products take both
-// operands in one type); scores, m, l and the accumulators are fp32.  Every
+// The products take both operands in one type, so P enters as its value rounded
+// to the type and what that rounding left, rounded: 16 bits of a weight in bf16,
+// 22 in fp16 (2^-32 of the row's largest at least), as many as the two parts have
+// columns in S's place.  One part alone (8 and 11 bits) made a sequence's weights
+// depend on how many others share its tokens, and where values of opposite signs
+// meet its output was up to 35 times further off than a decode of its own may be;
+// it took 43 us in place of 48 for 64 sequences behind 8192 tokens, 99 in place of
+// 103 for 8 behind 131072.  Scores, m, l and the accumulators are fp32.  Every
 // row of a tile sees all of its keys, but for those behind the shared tokens
 // and on pages outside the pool, which a mask of a bit per key leaves out.
 //
@@ -442,8 +448,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc_fence_after();
 #pragma unroll
                         for (int ks = WIDE ? 0 : half * 4; ks < half * 4 + 4 && ks < KEYS / 16; ++ks)
-                            mma_ts(tbase + kColO + u * kStepO, tbase + kColS + u * KEYS + ks * 8, db + ks * 128, idv,
-                                   k > (WIDE ? 0 : 1) || ks > 0);
+#pragma unroll
+                            for (int part = 0; part < 2; ++part)
+                                mma_ts(tbase + kColO + u * kStepO, tbase + kColS + u * KEYS + part * (KEYS / 2) + ks * 8, db + ks * 128, idv,
+                                       k > (WIDE ? 0 : 1) || ks > 0 || part > 0);
                     }
                     if (!ok) break;
                     steps ^= 1u << u;
@@ -575,6 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int half = WIDE ? 1 : 0; half < 2; ++half) {  // the products of the first 64 keys start under the second's exponentials
                     constexpr int H = 32;  // pairs of keys
                     const int c0 = WIDE ? 0 : half * H;
+                    uint32_t rest[H];
 #pragma unroll
                     for (int i = 0; i < H; ++i) {
                         const int c = c0 + i;
@@ -583,8 +592,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         e.y = ex2_approx(e.y);
                         sum[c & 1] = __fadd2_rn(sum[c & 1], e);
                         s[c] = pack2<BF>(e.x, e.y);
+                        const float2 r = minus2<BF>(e, s[c]);  // exact
+                        rest[i] = pack2<BF>(r.x, r.y);
                     }
                     st32(ts + c0, s + c0);
+                    st32(ts + KEYS / 2 + c0, rest);
                     wait_st();
                     tc_fence_before();
                     __syncwarp();
