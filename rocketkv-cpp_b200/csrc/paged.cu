@@ -249,7 +249,7 @@ __device__ __forceinline__ void merge_last(const DecodeArgs& a, Head head_of, in
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the shared tokens' parts are there
     if (a.res.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.res.clear = 0;
     const int some = shared_parts(a, shared);
-    if ((int)threadIdx.x < ng) xs[threadIdx.x] = a.tc.first_o && some > 0 ? a.tc.first_later[head_of(threadIdx.x)] : make_int2(0, 0);
+    if ((int)threadIdx.x < ng) xs[threadIdx.x] = a.tc.first_o && some > 0 ? parts_behind(a.tc, (long long)head_of(threadIdx.x), some) : make_int2(0, 0);
     __syncthreads();
     const int per = a.D / 4;
     float4 v[U];

@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const Join
     int shared = info.y;
     int2 x = make_int2(0, 0);
     if (TC && shared > 0) {
-        x = a.tc.first_later[row];
+        x = parts_behind(a.tc, row, shared);
         shared += x.x;
     }
     // own parts, then shared ones

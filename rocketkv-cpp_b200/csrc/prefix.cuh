@@ -2,6 +2,7 @@
 #pragma once
 
 #include "paged.cuh"
+#include "prefix_parts.cuh"
 
 namespace rkv {
 
@@ -101,12 +102,15 @@ struct TcParts {
     float2* later_ml;
     int* err;
 };
-constexpr int kTcSms = 148;
-constexpr int kTcRows = 256;
-// Parts of a row's shared tokens at most.
-constexpr int kMaxShared = 152;
-static_assert(kMaxShared >= kTcSms, "a unit may have a stretch per CTA");
-// Part p of row's shared tokens, wherever the pass over them left it; x: first_later[row].
+// first_later[row] for a row with a part of shared tokens (some: 1).  A pair that the kernel cannot have written, which
+// is there where it gave up a wait: the row is joined without shared tokens, and the call's error stays recorded.
+__device__ __forceinline__ int2 parts_behind(const TcParts& t, long long row, int some) {
+    const int2 x = t.first_later[row];
+    if (parts_in_buffer(x.x, x.y)) return x;
+    atomicCAS(t.err, 0, (int)RKV_ERR_DEVICE_TIMEOUT);
+    return make_int2(-some, 0);
+}
+// Part p of row's shared tokens, wherever the pass over them left it; x: parts_behind of row.
 __device__ __forceinline__ float2 shared_ml(const SharedArgs& s, const TcParts& t, long long row, int2 x, int p) {
     return !t.first_o ? s.part_ml[row * s.slots + s.own + p] : p == 0 ? t.first_ml[row] : t.later_ml[x.y + (p - 1) * kTcRows];
 }
