@@ -109,6 +109,7 @@ struct Bars {
     uint64_t q_full, o_full, o_empty, written, drained;
     uint64_t s_full[2], p_half[2], p_ready[2], pv_done;  // of an accumulator (above 128 columns: of a score buffer)
     uint64_t full[8], empty[8];
+    uint64_t pair[4];  // of the two softmax warps that hold the same rows
     Stretches next;
     alignas(16) uint32_t mask[kMasks][4];
     uint32_t tmem;
@@ -331,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&B.full[i], BOXES ? 1 : 4 * 33);  // 33: a copying warp's lanes' copies, and its part of the mask
             mbar_init(&B.empty[i], 1);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(&B.pair[i], 2);
         B.next.init(BOXES ? 14 : 13);
         *abort_flag = 0;
         // a wait gives up after two seconds at the soonest, long after this
@@ -650,13 +652,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) mbar_arrive1(&B.written);
                 continue;
             }
-            // the two accumulators hold the same rows: each softmax takes half of the columns of their sum
+            // the two accumulators hold the same rows: each softmax takes half of the columns of their sum.  The
+            // warps meet by a wait with a limit: one of them may have given up the wait before that the other did not
             float2* mine = reinterpret_cast<float2*>(so);
             const float2* others = reinterpret_cast<const float2*>(stage + ((warp - 8) ^ 4) * 4096);
             mine[lane] = ml;
-            group_sync(1 + q4, 64);
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(&B.pair[q4]);
+            if (!(ok = warp_wait(&B.pair[q4], 0, err, abort_flag))) break;
             const float2 ot = others[lane];
-            group_sync(1 + q4, 64);  // the stage's other use begins
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(&B.pair[q4]);
+            if (!(ok = warp_wait(&B.pair[q4], 1, err, abort_flag))) break;  // the stage's other use begins
             const float top = fmaxf(ml.x, ot.x), base = top == -INFINITY ? 0.0f : top;
             const float fm = exp2f(ml.x - base), fo = exp2f(ot.x - base);
             const float f0 = u ? fo : fm, f1 = u ? fm : fo;
