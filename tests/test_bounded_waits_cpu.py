@@ -26,5 +26,4 @@ def test_no_wait_without_a_limit():
     # the whole CTA's barriers: one before the roles part, one behind them, which every role reaches
     assert body.count("__syncthreads()") == 2
     roles = body[body.index("__syncthreads()") + 15: body.rindex("__syncthreads()")]
-    assert "return" not in re.sub(r"\[[&=]?\]\([^)]*\)\s*\{[^}]*\}", "", roles)
-    assert roles.count("warp_wait(") >= 10
+    assert "return" not in roles and "warp_wait(&B.pair" in roles
