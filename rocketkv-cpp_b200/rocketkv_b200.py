@@ -673,9 +673,12 @@ class PrefixDecoder:
         self.max_len, self.batch, self.num_groups = max_len, batch, num_groups
         self.ws_bytes = b.value
         self.ws = _workspace(b.value, device)
+        self.ws[:16].zero_()  # the error word: status() may look before a call has run
+        if not torch.cuda.is_current_stream_capturing():
+            # calls on other streams come behind it
+            torch.cuda.current_stream(self.ws.device).synchronize()
         self.lse = torch.empty((batch, num_heads), dtype=torch.float32, device=device)
         self._streams = {_handle(self.ws.device, None)}  # whose work its buffers outlive
-        self._ran = False  # a call has written the workspace's error word
 
     def _buffers(self):
         return self.ws, self.O, self.lse
@@ -701,14 +704,11 @@ class PrefixDecoder:
                 self.num_heads * self.dim_head * Q.element_size(), self.num_heads, cache.ref, self.max_len, self.batch,
                 group_starts.data_ptr(), group_tokens.data_ptr(), self.num_groups, self.O.data_ptr(), self.lse.data_ptr(),
                 self.ws.data_ptr(), self.ws_bytes, owner=self)
-        self._ran |= self.batch > 0
         return self.O
 
     def status(self, stream=None) -> int:
         """Waits for `stream`; the first error that a call recorded since the last look, or RKV_OK."""
         import torch
-        if not self._ran:
-            return RKV_OK
         with torch.cuda.device(self.ws.device):
             return lib().rkv_workspace_status(_ptr(self.ws), _stream(stream))
 
