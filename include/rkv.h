@@ -542,6 +542,9 @@ int rkv_paged_append_rotated(const rkv_paged_cache* cache, const rkv_rotary* rot
  * rkv_paged_decode takes 269 and 140).
  * Workspace: device, 16-byte aligned, not shared with a call that may run at
  * the same time; it begins with the error word that rkv_workspace_status reads.
+ * An error stays there until it is read, whatever calls and replays follow:
+ * set the first 4 bytes to 0 once, before the first call (anything that is no
+ * error code is taken for 0).
  * Asynchronous on `stream`; allocates nothing. */
 int rkv_prefix_decode_workspace_size(int dtype, int num_heads, int num_heads_kv, int dim_head, int max_len,
                                      int batch, int num_groups, size_t* bytes);

@@ -247,7 +247,6 @@ __device__ __forceinline__ void merge_last(const DecodeArgs& a, Head head_of, in
     int2* xs = reinterpret_cast<int2*>(inv + rows);
     float* share = inv + 3 * rows;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the shared tokens' parts are there
-    if (a.res.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.res.clear = 0;
     const int some = shared_parts(a, shared);
     if ((int)threadIdx.x < ng) xs[threadIdx.x] = a.tc.first_o && some > 0 ? parts_behind(a.tc, (long long)head_of(threadIdx.x), some) : make_int2(0, 0);
     __syncthreads();
@@ -324,6 +323,7 @@ __device__ __forceinline__ void merge_last(const DecodeArgs& a, Head head_of, in
                 make_uint2(round2<KIND == KIND_BF16>(o.x, o.y), round2<KIND == KIND_BF16>(o.z, o.w));
         }
     }
+    if (a.res.err && blockIdx.x == 0 && threadIdx.x == 0) keep_error(a.res.err);
 }
 
 // ---------------------------------------------------------------------------

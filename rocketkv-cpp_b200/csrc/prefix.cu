@@ -55,7 +55,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const Join
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long row = blockIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (a.r.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.r.clear = 0;
     const int2 info = s.info[row];
     const int own = info.x;
     int shared = info.y;
@@ -122,6 +121,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(const Join
         put4(static_cast<T*>(a.r.O) + row * s.D + c, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
     if (threadIdx.x == 0 && a.r.lse) a.r.lse[row] = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.693147180559945f;
+    if (a.r.err && blockIdx.x == 0 && threadIdx.x == 0) keep_error(a.r.err);
 }
 
 template <typename T>
@@ -235,7 +235,7 @@ extern "C" int rkv_prefix_decode(const void* Q, long long q_item_stride, int num
         a.tc.later_o = reinterpret_cast<float*>(ws + p.off_later_o);
         a.tc.err = static_cast<int*>(workspace);
     } else {
-        a.r.clear = static_cast<int*>(workspace);
+        a.r.err = static_cast<int*>(workspace);
     }
     if (p.own == 1) {
         // as many sequences as there is room for CTAs: each takes its own tokens in one part and joins the others' to it

@@ -119,11 +119,15 @@ __device__ __forceinline__ const float* shared_o(const SharedArgs& s, const TcPa
            : p == 0   ? t.first_o + row * s.D
                       : t.later_o + (long long)(x.y + (p - 1) * kTcRows) * s.D;
 }
-// Where the last pass leaves its rows, and the error word, where no pass before it has cleared it.
+// The error word of a workspace that may have held anything: an error stays until it is read, all else is none.
+__device__ __forceinline__ void keep_error(int* err) {
+    if (*err != (int)RKV_ERR_DEVICE_TIMEOUT) *err = RKV_OK;
+}
+// Where the last pass leaves its rows, and the error word, where no pass before it has looked at it.
 struct Result {
     void* O;  // [batch][H][D] of the cache's type
     float* lse;
-    int* clear;
+    int* err;
 };
 
 // Passes of the matrix-instruction kernel: the groups' shared tokens, every sequence's own, or both; or the own ones in

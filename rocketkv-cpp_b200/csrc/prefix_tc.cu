@@ -335,8 +335,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 4; ++i) mbar_init(&B.pair[i], 2);
         B.next.init(BOXES ? 14 : 13);
         *abort_flag = 0;
-        // a wait gives up after two seconds at the soonest, long after this
-        if (blockIdx.x == 0) *err = 0;
         fence_mbar_init();
     }
     if (warp == 4) tmem_alloc(&B.tmem, 512);
@@ -507,6 +505,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int s = 0; s < min(q, NS); ++s) mbar_wait_bounded(&B.full[s], (uint32_t)(((q - 1 - s) / NS) & 1), err);
         } else if (warp == 6) {
             for (int k = 0; B.next.put(k, x, err, abort_flag, lane); ++k) x = walk.next(a, lane);
+        } else if (warp == 7 && blockIdx.x == 0 && lane == 0) {
+            keep_error(err);  // a wait gives up after two seconds at the soonest, long after this
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(200));

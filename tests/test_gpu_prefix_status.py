@@ -30,6 +30,33 @@ def _call(name, cuda):
     return dec, (Q, cache, starts, shared)
 
 
+@pytest.mark.parametrize("name", PLANS)
+def test_an_error_stays_until_it_is_read(name, cuda):
+    dec, args = _call(name, cuda)
+    dec(*args)
+    assert dec.status() == rkv.RKV_OK
+    word = dec.ws[:4].view(torch.int32)
+    word.fill_(rkv.RKV_ERR_DEVICE_TIMEOUT)  # as the kernel records it
+    for _ in range(3):
+        dec(*args)
+    assert dec.status() == rkv.RKV_ERR_DEVICE_TIMEOUT
+    assert dec.status() == rkv.RKV_OK
+    # in a graph, over several replays
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dec(*args)
+    word.fill_(rkv.RKV_ERR_DEVICE_TIMEOUT)
+    g.replay()
+    g.replay()
+    assert dec.status() == rkv.RKV_ERR_DEVICE_TIMEOUT
+    g.replay()
+    assert dec.status() == rkv.RKV_OK
+    # a workspace in memory that held anything: not an error
+    word.fill_(12345)
+    dec(*args)
+    assert dec.status() == rkv.RKV_OK
+
+
 def test_status_of_an_object_whose_only_call_was_captured(cuda):
     """A captured call has not run: its workspace holds what the memory held."""
     warm, args = _call("few rows, one launch", cuda)
