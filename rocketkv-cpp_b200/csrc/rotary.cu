@@ -25,14 +25,12 @@
 // each thread's registers 78 us, all heads in one thread 61, products one by one
 // in place of two 73; 2 heads ahead 50 and with the next two behind them 61.
 #include "paged.cuh"
+#include "rotary_grid.cuh"
 
 namespace rkv {
 namespace {
 
-constexpr int kRotThreads = 256;
-constexpr int kRotAhead = 4;        // heads whose rows are on their way per thread
-constexpr int kRotHeads = 8;        // heads of a thread at most, where there are tokens for all threads
-constexpr int kRotBlocks = 148 * 2; // CTAs that the heads are spread for
+constexpr int kRotAhead = 4;  // heads whose rows are on their way per thread
 
 // Rows of one tensor: element (b, h, i, d) at b item + h head + i token + d elements.
 struct Rows {
@@ -254,22 +252,12 @@ int launch(RotArgs& a, const rkv_rotary* r, int dtype, uintptr_t al, cudaStream_
     a.num_axes = r->num_axes;
     const uintptr_t all = al | (uintptr_t)(r->pairs * es);
     const int bytes = (all & 15) == 0 ? 16 : (all & 7) == 0 ? 8 : es, vec = bytes / es;
-    a.turned = a.pairs / vec;
-    a.chunks = a.turned + ((a.D - 2 * a.pairs) / vec + 1) / 2;
-    a.slots = (a.heads + kRotHeads - 1) / kRotHeads;  // chunks: at most 128
-    if (a.slots > kRotThreads / a.chunks) a.slots = kRotThreads / a.chunks;
-    a.tile = kRotThreads / (a.chunks * a.slots);
-    if (a.tile > a.rows) a.tile = a.rows;
-    a.slots = kRotThreads / (a.chunks * a.tile);
-    if (a.slots > a.heads) a.slots = a.heads;
-    const long long tiles = (a.rows + a.tile - 1) / a.tile;
-    long long split = (kRotBlocks + tiles * a.batch - 1) / (tiles * a.batch);
-    const long long most = (a.heads + a.slots - 1) / a.slots;
-    if (split > most) split = most;
-    if (split > 65535) split = 65535;
-    const long long each = (most + split - 1) / split;  // heads of a thread
-    split = (most + each - 1) / each;
-    const dim3 grid((unsigned)tiles, (unsigned)split, a.batch);
+    const RotGrid g = rotary_grid(a.D, a.pairs, vec, a.heads, a.rows, a.batch);
+    a.turned = g.turned;
+    a.chunks = g.chunks;
+    a.slots = g.slots;
+    a.tile = g.tile;
+    const dim3 grid((unsigned)g.tiles, (unsigned)g.split, a.batch);
     switch (dtype) {
         case RKV_F32: launch_type<float, PAGED>(a, bytes, r->interleaved != 0, grid, st); break;
         case RKV_BF16: launch_type<__nv_bfloat16, PAGED>(a, bytes, r->interleaved != 0, grid, st); break;
