@@ -470,7 +470,7 @@ int rkv_sink_attention(const void* Q, const void* K, const void* V, int dtype, i
  * takes rows that its model has turned already.
  * freqs: device [pairs], 8-byte aligned, f_i as turns per position in units of
  * 2^-64, as rkv_rotary_frequencies makes them (so that angles of far positions
- * lose nothing: they are off by 2^-25 half turns at most); axes: device
+ * lose nothing: they are off by 2^-25 + 2^-30 half turns at most); axes: device
  * [pairs], NULL for axis 0 throughout; a pair of an axis >= num_axes stays at
  * position 0.
  * num_axes: at most 256.  Positions are 32-bit, negative ones turn back: the
@@ -484,7 +484,8 @@ typedef struct rkv_rotary {
     int interleaved;
 } rkv_rotary;
 
-/* Host: freqs[i] for radians[i] radians per position; both host arrays. */
+/* Host: freqs[i], the nearest step, for radians[i] radians per position; both
+ * host arrays.  Radians of 2^64 or more, infinities and NaN are refused. */
 int rkv_rotary_frequencies(const double* radians, int pairs, unsigned long long* freqs);
 
 /* q: [batch][num_heads][len][dim_head], k: [batch][num_heads_kv][len][dim_head]

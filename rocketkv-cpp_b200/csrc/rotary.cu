@@ -8,9 +8,10 @@
 // The angle.  f_i is kept as turns per position in units of 2^-64, so that the
 // 64-bit product with p wraps as the angle does: what is left is the fraction
 // of a turn, exact for every 32-bit position but for f_i's own rounding
-// (2^-65 |p| turns).  Its top 32 bits become the fp32 argument of sincospif (off
-// by 2^-25 half turns at most).  Products and sums are fp32 with one rounding
-// to the rows' type at the end.
+// (2^-65 |p| turns).  Its top 32 bits become the fp32 argument of sincospif: off
+// by 2^-25 half turns for the rounding to fp32, 2^-31 for the bits below, 2^-33
+// for f_i at most.  Products and sums are fp32 with one rounding to the rows'
+// type at the end.
 //
 // Memory bounds it: every row is read and written once, six operations per
 // pair.  A CTA has a tile of tokens; its threads ask for their first rows, form
@@ -24,6 +25,8 @@
 // with its append 3.3 us.  Measured at 4 x 4096 tokens: sines and cosines in
 // each thread's registers 78 us, all heads in one thread 61, products one by one
 // in place of two 73; 2 heads ahead 50 and with the next two behind them 61.
+#include <cmath>
+
 #include "paged.cuh"
 #include "rotary_grid.cuh"
 
@@ -274,12 +277,27 @@ using namespace rkv;
 extern "C" int rkv_rotary_frequencies(const double* radians, int pairs, unsigned long long* freqs) {
     if (!radians || !freqs || pairs < 0) return RKV_ERR_INVALID_ARG;
     for (int i = 0; i < pairs; ++i)
-        if (!(radians[i] >= -1e300 && radians[i] <= 1e300)) return RKV_ERR_INVALID_ARG;
+        if (!(radians[i] > -0x1p64 && radians[i] < 0x1p64)) return RKV_ERR_INVALID_ARG;
+    // floor(2^192 / 2 pi), low word first.  A double is an integer m < 2^53 times 2^e, e <= 11; the product of m with
+    // these 192 bits is off by m at most, and its bits from 128 - e on (117 or more) are the steps of 2^-64 turns.
+    constexpr unsigned long long inv[3] = {0x36d8a5664f10e410ull, 0x7f09d5f47d4d3770ull, 0x28be60db9391054aull};
     for (int i = 0; i < pairs; ++i) {
-        long double t = (long double)radians[i] / 6.283185307179586476925286766559006L;
-        t -= __builtin_floorl(t);
-        const long double s = __builtin_rintl(t * 18446744073709551616.0L);
-        freqs[i] = s >= 18446744073709551616.0L ? 0ull : (unsigned long long)s;  // a whole turn
+        int e = 0;
+        const double x = frexp(radians[i] < 0 ? -radians[i] : radians[i], &e);
+        const unsigned long long m = (unsigned long long)ldexp(x, 53);
+        unsigned long long p[5] = {};
+        for (int k = 0; k < 3; ++k) {
+            const unsigned __int128 y = (unsigned __int128)m * inv[k] + p[k];
+            p[k] = (unsigned long long)y;
+            p[k + 1] = (unsigned long long)(y >> 64);
+        }
+        auto word = [&](int at) {  // 64 bits from bit `at` on; those from 256 on are 0
+            const int w = at / 64, r = at % 64;
+            return w > 3 ? 0ull : r ? p[w] >> r | p[w + 1] << (64 - r) : p[w];
+        };
+        const int at = 128 - (e - 53);
+        const unsigned long long f = word(at) + (word(at - 1) & 1);  // rounded; a whole turn is none
+        freqs[i] = radians[i] < 0 ? 0 - f : f;
     }
     return RKV_OK;
 }
