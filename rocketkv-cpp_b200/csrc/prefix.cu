@@ -156,10 +156,10 @@ struct PrefixPlan {
     int own, slots;
     size_t off_ml, off_o, off_info, off_first, off_first_ml, off_first_o, off_later_ml, off_later_o, bytes;
 };
-PrefixPlan prefix_plan(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
+PrefixPlan prefix_plan(bool tc, int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
     PrefixPlan p{};
     const bool any = groups > 0 && batch > 0;
-    p.tc = any && on_tc(dtype, H, HK, D, max_len, batch, groups);
+    p.tc = any && tc && on_tc(dtype, H, HK, D, max_len, batch, groups);
     p.own = shared_own_parts(dtype, H, HK, D, max_len, batch, groups);
     p.slots = p.own + (any && !p.tc ? shared_prefix_parts(dtype, H, HK, D, max_len, batch, groups) : 0);
     size_t off = kWorkspaceHeader;
@@ -191,7 +191,11 @@ extern "C" int rkv_prefix_decode_workspace_size(int dtype, int num_heads, int nu
                                                 int num_groups, size_t* bytes) {
     const int rc = prefix_check(dtype, num_heads, num_heads_kv, dim_head, max_len, batch, num_groups);
     if (rc || !bytes) return rc ? rc : (int)RKV_ERR_INVALID_ARG;
-    *bytes = prefix_plan(dtype, num_heads, num_heads_kv, dim_head, max_len, batch, num_groups).bytes;
+    *bytes = 0;  // the larger of the plans with the tcgen05 kernel and without
+    for (bool tc : {true, false}) {
+        const size_t n = prefix_plan(tc, dtype, num_heads, num_heads_kv, dim_head, max_len, batch, num_groups).bytes;
+        if (n > *bytes) *bytes = n;
+    }
     return RKV_OK;
 }
 
@@ -206,7 +210,8 @@ extern "C" int rkv_prefix_decode(const void* Q, long long q_item_stride, int num
     if (!Q || !O || ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(O)) & 15)) return RKV_ERR_INVALID_ARG;
     if (batch > 1 && (q_item_stride < (long long)num_heads * D * es || (q_item_stride & 15))) return RKV_ERR_INVALID_ARG;
     if (num_groups > 0 && (!group_starts || !group_tokens)) return RKV_ERR_INVALID_ARG;
-    const PrefixPlan p = prefix_plan(cache->dtype, num_heads, cache->num_heads_kv, D, max_len, batch, num_groups);
+    const bool tc = on_tc(cache->dtype, num_heads, cache->num_heads_kv, D, max_len, batch, num_groups) && prefix_tc_usable(cache->dtype, D);
+    const PrefixPlan p = prefix_plan(tc, cache->dtype, num_heads, cache->num_heads_kv, D, max_len, batch, num_groups);
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < p.bytes) return RKV_ERR_WORKSPACE;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

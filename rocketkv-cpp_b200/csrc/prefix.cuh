@@ -135,6 +135,9 @@ struct Result {
 enum SharedPass { SHARED_TOKENS, OWN_TOKENS, ALL_TOKENS, OWN_AND_JOIN };
 // dependent: launched while the kernel before it still runs, which it waits for at its end only.
 int launch_shared_pass(const SharedArgs& s, SharedPass pass, const TcParts& t, const Result& r, bool dependent, cudaStream_t st);
+// Whether the tcgen05 kernel can run as compiled (also where that is not known: the launch says so then); where it
+// cannot, the matrix-instruction kernel attends the shared tokens.
+bool prefix_tc_usable(int dtype, int D);
 // spare: CTAs of the kernel before that hold an SM each; dependent as above.
 int launch_prefix_tc(const SharedArgs& s, const TcParts& p, int spare, bool dependent, cudaStream_t st);
 

@@ -1,4 +1,5 @@
-// prefix_parts.cuh -- what the joins may read of the tcgen05 kernel's parts.
+// prefix_parts.cuh -- what the joins may read of the tcgen05 kernel's parts, and how that kernel's roles divide its
+// registers.
 // Plain integer arithmetic, compiled for the host too (tests/prefix_parts_check.cpp).
 #pragma once
 
@@ -21,5 +22,11 @@ static_assert(kMaxShared >= kTcSms, "a unit may have a stretch per CTA");
 RKV_HOST_DEVICE bool parts_in_buffer(int behind, int row) {
     return behind == 0 || (behind > 0 && behind < kTcSms && row >= 0 && row < (kTcSms - (behind - 1)) * kTcRows);
 }
+
+// Threads of the tcgen05 kernel, and the registers that a thread of either half of them asks for once it has its role.
+constexpr int kTcThreads = 512, kTcFewRegs = 56, kTcManyRegs = 200;
+// Whether a kernel compiled to `regs` registers a thread was launched with as many as the roles ask for: where it was
+// not, those that ask for more would wait for ever.
+RKV_HOST_DEVICE bool split_fits(int regs) { return (long long)regs * kTcThreads >= (long long)(kTcFewRegs + kTcManyRegs) * (kTcThreads / 2); }
 
 }  // namespace rkv

@@ -46,13 +46,15 @@
 // the rows.  Not kept: a wait of the copying warps before each hand-over (103 us
 // -> 119 for the call at 131072 tokens), K and V by 16-byte copies where boxes can
 // be (this kernel 111 us there, 97 with boxes).
+#include <atomic>
+
 #include "attn_tc.cuh"
 #include "prefix.cuh"
 
 namespace rkv {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = kTcThreads;
 constexpr int kBlk = 128 * 128;  // bytes of a 128-row block of 64 columns
 constexpr int kMasks = 16;       // tiles whose masks are kept: more than the copies are ahead of the softmax
 
@@ -343,9 +345,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tbase = B.tmem;
 
-    // (56 + 56 + 200 + 200) * 128 registers are the 128 * 512 of the launch
+    // split_fits: together as many registers as the launch has
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(56));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcFewRegs));
         const int chunks = a.s.D / 8;
         int q = 0, nk = 0;  // slots, tiles
         bool ok = true;
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // every copy has landed before the CTA may end
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(56));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcFewRegs));
         if (warp == 4) {
             const uint32_t ids = mma_idesc(BF ? 1u : 0u, KEYS);
             const uint32_t idv = mma_idesc(BF ? 1u : 0u, KB * 64) | (1u << 16);  // B with N contiguous
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             keep_error(err);  // a wait gives up after two seconds at the soonest, long after this
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(200));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcManyRegs));
         const int u = (warp >> 2) - 2, q4 = warp & 3, row = q4 * 32 + lane;
         const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
         const uint32_t to = tbase + kColO + lane_off;
@@ -716,18 +718,28 @@ bool encode(CUtensorMap* m, const uint8_t* base, const SharedArgs& s, int box) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// What the kernel was compiled to, asked for until there is an answer; 0: none.
+template <int KB, bool BF, bool BOXES>
+int registers_of() {
+    static std::atomic<int> regs{0};
+    if (regs == 0) {
+        cudaFuncAttributes f;
+        if (cudaFuncGetAttributes(&f, prefix_tc_kernel<KB, BF, BOXES>) == cudaSuccess) regs = f.numRegs;
+        else (void)cudaGetLastError();
+    }
+    return regs;
+}
+template <int KB, bool BF>
+bool usable() {
+    const int boxes = registers_of<KB, BF, true>(), rows = registers_of<KB, BF, false>();
+    return (boxes == 0 || split_fits(boxes)) && (rows == 0 || split_fits(rows));
+}
+
 template <int KB, bool BF, bool BOXES>
 int launch_kernel(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, bool dependent, cudaStream_t st) {
     // the barriers, and up to 1023 bytes of alignment; Q and the ring
     const int smem = 2048 + unit_rows(KB) / 128 * KB * kBlk + ring_slots(KB) * KB * tile_keys(KB) * 128;
-    // the split of the registers is the launch's only where the kernel was compiled to 128 a thread
-    static const bool fits = [] {
-        cudaFuncAttributes f;
-        if (cudaFuncGetAttributes(&f, prefix_tc_kernel<KB, BF, BOXES>) == cudaSuccess) return f.numRegs == 128;
-        (void)cudaGetLastError();
-        return false;
-    }();
-    if (!fits) return RKV_ERR_CUDA;
+    if (!split_fits(registers_of<KB, BF, BOXES>())) return RKV_ERR_CUDA;  // not known
     if (cudaFuncSetAttribute(prefix_tc_kernel<KB, BF, BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
         (void)cudaGetLastError();
         return RKV_ERR_CUDA;
@@ -752,6 +764,13 @@ int launch(Args& a, bool dependent, cudaStream_t st) {
 }
 
 }  // namespace
+
+bool prefix_tc_usable(int dtype, int D) {
+    const bool bf = dtype == RKV_BF16;
+    if (D <= 64) return bf ? usable<1, true>() : usable<1, false>();
+    if (D <= 128) return bf ? usable<2, true>() : usable<2, false>();
+    return bf ? usable<4, true>() : usable<4, false>();
+}
 
 int launch_prefix_tc(const SharedArgs& s, const TcParts& p, int spare, bool dependent, cudaStream_t st) {
     Args a{};

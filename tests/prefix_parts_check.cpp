@@ -26,5 +26,8 @@ int main() {
                 if (at < 0 || at >= rows) fail("behind the buffer", behind, row);
             }
         }
+    // (56 + 200) * 256 registers are the 128 * 512 of an SM
+    for (int regs = 0; regs <= 255; ++regs)
+        if (split_fits(regs) != (regs >= 128)) fail("registers", regs, 0);
     return bad ? 1 : 0;
 }
