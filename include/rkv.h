@@ -539,8 +539,20 @@ int rkv_paged_append_rotated(const rkv_paged_cache* cache, const rkv_rotary* rot
  * results repeat bit for bit.  It is made for own tokens that are few beside the
  * shared ones and alike: a sequence with far more of them than the others runs
  * on few CTAs (24/8 heads of 128, bf16, 8192 shared tokens, 512 own ones, one
- * sequence with 65536 of its own: 64 sequences 225 us, 16 sequences 213, where
- * rkv_paged_decode takes 269 and 140).
+ * sequence with 65536 of its own: 64 sequences 223 us, 16 sequences 213, where
+ * rkv_paged_decode takes 265 and 139).
+ * max_len and num_groups fix the launch, the lengths and groups on the device do
+ * not.  The price of a loose max_len: from 12288 on own tokens are cut into more
+ * parts, most of them empty (64 sequences behind 8192 tokens as above: 49 us up
+ * to 12288, 57 under 16384, 67 under 131072; 192 in four groups behind 4096: 70
+ * and 109; 16 sequences or fewer, or fp32: 2 us or none).  The price of a loose
+ * num_groups: the kernel is chosen for a group of mean size, batch / num_groups,
+ * so one group of 64 takes 49 us under num_groups 1 to 11, 91 under 12 and 130
+ * under 64, and 32 sequences in one group beside 32 in groups of their own 94 (60
+ * with the other kernel): give it the number of groups that there are.  Batches
+ * that share little gain nothing: 2 sequences behind 1024 tokens 12 us, where
+ * rkv_paged_decode takes 8, 8 pairs behind 512 19 and 16, 64 groups of one
+ * sequence of 2048 tokens 104 and 95.
  * Workspace: device, 16-byte aligned, not shared with a call that may run at
  * the same time; it begins with the error word that rkv_workspace_status reads.
  * An error stays there until it is read, whatever calls and replays follow:

@@ -12,10 +12,11 @@
 // alone fill the GPU, the shared tokens, then the own ones with the join.  Each
 // is begun while the one before still runs.
 //
-// 24/8 heads of 128, bf16: 2 sequences behind 1024 tokens 11 us, 64 behind 8192
-// with up to 512 of their own 43, 8 behind 131072 107, 99 over one cache (0.78, 0.85
-// of a copy's rate; 640 without sharing).  Not kept: the shared tokens first where a join follows (45 us
-// -> 47), and the last CTA to arrive as the join (34 -> 42 for 24 sequences).
+// 24/8 heads of 128, bf16: 2 sequences behind 1024 tokens 11.6 us, 64 behind 8192
+// with up to 512 of their own 48 (244 without sharing), 8 behind 131072 121, 104 at
+// full clock (0.69, 0.81 of a copy's rate; 640 without sharing).  Not kept: the
+// shared tokens first where a join follows (45 us -> 47, when that took 45), and the
+// last CTA to arrive as the join (34 -> 42 for 24 sequences, when they took 34).
 #include "prefix.cuh"
 
 namespace rkv {
@@ -144,8 +145,11 @@ int prefix_check(int dtype, int H, int HK, int D, int max_len, int batch, int gr
     return RKV_OK;
 }
 
-// The shared tokens on the tcgen05 tensor cores: 16-bit types where a group of mean size has more rows of a KV head
-// than two CTAs of the matrix-instruction kernel take.
+// The shared tokens on the tcgen05 tensor cores: 16-bit types where a group of mean size has more than 16 rows of a KV
+// head (one CTA of the matrix-instruction kernel takes up to 16 with 128 columns, 8 above).  The groups themselves are
+// known on the device alone, and num_groups counts empty ones too.  24/8 heads of 128, bf16, 64 sequences: one group
+// behind 8192 tokens 49 us on the tensor cores, 91 as one of 12 groups and 130 as one of 64 on the other kernel; 16
+// groups of 4 behind 2048 tokens 55 on the latter and 65 on the tensor cores, 64 groups of one 104 and 139.
 bool on_tc(int dtype, int H, int HK, int D, int max_len, int batch, int groups) {
     const double tiles = ((double)groups + (double)batch * (H / HK) / 128) * HK * ((double)max_len / 64 + 1);
     return dtype != RKV_F32 && (long long)batch * (H / HK) > 16LL * groups && tiles < 1e9;  // counted in 32 bits

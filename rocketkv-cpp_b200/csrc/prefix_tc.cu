@@ -37,15 +37,17 @@
 // row of a tile sees all of its keys, but for those behind the shared tokens
 // and on pages outside the pool, which a mask of a bit per key leaves out.
 //
-// What bounds it.  Long prefixes and few rows: HBM, 8 sequences behind 131072
-// tokens (24/8 heads of 128, bf16) 87 us, 6.2 TB/s.  Many rows: a pair of tiles
-// takes 2.5 us, of which the products are 1.1 at their full rate and the
-// exponentials 1.1 at theirs; an accumulator's chain of scores, softmax and
-// products is covered by the other's in part.  Short ones: begin and end, 64
-// sequences behind 8192 tokens 21 us, 4 until the first scores, 4 tiles, 2 for
-// the rows.  Not kept: a wait of the copying warps before each hand-over (103 us
-// -> 119 for the call at 131072 tokens), K and V by 16-byte copies where boxes can
-// be (this kernel 111 us there, 97 with boxes).
+// What bounds it.  Many rows: a pair of tiles takes 3.2 us, of which the products
+// are 1.7 at their full rate and the exponentials 1.1 at theirs; an accumulator's
+// chain of scores, softmax and products is covered by the other's in part.  Long
+// prefixes and few rows: the same chain with one warp of each softmax at work, and
+// behind it HBM: 8 sequences behind 131072 tokens (24/8 heads of 128, bf16) 104 us
+// a call, 5.3 TB/s, at full clock, 115-121 where the power cap lowers it.  Short
+// ones: begin and end, 64 sequences behind 8192 tokens 25 us, 4 until the first
+// scores, 4 tiles, 2 for the rows.  Not kept, measured with P in one part: a wait
+// of the copying warps before each hand-over (a call at 131072 tokens 103 us ->
+// 119), K and V by 16-byte copies where boxes can be (its kernel 97 us with boxes,
+// 111 with copies, at a time when it took more than at the end).
 #include <atomic>
 
 #include "attn_tc.cuh"

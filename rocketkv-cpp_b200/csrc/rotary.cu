@@ -21,8 +21,8 @@
 // token and goes through the heads, so that a sine and a cosine serve up to 8 of
 // them.  Where there are few tokens the heads are spread over more threads and
 // CTAs.  bf16, 24/8 heads of 128: 4 x 4096 tokens on three axes (268 MB moved)
-// 47.5 us, 5.7 TB/s, 0.86 of a copy; 512 tokens 4.2 us; the step of 64 sequences
-// with its append 3.3 us.  Measured at 4 x 4096 tokens: sines and cosines in
+// 47.5 us, 5.6 TB/s, 0.86 of a copy; 512 tokens 4.5 us; the step of 64 sequences
+// with its append 3.8 us.  Measured at 4 x 4096 tokens: sines and cosines in
 // each thread's registers 78 us, all heads in one thread 61, products one by one
 // in place of two 73; 2 heads ahead 50 and with the next two behind them 61.
 #include <cmath>

@@ -661,7 +661,9 @@ class PrefixDecoder:
     group (rkv_prefix_decode): what a group shares is read once for all its
     sequences.  dtype: the cache's, and that of the output O [B, H, D]; lse
     [B, H] float32; both and the workspace are the object's, so calls that may
-    run at the same time need an object each."""
+    run at the same time need an object each.  max_len and num_groups decide
+    how the work is divided: bounds far above what the calls hold, empty groups
+    included, cost time (rkv.h has figures)."""
 
     def __init__(self, num_heads: int, num_heads_kv: int, dim_head: int, max_len: int, batch: int, dtype, device, num_groups: int = 1):
         import torch
@@ -842,8 +844,8 @@ class SinkAttention:
         return out
 
     def status(self, stream=None) -> int:
-        """Waits for `stream`; the first error that a call recorded in any
-        workspace since the last look, or RKV_OK."""
+        """Waits for `stream`; an error that the last call in any workspace
+        recorded (each call sets its workspace's error word anew), or RKV_OK."""
         import torch
         found = RKV_OK
         with torch.cuda.device(self.ws.device):
